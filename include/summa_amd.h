@@ -33,8 +33,17 @@ typedef enum sm_status {
  * holds K f16 "hi" values followed by K f16 "lo" values, x = hi + lo with
  * hi = f16(x), lo = f16(x - hi) (about 22 significant bits); the row stride
  * (ldx / ldy) counts f16 elements and is >= 2K. Matmul inputs of quantized
- * models use it so the f16 MFMA path keeps fp32-level activation precision. */
-typedef enum sm_dtype { SM_F32 = 0, SM_BF16 = 1, SM_F16 = 2, SM_F16X2 = 3 } sm_dtype;
+ * models use it so the f16 MFMA path keeps fp32-level activation precision.
+ *
+ * SM_F8E4M3: OCP e4m3 codes (4 exponent and 3 mantissa bits, largest value 448, no
+ * infinity), only as the type of a paged cache (sm_paged_cache). */
+typedef enum sm_dtype {
+  SM_F32 = 0,
+  SM_BF16 = 1,
+  SM_F16 = 2,
+  SM_F16X2 = 3,
+  SM_F8E4M3 = 4
+} sm_dtype;
 
 /* Library identity / diagnostics. */
 int sm_version(void);
@@ -397,6 +406,117 @@ int sm_attention_backward(const float* q, const float* k, const float* v, const 
                           const float* grad_out, const float* lse, int64_t B, int64_t H,
                           int64_t KVH, int64_t S, int64_t head_dim, int causal, float* dq,
                           float* dk, float* dv, float* delta_scratch, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Rotary positions in general form (MultiHeadAttention's RoPE, attention.rs:142-177,
+ * is the adjacent-pair layout over the whole head, without scaling).
+ * sm_rope_table: table [positions, rot_dim / 2, 2] f32 = magnitude * (cos, sin)(p f_i),
+ *   the rope_table of every call here that takes one; angles in f64, f_i =
+ *   theta^(-2 i / rot_dim), scaled for contexts `factor` times as long:
+ *   SM_ROPE_SCALE_LINEAR f_i / factor (position interpolation);
+ *   SM_ROPE_SCALE_THETA  theta * factor^(rot_dim / (rot_dim - 2)) for theta, which
+ *     leaves the fastest pair alone and divides the slowest by factor;
+ *   SM_ROPE_SCALE_PARTS  with r = original_positions f_i / 2 pi turns over the original
+ *     context: f_i where r >= high_turns, f_i / factor where r <= low_turns, in between
+ *     their mean weighted by (r - low_turns) / (high_turns - low_turns).
+ *   The arguments that a scaling does not name are ignored. rot_dim even.
+ * sm_rope: y [rows, heads, head_dim] = x with the first rot_dim dims of every head
+ *   rotated by table row positions[r]: (a, b) -> (a cos - b sin, b cos + a sin) over
+ *   dims (2 i, 2 i + 1) (SM_ROPE_INTERLEAVED) or (i, i + rot_dim / 2) (SM_ROPE_HALF);
+ *   backward != 0: by the opposite angle, which is the gradient with respect to x.
+ *   Rows are ldx / ldy values apart, so that the q and k heads of fused qkv rows are
+ *   rotated where they lie; y == x (with ldy == ldx) is allowed, other overlaps are
+ *   not. dtype SM_F32, SM_BF16 or SM_F16 (f32 arithmetic, one rounding); head_dim a
+ *   multiple of 16 up to 1024, rot_dim a multiple of 16 up to head_dim; rows, x, y and
+ *   table 16-byte aligned. A position outside [0, table_rows) gives NaN.
+ */
+enum { SM_ROPE_INTERLEAVED = 0, SM_ROPE_HALF = 1 };
+enum {
+  SM_ROPE_SCALE_NONE = 0,
+  SM_ROPE_SCALE_LINEAR = 1,
+  SM_ROPE_SCALE_THETA = 2,
+  SM_ROPE_SCALE_PARTS = 3
+};
+int sm_rope_table(double theta, int64_t rot_dim, int64_t positions, int scaling, double factor,
+                  double original_positions, double low_turns, double high_turns,
+                  double magnitude, float* table, void* stream);
+int sm_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, const float* table,
+            int64_t table_rows, const int32_t* positions, int64_t rows, int64_t heads,
+            int64_t head_dim, int64_t rot_dim, int layout, int backward, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Paged KV cache: AttnCache (attention.rs:20-40) in pages of page_tokens tokens that any
+ * sequence may hold in any order, so that rollouts of unequal length take what they use
+ * and rollouts of one prompt can share its full pages. 16-bit, or 8-bit: e4m3 codes with
+ * one power-of-two scale for every block of 16 tokens of a head.
+ *
+ * k [pages, kv_heads, page_tokens, head_dim].
+ * v [pages, kv_heads, page_tokens / 16, 16 * head_dim]: in each 16-token block, dim d of
+ *   token t is at (((d / (16 T) * 4 + t / 4) * 16 + d % 16) * T + d / 16 % T) * 4 + t % 4
+ *   with T = 4 (8-bit) or 2 (16-bit): four tokens' values of one dim lie together, as
+ *   the matrix cores take them.
+ * k_scales, v_scales (SM_F8E4M3; else ignored) [pages, kv_heads, page_tokens / 16]: the
+ *   exponent + 127; a stored code c stands for c * 2^(scale - 127).
+ * dtype SM_BF16, SM_F16 or SM_F8E4M3; head_dim 64 or 128; page_tokens a multiple of 16;
+ * k and v 16-byte aligned; fewer than 2^31 blocks in all.
+ *
+ * A batch: S sequences; block_table [S, table_cols] int32, entry j of a row the page of
+ * the sequence's tokens j page_tokens ..; pos0 [S] the tokens it holds before the call;
+ * its new rows are row_start[s] .. row_start[s + 1] - 1 (row_start [S + 1] int32), or,
+ * with row_start NULL, max_rows each (rows = S * max_rows). Row i of a sequence is at
+ * position pos0[s] + i. No sequence may have more than max_rows rows: what it has more is
+ * not processed. Rows that belong to no sequence are left as they are.
+ *
+ * sm_paged_append: k and v rows [rows, kv_heads, head_dim] (ldk, ldv values apart) of
+ *   `dtype` (SM_F32, SM_BF16, SM_F16) into the pages at their positions, k rotated by
+ *   rope_table [rope_rows, rot_dim / 2, 2] (as sm_rope; NULL: no rotation), and q rows
+ *   [rows, H, head_dim] (nullable) rotated into q_out [rows, H, head_dim] of q_dtype
+ *   (SM_BF16 or SM_F16), which must not overlap q. Rotation in f32, one rounding to the
+ *   cache's type. (project_qkv + slice_assign, attention.rs:142-177, 331-356.)
+ *   8-bit: a block's scale is the least 2^e, e >= -63, with every finite value of the
+ *   block within 448 * 2^e; it never falls while earlier tokens of the block stay, and
+ *   where a later token raises it their codes are scaled down and rounded again, which
+ *   is exact except among e4m3's subnormals. An infinity or NaN is stored as NaN (0x7f)
+ *   and does not enter the scale.
+ *   Tokens at a negative position, or for which the table names no page in [0, pages),
+ *   are not stored (nor is q of a negative position). Pages that several sequences hold
+ *   must not be written by two of them in one call.
+ * sm_paged_attention: out [rows, H, head_dim] of `dtype` (SM_BF16 or SM_F16; a 16-bit
+ *   cache must have the same): softmax(q . K / sqrt(head_dim)) . V over keys 0 .. position
+ *   of the row, query head h reading KV head h / (H / kv_heads); q rows ldq values apart,
+ *   16-byte aligned; lse (nullable) [rows, H] f32, the log-sum-exp of the scaled scores.
+ *   A row at a negative position sees no key: out 0, lse -inf. A row that sees a token
+ *   without a page gives NaN. What the pages hold behind a sequence's last token, and
+ *   values that a row does not see, do not enter its result, NaN and infinities among
+ *   them. (forward_cached / sdpa, attention.rs:216-265, 318-371.)
+ *   max_tokens: the tokens of the longest sequence, new rows included; it only decides
+ *   how the keys are split, a longer sequence is still attended to in full.
+ *   workspace: sm_paged_attention_workspace_bytes(...) bytes (-1 for a bad shape), 16-byte
+ *   aligned, for the partial sums of the splits; calls that share one must not overlap.
+ * Every length is read on the device, so a captured call may be replayed with other
+ * contents of the batch's arrays, up to max_rows.
+ */
+typedef struct sm_paged_cache {
+  void* k;
+  void* v;
+  uint8_t* k_scales;
+  uint8_t* v_scales;
+  int64_t pages, kv_heads, page_tokens, head_dim;
+  int32_t dtype;
+} sm_paged_cache;
+int sm_paged_append(const sm_paged_cache* cache, const int32_t* block_table, int64_t table_cols,
+                    const int32_t* pos0, const int32_t* row_start, int64_t S, int64_t rows,
+                    int64_t max_rows, const void* q, int64_t ldq, const void* k, int64_t ldk,
+                    const void* v, int64_t ldv, int dtype, int64_t H, const float* rope_table,
+                    int64_t rope_rows, int64_t rot_dim, int layout, void* q_out, int q_dtype,
+                    void* stream);
+int64_t sm_paged_attention_workspace_bytes(int64_t S, int64_t rows, int64_t max_rows, int64_t H,
+                                           int64_t KVH, int64_t head_dim, int64_t max_tokens);
+int sm_paged_attention(const sm_paged_cache* cache, const int32_t* block_table,
+                       int64_t table_cols, const int32_t* pos0, const int32_t* row_start,
+                       int64_t S, int64_t rows, int64_t max_rows, int64_t max_tokens,
+                       const void* q, int dtype, int64_t ldq, int64_t H, void* out, float* lse,
+                       void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Next-token selection for `rows` logits rows (select_next_token /
  * sample_from_logits, summa-llm/src/generate.rs:127-202). temperature <= 0:

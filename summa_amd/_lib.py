@@ -16,7 +16,7 @@ LIB_PATH = Path(os.environ.get("SUMMA_AMD_LIB",
                                Path(__file__).resolve().parent / "libsumma_amd.so"))
 
 SM_OK = 0
-SM_F32, SM_BF16, SM_F16, SM_F16X2 = 0, 1, 2, 3
+SM_F32, SM_BF16, SM_F16, SM_F16X2, SM_F8E4M3 = 0, 1, 2, 3, 4
 (SM_EPI_STORE_F32, SM_EPI_STORE_BF16, SM_EPI_ADD_F32, SM_EPI_SWIGLU_BF16, SM_EPI_SWIGLU_F16,
  SM_EPI_SWIGLU_F16X2) = 0, 1, 2, 3, 4, 5
 
@@ -28,6 +28,13 @@ class GemvJob(C.Structure):
     _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("x", C.c_void_p),
                 ("y", C.c_void_p), ("N", C.c_int64), ("K", C.c_int64),
                 ("epilogue", C.c_int32), ("first_block", C.c_int32)]
+
+class PagedCache(C.Structure):
+    """sm_paged_cache (include/summa_amd.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scales", C.c_void_p),
+                ("v_scales", C.c_void_p), ("pages", C.c_int64), ("kv_heads", C.c_int64),
+                ("page_tokens", C.c_int64), ("head_dim", C.c_int64), ("dtype", C.c_int32)]
+
 
 vp, i32, i64, u64, f32, f64 = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_float, C.c_double
 
@@ -73,6 +80,13 @@ SIGNATURES: dict[str, tuple] = {
     "sm_attention": (i32, [vp, vp, vp, i32, i64, i64, i64, i64, i64, i32, vp, vp, vp]),
     "sm_attention_backward": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i32, vp, vp,
                                     vp, vp, vp]),
+    "sm_rope_table": (i32, [f64, i64, i64, i32, f64, f64, f64, f64, f64, vp, vp]),
+    "sm_rope": (i32, [vp, i64, vp, i64, i32, vp, i64, vp, i64, i64, i64, i64, i32, i32, vp]),
+    "sm_paged_append": (i32, [vp, vp, i64, vp, vp, i64, i64, i64, vp, i64, vp, i64, vp, i64, i32,
+                              i64, vp, i64, i64, i32, vp, i32, vp]),
+    "sm_paged_attention_workspace_bytes": (i64, [i64, i64, i64, i64, i64, i64, i64]),
+    "sm_paged_attention": (i32, [vp, vp, i64, vp, vp, i64, i64, i64, i64, vp, i32, i64, i64, vp,
+                                 vp, vp, i64, vp]),
     "sm_sample": (i32, [vp, i64, i64, i64, f32, u64, i64, vp, i64, vp, i64, vp, vp]),
     "sm_sample_ex": (i32, [vp, i64, i64, i64, vp, u64, i64, vp, i64, vp, vp, vp, i64, vp, i64, vp,
                            vp]),

@@ -1,0 +1,505 @@
+// Attention over a paged KV cache, 16-bit or 8-bit (e4m3 codes with a power-of-two
+// scale per 16 tokens of a head). See sm_paged_attention for the layouts.
+#include <algorithm>
+#include <cmath>
+
+#include "attn_common.hpp"
+#include "common.hpp"
+#include "paged_map.hpp"
+
+namespace sm {
+namespace {
+
+struct PagedArgs {
+  const uint8_t *k, *v;          // cache pages
+  const uint8_t *ks, *vs;        // block scales (8-bit cache)
+  const uint16_t* q;
+  const int32_t *table, *pos0, *row_start;
+  void* out;
+  float* lse;
+  float *part_o, *part_ml;       // per (row, head, split): unnormalised O; (max, sum)
+  int64_t ldq;
+  int S, rows, max_rows, H, KVH, G, pages, bpp, cols, cb, nsplit, tiles;
+  float c2;                      // log2(e) / sqrt(hd)
+};
+
+// Four / eight cache codes of one packed word -> the MFMA operand's 16-bit values.
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+template <bool F16>
+__device__ inline uint32_t cvt2(uint32_t w, bool hi) {
+  if constexpr (F16)
+    return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true))
+              : __builtin_bit_cast(uint32_t,
+                                   __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
+  else
+    return hi ? __builtin_bit_cast(uint32_t,
+                                   __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true))
+              : __builtin_bit_cast(uint32_t,
+                                   __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
+}
+template <bool F16>
+__device__ inline u32x4 cvt8(uint32_t a, uint32_t b) {
+  return u32x4{cvt2<F16>(a, false), cvt2<F16>(a, true), cvt2<F16>(b, false), cvt2<F16>(b, true)};
+}
+
+template <bool F16>
+__device__ inline f4 mfma16(u32x4 a, u32x4 b, f4 c) {
+  return Op8<F16>::mfma(__builtin_bit_cast(typename Op8<F16>::T, a),
+                        __builtin_bit_cast(typename Op8<F16>::T, b), c);
+}
+template <bool F16>
+__device__ inline uint32_t pack2(float a, float b) {
+  if constexpr (F16) {
+    const f32x2_t v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));
+  } else {
+    return pack_bf16x2(a, b);
+  }
+}
+
+// Whether a word of cache values holds an infinity or a NaN.
+template <bool C8, bool F16>
+__device__ inline bool not_finite(uint32_t w) {
+  if constexpr (C8) {  // e4m3 has no infinity; NaN is 0x7f or 0xff
+    const uint32_t x = (w & 0x7f7f7f7fu) + 0x01010101u;
+    return (x & 0x80808080u) != 0;
+  } else {
+    constexpr uint32_t m = F16 ? 0x7c00u : 0x7f80u;
+    return (w & m) == m || ((w >> 16) & m) == m;
+  }
+}
+
+constexpr int kRows16 = 16;  // query rows of a workgroup
+
+template <int HD, bool QF16, bool C8>
+__global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
+  constexpr int ES = C8 ? 1 : 2;
+  constexpr bool PF16 = C8 || QF16;   // type of P and V in P.V
+  constexpr int NB = C8 ? 4 : 2;      // blocks a wave takes at a time
+  constexpr int NC = HD * ES / 64;    // 16-byte loads a lane makes of a block of K, and of V
+  constexpr int NT = HD / 16;         // 16-dim tiles of O
+  constexpr int BB = kBlock * HD * ES;  // bytes of a block
+  __shared__ float sm_m[4][kRows16], sm_l[4][kRows16];
+  __shared__ __attribute__((aligned(16))) float sm_o[4][kRows16][HD + 4];
+
+  uint32_t id = blockIdx.x;
+  const int split = (int)(id % a.nsplit);
+  id /= a.nsplit;
+  const int kvh = (int)(id % a.KVH);
+  id /= a.KVH;
+  const int tile = (int)(id % a.tiles), s = (int)(id / a.tiles);
+  const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
+  const int row0 = tile * kRows16, all = pr.n * a.G;
+  if (row0 >= all) return;
+  const int pos0 = a.pos0[s];
+  const PagedKeys pk(pos0, pr.n, a.G, row0, kRows16, a.cb, a.nsplit);
+  if (split >= max(pk.splits, 1)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int r = lane % 16, g = lane / 16;
+  const int b0 = pk.begin(split, a.cb), b1 = pk.keys > 0 ? pk.end(split, a.cb) : b0;
+
+  // this lane's query: row row0 + r
+  const int qr = min(row0 + r, all - 1);
+  const int qpos = pos0 + qr / a.G;
+  const int pos_first = pos0 + row0 / a.G;  // of the tile
+  u32x4 qf[HD / 32];
+  {
+    const uint16_t* qp = a.q + (int64_t)(pr.first + qr / a.G) * a.ldq +
+                         (int64_t)(kvh * a.G + qr % a.G) * HD;
+#pragma unroll
+    for (int c = 0; c < HD / 32; ++c) {
+      const int d = C8 ? (c / 2) * 64 + g * 16 + (c % 2) * 8 : c * 32 + g * 8;
+      qf[c] = *reinterpret_cast<const u32x4*>(qp + d);
+    }
+  }
+  f4 o[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) o[n] = f4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  const int32_t* trow = a.table + (int64_t)s * a.cols;
+
+  for (int seg = b0; seg < b1; seg += kWave) {
+    const int nb = min(kWave, b1 - seg);
+    // lane i: block seg + i
+    int bi = lane < nb ? paged_block(trow, a.cols, a.pages, a.KVH, kvh, a.bpp, seg + lane) : -1;
+    const bool bad = bi < 0;
+    bi = bad ? 0 : bi;
+    float kscale = a.c2, vexp = 0.f;
+    if constexpr (C8) {
+      kscale *= __uint_as_float((uint32_t)a.ks[bi] << 23);
+      vexp = (float)((int)a.vs[bi] - 127);
+    }
+    if (bad) kscale = NAN;
+    for (int st = wave * NB; st < nb; st += 4 * NB) {
+      u32x4 kr[NB][NC], vr[NB][NC];
+      float ksc[NB], vex[NB];
+#pragma unroll
+      for (int u = 0; u < NB; ++u) {
+        const int li = min(st + u, nb - 1);
+        const size_t at = (size_t)__builtin_amdgcn_readlane(bi, li) * BB;
+        ksc[u] = lane_f32(kscale, li);
+        vex[u] = lane_f32(vexp, li);
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          kr[u][c] = *reinterpret_cast<const u32x4*>(a.k + at + r * HD * ES + c * 64 + g * 16);
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          vr[u][c] = *reinterpret_cast<const u32x4*>(a.v + at + c * 1024 + lane * 16);
+      }
+      // scores, in units of log2 and raised by the exponent of V's scale
+      float t[NB][4];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < NB; ++u) {
+        f4 sc = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          if constexpr (C8) {
+            sc = mfma16<QF16>(cvt8<QF16>(kr[u][c].x, kr[u][c].y), qf[2 * c], sc);
+            sc = mfma16<QF16>(cvt8<QF16>(kr[u][c].z, kr[u][c].w), qf[2 * c + 1], sc);
+          } else {
+            sc = mfma16<QF16>(kr[u][c], qf[c], sc);
+          }
+        }
+        const int key0 = (seg + st + u) * kBlock;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          t[u][i] = C8 ? fmaf(sc[i], ksc[u], vex[u]) : sc[i] * ksc[u];
+          if (key0 + 4 * g + i > qpos || st + u >= nb) t[u][i] = -INFINITY;
+          mx = fmaxf(mx, t[u][i]);
+        }
+        // values past the tile's last key are not the cache's: no product sees them
+        if (key0 + kBlock > pk.keys || st + u >= nb || ksc[u] != ksc[u]) {
+          const int have = st + u >= nb || ksc[u] != ksc[u]
+                               ? 0 : max(0, min(4, pk.keys - key0 - 4 * g));
+          if constexpr (C8) {
+            const uint32_t keep = have >= 4 ? ~0u : (1u << (8 * have)) - 1;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) vr[u][c] &= keep;
+          } else {
+            const uint32_t k01 = have >= 2 ? ~0u : have == 1 ? 0xffffu : 0u;
+            const uint32_t k23 = have >= 4 ? ~0u : have == 3 ? 0xffffu : 0u;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) vr[u][c] &= u32x4{k01, k23, k01, k23};
+          }
+        }
+      }
+      if (__ballot(mx > m + 8.f)) {
+        mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+        const float mn = fmaxf(m, mx);
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[n] *= f;
+      }
+      const float ms = m == -INFINITY ? 0.f : m;
+      u32x4 p[NB / 2];
+#pragma unroll
+      for (int u = 0; u < NB; ++u) {
+        float e[4], sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(t[u][i] - ms);
+        sum = (e[0] + e[1]) + (e[2] + e[3]);
+        l = C8 ? fmaf(sum, __builtin_amdgcn_exp2f(-vex[u]), l) : l + sum;
+        p[u / 2][2 * (u % 2)] = pack2<PF16>(e[0], e[1]);
+        p[u / 2][2 * (u % 2) + 1] = pack2<PF16>(e[2], e[3]);
+      }
+      bool odd = false;  // values that are not finite where some row sees them and some not
+      if ((seg + st + NB) * kBlock - 1 > pos_first && pos_first + 1 < pk.keys) {
+        bool x = false;
+#pragma unroll
+        for (int u = 0; u < NB; ++u)
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x |= not_finite<C8, QF16>(vr[u][c][i]);
+        odd = __ballot(x) != 0;
+      }
+#pragma unroll
+      for (int w = 0; w < NB / 2; ++w) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          u32x4 va;
+          if constexpr (C8) {
+            va = cvt8<true>(vr[2 * w][n / 4][n % 4], vr[2 * w + 1][n / 4][n % 4]);
+          } else {
+            va = u32x4{vr[2 * w][n / 2][2 * (n % 2)], vr[2 * w][n / 2][2 * (n % 2) + 1],
+                       vr[2 * w + 1][n / 2][2 * (n % 2)], vr[2 * w + 1][n / 2][2 * (n % 2) + 1]};
+          }
+          if (!odd) {
+            o[n] = mfma16<PF16>(va, p[w], o[n]);
+          } else {  // key by key, each added only to the rows that see it
+            for (int key = 0; key < 2 * kBlock; ++key) {
+              const int e = key % 4 + 4 * (key / kBlock);
+              u32x4 one = va;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint32_t keep = e / 2 == i ? (e % 2 ? 0xffff0000u : 0xffffu) : 0u;
+                if (key % kBlock / 4 != g) keep = 0u;
+                one[i] &= keep;
+              }
+              const f4 part = mfma16<PF16>(one, p[w], f4{0.f, 0.f, 0.f, 0.f});
+              if ((seg + st + 2 * w) * kBlock + key <= qpos) o[n] += part;
+            }
+          }
+        }
+      }
+    }
+  }
+  l += __shfl_xor(l, 16, kWave);
+  l += __shfl_xor(l, 32, kWave);
+  if (g == 0) {
+    sm_m[wave][r] = m;
+    sm_l[wave][r] = l;
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) *reinterpret_cast<f4*>(&sm_o[wave][r][16 * n + 4 * g]) = o[n];
+  __syncthreads();
+
+  // row threadIdx.x / 16, HD / 16 of its dims
+  const int y = threadIdx.x / 16, d0 = (threadIdx.x % 16) * (HD / 16);
+  if (row0 + y >= all) return;
+  const int tok = (row0 + y) / a.G, head = kvh * a.G + (row0 + y) % a.G;
+  float mm = sm_m[0][y];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) mm = fmaxf(mm, sm_m[w][y]);
+  float ll = 0.f, f[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    // (a wave without keys has an empty sum, whatever its partner's maximum)
+    f[w] = sm_m[w][y] == -INFINITY ? (sm_l[w][y] == 0.f ? 0.f : NAN)
+                                   : __builtin_amdgcn_exp2f(sm_m[w][y] - mm);
+    ll = fmaf(sm_l[w][y], f[w], ll);
+  }
+  float acc[HD / 16];
+#pragma unroll
+  for (int i = 0; i < HD / 16; ++i) {
+    acc[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) acc[i] = fmaf(sm_o[w][y][d0 + i], f[w], acc[i]);
+  }
+  const size_t at = (size_t)(pr.first + tok) * a.H + head;
+  if (pk.splits > 1) {
+    float* po = a.part_o + (at * a.nsplit + split) * HD + d0;
+#pragma unroll
+    for (int i = 0; i < HD / 16; i += 4)
+      *reinterpret_cast<f4*>(po + i) = f4{acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
+    if (d0 == 0)
+      *reinterpret_cast<float2*>(a.part_ml + (at * a.nsplit + split) * 2) = float2{mm, ll};
+    return;
+  }
+  const bool none = pos0 + tok < 0;  // a row without keys
+  const float inv = 1.f / ll;
+  uint32_t w2[HD / 32];
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i)
+    w2[i] = none ? 0u : pack2<QF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  uint32_t* op = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at * HD + d0);
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i) op[i] = w2[i];
+  if (a.lse && d0 == 0)
+    a.lse[at] = none ? -INFINITY : (mm + __log2f(ll)) * 0.69314718055994530942f;
+}
+
+// Joins the splits of a (row, head): one wave each.
+template <int HD, bool QF16, int TILE>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
+  const int64_t id = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave;
+  const int head = (int)(id % a.H);
+  const int i = (int)(id / a.H % a.max_rows), s = (int)(id / a.H / a.max_rows);
+  if (s >= a.S) return;
+  const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
+  if (i >= pr.n) return;
+  const int pos0 = a.pos0[s], row = i * a.G + head % a.G;
+  const PagedKeys pk(pos0, pr.n, a.G, row / TILE * TILE, TILE, a.cb, a.nsplit);
+  if (pk.splits <= 1) return;  // written already
+  const size_t at = (size_t)(pr.first + i) * a.H + head;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at * a.nsplit;
+  const float* po = a.part_o + at * a.nsplit * HD;
+  constexpr int D = HD / kWave;
+  float mm = -INFINITY;
+  for (int x = lane; x < pk.splits; x += kWave) mm = fmaxf(mm, ml[x].x);
+  mm = wave_max(mm);
+  float ll = 0.f, acc[D];
+#pragma unroll
+  for (int d = 0; d < D; ++d) acc[d] = 0.f;
+  for (int x = 0; x < pk.splits; ++x) {
+    const float2 v = ml[x];
+    const float f = v.x == -INFINITY ? (v.y == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(v.x - mm);
+    ll = fmaf(v.y, f, ll);
+#pragma unroll
+    for (int d = 0; d < D; ++d) acc[d] = fmaf(po[(size_t)x * HD + lane * D + d], f, acc[d]);
+  }
+  const bool none = pos0 + i < 0;
+  const float inv = 1.f / ll;
+#pragma unroll
+  for (int d = 0; d < D; ++d) {
+    const float v = none ? 0.f : acc[d] * inv;
+    if constexpr (QF16)
+      static_cast<_Float16*>(a.out)[at * HD + lane * D + d] = (_Float16)v;
+    else
+      static_cast<uint16_t*>(a.out)[at * HD + lane * D + d] = f32_to_bf16(v);
+  }
+  if (a.lse && lane == 0)
+    a.lse[at] = none ? -INFINITY : (mm + __log2f(ll)) * 0.69314718055994530942f;
+}
+
+// How a call is split: rows of a tile, key blocks of a split and splits.
+struct PagedPlan {
+  int tile, cb, nsplit;
+  int64_t tiles, wgs;
+  PagedPlan(int64_t S, int64_t max_rows, int64_t G, int64_t KVH, int64_t max_tokens) {
+    tile = kRows16;
+    tiles = ceil_div(max_rows * G, tile);
+    const int64_t units = std::max<int64_t>(1, S * tiles * KVH);
+    const int64_t blocks = std::max<int64_t>(1, ceil_div(max_tokens, kBlock));
+    const int64_t want = std::max<int64_t>(1, ceil_div(1024, units));
+    cb = (int)(ceil_div(std::max<int64_t>(16, ceil_div(blocks, want)), 16) * 16);
+    nsplit = (int)ceil_div(blocks, cb);
+    wgs = S * tiles * KVH * nsplit;
+  }
+  int64_t bytes(int64_t rows, int64_t H, int64_t hd) const {
+    return nsplit > 1 ? rows * H * nsplit * (hd + 2) * 4 : 0;
+  }
+};
+
+int check_shape(const char* who, int64_t S, int64_t rows, int64_t max_rows, int64_t H,
+                int64_t KVH, int64_t hd, int64_t max_tokens) {
+  const int64_t most = 0x7fffffff;
+  SM_REQUIRE(S >= 0 && rows >= 0 && max_rows >= 0 && S < most && rows < most && max_rows <= rows,
+             "%s: need S >= 0 sequences and 0 <= max_rows <= rows", who);
+  SM_REQUIRE(H > 0 && KVH > 0 && H % KVH == 0 && H <= 65535,
+             "%s: H must be a multiple of KVH, at most 65535", who);
+  SM_REQUIRE(hd == 64 || hd == 128, "%s: head_dim must be 64 or 128", who);
+  SM_REQUIRE(max_tokens >= 0 && max_tokens <= most, "%s: max_tokens must be in 0..2^31 - 1", who);
+  // (the grid holds less than 2^24 workgroups of 256 threads, and 32 bits index a row)
+  if (max_rows * (H / KVH) >= most ||
+      (double)S * (double)ceil_div(max_rows * (H / KVH), 16) * (double)KVH >= (double)(1 << 24) ||
+      (double)S * (double)max_rows * (double)H >= (double)(1 << 26)) {
+    set_error("%s: problem too large", who);
+    return SM_ERR_UNSUPPORTED;
+  }
+  return SM_OK;
+}
+
+}  // namespace
+
+// Shared with the append: what a cache descriptor has to be.
+int check_paged_cache(const char* who, const sm_paged_cache* c) {
+  SM_REQUIRE(c, "%s: null cache", who);
+  SM_REQUIRE(c->dtype == SM_BF16 || c->dtype == SM_F16 || c->dtype == SM_F8E4M3,
+             "%s: cache dtype must be SM_BF16, SM_F16 or SM_F8E4M3", who);
+  SM_REQUIRE(c->head_dim == 64 || c->head_dim == 128, "%s: head_dim must be 64 or 128", who);
+  SM_REQUIRE(c->pages > 0 && c->kv_heads > 0 && c->page_tokens > 0 &&
+                 c->page_tokens % kBlock == 0,
+             "%s: need pages and kv_heads > 0 and page_tokens a positive multiple of 16", who);
+  const int64_t most = 0x7fffffff;
+  SM_REQUIRE(c->pages <= most && c->kv_heads <= 65535 && c->page_tokens <= most &&
+                 c->kv_heads * (c->page_tokens / kBlock) <= most / c->pages,
+             "%s: a cache holds less than 2^31 blocks of 16 tokens", who);
+  SM_REQUIRE(c->k && c->v, "%s: null cache pages", who);
+  SM_REQUIRE(reinterpret_cast<uintptr_t>(c->k) % 16 == 0 &&
+                 reinterpret_cast<uintptr_t>(c->v) % 16 == 0,
+             "%s: cache pages must be 16-byte aligned", who);
+  SM_REQUIRE(c->dtype != SM_F8E4M3 || (c->k_scales && c->v_scales),
+             "%s: an SM_F8E4M3 cache needs k_scales and v_scales", who);
+  return SM_OK;
+}
+
+}  // namespace sm
+
+extern "C" int64_t sm_paged_attention_workspace_bytes(int64_t S, int64_t rows, int64_t max_rows,
+                                                      int64_t H, int64_t KVH, int64_t head_dim,
+                                                      int64_t max_tokens) {
+  if (sm::check_shape("sm_paged_attention_workspace_bytes", S, rows, max_rows, H, KVH, head_dim,
+                      max_tokens) != SM_OK)
+    return -1;
+  if (S == 0 || max_rows == 0) return 0;
+  return sm::PagedPlan(S, max_rows, H / KVH, KVH, max_tokens).bytes(rows, H, head_dim);
+}
+
+extern "C" int sm_paged_attention(const sm_paged_cache* cache, const int32_t* block_table,
+                                  int64_t table_cols, const int32_t* pos0,
+                                  const int32_t* row_start, int64_t S, int64_t rows,
+                                  int64_t max_rows, int64_t max_tokens, const void* q, int dtype,
+                                  int64_t ldq, int64_t H, void* out, float* lse, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  using namespace sm;
+  const char* me = "sm_paged_attention";
+  SM_TRY(check_paged_cache(me, cache));
+  const int64_t KVH = cache->kv_heads, hd = cache->head_dim;
+  SM_TRY(check_shape(me, S, rows, max_rows, H, KVH, hd, max_tokens));
+  SM_REQUIRE(dtype == SM_BF16 || dtype == SM_F16, "%s: dtype must be SM_BF16 or SM_F16", me);
+  SM_REQUIRE(cache->dtype == SM_F8E4M3 || cache->dtype == dtype,
+             "%s: a 16-bit cache must have the query's dtype", me);
+  if (S == 0 || max_rows == 0) return SM_OK;
+  SM_REQUIRE(block_table && pos0 && q && out, "%s: null buffer", me);
+  SM_REQUIRE(table_cols > 0 && table_cols <= 0x7fffffff, "%s: table_cols must be positive", me);
+  SM_REQUIRE(row_start || rows == S * max_rows,
+             "%s: without row_start, rows must be S * max_rows", me);
+  SM_REQUIRE(ldq >= H * hd && ldq % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
+                 reinterpret_cast<uintptr_t>(out) % 16 == 0,
+             "%s: q rows and out must be 16-byte aligned, ldq >= H * head_dim", me);
+  const PagedPlan plan(S, max_rows, H / KVH, KVH, max_tokens);
+  const int64_t need = plan.bytes(rows, H, hd);
+  SM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need &&
+                           reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+             "%s: workspace of %lld bytes, %lld needed, 16-byte aligned", me,
+             (long long)workspace_bytes, (long long)need);
+  const int64_t joins = ceil_div(S * max_rows * H, 4);
+  if (plan.wgs >= (1 << 24) || joins >= (1 << 24)) {
+    set_error("%s: problem too large", me);
+    return SM_ERR_UNSUPPORTED;
+  }
+  hipStream_t st = as_stream(stream);
+  PagedArgs a;
+  a.k = static_cast<const uint8_t*>(cache->k);
+  a.v = static_cast<const uint8_t*>(cache->v);
+  a.ks = cache->k_scales;
+  a.vs = cache->v_scales;
+  a.q = static_cast<const uint16_t*>(q);
+  a.table = block_table;
+  a.pos0 = pos0;
+  a.row_start = row_start;
+  a.out = out;
+  a.lse = lse;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = need ? a.part_o + rows * H * plan.nsplit * hd : nullptr;
+  a.ldq = ldq;
+  a.S = (int)S;
+  a.rows = (int)rows;
+  a.max_rows = (int)max_rows;
+  a.H = (int)H;
+  a.KVH = (int)KVH;
+  a.G = (int)(H / KVH);
+  a.pages = (int)cache->pages;
+  a.bpp = (int)(cache->page_tokens / kBlock);
+  a.cols = (int)table_cols;
+  a.cb = plan.cb;
+  a.nsplit = plan.nsplit;
+  a.tiles = (int)plan.tiles;
+  a.c2 = 1.44269504088896340736f / sqrtf((float)hd);
+  const bool f16 = dtype == SM_F16, c8 = cache->dtype == SM_F8E4M3;
+#define SM_PAGED2(HD, F, C)                                                      \
+  do {                                                                           \
+    paged_split_kernel<HD, F, C><<<(unsigned)plan.wgs, 256, 0, st>>>(a);         \
+    if (plan.nsplit > 1)                                                         \
+      paged_join_kernel<HD, F, kRows16><<<(unsigned)joins, 256, 0, st>>>(a);     \
+  } while (0)
+#define SM_PAGED(HD)                             \
+  do {                                           \
+    if (f16 && c8) SM_PAGED2(HD, true, true);    \
+    else if (f16) SM_PAGED2(HD, true, false);    \
+    else if (c8) SM_PAGED2(HD, false, true);     \
+    else SM_PAGED2(HD, false, false);            \
+  } while (0)
+  if (hd == 64) SM_PAGED(64);
+  else SM_PAGED(128);
+#undef SM_PAGED
+#undef SM_PAGED2
+  SM_LAUNCH_CHECK();
+  return SM_OK;
+}

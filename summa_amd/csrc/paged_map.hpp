@@ -1,0 +1,72 @@
+// What a paged batch's sequences, rows and key splits are. Host and device, so that
+// the map can be walked on the CPU.
+#pragma once
+
+#include <cstdint>
+
+#include <hip/hip_runtime.h>
+
+namespace sm {
+
+constexpr int kBlock = 16;  // tokens of a cache block (and of a scale)
+
+// Rows [first, first + n) of sequence s: the ragged form's row_start [S + 1], or
+// max_rows each without one. Whatever row_start holds, they lie inside [0, rows).
+struct PagedRows {
+  int first, n;
+  __host__ __device__ PagedRows(const int32_t* row_start, int s, int rows, int max_rows) {
+    int a, b;
+    if (row_start) {
+      a = row_start[s];
+      b = row_start[s + 1];
+      a = a < 0 ? 0 : a > rows ? rows : a;
+      b = b < a ? a : b > rows ? rows : b;
+    } else {
+      a = s * max_rows;
+      b = a + max_rows;
+    }
+    first = a;
+    n = b - a < max_rows ? b - a : max_rows;
+  }
+};
+
+// The cache block of block `blk` of a sequence, as an index over [pages, KVH, page / 16];
+// -1 where the table has no such entry or the entry names no page.
+__host__ __device__ inline int paged_block(const int32_t* table_row, int cols, int pages, int KVH,
+                                           int kvh, int bpp, int blk) {
+  const int col = blk / bpp;
+  if (blk < 0 || col >= cols) return -1;
+  const int page = table_row[col];
+  if (page < 0 || page >= pages) return -1;
+  return (page * KVH + kvh) * bpp + (blk - col * bpp);
+}
+
+// Blocks that n tokens touch at most, wherever the first of them falls.
+__host__ __device__ inline int64_t paged_touched(int64_t n) { return (n + kBlock - 2) / kBlock + 1; }
+
+// Keys of one tile of `tile` query rows and their split. A row is a (token, head of
+// the KV head's group) pair, G heads to a token, so the tile's last row sees the most
+// keys. Split i of `nsplit` takes blocks [i cb, (i + 1) cb); the last one takes what is
+// left, so that no key is dropped however long the sequence is.
+struct PagedKeys {
+  int keys;    // keys that the tile's last row sees (<= 0: none)
+  int blocks;  // blocks that hold them
+  int splits;  // splits that have work (0 without keys)
+  __host__ __device__ PagedKeys(int pos0, int n, int G, int first_row, int tile, int cb,
+                                int nsplit) {
+    const int all = n * G;
+    int last = first_row + tile - 1;
+    if (last > all - 1) last = all - 1;
+    const int64_t k = (int64_t)pos0 + last / G + 1;
+    keys = k < 0 ? 0 : k > 0x7fffffff ? 0x7fffffff : (int)k;
+    blocks = (int)(((int64_t)keys + kBlock - 1) / kBlock);
+    const int64_t want = ((int64_t)blocks + cb - 1) / cb;
+    splits = want < nsplit ? (int)want : nsplit;
+  }
+  __host__ __device__ int begin(int split, int cb) const { return split * cb; }
+  __host__ __device__ int end(int split, int cb) const {
+    return split + 1 >= splits ? blocks : (split + 1) * cb;
+  }
+};
+
+}  // namespace sm

@@ -716,6 +716,90 @@ def row_permute(input: torch.Tensor, order: torch.Tensor, inverse: torch.Tensor 
     return out
 
 
+# ------------------------------------------------------ rotary positions ---
+
+_ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+_ROPE_SCALINGS = {"none": 0, "linear": 1, "theta": 2, "parts": 3}
+
+
+def _rope_layout(layout: str) -> int:
+    try:
+        return _ROPE_LAYOUTS[layout]
+    except KeyError as e:
+        raise ValueError("layout must be 'interleaved' or 'half'") from e
+
+
+def _on_current(device: torch.device) -> None:
+    """The library launches on the current device's stream."""
+    if device.type != "cuda":
+        raise ValueError("tensors must be on the device")
+    if device.index != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors are on {device}, which is not the current device")
+
+
+def _rope_angles(table: torch.Tensor | None, device):
+    """(pointer, rows, rot_dim) of a checked rotary table; None: no rotation."""
+    if table is None:
+        return None, 0, 0
+    if table.dtype != torch.float32 or table.dim() != 3 or table.shape[2] != 2 or \
+            not table.is_contiguous():
+        raise ValueError("a rotary table is contiguous float32 [positions, rot_dim / 2, 2]")
+    if table.device != device:
+        raise ValueError("the rotary table must be on the tensors' device")
+    return table.data_ptr(), table.shape[0], 2 * table.shape[1]
+
+
+def rope_table(positions: int, rot_dim: int, theta: float = 1e4, *, scaling: str = "none",
+               factor: float = 1.0, original_positions: float = 0.0, low_turns: float = 1.0,
+               high_turns: float = 32.0, magnitude: float = 1.0, device="cuda") -> torch.Tensor:
+    """The rotary table [positions, rot_dim / 2, 2] f32 of (cos, sin) that every call with a
+    rope_table reads (``sm_rope_table``; attention.rs:142-177 without scaling). ``scaling``
+    stretches it for longer contexts: "linear" divides every frequency by ``factor``,
+    "theta" raises the base, "parts" divides only the pairs that make at most ``low_turns``
+    turns over ``original_positions``, leaves those of ``high_turns`` and more, and mixes
+    between; ``magnitude`` multiplies cosines and sines."""
+    if scaling not in _ROPE_SCALINGS:
+        raise ValueError("scaling must be 'none', 'linear', 'theta' or 'parts'")
+    if positions < 0 or rot_dim <= 0 or rot_dim % 2:
+        raise ValueError("need positions >= 0 and an even rot_dim > 0")
+    t = torch.empty(positions, rot_dim // 2, 2, dtype=torch.float32, device=device)
+    _on_current(t.device)
+    call("sm_rope_table", float(theta), rot_dim, positions, _ROPE_SCALINGS[scaling], float(factor),
+         float(original_positions), float(low_turns), float(high_turns), float(magnitude),
+         t.data_ptr(), _stream())
+    return t
+
+
+def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
+         layout: str = "interleaved", backward: bool = False,
+         out: torch.Tensor | None = None) -> torch.Tensor:
+    """x [rows, heads, head_dim] (float32, bfloat16 or float16; rows may be strided, as the q
+    and k heads of fused qkv rows are) with the first ``2 * table.shape[1]`` dims of every
+    head rotated by the table's row ``positions[r]`` (int32 [rows]); ``backward``: by the
+    opposite angle, the gradient with respect to x. ``out`` may be x itself
+    (``sm_rope``; attention.rs:142-177)."""
+    if x.dim() != 3 or x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != x.shape[2]):
+        raise ValueError("x must be [rows, heads, head_dim] with contiguous heads")
+    rows, heads, hd = x.shape
+    dt = _dt(x)
+    _on_current(x.device)
+    if positions.dtype != torch.int32 or positions.shape != (rows,) or \
+            not positions.is_contiguous() or positions.device != x.device:
+        raise ValueError("positions must be contiguous int32 [rows] on x's device")
+    at, table_rows, rot = _rope_angles(table, x.device)
+    if out is None:
+        out = torch.empty((rows, heads, hd), dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or \
+            out.stride(2) != 1 or (heads > 1 and out.stride(1) != hd):
+        raise ValueError("out must have x's shape and dtype, with contiguous heads")
+    width = heads * hd
+    ldx, ldy = (t.stride(0) if rows > 1 else width for t in (x, out))
+    call("sm_rope", x.data_ptr(), ldx, out.data_ptr(), ldy, dt, at, table_rows,
+         positions.data_ptr(), rows, heads, hd, rot, _rope_layout(layout), int(backward),
+         _stream())
+    return out
+
+
 # ------------------------------------------------------------- attention ---
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = True,
