@@ -6,6 +6,7 @@
 #include "attn_common.hpp"
 #include "common.hpp"
 #include "paged_map.hpp"
+#include "prefill_map.hpp"
 
 namespace sm {
 namespace {
@@ -19,7 +20,7 @@ struct PagedArgs {
   float* lse;
   float *part_o, *part_ml;       // per (row, head, split): unnormalised O; (max, sum)
   int64_t ldq;
-  int S, rows, max_rows, H, KVH, G, pages, bpp, cols, cb, nsplit, tiles;
+  int S, rows, max_rows, H, KVH, G, pages, bpp, cols, cb, nsplit, tile, tiles;
   float c2;                      // log2(e) / sqrt(hd)
 };
 
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
     bi = bad ? 0 : bi;
     float kscale = a.c2, vexp = 0.f;
     if constexpr (C8) {
-      kscale *= __uint_as_float((uint32_t)a.ks[bi] << 23);
+      kscale = __builtin_amdgcn_ldexpf(kscale, (int)a.ks[bi] - 127);
       vexp = (float)((int)a.vs[bi] - 127);
     }
     if (bad) kscale = NAN;
@@ -303,8 +304,317 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
     a.lse[at] = none ? -INFINITY : (mm + __log2f(ll)) * 0.69314718055994530942f;
 }
 
+// ---- many query rows: 128 of them a workgroup, keys staged through LDS ----
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+template <bool F16>
+__device__ inline f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a),
+                                                  __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a),
+                                                   __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+}
+
+constexpr int kRowsTile = 128;  // query rows of a workgroup, 32 a wave
+constexpr int kTile = 64;       // keys of a tile: a block to a wave's staging
+
+template <int HD, bool QF16, bool C8>
+__global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
+  constexpr int ES = C8 ? 1 : 2;
+  constexpr bool PF16 = C8 || QF16;
+  constexpr int KS = HD / 16, DB = HD / 32;  // MFMA steps of a score, 32-dim blocks of O
+  constexpr int KP = HD + 8, VP = kTile + 8; // padded LDS rows (elements)
+  constexpr int NC = HD * ES / 64;           // 16-byte loads a lane makes of a block
+  constexpr int BB = kBlock * HD * ES;
+  __shared__ __attribute__((aligned(16))) uint16_t ks[2][kTile * KP];
+  __shared__ __attribute__((aligned(16))) uint16_t vts[2][HD * VP];
+  __shared__ float info[2][4][4];  // a tile's blocks: score factor, V exponent, not finite
+
+  const PrefillMap map((uint32_t)(a.S * a.KVH * a.nsplit), (uint32_t)a.tiles);
+  uint32_t grp, place;
+  if (!map.at(blockIdx.x, grp, place)) return;  // (uniform)
+  const int split = (int)(grp % a.nsplit);
+  const int kvh = (int)(grp / a.nsplit % a.KVH), s = (int)(grp / a.nsplit / a.KVH);
+  const int tile = a.tiles - 1 - (int)place;  // the rows with the most keys first
+  const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
+  const int row0 = tile * kRowsTile, all = pr.n * a.G;
+  if (row0 >= all) return;
+  const int pos0 = a.pos0[s];
+  const PagedKeys pk(pos0, pr.n, a.G, row0, kRowsTile, a.cb, a.nsplit);
+  if (split >= max(pk.splits, 1)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int j = lane % 32, hf = lane / 32;
+  const int b0 = pk.begin(split, a.cb), b1 = pk.keys > 0 ? pk.end(split, a.cb) : b0;
+  const int r0 = row0 + wave * 32;  // first row of this wave
+  const int qr = min(r0 + j, all - 1);
+  const int qpos = pos0 + qr / a.G;
+  const int pos_first = pos0 + row0 / a.G;
+  // positions of the wave's first and last row
+  const int wave_first = pos0 + min(r0, all - 1) / a.G;
+  const int wave_last = r0 < all ? pos0 + min(r0 + 31, all - 1) / a.G : -1;
+
+  u32x4 qa[KS];
+  {
+    const uint16_t* qp = a.q + (int64_t)(pr.first + qr / a.G) * a.ldq +
+                         (int64_t)(kvh * a.G + qr % a.G) * HD;
+#pragma unroll
+    for (int st = 0; st < KS; ++st)
+      qa[st] = *reinterpret_cast<const u32x4*>(qp + st * 16 + hf * 8);
+  }
+  f32x16 o[DB];  // o[d][e]: row j, dim 32 d + 8 (e / 4) + 4 hf + e % 4
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  // lane i: block seg + i of the segment at hand, and of the next
+  const int32_t* trow = a.table + (int64_t)s * a.cols;
+  int bi, bi_next;
+  float kscale, vexp, kscale_next, vexp_next;
+  auto look_up = [&](int seg, int& b, float& kf, float& vf) {
+    b = seg + lane < b1 ? paged_block(trow, a.cols, a.pages, a.KVH, kvh, a.bpp, seg + lane) : -1;
+    const bool bad = b < 0;
+    b = bad ? 0 : b;
+    kf = a.c2;
+    vf = 0.f;
+    if constexpr (C8) {
+      kf = __builtin_amdgcn_ldexpf(kf, (int)a.ks[b] - 127);
+      vf = (float)((int)a.vs[b] - 127);
+    }
+    if (bad) kf = NAN;
+  };
+  u32x4 kr[NC], vr[NC];
+  float kf_s, vf_s;
+  bool odd_s;
+  // wave w stages block w of a tile
+  auto load_tile = [&](int blk) {  // first block of the tile
+    const int li = (blk - b0 + wave) % kWave;
+    kf_s = lane_f32(kscale, li);
+    vf_s = lane_f32(vexp, li);
+    const size_t at = (size_t)__builtin_amdgcn_readlane(bi, li) * BB;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      kr[c] = *reinterpret_cast<const u32x4*>(a.k + at + c * 1024 + lane * 16);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      vr[c] = *reinterpret_cast<const u32x4*>(a.v + at + c * 1024 + lane * 16);
+  };
+  auto store_tile = [&](int blk, int buf) {
+    const int g = lane / 16, r = lane % 16;
+    const int key0 = (blk + wave) * kBlock;
+    odd_s = false;
+    if (key0 + kBlock > pk.keys || kf_s != kf_s) {  // not the cache's: no product sees them
+      const int have = kf_s != kf_s ? 0 : max(0, min(4, pk.keys - key0 - 4 * g));
+      if constexpr (C8) {
+        const uint32_t keep = have >= 4 ? ~0u : (1u << (8 * have)) - 1;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) vr[c] &= keep;
+      } else {
+        const uint32_t k01 = have >= 2 ? ~0u : have == 1 ? 0xffffu : 0u;
+        const uint32_t k23 = have >= 4 ? ~0u : have == 3 ? 0xffffu : 0u;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) vr[c] &= u32x4{k01, k23, k01, k23};
+      }
+    }
+    if (key0 + kBlock - 1 > pos_first) {  // some rows see these keys and some do not
+      bool x = false;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x |= not_finite<C8, QF16>(vr[c][i]);
+      odd_s = __ballot(x) != 0;
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int at = (c * 64 + lane) * (16 / ES);  // element of the block
+      uint16_t* kp = &ks[buf][(wave * kBlock + at / HD) * KP + at % HD];
+      if constexpr (C8) {
+        *reinterpret_cast<u32x4*>(kp) = cvt8<QF16>(kr[c].x, kr[c].y);
+        *reinterpret_cast<u32x4*>(kp + 8) = cvt8<QF16>(kr[c].z, kr[c].w);
+      } else {
+        *reinterpret_cast<u32x4*>(kp) = kr[c];
+      }
+      // quads of a block in the order 0, 2, 1, 3: the order in which a lane of the
+      // transposed score tile holds its keys
+      uint16_t* vp = &vts[buf][r * VP + wave * kBlock + (g % 2 * 2 + g / 2) * 4];
+#pragma unroll
+      for (int t = 0; t < 4 / ES; ++t) {
+        u32x2 w;
+        if constexpr (C8) w = u32x2{cvt2<true>(vr[c][t], false), cvt2<true>(vr[c][t], true)};
+        else w = u32x2{vr[c][2 * t], vr[c][2 * t + 1]};
+        *reinterpret_cast<u32x2*>(vp + (c * (4 / ES) + t) * 16 * VP) = w;
+      }
+    }
+    if (lane == 0)
+      *reinterpret_cast<f4*>(info[buf][wave]) = f4{kf_s, vf_s, odd_s ? 1.f : 0.f, 0.f};
+  };
+
+  if (b1 > b0) {
+    look_up(b0, bi, kscale, vexp);
+    load_tile(b0);
+    store_tile(b0, 0);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int blk = b0; blk < b1; blk += 4, buf ^= 1) {
+    const bool more = blk + 4 < b1;
+    if ((blk - b0) % kWave == 0 && blk + kWave < b1)
+      look_up(blk + kWave, bi_next, kscale_next, vexp_next);
+    if (more) {
+      if ((blk + 4 - b0) % kWave == 0) {
+        bi = bi_next;
+        kscale = kscale_next;
+        vexp = vexp_next;
+      }
+      load_tile(blk + 4);
+    }
+    const int key0 = blk * kBlock;
+    if (key0 <= wave_last) {  // (uniform per wave) later keys are hidden from all its rows
+      f32x16 sc[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[kb][e] = 0.f;
+#pragma unroll
+        for (int st = 0; st < KS; ++st) {
+          const u32x4 kf =
+              *reinterpret_cast<const u32x4*>(&ks[buf][(kb * 32 + j) * KP + st * 16 + hf * 8]);
+          sc[kb] = mfma32<QF16>(kf, qa[st], sc[kb]);
+        }
+      }
+      float kf[4], vf[4];
+      bool odd = false;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const f4 x = *reinterpret_cast<const f4*>(info[buf][b]);
+        kf[b] = x[0];
+        vf[b] = x[1];
+        odd |= x[2] != 0.f;
+      }
+      odd = __ballot(odd) != 0;
+      if (key0 + kTile - 1 > wave_first) {  // the diagonal, or past the last key
+        const int lim = qpos - key0 - 4 * hf;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (kb * 32 + 8 * (e / 4) + e % 4 > lim) sc[kb][e] = -INFINITY;
+        // (a block without a page has the factor NaN: only where it is seen)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (b * kBlock > qpos - key0) kf[b] = a.c2;
+      }
+      // scores in units of log2, raised by the exponent of V's scale
+      float mx = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        float x = sc[b / 2][8 * (b % 2)];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) x = fmaxf(x, sc[b / 2][8 * (b % 2) + e]);
+        mx = fmaxf(mx, C8 ? fmaf(x, kf[b], vf[b]) : x * kf[b]);
+      }
+      if (__ballot(mx > m + 8.f)) {
+        mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+        const float mn = fmaxf(m, mx);
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[d][e] *= f;
+      }
+      const float ms = m == -INFINITY ? 0.f : m;
+      u32x4 p[4];  // P^T of a block's 16 keys
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const float off = vf[b] - ms;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(sc[b / 2][8 * (b % 2) + 2 * e], kf[b], off));
+          const float y =
+              __builtin_amdgcn_exp2f(fmaf(sc[b / 2][8 * (b % 2) + 2 * e + 1], kf[b], off));
+          sum += x;
+          sum += y;
+          p[b][e] = pack2<PF16>(x, y);
+        }
+        l = C8 ? fmaf(sum, __builtin_amdgcn_exp2f(-vf[b]), l) : l + sum;
+      }
+      if (!odd) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            const u32x4 vb = *reinterpret_cast<const u32x4*>(
+                &vts[buf][(d * 32 + j) * VP + b * kBlock + hf * 8]);
+            o[d] = mfma32<PF16>(vb, p[b], o[d]);
+          }
+      } else {  // key by key, each added only to the rows that see it
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            const u32x4 vb = *reinterpret_cast<const u32x4*>(
+                &vts[buf][(d * 32 + j) * VP + b * kBlock + hf * 8]);
+            for (int key = 0; key < kBlock; ++key) {
+              const int e = key % 4 + key / 8 * 4;  // its place in the lane half key / 4 % 2
+              u32x4 one = vb;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint32_t keep = e / 2 == i ? (e % 2 ? 0xffff0000u : 0xffffu) : 0u;
+                if (key / 4 % 2 != hf) keep = 0u;
+                one[i] &= keep;
+              }
+              f32x16 part;
+#pragma unroll
+              for (int x = 0; x < 16; ++x) part[x] = 0.f;
+              part = mfma32<PF16>(one, p[b], part);
+              if (key0 + b * kBlock + key <= qpos) o[d] += part;
+            }
+          }
+      }
+    }
+    if (more) store_tile(blk + 4, buf ^ 1);  // last read before the previous barrier
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32, kWave);
+  const int row = r0 + j;
+  if (row >= all) return;
+  const int tok = row / a.G, head = kvh * a.G + row % a.G;
+  const size_t at = (size_t)(pr.first + tok) * a.H + head;
+  if (pk.splits > 1) {
+    float* po = a.part_o + (at * a.nsplit + split) * HD;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f4*>(po + d * 32 + 8 * i + 4 * hf) =
+            f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+    if (hf == 0)
+      *reinterpret_cast<float2*>(a.part_ml + (at * a.nsplit + split) * 2) = float2{m, l};
+    return;
+  }
+  const bool none = pos0 + tok < 0;  // a row without keys
+  const float inv = 1.f / l;
+  uint16_t* op = static_cast<uint16_t*>(a.out) + at * HD;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const u32x2 w = {pack2<QF16>(o[d][4 * i] * inv, o[d][4 * i + 1] * inv),
+                       pack2<QF16>(o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv)};
+      *reinterpret_cast<u32x2*>(op + d * 32 + 8 * i + 4 * hf) = none ? u32x2{0u, 0u} : w;
+    }
+  if (a.lse && hf == 0)
+    a.lse[at] = none ? -INFINITY : (m + __log2f(l)) * 0.69314718055994530942f;
+}
+
 // Joins the splits of a (row, head): one wave each.
-template <int HD, bool QF16, int TILE>
+template <int HD, bool QF16>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   const int64_t id = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
   const int lane = threadIdx.x % kWave;
@@ -314,7 +624,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
   if (i >= pr.n) return;
   const int pos0 = a.pos0[s], row = i * a.G + head % a.G;
-  const PagedKeys pk(pos0, pr.n, a.G, row / TILE * TILE, TILE, a.cb, a.nsplit);
+  const PagedKeys pk(pos0, pr.n, a.G, row / a.tile * a.tile, a.tile, a.cb, a.nsplit);
   if (pk.splits <= 1) return;  // written already
   const size_t at = (size_t)(pr.first + i) * a.H + head;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at * a.nsplit;
@@ -352,14 +662,15 @@ struct PagedPlan {
   int tile, cb, nsplit;
   int64_t tiles, wgs;
   PagedPlan(int64_t S, int64_t max_rows, int64_t G, int64_t KVH, int64_t max_tokens) {
-    tile = kRows16;
+    tile = max_rows * G <= kRows16 ? kRows16 : kRowsTile;
     tiles = ceil_div(max_rows * G, tile);
     const int64_t units = std::max<int64_t>(1, S * tiles * KVH);
     const int64_t blocks = std::max<int64_t>(1, ceil_div(max_tokens, kBlock));
-    const int64_t want = std::max<int64_t>(1, ceil_div(1024, units));
+    const int64_t want = std::max<int64_t>(1, ceil_div(tile == kRows16 ? 1024 : 512, units));
     cb = (int)(ceil_div(std::max<int64_t>(16, ceil_div(blocks, want)), 16) * 16);
     nsplit = (int)ceil_div(blocks, cb);
-    wgs = S * tiles * KVH * nsplit;
+    wgs = tile == kRows16 ? S * tiles * KVH * nsplit
+                          : PrefillMap((uint32_t)(S * KVH * nsplit), (uint32_t)tiles).workgroups();
   }
   int64_t bytes(int64_t rows, int64_t H, int64_t hd) const {
     return nsplit > 1 ? rows * H * nsplit * (hd + 2) * 4 : 0;
@@ -480,14 +791,18 @@ extern "C" int sm_paged_attention(const sm_paged_cache* cache, const int32_t* bl
   a.cols = (int)table_cols;
   a.cb = plan.cb;
   a.nsplit = plan.nsplit;
+  a.tile = plan.tile;
   a.tiles = (int)plan.tiles;
   a.c2 = 1.44269504088896340736f / sqrtf((float)hd);
   const bool f16 = dtype == SM_F16, c8 = cache->dtype == SM_F8E4M3;
 #define SM_PAGED2(HD, F, C)                                                      \
   do {                                                                           \
-    paged_split_kernel<HD, F, C><<<(unsigned)plan.wgs, 256, 0, st>>>(a);         \
+    if (plan.tile == kRows16)                                                    \
+      paged_split_kernel<HD, F, C><<<(unsigned)plan.wgs, 256, 0, st>>>(a);       \
+    else                                                                         \
+      paged_tile_kernel<HD, F, C><<<(unsigned)plan.wgs, 256, 0, st>>>(a);        \
     if (plan.nsplit > 1)                                                         \
-      paged_join_kernel<HD, F, kRows16><<<(unsigned)joins, 256, 0, st>>>(a);     \
+      paged_join_kernel<HD, F><<<(unsigned)joins, 256, 0, st>>>(a);              \
   } while (0)
 #define SM_PAGED(HD)                             \
   do {                                           \
