@@ -58,15 +58,51 @@ __device__ inline uint32_t pack2(float a, float b) {
   }
 }
 
-// Whether a word of cache values holds an infinity or a NaN.
+// A word of cache values with its infinities and NaN set to zero.
 template <bool C8, bool F16>
-__device__ inline bool not_finite(uint32_t w) {
+__device__ inline uint32_t finite_only(uint32_t w) {
   if constexpr (C8) {  // e4m3 has no infinity; NaN is 0x7f or 0xff
-    const uint32_t x = (w & 0x7f7f7f7fu) + 0x01010101u;
-    return (x & 0x80808080u) != 0;
+    const uint32_t x = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    return w & ~((x >> 7) * 0xffu);
   } else {
     constexpr uint32_t m = F16 ? 0x7c00u : 0x7f80u;
-    return (w & m) == m || ((w >> 16) & m) == m;
+    if ((w & m) == m) w &= 0xffff0000u;
+    if ((w >> 16 & m) == m) w &= 0x0000ffffu;
+    return w;
+  }
+}
+
+// Values that some of a tile's rows see and some do not go into the products only where
+// they are finite (a weight of zero would turn an infinity into a NaN for the rows that do
+// not see it). The others come here, after the sweep and only where there are any: each is
+// added to the rows that see it, whose sums it makes infinite or NaN as its weight, which
+// is positive, would. dim(i): the dims of this lane's sums.
+template <int HD, bool C8, bool F16, int N, typename Dim>
+__device__ inline void add_odd(const PagedArgs& a, const int32_t* trow, int kvh, int first_block,
+                               int end_block, int keys, int qpos, Dim dim, float (&sum)[N]) {
+  constexpr int T = C8 ? 4 : 2;
+  for (int blk = first_block; blk < end_block; ++blk) {
+    const int bi = paged_block(trow, a.cols, a.pages, a.KVH, kvh, a.bpp, blk);
+    if (bi < 0) continue;
+    const size_t base = (size_t)bi * (kBlock * HD);
+    for (int t = 0; t < kBlock; ++t) {
+      const int key = blk * kBlock + t;
+      if (key >= keys) break;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int d = dim(i), n = d / 16;
+        const size_t at = base + ((n / T * 4 + t / 4) * 16 + d % 16) * (4 * T) + n % T * 4 + t % 4;
+        float v;
+        if constexpr (C8) {
+          v = (a.v[at] & 0x7f) == 0x7f ? NAN : 0.f;
+        } else {
+          const uint16_t w = reinterpret_cast<const uint16_t*>(a.v)[at];
+          v = F16 ? (float)__builtin_bit_cast(_Float16, w) : bf16_to_f32(w);
+          if (fabsf(v) < INFINITY) v = 0.f;
+        }
+        if (key <= qpos) sum[i] += v;
+      }
+    }
   }
 }
 
@@ -117,6 +153,7 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
 #pragma unroll
   for (int n = 0; n < NT; ++n) o[n] = f4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
+  bool odd = false;  // values that are not finite, among keys that not all rows see
   const int32_t* trow = a.table + (int64_t)s * a.cols;
 
   for (int seg = b0; seg < b1; seg += kWave) {
@@ -184,6 +221,18 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
             for (int c = 0; c < NC; ++c) vr[u][c] &= u32x4{k01, k23, k01, k23};
           }
         }
+        if (key0 + kBlock - 1 > pos_first && pos_first + 1 < pk.keys) {
+          bool x = false;
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t y = finite_only<C8, QF16>(vr[u][c][i]);
+              x |= y != vr[u][c][i];
+              vr[u][c][i] = y;
+            }
+          odd |= __ballot(x) != 0;
+        }
       }
       if (__ballot(mx > m + 8.f)) {
         mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
@@ -207,17 +256,6 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
         p[u / 2][2 * (u % 2)] = pack2<PF16>(e[0], e[1]);
         p[u / 2][2 * (u % 2) + 1] = pack2<PF16>(e[2], e[3]);
       }
-      bool odd = false;  // values that are not finite where some row sees them and some not
-      if ((seg + st + NB) * kBlock - 1 > pos_first && pos_first + 1 < pk.keys) {
-        bool x = false;
-#pragma unroll
-        for (int u = 0; u < NB; ++u)
-#pragma unroll
-          for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x |= not_finite<C8, QF16>(vr[u][c][i]);
-        odd = __ballot(x) != 0;
-      }
 #pragma unroll
       for (int w = 0; w < NB / 2; ++w) {
 #pragma unroll
@@ -229,24 +267,22 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
             va = u32x4{vr[2 * w][n / 2][2 * (n % 2)], vr[2 * w][n / 2][2 * (n % 2) + 1],
                        vr[2 * w + 1][n / 2][2 * (n % 2)], vr[2 * w + 1][n / 2][2 * (n % 2) + 1]};
           }
-          if (!odd) {
-            o[n] = mfma16<PF16>(va, p[w], o[n]);
-          } else {  // key by key, each added only to the rows that see it
-            for (int key = 0; key < 2 * kBlock; ++key) {
-              const int e = key % 4 + 4 * (key / kBlock);
-              u32x4 one = va;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                uint32_t keep = e / 2 == i ? (e % 2 ? 0xffff0000u : 0xffffu) : 0u;
-                if (key % kBlock / 4 != g) keep = 0u;
-                one[i] &= keep;
-              }
-              const f4 part = mfma16<PF16>(one, p[w], f4{0.f, 0.f, 0.f, 0.f});
-              if ((seg + st + 2 * w) * kBlock + key <= qpos) o[n] += part;
-            }
-          }
+          o[n] = mfma16<PF16>(va, p[w], o[n]);
         }
       }
+    }
+  }
+  if (odd) {  // (uniform per wave)
+    // the blocks of this wave's steps among those that not all rows see
+    for (int st = b0 + wave * NB; st < b1; st += 4 * NB) {
+      const int from = max(st, (pos_first + 1) / kBlock);
+      float x[4 * NT];
+#pragma unroll
+      for (int i = 0; i < 4 * NT; ++i) x[i] = o[i / 4][i % 4];
+      add_odd<HD, C8, QF16>(a, trow, kvh, from, min(st + NB, b1), pk.keys, qpos,
+                            [&](int i) { return 16 * (i / 4) + 4 * g + i % 4; }, x);
+#pragma unroll
+      for (int i = 0; i < 4 * NT; ++i) o[i / 4][i % 4] = x[i];
     }
   }
   l += __shfl_xor(l, 16, kWave);
@@ -321,60 +357,38 @@ constexpr int kRowsTile = 128;  // query rows of a workgroup, 32 a wave
 constexpr int kTile = 64;       // keys of a tile: a block to a wave's staging
 
 template <int HD, bool QF16, bool C8>
-__global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
-  constexpr int ES = C8 ? 1 : 2;
-  constexpr bool PF16 = C8 || QF16;
-  constexpr int KS = HD / 16, DB = HD / 32;  // MFMA steps of a score, 32-dim blocks of O
-  constexpr int KP = HD + 8, VP = kTile + 8; // padded LDS rows (elements)
-  constexpr int NC = HD * ES / 64;           // 16-byte loads a lane makes of a block
-  constexpr int BB = kBlock * HD * ES;
-  __shared__ __attribute__((aligned(16))) uint16_t ks[2][kTile * KP];
-  __shared__ __attribute__((aligned(16))) uint16_t vts[2][HD * VP];
-  __shared__ float info[2][4][4];  // a tile's blocks: score factor, V exponent, not finite
+struct TileSweep {
+  static constexpr int ES = C8 ? 1 : 2;
+  static constexpr bool PF16 = C8 || QF16;
+  static constexpr int KS = HD / 16, DB = HD / 32;  // MFMA steps of a score, 32-dim blocks of O
+  static constexpr int KP = HD + 8, VP = kTile + 8; // padded LDS rows (elements)
+  static constexpr int NC = HD * ES / 64;           // 16-byte loads a lane makes of a block
+  static constexpr int BB = kBlock * HD * ES;
+  struct Lds {
+    __attribute__((aligned(16))) uint16_t ks[2][kTile * KP];
+    __attribute__((aligned(16))) uint16_t vts[2][HD * VP];
+    __attribute__((aligned(16))) float info[2][4][2];  // a block's score factor and V exponent
+    int odd;
+  };
 
-  const PrefillMap map((uint32_t)(a.S * a.KVH * a.nsplit), (uint32_t)a.tiles);
-  uint32_t grp, place;
-  if (!map.at(blockIdx.x, grp, place)) return;  // (uniform)
-  const int split = (int)(grp % a.nsplit);
-  const int kvh = (int)(grp / a.nsplit % a.KVH), s = (int)(grp / a.nsplit / a.KVH);
-  const int tile = a.tiles - 1 - (int)place;  // the rows with the most keys first
-  const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
-  const int row0 = tile * kRowsTile, all = pr.n * a.G;
-  if (row0 >= all) return;
-  const int pos0 = a.pos0[s];
-  const PagedKeys pk(pos0, pr.n, a.G, row0, kRowsTile, a.cb, a.nsplit);
-  if (split >= max(pk.splits, 1)) return;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
-  const int j = lane % 32, hf = lane / 32;
-  const int b0 = pk.begin(split, a.cb), b1 = pk.keys > 0 ? pk.end(split, a.cb) : b0;
-  const int r0 = row0 + wave * 32;  // first row of this wave
-  const int qr = min(r0 + j, all - 1);
-  const int qpos = pos0 + qr / a.G;
-  const int pos_first = pos0 + row0 / a.G;
-  // positions of the wave's first and last row
-  const int wave_first = pos0 + min(r0, all - 1) / a.G;
-  const int wave_last = r0 < all ? pos0 + min(r0 + 31, all - 1) / a.G : -1;
-
+  const PagedArgs& a;
+  Lds& s;
+  const int32_t* trow;
+  const uint16_t* qp;  // this lane's query row
+  int kvh, b0, b1, keys, qpos, pos_first, wave_first, wave_last, wave, lane, j, hf;
   u32x4 qa[KS];
-  {
-    const uint16_t* qp = a.q + (int64_t)(pr.first + qr / a.G) * a.ldq +
-                         (int64_t)(kvh * a.G + qr % a.G) * HD;
-#pragma unroll
-    for (int st = 0; st < KS; ++st)
-      qa[st] = *reinterpret_cast<const u32x4*>(qp + st * 16 + hf * 8);
-  }
   f32x16 o[DB];  // o[d][e]: row j, dim 32 d + 8 (e / 4) + 4 hf + e % 4
-#pragma unroll
-  for (int d = 0; d < DB; ++d)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-  float m = -INFINITY, l = 0.f;
+  float m, l;
 
   // lane i: block seg + i of the segment at hand, and of the next
-  const int32_t* trow = a.table + (int64_t)s * a.cols;
   int bi, bi_next;
   float kscale, vexp, kscale_next, vexp_next;
-  auto look_up = [&](int seg, int& b, float& kf, float& vf) {
+  u32x4 kr[NC], vr[NC];
+  float kf_s, vf_s;
+
+  __device__ TileSweep(const PagedArgs& a_, Lds& s_) : a(a_), s(s_) {}
+
+  __device__ inline void look_up(int seg, int& b, float& kf, float& vf) {
     b = seg + lane < b1 ? paged_block(trow, a.cols, a.pages, a.KVH, kvh, a.bpp, seg + lane) : -1;
     const bool bad = b < 0;
     b = bad ? 0 : b;
@@ -385,12 +399,9 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
       vf = (float)((int)a.vs[b] - 127);
     }
     if (bad) kf = NAN;
-  };
-  u32x4 kr[NC], vr[NC];
-  float kf_s, vf_s;
-  bool odd_s;
+  }
   // wave w stages block w of a tile
-  auto load_tile = [&](int blk) {  // first block of the tile
+  __device__ inline void load_tile(int blk) {  // first block of the tile
     const int li = (blk - b0 + wave) % kWave;
     kf_s = lane_f32(kscale, li);
     vf_s = lane_f32(vexp, li);
@@ -401,13 +412,12 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
 #pragma unroll
     for (int c = 0; c < NC; ++c)
       vr[c] = *reinterpret_cast<const u32x4*>(a.v + at + c * 1024 + lane * 16);
-  };
-  auto store_tile = [&](int blk, int buf) {
+  }
+  __device__ inline void store_tile(int blk, int buf) {
     const int g = lane / 16, r = lane % 16;
     const int key0 = (blk + wave) * kBlock;
-    odd_s = false;
-    if (key0 + kBlock > pk.keys || kf_s != kf_s) {  // not the cache's: no product sees them
-      const int have = kf_s != kf_s ? 0 : max(0, min(4, pk.keys - key0 - 4 * g));
+    if (key0 + kBlock > keys || kf_s != kf_s) {  // not the cache's: no product sees them
+      const int have = kf_s != kf_s ? 0 : max(0, min(4, keys - key0 - 4 * g));
       if constexpr (C8) {
         const uint32_t keep = have >= 4 ? ~0u : (1u << (8 * have)) - 1;
 #pragma unroll
@@ -424,13 +434,17 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x |= not_finite<C8, QF16>(vr[c][i]);
-      odd_s = __ballot(x) != 0;
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t y = finite_only<C8, QF16>(vr[c][i]);
+          x |= y != vr[c][i];
+          vr[c][i] = y;
+        }
+      if (x) s.odd = 1;
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int at = (c * 64 + lane) * (16 / ES);  // element of the block
-      uint16_t* kp = &ks[buf][(wave * kBlock + at / HD) * KP + at % HD];
+      uint16_t* kp = &s.ks[buf][(wave * kBlock + at / HD) * KP + at % HD];
       if constexpr (C8) {
         *reinterpret_cast<u32x4*>(kp) = cvt8<QF16>(kr[c].x, kr[c].y);
         *reinterpret_cast<u32x4*>(kp + 8) = cvt8<QF16>(kr[c].z, kr[c].w);
@@ -439,7 +453,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
       }
       // quads of a block in the order 0, 2, 1, 3: the order in which a lane of the
       // transposed score tile holds its keys
-      uint16_t* vp = &vts[buf][r * VP + wave * kBlock + (g % 2 * 2 + g / 2) * 4];
+      uint16_t* vp = &s.vts[buf][r * VP + wave * kBlock + (g % 2 * 2 + g / 2) * 4];
 #pragma unroll
       for (int t = 0; t < 4 / ES; ++t) {
         u32x2 w;
@@ -448,140 +462,172 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
         *reinterpret_cast<u32x2*>(vp + (c * (4 / ES) + t) * 16 * VP) = w;
       }
     }
-    if (lane == 0)
-      *reinterpret_cast<f4*>(info[buf][wave]) = f4{kf_s, vf_s, odd_s ? 1.f : 0.f, 0.f};
-  };
+    if (lane == 0) *reinterpret_cast<float2*>(s.info[buf][wave]) = float2{kf_s, vf_s};
+  }
 
-  if (b1 > b0) {
+  // One pass over the keys.
+  __device__ inline void sweep() {
+#pragma unroll
+    for (int st = 0; st < KS; ++st)
+      qa[st] = *reinterpret_cast<const u32x4*>(qp + st * 16 + hf * 8);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+    m = -INFINITY;
+    l = 0.f;
+    if (b1 <= b0) return;
+    if (threadIdx.x == 0) s.odd = 0;
+    __syncthreads();
     look_up(b0, bi, kscale, vexp);
     load_tile(b0);
     store_tile(b0, 0);
-  }
-  __syncthreads();
-  int buf = 0;
-  for (int blk = b0; blk < b1; blk += 4, buf ^= 1) {
-    const bool more = blk + 4 < b1;
-    if ((blk - b0) % kWave == 0 && blk + kWave < b1)
-      look_up(blk + kWave, bi_next, kscale_next, vexp_next);
-    if (more) {
-      if ((blk + 4 - b0) % kWave == 0) {
-        bi = bi_next;
-        kscale = kscale_next;
-        vexp = vexp_next;
-      }
-      load_tile(blk + 4);
-    }
-    const int key0 = blk * kBlock;
-    if (key0 <= wave_last) {  // (uniform per wave) later keys are hidden from all its rows
-      f32x16 sc[2];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sc[kb][e] = 0.f;
-#pragma unroll
-        for (int st = 0; st < KS; ++st) {
-          const u32x4 kf =
-              *reinterpret_cast<const u32x4*>(&ks[buf][(kb * 32 + j) * KP + st * 16 + hf * 8]);
-          sc[kb] = mfma32<QF16>(kf, qa[st], sc[kb]);
-        }
-      }
-      float kf[4], vf[4];
-      bool odd = false;
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const f4 x = *reinterpret_cast<const f4*>(info[buf][b]);
-        kf[b] = x[0];
-        vf[b] = x[1];
-        odd |= x[2] != 0.f;
-      }
-      odd = __ballot(odd) != 0;
-      if (key0 + kTile - 1 > wave_first) {  // the diagonal, or past the last key
-        const int lim = qpos - key0 - 4 * hf;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (kb * 32 + 8 * (e / 4) + e % 4 > lim) sc[kb][e] = -INFINITY;
-        // (a block without a page has the factor NaN: only where it is seen)
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-          if (b * kBlock > qpos - key0) kf[b] = a.c2;
-      }
-      // scores in units of log2, raised by the exponent of V's scale
-      float mx = -INFINITY;
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        float x = sc[b / 2][8 * (b % 2)];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) x = fmaxf(x, sc[b / 2][8 * (b % 2) + e]);
-        mx = fmaxf(mx, C8 ? fmaf(x, kf[b], vf[b]) : x * kf[b]);
-      }
-      if (__ballot(mx > m + 8.f)) {
-        mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-        const float mn = fmaxf(m, mx);
-        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-        m = mn;
-        l *= f;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[d][e] *= f;
-      }
-      const float ms = m == -INFINITY ? 0.f : m;
-      u32x4 p[4];  // P^T of a block's 16 keys
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const float off = vf[b] - ms;
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(sc[b / 2][8 * (b % 2) + 2 * e], kf[b], off));
-          const float y =
-              __builtin_amdgcn_exp2f(fmaf(sc[b / 2][8 * (b % 2) + 2 * e + 1], kf[b], off));
-          sum += x;
-          sum += y;
-          p[b][e] = pack2<PF16>(x, y);
-        }
-        l = C8 ? fmaf(sum, __builtin_amdgcn_exp2f(-vf[b]), l) : l + sum;
-      }
-      if (!odd) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            const u32x4 vb = *reinterpret_cast<const u32x4*>(
-                &vts[buf][(d * 32 + j) * VP + b * kBlock + hf * 8]);
-            o[d] = mfma32<PF16>(vb, p[b], o[d]);
-          }
-      } else {  // key by key, each added only to the rows that see it
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            const u32x4 vb = *reinterpret_cast<const u32x4*>(
-                &vts[buf][(d * 32 + j) * VP + b * kBlock + hf * 8]);
-            for (int key = 0; key < kBlock; ++key) {
-              const int e = key % 4 + key / 8 * 4;  // its place in the lane half key / 4 % 2
-              u32x4 one = vb;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                uint32_t keep = e / 2 == i ? (e % 2 ? 0xffff0000u : 0xffffu) : 0u;
-                if (key / 4 % 2 != hf) keep = 0u;
-                one[i] &= keep;
-              }
-              f32x16 part;
-#pragma unroll
-              for (int x = 0; x < 16; ++x) part[x] = 0.f;
-              part = mfma32<PF16>(one, p[b], part);
-              if (key0 + b * kBlock + key <= qpos) o[d] += part;
-            }
-          }
-      }
-    }
-    if (more) store_tile(blk + 4, buf ^ 1);  // last read before the previous barrier
     __syncthreads();
+    int buf = 0;
+    for (int blk = b0; blk < b1; blk += 4, buf ^= 1) {
+      const bool more = blk + 4 < b1;
+      if ((blk - b0) % kWave == 0 && blk + kWave < b1)
+        look_up(blk + kWave, bi_next, kscale_next, vexp_next);
+      if (more) {
+        if ((blk + 4 - b0) % kWave == 0) {
+          bi = bi_next;
+          kscale = kscale_next;
+          vexp = vexp_next;
+        }
+        load_tile(blk + 4);
+      }
+      const int key0 = blk * kBlock;
+      if (key0 <= wave_last) tile(buf, key0);  // (uniform per wave) later keys: no row sees them
+      if (more) store_tile(blk + 4, buf ^ 1);  // last read before the previous barrier
+      __syncthreads();
+    }
+    if (s.odd) {
+      float x[16 * DB];
+#pragma unroll
+      for (int i = 0; i < 16 * DB; ++i) x[i] = o[i / 16][i % 16];
+      add_odd<HD, C8, QF16>(
+          a, trow, kvh, max(b0, (pos_first + 1) / kBlock), b1, keys, qpos,
+          [&](int i) { return 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * hf + i % 4; }, x);
+#pragma unroll
+      for (int i = 0; i < 16 * DB; ++i) o[i / 16][i % 16] = x[i];
+    }
   }
-  l += __shfl_xor(l, 32, kWave);
+
+  __device__ inline void tile(int buf, int key0) {
+    f32x16 sc[2];
+    float kf[4], vf[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const float2 x = *reinterpret_cast<const float2*>(s.info[buf][b]);
+      kf[b] = x.x;
+      vf[b] = x.y;
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[kb][e] = 0.f;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        const u32x4 k =
+            *reinterpret_cast<const u32x4*>(&s.ks[buf][(kb * 32 + j) * KP + st * 16 + hf * 8]);
+        sc[kb] = mfma32<QF16>(k, qa[st], sc[kb]);
+      }
+    }
+    if (key0 + kTile - 1 > wave_first) {  // the diagonal, or past the last key
+      const int lim = qpos - key0 - 4 * hf;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (kb * 32 + 8 * (e / 4) + e % 4 > lim) sc[kb][e] = -INFINITY;
+      // (a block without a page has the factor NaN: only for the rows that see it)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (b * kBlock > qpos - key0) kf[b] = a.c2;
+    }
+    // scores in units of log2, raised by the exponent of V's scale
+    float mx = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      float x = sc[b / 2][8 * (b % 2)];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) x = fmaxf(x, sc[b / 2][8 * (b % 2) + e]);
+      mx = fmaxf(mx, C8 ? fmaf(x, kf[b], vf[b]) : x * kf[b]);
+    }
+    if (__ballot(mx > m + 8.f)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+      const float mn = fmaxf(m, mx);
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] *= f;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const float off = vf[b] - ms;
+      float sum = 0.f;
+      u32x4 p;  // P^T of the block's 16 keys
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(sc[b / 2][8 * (b % 2) + 2 * e], kf[b], off));
+        const float y =
+            __builtin_amdgcn_exp2f(fmaf(sc[b / 2][8 * (b % 2) + 2 * e + 1], kf[b], off));
+        sum += x;
+        sum += y;
+        p[e] = pack2<PF16>(x, y);
+      }
+      l = C8 ? fmaf(sum, __builtin_amdgcn_exp2f(-vf[b]), l) : l + sum;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(
+            &s.vts[buf][(d * 32 + j) * VP + b * kBlock + hf * 8]);
+        o[d] = mfma32<PF16>(v, p, o[d]);
+      }
+    }
+  }
+};
+
+template <int HD, bool QF16, bool C8>
+__global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
+  typedef TileSweep<HD, QF16, C8> T;
+  __shared__ typename T::Lds lds;
+  const PrefillMap map((uint32_t)(a.S * a.KVH * a.nsplit), (uint32_t)a.tiles);
+  uint32_t grp, place;
+  if (!map.at(blockIdx.x, grp, place)) return;  // (uniform)
+  const int split = (int)(grp % a.nsplit);
+  const int kvh = (int)(grp / a.nsplit % a.KVH), s = (int)(grp / a.nsplit / a.KVH);
+  const int tile = a.tiles - 1 - (int)place;  // the rows with the most keys first
+  const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
+  const int row0 = tile * kRowsTile, all = pr.n * a.G;
+  if (row0 >= all) return;
+  const int pos0 = a.pos0[s];
+  const PagedKeys pk(pos0, pr.n, a.G, row0, kRowsTile, a.cb, a.nsplit);
+  if (split >= max(pk.splits, 1)) return;
+  T t(a, lds);
+  t.trow = a.table + (int64_t)s * a.cols;
+  t.kvh = kvh;
+  t.wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  t.lane = threadIdx.x % kWave;
+  const int j = t.j = t.lane % 32, hf = t.hf = t.lane / 32;
+  t.b0 = pk.begin(split, a.cb);
+  t.b1 = pk.keys > 0 ? pk.end(split, a.cb) : t.b0;
+  t.keys = pk.keys;
+  const int r0 = row0 + t.wave * 32;  // first row of this wave
+  const int qr = min(r0 + j, all - 1);
+  t.qpos = pos0 + qr / a.G;
+  t.pos_first = pos0 + row0 / a.G;
+  // positions of the wave's first and last row
+  t.wave_first = pos0 + min(r0, all - 1) / a.G;
+  t.wave_last = r0 < all ? pos0 + min(r0 + 31, all - 1) / a.G : -1;
+  t.qp = a.q + (int64_t)(pr.first + qr / a.G) * a.ldq + (int64_t)(kvh * a.G + qr % a.G) * HD;
+  t.sweep();
+  f32x16(&o)[T::DB] = t.o;
+  constexpr int DB = T::DB;
+  const float l = t.l + __shfl_xor(t.l, 32, kWave), m = t.m;
   const int row = r0 + j;
   if (row >= all) return;
   const int tok = row / a.G, head = kvh * a.G + row % a.G;
@@ -636,12 +682,28 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   float ll = 0.f, acc[D];
 #pragma unroll
   for (int d = 0; d < D; ++d) acc[d] = 0.f;
-  for (int x = 0; x < pk.splits; ++x) {
-    const float2 v = ml[x];
+  for (int x0 = 0; x0 < pk.splits; x0 += kWave) {
+    const int n = min(kWave, pk.splits - x0);
+    const float2 v = lane < n ? ml[x0 + lane] : float2{-INFINITY, 0.f};
+    // (a split without visible keys has the maximum -inf and the sum 0)
     const float f = v.x == -INFINITY ? (v.y == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(v.x - mm);
-    ll = fmaf(v.y, f, ll);
+    ll += wave_sum(v.y * f);
+    for (int x = 0; x < n; x += 8) {  // eight splits' sums in flight
+      float y[8][D];
 #pragma unroll
-    for (int d = 0; d < D; ++d) acc[d] = fmaf(po[(size_t)x * HD + lane * D + d], f, acc[d]);
+      for (int k = 0; k < 8; ++k) {
+        const float* p = po + (size_t)(x0 + min(x + k, n - 1)) * HD + lane * D;
+#pragma unroll
+        for (int d = 0; d < D; ++d) y[k][d] = p[d];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = x + k < n ? lane_f32(f, min(x + k, n - 1)) : 0.f;
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+          if (x + k < n) acc[d] = fmaf(y[k][d], w, acc[d]);
+      }
+    }
   }
   const bool none = pos0 + i < 0;
   const float inv = 1.f / ll;
