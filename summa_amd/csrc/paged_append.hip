@@ -27,7 +27,8 @@ struct AppendArgs {
   int64_t rope_rows;
   const int32_t *table, *pos0, *row_start;
   void* q_out;
-  int S, rows, max_rows, H, KVH, pages, bpp, cols, rot, half_layout, q_f16, touched, groups;
+  Divide bpp, touched, groups;
+  int S, rows, max_rows, H, KVH, pages, cols, rot, half_layout, q_f16;
 };
 
 // D consecutive values of a row as f32 (8: 16-byte loads; 4: 8- or 16-byte ones).
@@ -84,17 +85,16 @@ __device__ inline int scale_exponent(float amax) {
 template <typename T, int HD, int CT>  // CT: cache type, 0 bf16, 1 f16, 2 e4m3
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   constexpr int D = HD / 16;
-  uint32_t id = blockIdx.x;
-  const int slot = (int)(id % a.groups) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  id /= a.groups;
-  const int s = (int)(id / a.touched);
+  int s = (int)blockIdx.x;
+  const int slot = a.groups.mod(s) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int nth = a.touched.mod(s);  // of the blocks that the sequence's rows touch
   const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
   const int first_slot = a.q ? 0 : a.H;
   if (slot + first_slot >= a.H + 2 * a.KVH || pr.n == 0) return;
   const int head = slot + first_slot;
   const int pos0 = a.pos0[s];
   const int64_t end = (int64_t)pos0 + pr.n;            // one past the last position
-  const int64_t base = (int64_t)(max(pos0, 0) / kBlock + (int)(id % a.touched)) * kBlock;
+  const int64_t base = (int64_t)(max(pos0, 0) / kBlock + nth) * kBlock;
   const int t0 = (int)max((int64_t)max(pos0, 0) - base, (int64_t)0);
   const int t1 = (int)min(end - base, (int64_t)kBlock);
   if (t0 >= t1) return;  // (uniform: the wave's block holds none of the rows)
@@ -337,18 +337,18 @@ extern "C" int sm_paged_append(const sm_paged_cache* cache, const int32_t* block
   a.H = q ? (int)H : 0;
   a.KVH = (int)KVH;
   a.pages = (int)cache->pages;
-  a.bpp = (int)(cache->page_tokens / kBlock);
+  a.bpp = Divide((int)(cache->page_tokens / kBlock));
   a.cols = (int)table_cols;
   a.rot = rope_table ? (int)rot_dim : 0;
   a.half_layout = layout == SM_ROPE_HALF;
   a.q_f16 = q_dtype == SM_F16;
-  a.touched = (int)paged_touched(max_rows);
-  a.groups = (int)ceil_div(a.H + 2 * KVH, 4);
-  if ((double)S * a.touched * a.groups >= (double)(1 << 24)) {
+  a.touched = Divide((int)paged_touched(max_rows));
+  a.groups = Divide((int)ceil_div(a.H + 2 * KVH, 4));
+  if ((double)S * a.touched.d * a.groups.d >= (double)(1 << 24)) {
     set_error("%s: problem too large", me);
     return SM_ERR_UNSUPPORTED;
   }
-  const unsigned wgs = (unsigned)(S * a.touched * a.groups);
+  const unsigned wgs = (unsigned)(S * a.touched.d * a.groups.d);
   hipStream_t st = as_stream(stream);
 #define SM_APP3(T, HD, CT) paged_append_kernel<T, HD, CT><<<wgs, 256, 0, st>>>(a)
 #define SM_APP2(T, HD)                                  \

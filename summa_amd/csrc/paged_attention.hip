@@ -20,7 +20,8 @@ struct PagedArgs {
   float* lse;
   float *part_o, *part_ml;       // per (row, head, split): unnormalised O; (max, sum)
   int64_t ldq;
-  int S, rows, max_rows, H, KVH, G, pages, bpp, cols, cb, nsplit, tile, tiles;
+  Divide H, KVH, G, bpp, nsplit, tiles, rows_each, tile;
+  int S, rows, max_rows, pages, cols, cb;
   float c2;                      // log2(e) / sqrt(hd)
 };
 
@@ -82,7 +83,7 @@ __device__ inline void add_odd(const PagedArgs& a, const int32_t* trow, int kvh,
                                int end_block, int keys, int qpos, Dim dim, float (&sum)[N]) {
   constexpr int T = C8 ? 4 : 2;
   for (int blk = first_block; blk < end_block; ++blk) {
-    const int bi = paged_block(trow, a.cols, a.pages, a.KVH, kvh, a.bpp, blk);
+    const int bi = paged_block(trow, a.cols, a.pages, (int)a.KVH.d, kvh, a.bpp, blk);
     if (bi < 0) continue;
     const size_t base = (size_t)bi * (kBlock * HD);
     for (int t = 0; t < kBlock; ++t) {
@@ -106,43 +107,68 @@ __device__ inline void add_odd(const PagedArgs& a, const int32_t* trow, int kvh,
   }
 }
 
+// Where 64 blocks of a sequence lie, one to a lane, and their scales.
+struct Blocks {
+  int at;       // cache block; 0 where there is none
+  bool none;
+  int ke, ve;   // scale bytes (8-bit cache)
+  __device__ inline void find(const PagedArgs& a, const int32_t* trow, int kvh, int blk) {
+    const int b = paged_block(trow, a.cols, a.pages, (int)a.KVH.d, kvh, a.bpp, blk);
+    none = b < 0;
+    at = none ? 0 : b;
+    if (a.ks) {  // (uniform)
+      ke = a.ks[at];
+      ve = a.vs[at];
+    }
+  }
+  // factor of a score in units of log2, NaN without a block; exponent of V's scale
+  template <bool C8>
+  __device__ inline float kscale(float c2) const {
+    return none ? NAN : C8 ? __builtin_amdgcn_ldexpf(c2, ke - 127) : c2;
+  }
+  template <bool C8>
+  __device__ inline float vexp() const {
+    return C8 ? (float)(ve - 127) : 0.f;
+  }
+};
+
 constexpr int kRows16 = 16;  // query rows of a workgroup
 
 template <int HD, bool QF16, bool C8>
 __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
   constexpr int ES = C8 ? 1 : 2;
   constexpr bool PF16 = C8 || QF16;   // type of P and V in P.V
-  constexpr int NB = C8 ? 4 : 2;      // blocks a wave takes at a time
+  constexpr int NB = 2;               // blocks a wave takes at a time
   constexpr int NC = HD * ES / 64;    // 16-byte loads a lane makes of a block of K, and of V
   constexpr int NT = HD / 16;         // 16-dim tiles of O
   constexpr int BB = kBlock * HD * ES;  // bytes of a block
   __shared__ float sm_m[4][kRows16], sm_l[4][kRows16];
   __shared__ __attribute__((aligned(16))) float sm_o[4][kRows16][HD + 4];
 
-  uint32_t id = blockIdx.x;
-  const int split = (int)(id % a.nsplit);
-  id /= a.nsplit;
-  const int kvh = (int)(id % a.KVH);
-  id /= a.KVH;
-  const int tile = (int)(id % a.tiles), s = (int)(id / a.tiles);
-  const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
-  const int row0 = tile * kRows16, all = pr.n * a.G;
-  if (row0 >= all) return;
-  const int pos0 = a.pos0[s];
-  const PagedKeys pk(pos0, pr.n, a.G, row0, kRows16, a.cb, a.nsplit);
-  if (split >= max(pk.splits, 1)) return;
+  int s = (int)blockIdx.x;
+  const int split = a.nsplit.mod(s), kvh = a.KVH.mod(s), tile = a.tiles.mod(s);
+  // What the first loads need does not wait for the sequence's lengths: a workgroup without
+  // work goes through them too (its rows and table row are there) and leaves after the loop.
+  const int32_t* trow = a.table + (int64_t)s * a.cols;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int r = lane % 16, g = lane / 16;
-  const int b0 = pk.begin(split, a.cb), b1 = pk.keys > 0 ? pk.end(split, a.cb) : b0;
+  Blocks cur, next;
+  cur.find(a, trow, kvh, split * a.cb + lane);
+  const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
+  const int pos0 = a.pos0[s];
+  const int row0 = tile * kRows16, all = pr.n * (int)a.G.d;
+  const PagedKeys pk(pos0, pr.n, a.G, row0, kRows16, a.cb, (int)a.nsplit.d);
+  const bool idle = row0 >= all || split >= max(pk.splits, 1);
+  const int b0 = split * a.cb, b1 = idle || pk.keys <= 0 ? b0 : pk.end(split, a.cb);
 
   // this lane's query: row row0 + r
-  const int qr = min(row0 + r, all - 1);
-  const int qpos = pos0 + qr / a.G;
-  const int pos_first = pos0 + row0 / a.G;  // of the tile
+  const int qr = max(0, min(row0 + r, all - 1));
+  const int qt = a.G.div(qr), qpos = pos0 + qt;
+  const int pos_first = pos0 + a.G.div(row0);  // of the tile
   u32x4 qf[HD / 32];
   {
-    const uint16_t* qp = a.q + (int64_t)(pr.first + qr / a.G) * a.ldq +
-                         (int64_t)(kvh * a.G + qr % a.G) * HD;
+    const uint16_t* qp = a.q + (idle ? 0 : (int64_t)(pr.first + qt) * a.ldq) +
+                         (int64_t)(kvh * (int)a.G.d + qr - qt * (int)a.G.d) * HD;
 #pragma unroll
     for (int c = 0; c < HD / 32; ++c) {
       const int d = C8 ? (c / 2) * 64 + g * 16 + (c % 2) * 8 : c * 32 + g * 8;
@@ -154,35 +180,29 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
   for (int n = 0; n < NT; ++n) o[n] = f4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
   bool odd = false;  // values that are not finite, among keys that not all rows see
-  const int32_t* trow = a.table + (int64_t)s * a.cols;
 
-  for (int seg = b0; seg < b1; seg += kWave) {
+  for (int seg = b0; seg < b1; seg += kWave, cur = next) {
     const int nb = min(kWave, b1 - seg);
-    // lane i: block seg + i
-    int bi = lane < nb ? paged_block(trow, a.cols, a.pages, a.KVH, kvh, a.bpp, seg + lane) : -1;
-    const bool bad = bi < 0;
-    bi = bad ? 0 : bi;
-    float kscale = a.c2, vexp = 0.f;
-    if constexpr (C8) {
-      kscale = __builtin_amdgcn_ldexpf(kscale, (int)a.ks[bi] - 127);
-      vexp = (float)((int)a.vs[bi] - 127);
-    }
-    if (bad) kscale = NAN;
+    if (seg + kWave < b1) next.find(a, trow, kvh, seg + kWave + lane);
     for (int st = wave * NB; st < nb; st += 4 * NB) {
       u32x4 kr[NB][NC], vr[NB][NC];
       float ksc[NB], vex[NB];
 #pragma unroll
       for (int u = 0; u < NB; ++u) {
-        const int li = min(st + u, nb - 1);
-        const size_t at = (size_t)__builtin_amdgcn_readlane(bi, li) * BB;
-        ksc[u] = lane_f32(kscale, li);
-        vex[u] = lane_f32(vexp, li);
+        const size_t at = (size_t)__builtin_amdgcn_readlane(cur.at, min(st + u, nb - 1)) * BB;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
           kr[u][c] = *reinterpret_cast<const u32x4*>(a.k + at + r * HD * ES + c * 64 + g * 16);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
           vr[u][c] = *reinterpret_cast<const u32x4*>(a.v + at + c * 1024 + lane * 16);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // (the scales are waited for behind these loads)
+      const float kscale = cur.template kscale<C8>(a.c2), vexp = cur.template vexp<C8>();
+#pragma unroll
+      for (int u = 0; u < NB; ++u) {
+        ksc[u] = lane_f32(kscale, min(st + u, nb - 1));
+        vex[u] = lane_f32(vexp, min(st + u, nb - 1));
       }
       // scores, in units of log2 and raised by the exponent of V's scale
       float t[NB][4];
@@ -285,6 +305,7 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
       for (int i = 0; i < 4 * NT; ++i) o[i / 4][i % 4] = x[i];
     }
   }
+  if (idle) return;  // (uniform)
   l += __shfl_xor(l, 16, kWave);
   l += __shfl_xor(l, 32, kWave);
   if (g == 0) {
@@ -298,7 +319,8 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
   // row threadIdx.x / 16, HD / 16 of its dims
   const int y = threadIdx.x / 16, d0 = (threadIdx.x % 16) * (HD / 16);
   if (row0 + y >= all) return;
-  const int tok = (row0 + y) / a.G, head = kvh * a.G + (row0 + y) % a.G;
+  int tok = row0 + y;
+  const int head = kvh * (int)a.G.d + a.G.mod(tok);
   float mm = sm_m[0][y];
 #pragma unroll
   for (int w = 1; w < 4; ++w) mm = fmaxf(mm, sm_m[w][y]);
@@ -317,14 +339,14 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) acc[i] = fmaf(sm_o[w][y][d0 + i], f[w], acc[i]);
   }
-  const size_t at = (size_t)(pr.first + tok) * a.H + head;
+  const size_t at = (size_t)(pr.first + tok) * a.H.d + head;
   if (pk.splits > 1) {
-    float* po = a.part_o + (at * a.nsplit + split) * HD + d0;
+    float* po = a.part_o + (at * a.nsplit.d + split) * HD + d0;
 #pragma unroll
     for (int i = 0; i < HD / 16; i += 4)
       *reinterpret_cast<f4*>(po + i) = f4{acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
     if (d0 == 0)
-      *reinterpret_cast<float2*>(a.part_ml + (at * a.nsplit + split) * 2) = float2{mm, ll};
+      *reinterpret_cast<float2*>(a.part_ml + (at * a.nsplit.d + split) * 2) = float2{mm, ll};
     return;
   }
   const bool none = pos0 + tok < 0;  // a row without keys
@@ -353,8 +375,15 @@ __device__ inline f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
                                                    __builtin_bit_cast(bf8, b), c, 0, 0, 0);
 }
 
+// (fmaxf of values behind a branch costs the compiler's quieting of each)
+__device__ inline float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 constexpr int kRowsTile = 128;  // query rows of a workgroup, 32 a wave
-constexpr int kTile = 64;       // keys of a tile: a block to a wave's staging
+constexpr int kTile = 64;       // keys of a tile
 
 template <int HD, bool QF16, bool C8>
 struct TileSweep {
@@ -362,12 +391,14 @@ struct TileSweep {
   static constexpr bool PF16 = C8 || QF16;
   static constexpr int KS = HD / 16, DB = HD / 32;  // MFMA steps of a score, 32-dim blocks of O
   static constexpr int KP = HD + 8, VP = kTile + 8; // padded LDS rows (elements)
-  static constexpr int NC = HD * ES / 64;           // 16-byte loads a lane makes of a block
+  static constexpr int NB = kTile / kBlock;         // blocks of a tile
+  static constexpr int NC = HD * ES / 64;           // kilobytes of a block, each one wave's load
+  static constexpr int PER = (NB * NC + 3) / 4;     // of a tile's K, and of its V, for each wave
   static constexpr int BB = kBlock * HD * ES;
   struct Lds {
     __attribute__((aligned(16))) uint16_t ks[2][kTile * KP];
     __attribute__((aligned(16))) uint16_t vts[2][HD * VP];
-    __attribute__((aligned(16))) float info[2][4][2];  // a block's score factor and V exponent
+    __attribute__((aligned(16))) float info[2][NB][2];  // a block's score factor and V exponent
     int odd;
   };
 
@@ -380,89 +411,80 @@ struct TileSweep {
   f32x16 o[DB];  // o[d][e]: row j, dim 32 d + 8 (e / 4) + 4 hf + e % 4
   float m, l;
 
-  // lane i: block seg + i of the segment at hand, and of the next
-  int bi, bi_next;
-  float kscale, vexp, kscale_next, vexp_next;
-  u32x4 kr[NC], vr[NC];
-  float kf_s, vf_s;
+  Blocks cur, next;  // of the 64 blocks at hand, and of the next
+  u32x4 kr[PER], vr[PER];
 
   __device__ TileSweep(const PagedArgs& a_, Lds& s_) : a(a_), s(s_) {}
 
-  __device__ inline void look_up(int seg, int& b, float& kf, float& vf) {
-    b = seg + lane < b1 ? paged_block(trow, a.cols, a.pages, a.KVH, kvh, a.bpp, seg + lane) : -1;
-    const bool bad = b < 0;
-    b = bad ? 0 : b;
-    kf = a.c2;
-    vf = 0.f;
-    if constexpr (C8) {
-      kf = __builtin_amdgcn_ldexpf(kf, (int)a.ks[b] - 127);
-      vf = (float)((int)a.vs[b] - 127);
-    }
-    if (bad) kf = NAN;
+  // The n-th kilobyte that this wave stages of a tile's K and V: whose block, and which of it.
+  __device__ inline bool part(int n, int& block, int& c) const {
+    const int x = wave * PER + n;
+    block = x / NC;
+    c = x % NC;
+    return 4 * PER == NB * NC || x < NB * NC;
   }
-  // wave w stages block w of a tile
   __device__ inline void load_tile(int blk) {  // first block of the tile
-    const int li = (blk - b0 + wave) % kWave;
-    kf_s = lane_f32(kscale, li);
-    vf_s = lane_f32(vexp, li);
-    const size_t at = (size_t)__builtin_amdgcn_readlane(bi, li) * BB;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-      kr[c] = *reinterpret_cast<const u32x4*>(a.k + at + c * 1024 + lane * 16);
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-      vr[c] = *reinterpret_cast<const u32x4*>(a.v + at + c * 1024 + lane * 16);
-  }
-  __device__ inline void store_tile(int blk, int buf) {
-    const int g = lane / 16, r = lane % 16;
-    const int key0 = (blk + wave) * kBlock;
-    if (key0 + kBlock > keys || kf_s != kf_s) {  // not the cache's: no product sees them
-      const int have = kf_s != kf_s ? 0 : max(0, min(4, keys - key0 - 4 * g));
-      if constexpr (C8) {
-        const uint32_t keep = have >= 4 ? ~0u : (1u << (8 * have)) - 1;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) vr[c] &= keep;
-      } else {
-        const uint32_t k01 = have >= 2 ? ~0u : have == 1 ? 0xffffu : 0u;
-        const uint32_t k23 = have >= 4 ? ~0u : have == 3 ? 0xffffu : 0u;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) vr[c] &= u32x4{k01, k23, k01, k23};
-      }
+    for (int n = 0; n < PER; ++n) {
+      int block, c;
+      if (!part(n, block, c)) continue;
+      const size_t at =
+          (size_t)__builtin_amdgcn_readlane(cur.at, (blk - b0 + block) % kWave) * BB + c * 1024;
+      kr[n] = *reinterpret_cast<const u32x4*>(a.k + at + lane * 16);
+      vr[n] = *reinterpret_cast<const u32x4*>(a.v + at + lane * 16);
     }
-    if (key0 + kBlock - 1 > pos_first) {  // some rows see these keys and some do not
-      bool x = false;
+  }
+  __device__ inline void store_tile(int blk, int buf, const Blocks& of) {
+    const int g = lane / 16, r = lane % 16;
+    const float kscale = of.template kscale<C8>(a.c2), vexp = of.template vexp<C8>();
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
+    for (int n = 0; n < PER; ++n) {
+      int block, c;
+      if (!part(n, block, c)) continue;
+      const int key0 = (blk + block) * kBlock;
+      const float kf = lane_f32(kscale, (blk - b0 + block) % kWave);
+      if (key0 + kBlock > keys || kf != kf) {  // not the cache's: no product sees them
+        const int have = kf != kf ? 0 : max(0, min(4, keys - key0 - 4 * g));
+        if constexpr (C8) {
+          vr[n] &= have >= 4 ? ~0u : (1u << (8 * have)) - 1;
+        } else {
+          const uint32_t k01 = have >= 2 ? ~0u : have == 1 ? 0xffffu : 0u;
+          const uint32_t k23 = have >= 4 ? ~0u : have == 3 ? 0xffffu : 0u;
+          vr[n] &= u32x4{k01, k23, k01, k23};
+        }
+      }
+      if (key0 + kBlock - 1 > pos_first) {  // some rows see these keys and some do not
+        bool x = false;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t y = finite_only<C8, QF16>(vr[c][i]);
-          x |= y != vr[c][i];
-          vr[c][i] = y;
+          const uint32_t y = finite_only<C8, QF16>(vr[n][i]);
+          x |= y != vr[n][i];
+          vr[n][i] = y;
         }
-      if (x) s.odd = 1;
-    }
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
+        if (x) s.odd = 1;
+      }
       const int at = (c * 64 + lane) * (16 / ES);  // element of the block
-      uint16_t* kp = &s.ks[buf][(wave * kBlock + at / HD) * KP + at % HD];
+      uint16_t* kp = &s.ks[buf][(block * kBlock + at / HD) * KP + at % HD];
       if constexpr (C8) {
-        *reinterpret_cast<u32x4*>(kp) = cvt8<QF16>(kr[c].x, kr[c].y);
-        *reinterpret_cast<u32x4*>(kp + 8) = cvt8<QF16>(kr[c].z, kr[c].w);
+        *reinterpret_cast<u32x4*>(kp) = cvt8<QF16>(kr[n].x, kr[n].y);
+        *reinterpret_cast<u32x4*>(kp + 8) = cvt8<QF16>(kr[n].z, kr[n].w);
       } else {
-        *reinterpret_cast<u32x4*>(kp) = kr[c];
+        *reinterpret_cast<u32x4*>(kp) = kr[n];
       }
       // quads of a block in the order 0, 2, 1, 3: the order in which a lane of the
       // transposed score tile holds its keys
-      uint16_t* vp = &s.vts[buf][r * VP + wave * kBlock + (g % 2 * 2 + g / 2) * 4];
+      uint16_t* vp = &s.vts[buf][r * VP + block * kBlock + (g % 2 * 2 + g / 2) * 4];
 #pragma unroll
       for (int t = 0; t < 4 / ES; ++t) {
         u32x2 w;
-        if constexpr (C8) w = u32x2{cvt2<true>(vr[c][t], false), cvt2<true>(vr[c][t], true)};
-        else w = u32x2{vr[c][2 * t], vr[c][2 * t + 1]};
+        if constexpr (C8) w = u32x2{cvt2<true>(vr[n][t], false), cvt2<true>(vr[n][t], true)};
+        else w = u32x2{vr[n][2 * t], vr[n][2 * t + 1]};
         *reinterpret_cast<u32x2*>(vp + (c * (4 / ES) + t) * 16 * VP) = w;
       }
     }
-    if (lane == 0) *reinterpret_cast<float2*>(s.info[buf][wave]) = float2{kf_s, vf_s};
+    // (wave 0's lanes that hold the tile's blocks)
+    const unsigned i = (unsigned)(threadIdx.x - (blk - b0) % kWave);
+    if (i < NB) *reinterpret_cast<float2*>(s.info[buf][i]) = float2{kscale, vexp};
   }
 
   // One pass over the keys.
@@ -479,26 +501,21 @@ struct TileSweep {
     if (b1 <= b0) return;
     if (threadIdx.x == 0) s.odd = 0;
     __syncthreads();
-    look_up(b0, bi, kscale, vexp);
     load_tile(b0);
-    store_tile(b0, 0);
+    store_tile(b0, 0, cur);
     __syncthreads();
     int buf = 0;
-    for (int blk = b0; blk < b1; blk += 4, buf ^= 1) {
-      const bool more = blk + 4 < b1;
+    for (int blk = b0; blk < b1; blk += NB, buf ^= 1) {
+      const bool more = blk + NB < b1;
       if ((blk - b0) % kWave == 0 && blk + kWave < b1)
-        look_up(blk + kWave, bi_next, kscale_next, vexp_next);
+        next.find(a, trow, kvh, blk + kWave + lane);
       if (more) {
-        if ((blk + 4 - b0) % kWave == 0) {
-          bi = bi_next;
-          kscale = kscale_next;
-          vexp = vexp_next;
-        }
-        load_tile(blk + 4);
+        if ((blk + NB - b0) % kWave == 0) cur = next;
+        load_tile(blk + NB);
       }
       const int key0 = blk * kBlock;
       if (key0 <= wave_last) tile(buf, key0);  // (uniform per wave) later keys: no row sees them
-      if (more) store_tile(blk + 4, buf ^ 1);  // last read before the previous barrier
+      if (more) store_tile(blk + NB, buf ^ 1, cur);  // last read before the previous barrier
       __syncthreads();
     }
     if (s.odd) {
@@ -514,44 +531,69 @@ struct TileSweep {
   }
 
   __device__ inline void tile(int buf, int key0) {
-    f32x16 sc[2];
-    float kf[4], vf[4];
+    f32x16 sc[kTile / 32];
+    float kf[NB], vf[NB];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
+    for (int b = 0; b < NB; ++b) {
       const float2 x = *reinterpret_cast<const float2*>(s.info[buf][b]);
       kf[b] = x.x;
       vf[b] = x.y;
     }
+    constexpr int KG = KS / 2;  // steps of a group of key fragments; two groups in flight
+    u32x4 kfr[2][KG];
+    auto read_k = [&](int g) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+      for (int i = 0; i < KG; ++i)
+        kfr[g % 2][i] = *reinterpret_cast<const u32x4*>(
+            &s.ks[buf][(g / 2 * 32 + j) * KP + (g % 2 * KG + i) * 16 + hf * 8]);
+    };
+    u32x4 vfr[2][DB];
+    auto read_v = [&](int b) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sc[kb][e] = 0.f;
+      for (int d = 0; d < DB; ++d)
+        vfr[b % 2][d] = *reinterpret_cast<const u32x4*>(
+            &s.vts[buf][(d * 32 + j) * VP + b * kBlock + hf * 8]);
+    };
+    // Two groups of fragments are on their way from LDS while one is multiplied: left to
+    // itself the compiler reads each just before its use. The wave in its scores goes before
+    // the one of the other workgroup that is in its softmax.
+    read_k(0);
+    read_k(1);
+    __builtin_amdgcn_s_setprio(2);
 #pragma unroll
-      for (int st = 0; st < KS; ++st) {
-        const u32x4 k =
-            *reinterpret_cast<const u32x4*>(&s.ks[buf][(kb * 32 + j) * KP + st * 16 + hf * 8]);
-        sc[kb] = mfma32<QF16>(k, qa[st], sc[kb]);
-      }
+    for (int g = 0; g < NB; ++g) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (g % 2 == 0)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[g / 2][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KG; ++i) sc[g / 2] = mfma32<QF16>(kfr[g % 2][i], qa[g % 2 * KG + i], sc[g / 2]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (g + 2 < NB) read_k(g + 2);
+      else read_v(g + 2 - NB);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
     if (key0 + kTile - 1 > wave_first) {  // the diagonal, or past the last key
       const int lim = qpos - key0 - 4 * hf;
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < kTile / 32; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (kb * 32 + 8 * (e / 4) + e % 4 > lim) sc[kb][e] = -INFINITY;
       // (a block without a page has the factor NaN: only for the rows that see it)
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      for (int b = 0; b < NB; ++b)
         if (b * kBlock > qpos - key0) kf[b] = a.c2;
     }
     // scores in units of log2, raised by the exponent of V's scale
     float mx = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      float x = sc[b / 2][8 * (b % 2)];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) x = fmaxf(x, sc[b / 2][8 * (b % 2) + e]);
+    for (int b = 0; b < NB; ++b) {
+      const f32x16& z = sc[b / 2];
+      const int e = 8 * (b % 2);
+      const float x = max3(max3(max3(z[e], z[e + 1], z[e + 2]), z[e + 3], z[e + 4]), z[e + 5],
+                           fmaxf(z[e + 6], z[e + 7]));
       mx = fmaxf(mx, C8 ? fmaf(x, kf[b], vf[b]) : x * kf[b]);
     }
     if (__ballot(mx > m + 8.f)) {
@@ -566,26 +608,36 @@ struct TileSweep {
         for (int e = 0; e < 16; ++e) o[d][e] *= f;
     }
     const float ms = m == -INFINITY ? 0.f : m;
+    u32x4 p[NB];  // P^T of a block's 16 keys
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const float off = vf[b] - ms;
-      float sum = 0.f;
-      u32x4 p;  // P^T of the block's 16 keys
+    for (int b = 0; b < NB + 1; ++b) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (b < NB) {
+        const float off = vf[b] - ms;
+        float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(sc[b / 2][8 * (b % 2) + 2 * e], kf[b], off));
-        const float y =
-            __builtin_amdgcn_exp2f(fmaf(sc[b / 2][8 * (b % 2) + 2 * e + 1], kf[b], off));
-        sum += x;
-        sum += y;
-        p[e] = pack2<PF16>(x, y);
+        for (int e = 0; e < 4; ++e) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(sc[b / 2][8 * (b % 2) + 2 * e], kf[b], off));
+          const float y =
+              __builtin_amdgcn_exp2f(fmaf(sc[b / 2][8 * (b % 2) + 2 * e + 1], kf[b], off));
+          sum += x;
+          sum += y;
+          p[b][e] = pack2<PF16>(x, y);
+        }
+        l = C8 ? fmaf(sum, __builtin_amdgcn_exp2f(-vf[b]), l) : l + sum;
       }
-      l = C8 ? fmaf(sum, __builtin_amdgcn_exp2f(-vf[b]), l) : l + sum;
+      if (b > 0) {
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(
-            &s.vts[buf][(d * 32 + j) * VP + b * kBlock + hf * 8]);
-        o[d] = mfma32<PF16>(v, p, o[d]);
+        for (int d = 0; d < DB; ++d) o[d] = mfma32<PF16>(vfr[(b - 1) % 2][d], p[b - 1], o[d]);
+        if (b + 1 < NB) read_v(b + 1);
+      }
+      if (b > 0 && b < NB) {  // P V of a block among the exponentials of the next
+#pragma unroll
+        for (int i = 0; i < DB; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+          __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);  // VALU
+          __builtin_amdgcn_sched_group_barrier(0x400, 2, 0);  // transcendental
+        }
       }
     }
   }
@@ -595,45 +647,50 @@ template <int HD, bool QF16, bool C8>
 __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
   typedef TileSweep<HD, QF16, C8> T;
   __shared__ typename T::Lds lds;
-  const PrefillMap map((uint32_t)(a.S * a.KVH * a.nsplit), (uint32_t)a.tiles);
+  const PrefillMap map((uint32_t)a.S * a.KVH.d * a.nsplit.d, a.tiles.d);
   uint32_t grp, place;
   if (!map.at(blockIdx.x, grp, place)) return;  // (uniform)
-  const int split = (int)(grp % a.nsplit);
-  const int kvh = (int)(grp / a.nsplit % a.KVH), s = (int)(grp / a.nsplit / a.KVH);
-  const int tile = a.tiles - 1 - (int)place;  // the rows with the most keys first
-  const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
-  const int row0 = tile * kRowsTile, all = pr.n * a.G;
-  if (row0 >= all) return;
-  const int pos0 = a.pos0[s];
-  const PagedKeys pk(pos0, pr.n, a.G, row0, kRowsTile, a.cb, a.nsplit);
-  if (split >= max(pk.splits, 1)) return;
+  int s = (int)grp;
+  const int split = a.nsplit.mod(s), kvh = a.KVH.mod(s);
+  const int tile = (int)a.tiles.d - 1 - (int)place;  // the rows with the most keys first
   T t(a, lds);
+  // (as in paged_split_kernel: the first loads do not wait for the lengths)
   t.trow = a.table + (int64_t)s * a.cols;
   t.kvh = kvh;
   t.wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   t.lane = threadIdx.x % kWave;
+  t.cur.find(a, t.trow, kvh, split * a.cb + t.lane);
+  const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
+  const int pos0 = a.pos0[s];
+  const int row0 = tile * kRowsTile, all = pr.n * (int)a.G.d;
+  const PagedKeys pk(pos0, pr.n, a.G, row0, kRowsTile, a.cb, (int)a.nsplit.d);
+  const bool idle = row0 >= all || split >= max(pk.splits, 1);
   const int j = t.j = t.lane % 32, hf = t.hf = t.lane / 32;
-  t.b0 = pk.begin(split, a.cb);
-  t.b1 = pk.keys > 0 ? pk.end(split, a.cb) : t.b0;
+  t.b0 = split * a.cb;
+  t.b1 = idle || pk.keys <= 0 ? t.b0 : pk.end(split, a.cb);
   t.keys = pk.keys;
   const int r0 = row0 + t.wave * 32;  // first row of this wave
-  const int qr = min(r0 + j, all - 1);
-  t.qpos = pos0 + qr / a.G;
-  t.pos_first = pos0 + row0 / a.G;
+  const int qr = max(0, min(r0 + j, all - 1));
+  const int qt = a.G.div(qr);
+  t.qpos = pos0 + qt;
+  t.pos_first = pos0 + a.G.div(row0);
   // positions of the wave's first and last row
-  t.wave_first = pos0 + min(r0, all - 1) / a.G;
-  t.wave_last = r0 < all ? pos0 + min(r0 + 31, all - 1) / a.G : -1;
-  t.qp = a.q + (int64_t)(pr.first + qr / a.G) * a.ldq + (int64_t)(kvh * a.G + qr % a.G) * HD;
+  t.wave_first = pos0 + a.G.div(max(0, min(r0, all - 1)));
+  t.wave_last = r0 < all ? pos0 + a.G.div(min(r0 + 31, all - 1)) : -1;
+  t.qp = a.q + (idle ? 0 : (int64_t)(pr.first + qt) * a.ldq) +
+         (int64_t)(kvh * (int)a.G.d + qr - qt * (int)a.G.d) * HD;
   t.sweep();
+  if (idle) return;  // (uniform)
   f32x16(&o)[T::DB] = t.o;
   constexpr int DB = T::DB;
   const float l = t.l + __shfl_xor(t.l, 32, kWave), m = t.m;
   const int row = r0 + j;
-  if (row >= all) return;
-  const int tok = row / a.G, head = kvh * a.G + row % a.G;
-  const size_t at = (size_t)(pr.first + tok) * a.H + head;
+  int tok = row;
+  const int head = kvh * (int)a.G.d + a.G.mod(tok);
+  const size_t at = (size_t)(pr.first + tok) * a.H.d + head;
   if (pk.splits > 1) {
-    float* po = a.part_o + (at * a.nsplit + split) * HD;
+    if (row >= all) return;
+    float* po = a.part_o + (at * a.nsplit.d + split) * HD;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -641,40 +698,58 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
         *reinterpret_cast<f4*>(po + d * 32 + 8 * i + 4 * hf) =
             f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
     if (hf == 0)
-      *reinterpret_cast<float2*>(a.part_ml + (at * a.nsplit + split) * 2) = float2{m, l};
+      *reinterpret_cast<float2*>(a.part_ml + (at * a.nsplit.d + split) * 2) = float2{m, l};
     return;
   }
-  const bool none = pos0 + tok < 0;  // a row without keys
+  // Through LDS, so that a store instruction writes whole rows: a lane holds 8 bytes of its
+  // row at a time, and 16-byte pieces of 32 rows reach the L2 as as many requests.
   const float inv = 1.f / l;
-  uint16_t* op = static_cast<uint16_t*>(a.out) + at * HD;
+  const bool none = pos0 + tok < 0;  // a row without keys
+  constexpr int OP = HD + 8;
+  uint16_t* lo = &lds.ks[0][0] + t.wave * 32 * OP;  // (the buffers are free: 4 x 32 x OP fit)
+  static_assert(4 * 32 * OP <= 2 * kTile * T::KP, "the rows of O fit the keys' buffers");
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const u32x2 w = {pack2<QF16>(o[d][4 * i] * inv, o[d][4 * i + 1] * inv),
                        pack2<QF16>(o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv)};
-      *reinterpret_cast<u32x2*>(op + d * 32 + 8 * i + 4 * hf) = none ? u32x2{0u, 0u} : w;
+      *reinterpret_cast<u32x2*>(lo + j * OP + d * 32 + 8 * i + 4 * hf) = none ? u32x2{0u, 0u} : w;
     }
-  if (a.lse && hf == 0)
+  if (a.lse && hf == 0 && row < all)
     a.lse[at] = none ? -INFINITY : (m + __log2f(l)) * 0.69314718055994530942f;
+  __builtin_amdgcn_wave_barrier();  // (one wave's rows: its LDS accesses are in order)
+  constexpr int LR = HD / 8;        // lanes of a row
+#pragma unroll
+  for (int i = 0; i < 32 / (kWave / LR); ++i) {
+    const int x = i * (kWave / LR) + t.lane / LR;
+    const u32x4 w = *reinterpret_cast<const u32x4*>(lo + x * OP + t.lane % LR * 8);
+    if (r0 + x < all) {
+      int tk = r0 + x;
+      const int hd = kvh * (int)a.G.d + a.G.mod(tk);
+      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.out) +
+                                ((size_t)(pr.first + tk) * a.H.d + hd) * HD + t.lane % LR * 8) = w;
+    }
+  }
 }
 
 // Joins the splits of a (row, head): one wave each.
 template <int HD, bool QF16>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
-  const int64_t id = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+  int s = (int)(blockIdx.x * 4 + threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
-  const int head = (int)(id % a.H);
-  const int i = (int)(id / a.H % a.max_rows), s = (int)(id / a.H / a.max_rows);
+  const int head = a.H.mod(s), i = a.rows_each.mod(s);
   if (s >= a.S) return;
   const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
   if (i >= pr.n) return;
-  const int pos0 = a.pos0[s], row = i * a.G + head % a.G;
-  const PagedKeys pk(pos0, pr.n, a.G, row / a.tile * a.tile, a.tile, a.cb, a.nsplit);
+  int x = head;
+  const int pos0 = a.pos0[s], row = i * (int)a.G.d + a.G.mod(x);
+  const PagedKeys pk(pos0, pr.n, a.G, a.tile.div(row) * (int)a.tile.d, (int)a.tile.d, a.cb,
+                     (int)a.nsplit.d);
   if (pk.splits <= 1) return;  // written already
-  const size_t at = (size_t)(pr.first + i) * a.H + head;
-  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at * a.nsplit;
-  const float* po = a.part_o + at * a.nsplit * HD;
+  const size_t at = (size_t)(pr.first + i) * a.H.d + head;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at * a.nsplit.d;
+  const float* po = a.part_o + at * a.nsplit.d * HD;
   constexpr int D = HD / kWave;
   float mm = -INFINITY;
   for (int x = lane; x < pk.splits; x += kWave) mm = fmaxf(mm, ml[x].x);
@@ -831,7 +906,7 @@ extern "C" int sm_paged_attention(const sm_paged_cache* cache, const int32_t* bl
   PagedArgs a;
   a.k = static_cast<const uint8_t*>(cache->k);
   a.v = static_cast<const uint8_t*>(cache->v);
-  a.ks = cache->k_scales;
+  a.ks = cache->dtype == SM_F8E4M3 ? cache->k_scales : nullptr;
   a.vs = cache->v_scales;
   a.q = static_cast<const uint16_t*>(q);
   a.table = block_table;
@@ -845,16 +920,17 @@ extern "C" int sm_paged_attention(const sm_paged_cache* cache, const int32_t* bl
   a.S = (int)S;
   a.rows = (int)rows;
   a.max_rows = (int)max_rows;
-  a.H = (int)H;
-  a.KVH = (int)KVH;
-  a.G = (int)(H / KVH);
+  a.H = Divide((int)H);
+  a.KVH = Divide((int)KVH);
+  a.G = Divide((int)(H / KVH));
+  a.rows_each = Divide((int)max_rows);
   a.pages = (int)cache->pages;
-  a.bpp = (int)(cache->page_tokens / kBlock);
+  a.bpp = Divide((int)(cache->page_tokens / kBlock));
   a.cols = (int)table_cols;
   a.cb = plan.cb;
-  a.nsplit = plan.nsplit;
-  a.tile = plan.tile;
-  a.tiles = (int)plan.tiles;
+  a.nsplit = Divide(plan.nsplit);
+  a.tile = Divide(plan.tile);
+  a.tiles = Divide((int)plan.tiles);
   a.c2 = 1.44269504088896340736f / sqrtf((float)hd);
   const bool f16 = dtype == SM_F16, c8 = cache->dtype == SM_F8E4M3;
 #define SM_PAGED2(HD, F, C)                                                      \

@@ -10,6 +10,28 @@ namespace sm {
 
 constexpr int kBlock = 16;  // tokens of a cache block (and of a scale)
 
+// Division of 0 <= n < 2^31 by a divisor that the host knows: a multiply and a shift (round-up
+// method: with 2^shift >= d and mul = ceil(2^32 (2^shift - d) / d), or one more where that is
+// whole, the quotient is ((n mul >> 32) + n) >> shift). The compiler's own division takes
+// about 20 instructions, and a workgroup of few keys makes eight.
+struct Divide {
+  uint32_t d = 1, mul = 1, shift = 0;
+  Divide() = default;
+  __host__ __device__ Divide(int by) : d((uint32_t)by), shift(0) {
+    while (((uint64_t)1 << shift) < d) ++shift;
+    mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1);
+  }
+  __host__ __device__ int div(int n) const {
+    return (int)(((uint32_t)((uint64_t)(uint32_t)n * mul >> 32) + (uint32_t)n) >> shift);
+  }
+  // n becomes the quotient, the remainder is returned
+  __host__ __device__ int mod(int& n) const {
+    const int q = div(n), r = n - q * (int)d;
+    n = q;
+    return r;
+  }
+};
+
 // Rows [first, first + n) of sequence s: the ragged form's row_start [S + 1], or
 // max_rows each without one. Whatever row_start holds, they lie inside [0, rows).
 struct PagedRows {
@@ -33,12 +55,13 @@ struct PagedRows {
 // The cache block of block `blk` of a sequence, as an index over [pages, KVH, page / 16];
 // -1 where the table has no such entry or the entry names no page.
 __host__ __device__ inline int paged_block(const int32_t* table_row, int cols, int pages, int KVH,
-                                           int kvh, int bpp, int blk) {
-  const int col = blk / bpp;
-  if (blk < 0 || col >= cols) return -1;
+                                           int kvh, const Divide& bpp, int blk) {
+  if (blk < 0) return -1;
+  const int col = bpp.div(blk);
+  if (col >= cols) return -1;
   const int page = table_row[col];
   if (page < 0 || page >= pages) return -1;
-  return (page * KVH + kvh) * bpp + (blk - col * bpp);
+  return (page * KVH + kvh) * (int)bpp.d + (blk - col * (int)bpp.d);
 }
 
 // Blocks that n tokens touch at most, wherever the first of them falls.
@@ -52,12 +75,12 @@ struct PagedKeys {
   int keys;    // keys that the tile's last row sees (<= 0: none)
   int blocks;  // blocks that hold them
   int splits;  // splits that have work (0 without keys)
-  __host__ __device__ PagedKeys(int pos0, int n, int G, int first_row, int tile, int cb,
-                                int nsplit) {
-    const int all = n * G;
+  __host__ __device__ PagedKeys(int pos0, int n, const Divide& G, int first_row, int tile,
+                                int cb, int nsplit) {
+    const int all = n * (int)G.d;
     int last = first_row + tile - 1;
     if (last > all - 1) last = all - 1;
-    const int64_t k = (int64_t)pos0 + last / G + 1;
+    const int64_t k = last < 0 ? 0 : (int64_t)pos0 + G.div(last) + 1;
     keys = k < 0 ? 0 : k > 0x7fffffff ? 0x7fffffff : (int)k;
     blocks = (int)(((int64_t)keys + kBlock - 1) / kBlock);
     const int64_t want = ((int64_t)blocks + cb - 1) / cb;
