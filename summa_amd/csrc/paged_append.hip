@@ -4,10 +4,18 @@
 //   (summa-llm/src/model/attention.rs:142-177, 331-356) over the paged cache of
 //   sm_paged_cache.
 //
-// One wave takes one head of one 16-token cache block: a block's scale is the maximum
-// over its tokens, so the wave needs no other wave's values and no two waves write one
-// scale. Lane (g, c) holds dims D c .. D c + D - 1 (D = head_dim / 16) of tokens 4 g .. 4 g + 3.
+// One wave takes one head of one 16-token cache block at a time: a block's scale is the
+// maximum over its tokens, so the wave needs no other wave's values, no two waves write one
+// scale, and there is no barrier. A wave goes through several heads of its block where
+// there are blocks enough, with the angles of its tokens in registers.
+// Queries and keys: lane (i, c) of 64 / (head_dim / 8) x head_dim / 8 holds two times four
+// dims of tokens i, i + 64 / (head_dim / 8), ..: in the half layout 4 c .. and 4 c + rot_dim / 2 ..,
+// so that both of a pair are in one lane.
+// Values: lane (g, c) holds head_dim / 16 dims of tokens 4 g .. 4 g + 3, which is a word (8-bit)
+// or two of the stored block a dim; the block goes through LDS to be stored as it lies.
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.hpp"
 #include "paged_map.hpp"
@@ -28,7 +36,7 @@ struct AppendArgs {
   const int32_t *table, *pos0, *row_start;
   void* q_out;
   Divide bpp, touched, groups;
-  int S, rows, max_rows, H, KVH, pages, cols, rot, half_layout, q_f16;
+  int S, rows, max_rows, H, KVH, pages, cols, rot, half_layout, q_f16, each;
 };
 
 // D consecutive values of a row as f32 (8: 16-byte loads; 4: 8- or 16-byte ones).
@@ -82,190 +90,320 @@ __device__ inline int scale_exponent(float amax) {
   return max(-63, (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0));
 }
 
-template <typename T, int HD, int CT>  // CT: cache type, 0 bf16, 1 f16, 2 e4m3
-__global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
-  constexpr int D = HD / 16;
-  int s = (int)blockIdx.x;
-  const int slot = a.groups.mod(s) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int nth = a.touched.mod(s);  // of the blocks that the sequence's rows touch
-  const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
-  const int first_slot = a.q ? 0 : a.H;
-  if (slot + first_slot >= a.H + 2 * a.KVH || pr.n == 0) return;
-  const int head = slot + first_slot;
-  const int pos0 = a.pos0[s];
-  const int64_t end = (int64_t)pos0 + pr.n;            // one past the last position
-  const int64_t base = (int64_t)(max(pos0, 0) / kBlock + nth) * kBlock;
-  const int t0 = (int)max((int64_t)max(pos0, 0) - base, (int64_t)0);
-  const int t1 = (int)min(end - base, (int64_t)kBlock);
-  if (t0 >= t1) return;  // (uniform: the wave's block holds none of the rows)
-  const int lane = threadIdx.x % kWave, g = lane / 16, c = lane % 16, d0 = D * c;
-
-  const bool is_q = head < a.H, is_k = !is_q && head < a.H + a.KVH;
-  const int hd_at = (is_q ? head : is_k ? head - a.H : head - a.H - a.KVH);
-  const T* src = static_cast<const T*>(is_q ? a.q : is_k ? a.k : a.v) + (int64_t)hd_at * HD;
-  const int64_t ld = is_q ? a.ldq : is_k ? a.ldk : a.ldv;
-  const int64_t row0 = pr.first + (base - pos0);  // the row of token 0 of the block
-  float x[4][D];
+// Four consecutive values of a row as they lie, and as f32.
+template <typename T>
+struct Four {
+  u32x2 w;
+  __device__ inline void get(float (&f)[4]) const {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int t = 4 * g + j;
-    if (t >= t0 && t < t1) {
-      load_dims<T, D>(src + (row0 + t) * ld + d0, x[j]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < D; ++i) x[j][i] = 0.f;
-    }
-  }
-  if ((is_q || is_k) && d0 < a.rot) {
-    const int half = a.rot / 2;
-    const bool low = d0 < half;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int t = 4 * g + j;
-      if (t < t0 || t >= t1) continue;
-      if (a.half_layout) {
-        float p[D], cs[D], sn[D];
-        load_dims<T, D>(src + (row0 + t) * ld + (low ? d0 + half : d0 - half), p);
-        load_angles<D>(a.rope, a.rope_rows, half, base + t, low ? d0 : d0 - half, cs, sn);
-#pragma unroll
-        for (int i = 0; i < D; ++i) {
-          float u = low ? x[j][i] : p[i], w = low ? p[i] : x[j][i];
-          rotate_pair(u, w, cs[i], sn[i]);
-          x[j][i] = low ? u : w;
-        }
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (__is_same(T, _Float16)) {
+        const h2 x = as_h2(w[i]);
+        f[2 * i] = (float)x[0];
+        f[2 * i + 1] = (float)x[1];
       } else {
-        float cs[D / 2], sn[D / 2];
-        load_angles<D / 2>(a.rope, a.rope_rows, half, base + t, d0 / 2, cs, sn);
-#pragma unroll
-        for (int i = 0; i < D / 2; ++i) rotate_pair(x[j][2 * i], x[j][2 * i + 1], cs[i], sn[i]);
+        f[2 * i] = bf16lo(w[i]);
+        f[2 * i + 1] = bf16hi(w[i]);
       }
     }
   }
-  if (is_q) {
+};
+template <>
+struct Four<float> {
+  u32x4 w;
+  __device__ inline void get(float (&f)[4]) const {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int t = 4 * g + j;
-      if (t < t0 || t >= t1) continue;
-      const int64_t at = ((row0 + t) * a.H + head) * HD + d0;
-      if (a.q_f16) store_dims<_Float16, D>(static_cast<_Float16*>(a.q_out) + at, x[j]);
-      else store_dims<uint16_t, D>(static_cast<uint16_t*>(a.q_out) + at, x[j]);
-    }
-    return;
+    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
   }
-  const int bi = paged_block(a.table + (int64_t)s * a.cols, a.cols, a.pages, a.KVH, hd_at, a.bpp,
-                             (int)(base / kBlock));
-  if (bi < 0) return;  // (uniform) no page for these tokens
-  if constexpr (CT == 2) {
-    float amax = 0.f;
-    bool odd = false;
+};
+
+template <typename T, int HD, int CT>  // CT: cache type, 0 bf16, 1 f16, 2 e4m3
+struct Append {
+  static constexpr int LPT = HD / 8, TPL = HD / 32, STEP = kWave / LPT;
+  static constexpr int D = HD / 16;
+  static constexpr int ES = CT == 2 ? 1 : 2;
+  static constexpr int NC = HD * ES / 64;  // kilobytes of a block
+  typedef typename std::conditional<CT == 1, _Float16, uint16_t>::type TC;
+
+  const AppendArgs& a;
+  int lane, t0, t1;
+  int64_t base, row0;  // position and row of the block's token 0
+  const int32_t* trow;
+  u32x4* lds;          // this wave's NC kilobytes
+  float cs[TPL][4], sn[TPL][4];
+  Four<T> x[TPL][2];   // the slot at hand, as loaded
+  bool turn;           // this lane's dims are rotated
+
+  // The lane number anew: what a head's addresses are made of, so that those of all heads
+  // (30 registers) are not kept through the loop over heads.
+  __device__ inline int lane_again() const {
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    return l;
+  }
+  __device__ inline bool mine(int t) const { return t >= t0 && t < t1; }
+  static __device__ inline int token(int l, int j) { return l / LPT + j * STEP; }
+  // first dims of a lane's two fours
+  __device__ inline int dim_a(int l) const {
+    return a.half_layout && turn ? 4 * (l % LPT) : 8 * (l % LPT);
+  }
+  __device__ inline int dim_b(int l) const {
+    return dim_a(l) + (a.half_layout && turn ? a.rot / 2 : 4);
+  }
+
+  __device__ inline void angles() {
+    turn = 8 * (lane % LPT) < a.rot;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < TPL; ++j) {  // (tokens that are not the call's read some row too)
+      const int64_t pos = base + token(lane, j);
+      const bool in = pos < a.rope_rows;
+      const float4* p = reinterpret_cast<const float4*>(
+          a.rope + ((in ? pos : 0) * (a.rot / 2) + (turn ? 4 * (lane % LPT) : 0)) * 2);
+      const float4 u = p[0], w = p[1];
+      const float f[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int i = 0; i < D; ++i) {
-        const float v = fabsf(x[j][i]);
-        if (v < INFINITY) amax = fmaxf(amax, v);
-        else odd = true;
+      for (int i = 0; i < 4; ++i) {
+        cs[j][i] = in ? f[2 * i] : NAN;
+        sn[j][i] = in ? f[2 * i + 1] : NAN;
       }
-    int e = scale_exponent(wave_max(amax));
-    uint8_t* sp = (is_k ? a.ks : a.vs) + bi;
-    int old = e;
+    }
+  }
+  // a query's or key's head
+  __device__ inline void load_row(const void* p, int64_t ld, int head) {
+    const T* src = static_cast<const T*>(p) + (int64_t)head * HD;
+    const int l = lane_again();
+#pragma unroll
+    for (int j = 0; j < TPL; ++j) {
+      const int t = token(l, j);
+      x[j][0] = x[j][1] = Four<T>{};
+      if (mine(t)) {
+        x[j][0] = *reinterpret_cast<const Four<T>*>(src + (row0 + t) * ld + dim_a(l));
+        x[j][1] = *reinterpret_cast<const Four<T>*>(src + (row0 + t) * ld + dim_b(l));
+      }
+    }
+  }
+  __device__ inline void rotate(float (&y)[TPL * 8]) const {
+    const bool half = a.half_layout;  // (values are chosen, not places: those would go to memory)
+#pragma unroll
+    for (int j = 0; j < TPL; ++j) {
+      const bool on = turn && mine(token(lane, j));
+      float u[4], w[4], p[4], q[4];
+      x[j][0].get(u);
+      x[j][1].get(w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = half ? u[i] : i < 2 ? u[2 * i] : w[2 * i - 4];
+        q[i] = half ? w[i] : i < 2 ? u[2 * i + 1] : w[2 * i - 3];
+        if (on) rotate_pair(p[i], q[i], cs[j][i], sn[j][i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        y[8 * j + i] = half ? p[i] : i % 2 ? q[i / 2] : p[i / 2];
+        y[8 * j + 4 + i] = half ? q[i] : i % 2 ? q[2 + i / 2] : p[2 + i / 2];
+      }
+    }
+  }
+  template <typename TQ>
+  __device__ inline void store_q(const float (&y)[TPL * 8], int head) const {
+    const int l = lane_again();
+#pragma unroll
+    for (int j = 0; j < TPL; ++j) {
+      const int t = token(l, j);
+      if (!mine(t)) continue;
+      TQ* p = static_cast<TQ*>(a.q_out) + ((row0 + t) * a.H + head) * HD;
+      *reinterpret_cast<u32x2*>(p + dim_a(l)) =
+          u32x2{round2<TQ>(y[8 * j + 0], y[8 * j + 1]), round2<TQ>(y[8 * j + 2], y[8 * j + 3])};
+      *reinterpret_cast<u32x2*>(p + dim_b(l)) =
+          u32x2{round2<TQ>(y[8 * j + 4], y[8 * j + 5]), round2<TQ>(y[8 * j + 6], y[8 * j + 7])};
+    }
+  }
+
+  // The block's exponent for the values y of this call, with the earlier tokens' where some
+  // stay; `again` scales those down.
+  template <int N>
+  __device__ inline void scale(const float (&y)[N], uint8_t* sp, float& inv, float& again,
+                               bool& grown, bool& odd) const {
+    // (as bits, infinities and NaN are above every finite value)
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) most = max(most, __float_as_uint(y[i]) & 0x7fffffffu);
+    odd = __ballot(most >= 0x7f800000u) != 0;
+    if (odd) {
+      most = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t v = __float_as_uint(y[i]) & 0x7fffffffu;
+        most = max(most, v < 0x7f800000u ? v : 0u);
+      }
+    }
+    const float amax = __uint_as_float(most);
+    int e = scale_exponent(wave_max(amax)), old = e;
     if (t0 > 0) {
       old = (int)*sp - 127;
       e = max(e, old);
     }
-    const bool grown = e > old;  // (uniform)
-    const float again = pow2f(old - e), inv = pow2f(-e);
+    grown = e > old;  // (uniform)
+    again = pow2f(old - e);
+    inv = pow2f(-e);
     if (lane == 0) *sp = (uint8_t)(e + 127);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int i = 0; i < D; ++i) x[j][i] *= inv;
-    uint8_t* page = (is_k ? a.kc : a.vc) + (size_t)bi * (kBlock * HD);
-    // infinities and NaN are the NaN code: the scale is that of the finite values
-    auto nan4 = [&](uint32_t w, float p, float q, float r, float z) {
-      const float y[4] = {p, q, r, z};
+  }
+  // Four values -> codes; infinities and NaN are the NaN code.
+  static __device__ inline uint32_t encode(const float (&y)[4], bool odd) {
+    uint32_t w = pack_e4m3(y[0], y[1], y[2], y[3]);
+    if (odd) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (!(fabsf(y[i]) < INFINITY)) w = (w & ~(0xffu << (8 * i))) | (0x7fu << (8 * i));
-      return w;
-    };
-    const bool any_odd = __ballot(odd) != 0;
-    if (is_k) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = 4 * g + j;
-        uint32_t* p = reinterpret_cast<uint32_t*>(page + t * HD + d0);
-        if (t >= t0 && t < t1) {
-          uint32_t w[D / 4];
-#pragma unroll
-          for (int i = 0; i < D / 4; ++i) {
-            w[i] = pack_e4m3(x[j][4 * i], x[j][4 * i + 1], x[j][4 * i + 2], x[j][4 * i + 3]);
-            if (any_odd)
-              w[i] = nan4(w[i], x[j][4 * i], x[j][4 * i + 1], x[j][4 * i + 2], x[j][4 * i + 3]);
-          }
-          if constexpr (D == 8) *reinterpret_cast<u32x2*>(p) = u32x2{w[0], w[1]};
-          else *p = w[0];
-        } else if (t < t0 && grown) {
-#pragma unroll
-          for (int i = 0; i < D / 4; ++i) p[i] = rescale_e4m3(p[i], again);
-        }
-      }
-    } else {
-      uint32_t mine = 0, older = 0;  // bytes of the quad: the call's tokens, earlier ones
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = 4 * g + j;
-        if (t >= t0 && t < t1) mine |= 0xffu << (8 * j);
-        if (t < t0) older |= 0xffu << (8 * j);
-      }
-      if (mine || (grown && older)) {
-#pragma unroll
-        for (int i = 0; i < D; ++i) {
-          const int d = d0 + i, n = d / 16;
-          uint32_t* p =
-              reinterpret_cast<uint32_t*>(page + ((n / 4 * 4 + g) * 16 + d % 16) * 16 + n % 4 * 4);
-          uint32_t w = pack_e4m3(x[0][i], x[1][i], x[2][i], x[3][i]);
-          if (any_odd) w = nan4(w, x[0][i], x[1][i], x[2][i], x[3][i]);
-          if (~mine) {
-            uint32_t was = *p;
-            if (grown) was = (was & ~older) | (rescale_e4m3(was, again) & older);
-            w = (w & mine) | (was & ~mine);
-          }
-          *p = w;
-        }
-      }
     }
-  } else {
-    typedef typename std::conditional<CT == 1, _Float16, uint16_t>::type TC;
-    TC* page = reinterpret_cast<TC*>(is_k ? a.kc : a.vc) + (size_t)bi * (kBlock * HD);
-    if (is_k) {
+    return w;
+  }
+
+  __device__ inline int block(int head) const {
+    return paged_block(trow, a.cols, a.pages, a.KVH, head, a.bpp, (int)(base / kBlock));
+  }
+  __device__ inline void store_k(float (&y)[TPL * 8], int head) const {
+    const int bi = block(head);
+    if (bi < 0) return;  // (uniform) no page for these tokens
+    const int l = lane_again();
+    if constexpr (CT == 2) {
+      float inv, again;
+      bool grown, odd;
+      scale(y, a.ks + bi, inv, again, grown, odd);
+      uint8_t* page = a.kc + (size_t)bi * (kBlock * HD);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = 4 * g + j;
-        if (t >= t0 && t < t1) store_dims<TC, D>(page + t * HD + d0, x[j]);
+      for (int j = 0; j < TPL; ++j) {
+        const int t = token(l, j);
+        uint32_t* pa = reinterpret_cast<uint32_t*>(page + t * HD + dim_a(l));
+        uint32_t* pb = reinterpret_cast<uint32_t*>(page + t * HD + dim_b(l));
+        if (mine(t)) {
+          const float u[4] = {y[8 * j + 0] * inv, y[8 * j + 1] * inv, y[8 * j + 2] * inv, y[8 * j + 3] * inv};
+          const float w[4] = {y[8 * j + 4] * inv, y[8 * j + 5] * inv, y[8 * j + 6] * inv, y[8 * j + 7] * inv};
+          *pa = encode(u, odd);
+          *pb = encode(w, odd);
+        } else if (t < t0 && grown) {
+          *pa = rescale_e4m3(*pa, again);
+          *pb = rescale_e4m3(*pb, again);
+        }
       }
     } else {
-      uint32_t m01 = 0, m23 = 0;
+      TC* page = reinterpret_cast<TC*>(a.kc) + (size_t)bi * (kBlock * HD);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = 4 * g + j;
-        if (t >= t0 && t < t1) (j < 2 ? m01 : m23) |= 0xffffu << (16 * (j % 2));
-      }
-      if (m01 | m23) {
-#pragma unroll
-        for (int i = 0; i < D; ++i) {
-          const int d = d0 + i, n = d / 16;
-          u32x2* p = reinterpret_cast<u32x2*>(page + ((n / 2 * 4 + g) * 16 + d % 16) * 8 + n % 2 * 4);
-          u32x2 w = {round2<TC>(x[0][i], x[1][i]), round2<TC>(x[2][i], x[3][i])};
-          if (~(m01 & m23)) {
-            const u32x2 was = *p;
-            w = (w & u32x2{m01, m23}) | (was & u32x2{~m01, ~m23});
-          }
-          *p = w;
-        }
+      for (int j = 0; j < TPL; ++j) {
+        const int t = token(l, j);
+        if (!mine(t)) continue;
+        *reinterpret_cast<u32x2*>(page + t * HD + dim_a(l)) =
+            u32x2{round2<TC>(y[8 * j + 0], y[8 * j + 1]), round2<TC>(y[8 * j + 2], y[8 * j + 3])};
+        *reinterpret_cast<u32x2*>(page + t * HD + dim_b(l)) =
+            u32x2{round2<TC>(y[8 * j + 4], y[8 * j + 5]), round2<TC>(y[8 * j + 6], y[8 * j + 7])};
       }
     }
   }
+
+  __device__ inline void append_v(int head) const {
+    const int bi = block(head);
+    if (bi < 0) return;  // (uniform)
+    const int g = lane / 16, c = lane % 16;
+    const T* src = static_cast<const T*>(a.v) + (int64_t)head * HD + D * c;
+    float v[4 * D];  // [token 4 g + j][dim D c + i]
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float f[D];
+      const int t = 4 * g + j;
+#pragma unroll
+      for (int i = 0; i < D; ++i) f[i] = 0.f;
+      if (mine(t)) load_dims<T, D>(src + (row0 + t) * a.ldv, f);
+#pragma unroll
+      for (int i = 0; i < D; ++i) v[j * D + i] = f[i];
+    }
+    float inv = 1.f, again = 1.f;
+    bool grown = false, odd = false;
+    if constexpr (CT == 2) scale(v, a.vs + bi, inv, again, grown, odd);
+    // To LDS: 16-byte pieces in the block's order (piece ((d / 16 T) 4 + g) 16 + d % 16), each
+    // eight times 16 pieces in an order of their own, which spreads the words over the banks.
+    constexpr int TT = 4 / ES;
+#pragma unroll
+    for (int i = 0; i < D; ++i) {
+      const int d = D * c + i, n = d / 16;
+      const int piece = (n / TT * 4 + g) * 16 + d % 16, at = piece ^ (piece / 16 % 8);
+      const float y[4] = {v[i] * inv, v[D + i] * inv, v[2 * D + i] * inv, v[3 * D + i] * inv};
+      if constexpr (CT == 2)
+        reinterpret_cast<uint32_t*>(lds + at)[n % TT] = encode(y, odd);
+      else
+        reinterpret_cast<u32x2*>(lds + at)[n % TT] = u32x2{round2<TC>(y[0], y[1]), round2<TC>(y[2], y[3])};
+    }
+    __builtin_amdgcn_wave_barrier();  // (one wave's LDS accesses are in order)
+    // masks of the call's tokens and of earlier ones in the quad of this lane's pieces
+    uint32_t m[2] = {0, 0}, older = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int t = 4 * g + j;
+      if constexpr (CT == 2) {
+        if (mine(t)) m[0] |= 0xffu << (8 * j);
+        if (t < t0) older |= 0xffu << (8 * j);
+      } else if (mine(t)) {
+        m[j / 2] |= 0xffffu << (16 * (j % 2));
+      }
+    }
+    if constexpr (CT == 2) m[1] = m[0];
+    u32x4* page = reinterpret_cast<u32x4*>(a.vc + (size_t)bi * (kBlock * HD * ES)) + lane;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int piece = k * kWave + lane;
+      u32x4 w = lds[piece ^ (piece / 16 % 8)];
+      if (!(m[0] | m[1]) && !(grown && older)) continue;
+      const u32x4 keep = {m[0], m[1], m[0], m[1]};
+      if (~(m[0] & m[1])) {
+        u32x4 was = page[k * kWave];
+        if constexpr (CT == 2) {
+          if (grown) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              was[i] = (was[i] & ~older) | (rescale_e4m3(was[i], again) & older);
+          }
+        }
+        w = (w & keep) | (was & ~keep);
+      }
+      page[k * kWave] = w;
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+};
+
+template <typename T, int HD, int CT>
+__global__ __launch_bounds__(256, 4) void paged_append_kernel(AppendArgs a) {
+  typedef Append<T, HD, CT> A;
+  __shared__ u32x4 lds[4][A::NC * kWave];
+  int s = (int)blockIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int group = a.groups.mod(s), nth = a.touched.mod(s);
+  const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
+  const int pos0 = a.pos0[s];
+  const int64_t end = (int64_t)pos0 + pr.n;  // one past the last position
+  A x{a};
+  x.lane = threadIdx.x % kWave;
+  x.base = (int64_t)(max(pos0, 0) / kBlock + nth) * kBlock;
+  x.t0 = (int)max((int64_t)max(pos0, 0) - x.base, (int64_t)0);
+  x.t1 = (int)min(end - x.base, (int64_t)kBlock);
+  if (x.t0 >= x.t1) return;  // (uniform) the block holds none of the rows
+  x.row0 = pr.first + (x.base - pos0);
+  x.trow = a.table + (int64_t)s * a.cols;
+  x.lds = lds[wave];
+  x.turn = false;
+  // slots: query heads, key heads, value heads
+  const int slots = a.H + 2 * a.KVH, turned = a.H + a.KVH;
+  int slot = group * 4 * a.each + wave;
+  const int stop = min(slots, (group + 1) * 4 * a.each);
+  if (slot < turned && a.rot > 0) x.angles();
+  for (; slot < min(stop, turned); slot += 4) {
+    float y[A::TPL * 8];
+    if (slot < a.H) x.load_row(a.q, a.ldq, slot);
+    else x.load_row(a.k, a.ldk, slot - a.H);
+    x.rotate(y);
+    if (slot >= a.H) x.store_k(y, slot - a.H);
+    else if (a.q_f16) x.template store_q<_Float16>(y, slot);
+    else x.template store_q<uint16_t>(y, slot);
+  }
+  for (; slot < stop; slot += 4) x.append_v(slot - turned);
 }
 
 }  // namespace
@@ -294,8 +432,10 @@ extern "C" int sm_paged_append(const sm_paged_cache* cache, const int32_t* block
                "%s: layout must be SM_ROPE_INTERLEAVED or SM_ROPE_HALF", me);
     SM_REQUIRE(rot_dim >= 16 && rot_dim % 16 == 0 && rot_dim <= hd,
                "%s: rot_dim must be a multiple of 16 up to head_dim", me);
-    SM_REQUIRE(rope_rows >= 0 && reinterpret_cast<uintptr_t>(rope_table) % 16 == 0,
-               "%s: rope_table must be 16-byte aligned", me);
+    SM_REQUIRE(rope_rows > 0 && reinterpret_cast<uintptr_t>(rope_table) % 16 == 0,
+               "%s: rope_table must be 16-byte aligned and have rows", me);
+  } else {
+    SM_REQUIRE(rot_dim == 0, "%s: rot_dim without a rope_table", me);
   }
   if (S == 0 || max_rows == 0) return SM_OK;
   SM_REQUIRE(block_table && pos0 && k && v && (!q || q_out), "%s: null buffer", me);
@@ -343,7 +483,13 @@ extern "C" int sm_paged_append(const sm_paged_cache* cache, const int32_t* block
   a.half_layout = layout == SM_ROPE_HALF;
   a.q_f16 = q_dtype == SM_F16;
   a.touched = Divide((int)paged_touched(max_rows));
-  a.groups = Divide((int)ceil_div(a.H + 2 * KVH, 4));
+  // Heads that a wave goes through, for the angles that it then reads once: as many as leave
+  // 2048 workgroups, two for every place on the chip. (12.6 k bf16 rows of 16 + 2 x 4 heads of
+  // 128, 3.3 times that many blocks of work: one head a wave 40 us, three 33.)
+  const int64_t slots = a.H + 2 * KVH;
+  a.each = (int)std::max<int64_t>(
+      1, std::min<int64_t>(ceil_div(slots, 4), S * a.touched.d * ceil_div(slots, 4) / 2048));
+  a.groups = Divide((int)ceil_div(slots, 4 * a.each));
   if ((double)S * a.touched.d * a.groups.d >= (double)(1 << 24)) {
     set_error("%s: problem too large", me);
     return SM_ERR_UNSUPPORTED;

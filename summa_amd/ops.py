@@ -729,24 +729,37 @@ def _rope_layout(layout: str) -> int:
         raise ValueError("layout must be 'interleaved' or 'half'") from e
 
 
-def _on_current(device: torch.device) -> None:
+def _on_current(index: int) -> None:
     """The library launches on the current device's stream."""
-    if device.type != "cuda":
+    if index < 0:
         raise ValueError("tensors must be on the device")
-    if device.index != torch._C._cuda_getDevice():
-        raise ValueError(f"tensors are on {device}, which is not the current device")
+    if index != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors are on device {index}, which is not the current device")
 
 
-def _rope_angles(table: torch.Tensor | None, device):
+def _head_rows(t: torch.Tensor, name: str):
+    """(rows, heads, head_dim, row stride) of rows whose heads lie side by side."""
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [rows, heads, head_dim]")
+    (rows, heads, hd), (ld, step, unit) = t.shape, t.stride()
+    if unit != 1 or (step != hd and heads > 1):
+        raise ValueError(f"{name} must be [rows, heads, head_dim] with contiguous heads")
+    return rows, heads, hd, ld if rows > 1 else heads * hd
+
+
+def _rope_angles(table: torch.Tensor | None, index: int):
     """(pointer, rows, rot_dim) of a checked rotary table; None: no rotation."""
     if table is None:
         return None, 0, 0
-    if table.dtype != torch.float32 or table.dim() != 3 or table.shape[2] != 2 or \
+    if table.dtype is not torch.float32 or table.dim() != 3 or table.shape[2] != 2 or \
             not table.is_contiguous():
         raise ValueError("a rotary table is contiguous float32 [positions, rot_dim / 2, 2]")
-    if table.device != device:
+    if table.get_device() != index:
         raise ValueError("the rotary table must be on the tensors' device")
-    return table.data_ptr(), table.shape[0], 2 * table.shape[1]
+    rows, half, _ = table.shape
+    if rows == 0 or half == 0:
+        raise ValueError("the rotary table is empty")
+    return table.data_ptr(), rows, 2 * half
 
 
 def rope_table(positions: int, rot_dim: int, theta: float = 1e4, *, scaling: str = "none",
@@ -763,7 +776,7 @@ def rope_table(positions: int, rot_dim: int, theta: float = 1e4, *, scaling: str
     if positions < 0 or rot_dim <= 0 or rot_dim % 2:
         raise ValueError("need positions >= 0 and an even rot_dim > 0")
     t = torch.empty(positions, rot_dim // 2, 2, dtype=torch.float32, device=device)
-    _on_current(t.device)
+    _on_current(t.get_device())
     call("sm_rope_table", float(theta), rot_dim, positions, _ROPE_SCALINGS[scaling], float(factor),
          float(original_positions), float(low_turns), float(high_turns), float(magnitude),
          t.data_ptr(), _stream())
@@ -778,22 +791,20 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
     head rotated by the table's row ``positions[r]`` (int32 [rows]); ``backward``: by the
     opposite angle, the gradient with respect to x. ``out`` may be x itself
     (``sm_rope``; attention.rs:142-177)."""
-    if x.dim() != 3 or x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != x.shape[2]):
-        raise ValueError("x must be [rows, heads, head_dim] with contiguous heads")
-    rows, heads, hd = x.shape
-    dt = _dt(x)
-    _on_current(x.device)
-    if positions.dtype != torch.int32 or positions.shape != (rows,) or \
-            not positions.is_contiguous() or positions.device != x.device:
+    rows, heads, hd, ldx = _head_rows(x, "x")
+    dt, index = _dt(x), x.get_device()
+    _on_current(index)
+    if positions.dtype is not torch.int32 or positions.shape != (rows,) or \
+            not positions.is_contiguous() or positions.get_device() != index:
         raise ValueError("positions must be contiguous int32 [rows] on x's device")
-    at, table_rows, rot = _rope_angles(table, x.device)
+    at, table_rows, rot = _rope_angles(table, index)
     if out is None:
-        out = torch.empty((rows, heads, hd), dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or \
-            out.stride(2) != 1 or (heads > 1 and out.stride(1) != hd):
-        raise ValueError("out must have x's shape and dtype, with contiguous heads")
-    width = heads * hd
-    ldx, ldy = (t.stride(0) if rows > 1 else width for t in (x, out))
+        ldy = heads * hd
+        out = torch.empty_strided((rows, heads, hd), (ldy, hd, 1), dtype=x.dtype, device=x.device)
+    else:
+        if out.shape != x.shape or out.dtype is not x.dtype or out.get_device() != index:
+            raise ValueError("out must have x's shape and dtype, on x's device")
+        ldy = _head_rows(out, "out")[3]
     call("sm_rope", x.data_ptr(), ldx, out.data_ptr(), ldy, dt, at, table_rows,
          positions.data_ptr(), rows, heads, hd, rot, _rope_layout(layout), int(backward),
          _stream())

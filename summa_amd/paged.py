@@ -19,7 +19,7 @@ import torch
 
 from . import _lib
 from ._lib import SM_BF16, SM_F8E4M3, SM_F16, SM_F32, call
-from .ops import _on_current, _rope_angles, _rope_layout, _stream
+from .ops import _head_rows, _on_current, _rope_angles, _rope_layout, _stream
 
 BLOCK = 16  # tokens of a cache block and of a scale
 _CACHE = {torch.bfloat16: SM_BF16, torch.float16: SM_F16, torch.float8_e4m3fn: SM_F8E4M3}
@@ -84,7 +84,7 @@ class PagedKVCache:
                 raise ValueError(f"{name} must be contiguous")
         self.k, self.v, self.k_scales, self.v_scales = k, v, ks, vs
         self.pages, self.kv_heads, self.page_tokens, self.head_dim = k.shape
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self.index = k.dtype, k.device, k.get_device()
         self._c = _lib.PagedCache(k.data_ptr(), v.data_ptr(), ks.data_ptr() if ks is not None else 0,
                                   vs.data_ptr() if vs is not None else 0, self.pages,
                                   self.kv_heads, self.page_tokens, self.head_dim,
@@ -98,44 +98,47 @@ class PagedKVCache:
         return sum(t.numel() * t.element_size() for t in tensors)
 
 
-def _heads(t: torch.Tensor, name: str, hd: int, device) -> int:
-    """Row stride of [rows, heads, head_dim] rows whose heads lie side by side."""
-    if t.dim() != 3 or t.shape[2] != hd or t.stride(2) != 1 or \
-            (t.shape[1] > 1 and t.stride(1) != hd):
-        raise ValueError(f"{name} must be [rows, heads, {hd}] with contiguous heads")
-    if t.device != device:
+def _rows(cache, t: torch.Tensor, name: str):
+    """(rows, heads, row stride) of checked [rows, heads, head_dim] rows."""
+    rows, heads, hd, ld = _head_rows(t, name)
+    if hd != cache.head_dim:
+        raise ValueError(f"{name} must be [rows, heads, {cache.head_dim}]")
+    if t.get_device() != cache.index:
         raise ValueError(f"{name} must be on the cache's device")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * hd
+    return rows, heads, ld
 
 
-def _out(out, shape, dtype, device) -> torch.Tensor:
+def _out(cache, out, rows, heads, dtype) -> torch.Tensor:
+    hd = cache.head_dim
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if tuple(out.shape) != shape or out.dtype != dtype or out.device != device or \
-            not out.is_contiguous():
-        raise ValueError(f"out must be contiguous {list(shape)} {dtype} on the cache's device")
+        return torch.empty_strided((rows, heads, hd), (heads * hd, hd, 1), dtype=dtype,
+                                   device=cache.device)
+    if out.shape != (rows, heads, hd) or out.dtype is not dtype or not out.is_contiguous() or \
+            out.get_device() != cache.index:
+        raise ValueError(f"out must be contiguous [{rows}, {heads}, {hd}] {dtype} on the cache's "
+                         "device")
     return out
 
 
 def _batch(cache, rows, block_table, pos0, row_start, max_rows):
     """(sequences, columns, row_start pointer, max_rows) of a checked batch."""
+    index = cache.index
+    _on_current(index)
     if block_table.dim() != 2 or not block_table.is_contiguous():
         raise ValueError("block_table must be contiguous [sequences, columns]")
     S, cols = block_table.shape
     if pos0.shape != (S,) or not pos0.is_contiguous():
         raise ValueError("pos0 must be contiguous [sequences]")
-    dev, i32 = cache.device, torch.int32
-    _on_current(dev)
-    if block_table.dtype != i32 or pos0.dtype != i32:
+    if block_table.dtype is not torch.int32 or pos0.dtype is not torch.int32:
         raise TypeError("block_table and pos0 must be int32")
-    if block_table.device != dev or pos0.device != dev:
+    if block_table.get_device() != index or pos0.get_device() != index:
         raise ValueError("block_table and pos0 must be on the cache's device")
     if row_start is None:
         if S and rows % S:
             raise ValueError("without row_start every sequence has rows / sequences rows")
         return S, cols, None, rows // S if S else 0
-    if row_start.dtype != i32 or row_start.shape != (S + 1,) or not row_start.is_contiguous() \
-            or row_start.device != dev:
+    if row_start.dtype is not torch.int32 or row_start.shape != (S + 1,) or \
+            not row_start.is_contiguous() or row_start.get_device() != index:
         raise ValueError("row_start must be int32 [sequences + 1] on the cache's device")
     if max_rows is None:
         raise ValueError("row_start needs max_rows")
@@ -155,22 +158,19 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
     cache's 16-bit type, or that of ``q``, or float16), in ``out`` where given; rows of no
     sequence are not written. (project_qkv + slice_assign,
     summa-llm/src/model/attention.rs:142-177, 331-356.)"""
-    hd = cache.head_dim
-    ldk, ldv = _heads(k, "k", hd, cache.device), _heads(v, "v", hd, cache.device)
-    rows = k.shape[0]
-    if k.shape[1] != cache.kv_heads or v.shape != k.shape:
-        raise ValueError(f"k and v must be [rows, {cache.kv_heads}, {hd}]")
+    rows, heads, ldk = _rows(cache, k, "k")
+    _, _, ldv = _rows(cache, v, "v")
+    if heads != cache.kv_heads or v.shape != k.shape:
+        raise ValueError(f"k and v must be [rows, {cache.kv_heads}, {cache.head_dim}]")
     dt = _ROWS.get(k.dtype)
-    if dt is None or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+    if dt is None or v.dtype is not k.dtype or (q is not None and q.dtype is not k.dtype):
         raise TypeError("q, k and v must be float32, bfloat16 or float16, of one dtype")
     S, cols, starts, most = _batch(cache, rows, block_table, pos0, row_start, max_rows)
     H = ldq = 0
-    qd = SM_F16
-    if q is None and out is not None:
-        raise ValueError("out is for the queries: q is needed")
+    qd, at_q, at_out = SM_F16, None, None
     if q is not None:
-        ldq, H = _heads(q, "q", hd, cache.device), q.shape[1]
-        if q.shape[0] != rows:
+        q_rows, H, ldq = _rows(cache, q, "q")
+        if q_rows != rows:
             raise ValueError("q must have the rows of k")
         if out is not None:
             if q_dtype not in (None, out.dtype):
@@ -179,15 +179,17 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
         elif q_dtype is None:
             q_dtype = cache.dtype if cache.dtype.itemsize == 2 else \
                 q.dtype if q.dtype.itemsize == 2 else torch.float16
-        if q_dtype not in (torch.bfloat16, torch.float16):
+        if q_dtype is not torch.bfloat16 and q_dtype is not torch.float16:
             raise TypeError("q_dtype must be bfloat16 or float16")
         qd = _ROWS[q_dtype]
-        out = _out(out, (rows, H, hd), q_dtype, cache.device)
-    table, table_rows, rot = _rope_angles(rope_table, cache.device)
+        out = _out(cache, out, rows, H, q_dtype)
+        at_q, at_out = q.data_ptr(), out.data_ptr()
+    elif out is not None:
+        raise ValueError("out is for the queries: q is needed")
+    table, table_rows, rot = _rope_angles(rope_table, cache.index)
     call("sm_paged_append", cache._at, block_table.data_ptr(), cols, pos0.data_ptr(), starts, S,
-         rows, most, None if q is None else q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(),
-         ldv, dt, H, table, table_rows, rot, _rope_layout(layout),
-         None if out is None else out.data_ptr(), qd, _stream())
+         rows, most, at_q, ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, dt, H, table, table_rows,
+         rot, _rope_layout(layout), at_out, qd, _stream())
     return out
 
 
@@ -202,23 +204,22 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_table: torch.Ten
     included (default: what the block table can hold); it decides how the keys are
     split, not which are read. (forward_cached / sdpa,
     summa-llm/src/model/attention.rs:216-265, 318-371.)"""
-    hd = cache.head_dim
-    ldq = _heads(q, "q", hd, cache.device)
-    rows, H = q.shape[:2]
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    rows, H, ldq = _rows(cache, q, "q")
+    dt = _ROWS.get(q.dtype)
+    if dt is None or dt == SM_F32:
         raise TypeError("q must be bfloat16 or float16")
     S, cols, starts, most = _batch(cache, rows, block_table, pos0, row_start, max_rows)
     if max_tokens is None:
         max_tokens = min(cols * cache.page_tokens, 0x7fffffff)
-    nbytes = _lib.lib().sm_paged_attention_workspace_bytes(S, rows, most, H, cache.kv_heads, hd,
-                                                           max_tokens)
+    nbytes = _lib.lib().sm_paged_attention_workspace_bytes(S, rows, most, H, cache.kv_heads,
+                                                           cache.head_dim, max_tokens)
     if nbytes < 0:
         raise _lib.SummaError(-1, _lib.lib().sm_last_error().decode())
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    out = _out(out, (rows, H, hd), q.dtype, cache.device)
-    lse = torch.empty((rows, H), dtype=torch.float32, device=q.device) if want_lse else None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None
+    out = _out(cache, out, rows, H, q.dtype)
+    lse = torch.empty((rows, H), dtype=torch.float32, device=cache.device) if want_lse else None
     call("sm_paged_attention", cache._at, block_table.data_ptr(), cols, pos0.data_ptr(), starts,
-         S, rows, most, max_tokens, q.data_ptr(), _ROWS[q.dtype], ldq, H, out.data_ptr(),
+         S, rows, most, max_tokens, q.data_ptr(), dt, ldq, H, out.data_ptr(),
          None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
          _stream())
     return (out, lse) if want_lse else out
