@@ -428,7 +428,8 @@ int sm_attention_backward(const float* q, const float* k, const float* v, const 
  *   rotated where they lie; y == x (with ldy == ldx) is allowed, other overlaps are
  *   not. dtype SM_F32, SM_BF16 or SM_F16 (f32 arithmetic, one rounding); head_dim a
  *   multiple of 16 up to 1024, rot_dim a multiple of 16 up to head_dim; rows, x, y and
- *   table 16-byte aligned. A position outside [0, table_rows) gives NaN.
+ *   table 16-byte aligned. A position outside [0, table_rows) gives NaN;
+ *   table_rows > 0.
  */
 enum { SM_ROPE_INTERLEAVED = 0, SM_ROPE_HALF = 1 };
 enum {
@@ -464,15 +465,16 @@ int sm_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, const f
  * the sequence's tokens j page_tokens ..; pos0 [S] the tokens it holds before the call;
  * its new rows are row_start[s] .. row_start[s + 1] - 1 (row_start [S + 1] int32), or,
  * with row_start NULL, max_rows each (rows = S * max_rows). Row i of a sequence is at
- * position pos0[s] + i. No sequence may have more than max_rows rows: what it has more is
- * not processed. Rows that belong to no sequence are left as they are.
+ * position pos0[s] + i. What a sequence has beyond max_rows rows is not processed, and
+ * rows that belong to no sequence are left as they are. The grid is sized for max_rows
+ * rows of every sequence: it should be the longest's.
  *
  * sm_paged_append: k and v rows [rows, kv_heads, head_dim] (ldk, ldv values apart) of
  *   `dtype` (SM_F32, SM_BF16, SM_F16) into the pages at their positions, k rotated by
- *   rope_table [rope_rows, rot_dim / 2, 2] (as sm_rope; NULL: no rotation), and q rows
+ *   rope_table [rope_rows, rot_dim / 2, 2] (as sm_rope; NULL with rot_dim 0: none), and q rows
  *   [rows, H, head_dim] (nullable) rotated into q_out [rows, H, head_dim] of q_dtype
- *   (SM_BF16 or SM_F16), which must not overlap q. Rotation in f32, one rounding to the
- *   cache's type. (project_qkv + slice_assign, attention.rs:142-177, 331-356.)
+ *   (SM_BF16 or SM_F16), which must not overlap q, k or v. Rotation in f32, one rounding
+ *   to the cache's type; a position outside the table gives NaN. (project_qkv + slice_assign, attention.rs:142-177, 331-356.)
  *   8-bit: a block's scale is the least 2^e, e >= -63, with every finite value of the
  *   block within 448 * 2^e; it never falls while earlier tokens of the block stay, and
  *   where a later token raises it their codes are scaled down and rounded again, which

@@ -154,19 +154,9 @@ struct Append {
   __device__ inline void angles() {
     turn = 8 * (lane % LPT) < a.rot;
 #pragma unroll
-    for (int j = 0; j < TPL; ++j) {  // (tokens that are not the call's read some row too)
-      const int64_t pos = base + token(lane, j);
-      const bool in = pos < a.rope_rows;
-      const float4* p = reinterpret_cast<const float4*>(
-          a.rope + ((in ? pos : 0) * (a.rot / 2) + (turn ? 4 * (lane % LPT) : 0)) * 2);
-      const float4 u = p[0], w = p[1];
-      const float f[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        cs[j][i] = in ? f[2 * i] : NAN;
-        sn[j][i] = in ? f[2 * i + 1] : NAN;
-      }
-    }
+    for (int j = 0; j < TPL; ++j)  // (dims and tokens that are not to be rotated read some too)
+      load_angles<4>(a.rope, a.rope_rows, a.rot / 2, base + token(lane, j),
+                     turn ? 4 * (lane % LPT) : 0, cs[j], sn[j]);
   }
   // a query's or key's head
   __device__ inline void load_row(const void* p, int64_t ld, int head) {
@@ -447,10 +437,14 @@ extern "C" int sm_paged_append(const sm_paged_cache* cache, const int32_t* block
                  (!q || (ldq >= H * hd && ldq % each == 0)),
              "%s: rows must be 16-byte aligned and hold their heads", me);
   if (q) {
-    const uintptr_t qa = reinterpret_cast<uintptr_t>(q), oa = reinterpret_cast<uintptr_t>(q_out);
-    SM_REQUIRE(qa + (size_t)(((rows - 1) * ldq + H * hd) * (16 / each)) <= oa ||
-                   oa + (size_t)(rows * H * hd * 2) <= qa,
-               "%s: q_out must not overlap q", me);
+    const size_t size = 16 / each;
+    const uintptr_t o0 = reinterpret_cast<uintptr_t>(q_out), o1 = o0 + (size_t)(rows * H * hd * 2);
+    auto apart = [&](const void* p, int64_t ld, int64_t width) {
+      const uintptr_t a0 = reinterpret_cast<uintptr_t>(p);
+      return a0 + (size_t)((rows - 1) * ld + width) * size <= o0 || o1 <= a0;
+    };
+    SM_REQUIRE(apart(q, ldq, H * hd) && apart(k, ldk, KVH * hd) && apart(v, ldv, KVH * hd),
+               "%s: q_out must not overlap q, k or v", me);
   }
   for (const void* p : {k, v, q, (const void*)q_out})
     SM_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "%s: buffers must be 16-byte aligned", me);

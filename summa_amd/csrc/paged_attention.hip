@@ -6,7 +6,6 @@
 #include "attn_common.hpp"
 #include "common.hpp"
 #include "paged_map.hpp"
-#include "prefill_map.hpp"
 
 namespace sm {
 namespace {
@@ -20,6 +19,7 @@ struct PagedArgs {
   float* lse;
   float *part_o, *part_ml;       // per (row, head, split): unnormalised O; (max, sum)
   int64_t ldq;
+  PagedMap map;                  // of paged_tile_kernel
   Divide H, KVH, G, bpp, nsplit, tiles, rows_each, tile;
   int S, rows, max_rows, pages, cols, cb;
   float c2;                      // log2(e) / sqrt(hd)
@@ -647,9 +647,8 @@ template <int HD, bool QF16, bool C8>
 __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
   typedef TileSweep<HD, QF16, C8> T;
   __shared__ typename T::Lds lds;
-  const PrefillMap map((uint32_t)a.S * a.KVH.d * a.nsplit.d, a.tiles.d);
   uint32_t grp, place;
-  if (!map.at(blockIdx.x, grp, place)) return;  // (uniform)
+  if (!a.map.at(blockIdx.x, grp, place)) return;  // (uniform)
   int s = (int)grp;
   const int split = a.nsplit.mod(s), kvh = a.KVH.mod(s);
   const int tile = (int)a.tiles.d - 1 - (int)place;  // the rows with the most keys first
@@ -931,6 +930,11 @@ extern "C" int sm_paged_attention(const sm_paged_cache* cache, const int32_t* bl
   a.nsplit = Divide(plan.nsplit);
   a.tile = Divide(plan.tile);
   a.tiles = Divide((int)plan.tiles);
+  // the keys of a group, and whether an XCD's groups leave a quarter of its 4 MiB L2
+  const int64_t span = plan.nsplit > 1 ? (int64_t)plan.cb * kBlock : max_tokens;
+  const int64_t kv = span * hd * (cache->dtype == SM_F8E4M3 ? 2 : 4);
+  a.map = PagedMap((uint32_t)(S * KVH * plan.nsplit), (uint32_t)plan.tiles,
+                   S * KVH * plan.nsplit / 8 * kv <= 3 << 20);
   a.c2 = 1.44269504088896340736f / sqrtf((float)hd);
   const bool f16 = dtype == SM_F16, c8 = cache->dtype == SM_F8E4M3;
 #define SM_PAGED2(HD, F, C)                                                      \

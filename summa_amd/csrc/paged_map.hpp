@@ -6,6 +6,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include "prefill_map.hpp"
+
 namespace sm {
 
 constexpr int kBlock = 16;  // tokens of a cache block (and of a scale)
@@ -89,6 +91,37 @@ struct PagedKeys {
   __host__ __device__ int begin(int split, int cb) const { return split * cb; }
   __host__ __device__ int end(int split, int cb) const {
     return split + 1 >= splits ? blocks : (split + 1) * cb;
+  }
+};
+
+// Which workgroup takes which (KV head of a sequence's split) and row tile: PrefillMap's
+// share of groups for every XCD, whose L2 then reads a group's K and V once, but
+// - the eight groups of a set go to the XCDs in another turn in each set, so that a long
+//   sequence's KV heads and a short one's do not meet the same XCDs every time, and
+// - with by_place, where the K and V of all an XCD's groups stay in its L2, every group's
+//   tile with the most keys comes before any group's next, and what runs last is short.
+// Prefill of 32 prompts of 257-512 tokens, 4 KV heads: 58.6 -> 57.2 us with the turns,
+// 52.4 with both.
+struct PagedMap {
+  PrefillMap map;
+  Divide per, sets;
+  bool by_place;
+  PagedMap() : map(1, 1), by_place(false) {}
+  __host__ __device__ PagedMap(uint32_t groups, uint32_t per_, bool by_place_)
+      : map(groups, per_), per((int)per_), sets((int)(groups / 8 ? groups / 8 : 1)),
+        by_place(by_place_) {}
+  __host__ __device__ bool at(uint32_t wg, uint32_t& group, uint32_t& place) const {
+    int set = (int)(wg / 8);
+    if (set >= (int)(map.whole / 8 * map.per)) return map.at(wg, group, place);
+    if (by_place) {
+      const int s = sets.mod(set);
+      place = (uint32_t)set;
+      set = s;
+    } else {
+      place = (uint32_t)per.mod(set);
+    }
+    group = (uint32_t)set * 8 + (wg + 3 * (uint32_t)set) % 8;
+    return true;
   }
 };
 

@@ -61,28 +61,40 @@ __global__ __launch_bounds__(256) void rope_kernel(const T* x, int64_t ldx,
   constexpr int N = HALF ? 8 : 4;
   float c0[N], s0[N], c1[4], s1[4];
   const int64_t pos = positions[row];
-  if (turn0) load_angles<N>(table, table_rows, half, pos, HALF ? d0 : d0 / 2, c0, s0);
-  if (!HALF && turn1) load_angles<4>(table, table_rows, half, pos, d1 / 2, c1, s1);
+  // (dims that are not rotated read the first pairs' angles and do not use them)
+  load_angles<N>(table, table_rows, half, pos, !turn0 ? 0 : HALF ? d0 : d0 / 2, c0, s0);
+  if (!HALF) load_angles<4>(table, table_rows, half, pos, turn1 ? d1 / 2 : 0, c1, s1);
   const T* xr = x + row * ldx;
   T* yr = y + row * ldy;
-  for (int h = h0; h < heads; h += hpp) {
-    float a[8], b[8];
-    load8<T>(xr + (int64_t)h * hd + d0, a);
-    load8<T>(xr + (int64_t)h * hd + d1, b);
-    if constexpr (HALF) {
-      if (turn0)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) rotate_pair(a[i], b[i], c0[i], s0[i] * sign);
-    } else {
-      if (turn0)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) rotate_pair(a[2 * i], a[2 * i + 1], c0[i], s0[i] * sign);
-      if (turn1)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) rotate_pair(b[2 * i], b[2 * i + 1], c1[i], s1[i] * sign);
+  for (int h = h0; h < heads; h += 2 * hpp) {  // two heads' loads in flight
+    float a[2][8], b[2][8];
+    const bool second = h + hpp < heads;
+    load8<T>(xr + (int64_t)h * hd + d0, a[0]);
+    load8<T>(xr + (int64_t)h * hd + d1, b[0]);
+    if (second) {
+      load8<T>(xr + (int64_t)(h + hpp) * hd + d0, a[1]);
+      load8<T>(xr + (int64_t)(h + hpp) * hd + d1, b[1]);
     }
-    store8<T>(yr + (int64_t)h * hd + d0, a);
-    store8<T>(yr + (int64_t)h * hd + d1, b);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (k && !second) break;
+      if constexpr (HALF) {
+        if (turn0)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) rotate_pair(a[k][i], b[k][i], c0[i], s0[i] * sign);
+      } else {
+        if (turn0)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            rotate_pair(a[k][2 * i], a[k][2 * i + 1], c0[i], s0[i] * sign);
+        if (turn1)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            rotate_pair(b[k][2 * i], b[k][2 * i + 1], c1[i], s1[i] * sign);
+      }
+      store8<T>(yr + (int64_t)(h + k * hpp) * hd + d0, a[k]);
+      store8<T>(yr + (int64_t)(h + k * hpp) * hd + d1, b[k]);
+    }
   }
 }
 
@@ -137,13 +149,14 @@ extern "C" int sm_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int dty
              "sm_rope: dtype must be SM_F32, SM_BF16 or SM_F16");
   SM_REQUIRE(layout == SM_ROPE_INTERLEAVED || layout == SM_ROPE_HALF,
              "sm_rope: layout must be SM_ROPE_INTERLEAVED or SM_ROPE_HALF");
-  SM_REQUIRE(rows >= 0 && rows < ((int64_t)1 << 26) && heads > 0 && heads <= 65535,
-             "sm_rope: need 0 <= rows < 2^26 and 0 < heads <= 65535");
+  // (four rows a workgroup, and a grid holds less than 2^24 workgroups of 256 threads)
+  SM_REQUIRE(rows >= 0 && rows < ((int64_t)1 << 26) - 4 && heads > 0 && heads <= 65535,
+             "sm_rope: need 0 <= rows < 2^26 - 4 and 0 < heads <= 65535");
   SM_REQUIRE(head_dim >= 16 && head_dim % 16 == 0 && head_dim <= 1024,
              "sm_rope: head_dim must be a multiple of 16 up to 1024");
   SM_REQUIRE(rot_dim >= 16 && rot_dim % 16 == 0 && rot_dim <= head_dim,
              "sm_rope: rot_dim must be a multiple of 16 up to head_dim");
-  SM_REQUIRE(table_rows >= 0, "sm_rope: bad table");
+  SM_REQUIRE(table_rows > 0, "sm_rope: the table has no rows");
   const int64_t size = dtype == SM_F32 ? 4 : 2, each = 16 / size, width = heads * head_dim;
   SM_REQUIRE(ldx >= width && ldy >= width && ldx % each == 0 && ldy % each == 0 &&
                  ldx < ((int64_t)1 << 31) && ldy < ((int64_t)1 << 31),

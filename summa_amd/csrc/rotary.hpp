@@ -59,23 +59,21 @@ __device__ inline void store8(T* p, const float (&f)[8]) {
   }
 }
 
-// (cos, sin) of N consecutive pairs at table row `pos`; NaN outside the table.
+// (cos, sin) of N consecutive pairs at table row `pos`; NaN outside the table, which has a
+// row at least. (Values are chosen, and one row is always read: stores on two paths would
+// keep c and s in memory.)
 template <int N>
 __device__ inline void load_angles(const float* table, int64_t table_rows, int half, int64_t pos,
                                    int pair, float (&c)[N], float (&s)[N]) {
-  if (pos < 0 || pos >= table_rows) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) c[i] = s[i] = NAN;
-    return;
-  }
-  const float4* p = reinterpret_cast<const float4*>(table + (pos * half + pair) * 2);
+  const bool in = pos >= 0 && pos < table_rows;
+  const float4* p = reinterpret_cast<const float4*>(table + ((in ? pos : 0) * half + pair) * 2);
 #pragma unroll
   for (int i = 0; i < N / 2; ++i) {
     const float4 v = p[i];
-    c[2 * i] = v.x;
-    s[2 * i] = v.y;
-    c[2 * i + 1] = v.z;
-    s[2 * i + 1] = v.w;
+    c[2 * i] = in ? v.x : NAN;
+    s[2 * i] = in ? v.y : NAN;
+    c[2 * i + 1] = in ? v.z : NAN;
+    s[2 * i + 1] = in ? v.w : NAN;
   }
 }
 

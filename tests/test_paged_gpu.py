@@ -522,6 +522,27 @@ def test_a_rollout(dev, cdt):
             torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("cdt", [F8, F16])
+def test_many_sequences(dev, cdt):
+    """70000 sequences of one token: more than one grid dimension's 65535. The one weight is
+    1, so the output is V as the cache holds it."""
+    from summa_amd import paged
+    S = 70000
+    cache = paged.PagedKVCache(S, 1, 64, 16, cdt, dev)
+    table = torch.randperm(S, device=dev).to(torch.int32)[:, None].contiguous()
+    zero = torch.zeros(S, dtype=torch.int32, device=dev)
+    v = torch.randint(-8, 9, (S, 1, 64), device=dev).half() / 4  # (exact in either type)
+    q = torch.randn(S, 2, 64, device=dev).half()
+    got = paged.paged_append(cache, v, v, table, zero, q=q)
+    assert torch.equal(got, q)
+    out, lse = paged.paged_attention(cache, q, table, zero, max_tokens=1, want_lse=True)
+    assert torch.equal(out, v.expand(S, 2, 64))
+    score = (q.double() * v.double()).sum(-1) / 8
+    tol = (q.double().abs() * v.double().abs()).sum(-1) / 8 * 70 * 2.0 ** -24 + 2.0 ** -21 + \
+        2.0 ** -22 * score.abs()
+    assert bool(((lse.double() - score).abs() <= tol).all())
+
+
 def test_two_calls_at_once(dev):
     """Two attention calls over one cache on two streams, each with its own workspace."""
     b = Batch(dev, [3000, 3000], [1, 1], 2, 64, 64, F8)
@@ -565,6 +586,8 @@ def test_python_refusals(dev):
         paged.paged_append(b.cache, k.transpose(1, 2), v, b.t, b.p)
     with pytest.raises(ValueError, match="rotary table"):
         paged.paged_append(b.cache, k, v, b.t, b.p, rope_table=torch.zeros(4, 8, device=dev))
+    with pytest.raises(ValueError, match="table is empty"):
+        paged.paged_append(b.cache, k, v, b.t, b.p, rope_table=torch.zeros(0, 8, 2, device=dev))
     with pytest.raises(ValueError, match="device"):
         paged.paged_append(b.cache, k.cpu(), v, b.t, b.p)
     with pytest.raises(TypeError, match="q must be"):

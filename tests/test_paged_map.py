@@ -15,6 +15,7 @@ ROOT = Path(__file__).resolve().parent.parent
 PROGRAM = r"""
 #include <cstdio>
 #include <cstdlib>
+#include <vector>
 #include "paged_map.hpp"
 using namespace sm;
 static unsigned long long z = 88172645463325252ull;
@@ -53,6 +54,41 @@ int main() {
     }
     CHECK(paged_touched(n) == most);
   }
+  // division by a known divisor
+  const int ds[] = {1, 2, 3, 5, 7, 10, 12, 48, 641, 65535, 65536, 1 << 24, 0x3fffffff, 0x40000001, 0x7fffffff};
+  for (int d : ds) {
+    const Divide by(d);
+    for (int it = 0; it < 20000; ++it) {
+      int n = it < 4 ? 0x7fffffff - it : it < 8 ? it - 4 : (int)(rnd() & 0x7fffffff) >> (it % 31);
+      CHECK(by.div(n) == n / d);
+      int q = n;
+      CHECK(by.mod(q) == n % d && q == n / d);
+    }
+  }
+  // workgroups: every (group, place) once; whole eights of groups one XCD each, every XCD
+  // every group of a set in some set
+  for (int wide = 0; wide < 2; ++wide)
+    for (uint32_t groups : {1u, 3u, 4u, 8u, 16u, 23u, 128u, 1000u})
+      for (uint32_t per : {1u, 2u, 7u, 16u, 33u}) {
+        const PagedMap map(groups, per, wide != 0);
+        std::vector<int> seen(groups * per, 0), home(groups, -1);
+        uint32_t last = 0;
+        for (long w = 0; w < map.map.workgroups(); ++w) {
+          uint32_t g, p;
+          if (!map.at((uint32_t)w, g, p)) continue;
+          CHECK(g < groups && p < per);
+          seen[g * per + p]++;
+          if (g < groups / 8 * 8) {
+            CHECK(home[g] < 0 || home[g] == w % 8);
+            home[g] = (int)(w % 8);
+            if (wide) {
+              CHECK(p >= last);
+              last = p;
+            }
+          }
+        }
+        for (int n : seen) CHECK(n == 1);
+      }
   // splits: every key block of a tile exactly once, none beyond the last key
   for (int it = 0; it < 100000; ++it) {
     const int G = 1 + rnd() % 9, n = 1 + rnd() % 40, tile = it % 2 ? 16 : 128;
@@ -148,9 +184,12 @@ def test_null_cache_refused():
     (dict(q=D, ldq=128, H=4, out=4 * D), "hold their heads"),
     (dict(q=D, ldq=256, H=4, out=4 * D, qd=_lib.SM_F32), "q_dtype must be"),
     (dict(q=D, ldq=256, H=4, out=D + 512), "must not overlap"),
-    (dict(rope=D, rot=24), "multiple of 16 up to head_dim"),
-    (dict(rope=D, rot=128), "multiple of 16 up to head_dim"),
-    (dict(rope=D, rot=32, layout=2), "layout must be"), (dict(rope=D + 4, rot=32), "rope_table must"),
+    (dict(q=D, ldq=256, H=4, out=8 * D, k=8 * D + 64), "must not overlap q, k or v"),
+    (dict(q=D, ldq=256, H=4, out=8 * D, v=8 * D - 128), "must not overlap q, k or v"),
+    (dict(rot=32), "rot_dim without"), (dict(rope=D, rot=32), "have rows"),
+    (dict(rope=D, rot=24, rope_rows=8), "multiple of 16 up to head_dim"),
+    (dict(rope=D, rot=128, rope_rows=8), "multiple of 16 up to head_dim"),
+    (dict(rope=D, rot=32, rope_rows=8, layout=2), "layout must be"), (dict(rope=D + 4, rot=32), "rope_table must"),
 ])
 def test_append_refusals(kw, msg):
     st, err = append(cache(), **kw)
@@ -207,6 +246,7 @@ def test_rope_host_refusals():
     ok = dict(x=D, ldx=128, y=2 * D, ldy=128, dt=0, t=D, tr=8, p=D, rows=4, heads=2, hd=64, rot=32,
               layout=0, back=0)
     for kw, msg in [(dict(dt=3), "dtype"), (dict(layout=5), "layout"), (dict(rows=-1), "rows"),
+                    (dict(rows=(1 << 26) - 4), "rows"), (dict(tr=0), "no rows"),
                     (dict(heads=0), "heads"), (dict(hd=72), "head_dim"), (dict(rot=8), "rot_dim"),
                     (dict(rot=80), "rot_dim"), (dict(ldx=64), "hold heads"), (dict(ldy=130), "aligned"),
                     (dict(x=D + 4), "aligned"), (dict(t=D + 8), "aligned"), (dict(y=D + 64), "overlap"),
