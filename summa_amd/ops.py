@@ -729,12 +729,14 @@ def _rope_layout(layout: str) -> int:
         raise ValueError("layout must be 'interleaved' or 'half'") from e
 
 
-def _on_current(index: int) -> None:
-    """The library launches on the current device's stream."""
+def _stream_on(index: int) -> int:
+    """The current stream of device ``index``, which must be the current device: the library
+    launches there."""
     if index < 0:
         raise ValueError("tensors must be on the device")
     if index != torch._C._cuda_getDevice():
         raise ValueError(f"tensors are on device {index}, which is not the current device")
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _head_rows(t: torch.Tensor, name: str):
@@ -776,10 +778,10 @@ def rope_table(positions: int, rot_dim: int, theta: float = 1e4, *, scaling: str
     if positions < 0 or rot_dim <= 0 or rot_dim % 2:
         raise ValueError("need positions >= 0 and an even rot_dim > 0")
     t = torch.empty(positions, rot_dim // 2, 2, dtype=torch.float32, device=device)
-    _on_current(t.get_device())
+    stream = _stream_on(t.get_device())
     call("sm_rope_table", float(theta), rot_dim, positions, _ROPE_SCALINGS[scaling], float(factor),
          float(original_positions), float(low_turns), float(high_turns), float(magnitude),
-         t.data_ptr(), _stream())
+         t.data_ptr(), stream)
     return t
 
 
@@ -793,7 +795,7 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
     (``sm_rope``; attention.rs:142-177)."""
     rows, heads, hd, ldx = _head_rows(x, "x")
     dt, index = _dt(x), x.get_device()
-    _on_current(index)
+    stream = _stream_on(index)
     if positions.dtype is not torch.int32 or positions.shape != (rows,) or \
             not positions.is_contiguous() or positions.get_device() != index:
         raise ValueError("positions must be contiguous int32 [rows] on x's device")
@@ -807,7 +809,7 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
         ldy = _head_rows(out, "out")[3]
     call("sm_rope", x.data_ptr(), ldx, out.data_ptr(), ldy, dt, at, table_rows,
          positions.data_ptr(), rows, heads, hd, rot, _rope_layout(layout), int(backward),
-         _stream())
+         stream)
     return out
 
 

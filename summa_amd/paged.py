@@ -19,7 +19,7 @@ import torch
 
 from . import _lib
 from ._lib import SM_BF16, SM_F8E4M3, SM_F16, SM_F32, call
-from .ops import _head_rows, _on_current, _rope_angles, _rope_layout, _stream
+from .ops import _head_rows, _rope_angles, _rope_layout, _stream_on
 
 BLOCK = 16  # tokens of a cache block and of a scale
 _CACHE = {torch.bfloat16: SM_BF16, torch.float16: SM_F16, torch.float8_e4m3fn: SM_F8E4M3}
@@ -121,9 +121,9 @@ def _out(cache, out, rows, heads, dtype) -> torch.Tensor:
 
 
 def _batch(cache, rows, block_table, pos0, row_start, max_rows):
-    """(sequences, columns, row_start pointer, max_rows) of a checked batch."""
+    """(stream, sequences, columns, row_start pointer, max_rows) of a checked batch."""
     index = cache.index
-    _on_current(index)
+    stream = _stream_on(index)
     if block_table.dim() != 2 or not block_table.is_contiguous():
         raise ValueError("block_table must be contiguous [sequences, columns]")
     S, cols = block_table.shape
@@ -136,13 +136,13 @@ def _batch(cache, rows, block_table, pos0, row_start, max_rows):
     if row_start is None:
         if S and rows % S:
             raise ValueError("without row_start every sequence has rows / sequences rows")
-        return S, cols, None, rows // S if S else 0
+        return stream, S, cols, None, rows // S if S else 0
     if row_start.dtype is not torch.int32 or row_start.shape != (S + 1,) or \
             not row_start.is_contiguous() or row_start.get_device() != index:
         raise ValueError("row_start must be int32 [sequences + 1] on the cache's device")
     if max_rows is None:
         raise ValueError("row_start needs max_rows")
-    return S, cols, row_start.data_ptr(), min(int(max_rows), rows)
+    return stream, S, cols, row_start.data_ptr(), min(int(max_rows), rows)
 
 
 def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
@@ -165,7 +165,7 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
     dt = _ROWS.get(k.dtype)
     if dt is None or v.dtype is not k.dtype or (q is not None and q.dtype is not k.dtype):
         raise TypeError("q, k and v must be float32, bfloat16 or float16, of one dtype")
-    S, cols, starts, most = _batch(cache, rows, block_table, pos0, row_start, max_rows)
+    stream, S, cols, starts, most = _batch(cache, rows, block_table, pos0, row_start, max_rows)
     H = ldq = 0
     qd, at_q, at_out = SM_F16, None, None
     if q is not None:
@@ -189,7 +189,7 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
     table, table_rows, rot = _rope_angles(rope_table, cache.index)
     call("sm_paged_append", cache._at, block_table.data_ptr(), cols, pos0.data_ptr(), starts, S,
          rows, most, at_q, ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, dt, H, table, table_rows,
-         rot, _rope_layout(layout), at_out, qd, _stream())
+         rot, _rope_layout(layout), at_out, qd, stream)
     return out
 
 
@@ -208,18 +208,21 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_table: torch.Ten
     dt = _ROWS.get(q.dtype)
     if dt is None or dt == SM_F32:
         raise TypeError("q must be bfloat16 or float16")
-    S, cols, starts, most = _batch(cache, rows, block_table, pos0, row_start, max_rows)
+    stream, S, cols, starts, most = _batch(cache, rows, block_table, pos0, row_start, max_rows)
     if max_tokens is None:
         max_tokens = min(cols * cache.page_tokens, 0x7fffffff)
-    nbytes = _lib.lib().sm_paged_attention_workspace_bytes(S, rows, most, H, cache.kv_heads,
-                                                           cache.head_dim, max_tokens)
-    if nbytes < 0:
-        raise _lib.SummaError(-1, _lib.lib().sm_last_error().decode())
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None
+    nbytes, ws = 0, None
+    if max_tokens > 256:  # (none for fewer)
+        nbytes = _lib.lib().sm_paged_attention_workspace_bytes(S, rows, most, H, cache.kv_heads,
+                                                               cache.head_dim, max_tokens)
+        if nbytes < 0:
+            raise _lib.SummaError(-1, _lib.lib().sm_last_error().decode())
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device)
     out = _out(cache, out, rows, H, q.dtype)
     lse = torch.empty((rows, H), dtype=torch.float32, device=cache.device) if want_lse else None
     call("sm_paged_attention", cache._at, block_table.data_ptr(), cols, pos0.data_ptr(), starts,
          S, rows, most, max_tokens, q.data_ptr(), dt, ldq, H, out.data_ptr(),
          None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
-         _stream())
+         stream)
     return (out, lse) if want_lse else out
