@@ -494,7 +494,7 @@ int sm_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, const f
  *   max_tokens: the tokens of the longest sequence, new rows included; it only decides
  *   how the keys are split, a longer sequence is still attended to in full.
  *   workspace: sm_paged_attention_workspace_bytes(...) bytes (-1 for a bad shape; 0 where
- *   the keys are not split, so always for max_tokens <= 256), 16-byte aligned, for the
+ *   the keys are not split, so always for max_tokens <= 512), 16-byte aligned, for the
  *   partial sums of the splits; calls that share one must not overlap.
  * Every length is read on the device, so a captured call may be replayed with other
  * contents of the batch's arrays, up to max_rows.

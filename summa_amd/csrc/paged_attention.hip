@@ -732,6 +732,25 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
   }
 }
 
+// acc += the sums of N splits, all on their way at once, each times its weight: lane x + k
+// holds that of split k.
+template <int HD, int N>
+__device__ inline void add_splits(const float* po, float weight, int x, int lane,
+                                  float (&acc)[HD / kWave]) {
+  constexpr int D = HD / kWave;
+  float y[N][D];
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+#pragma unroll
+    for (int d = 0; d < D; ++d) y[k][d] = po[(size_t)k * HD + lane * D + d];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float w = lane_f32(weight, x + k);
+#pragma unroll
+    for (int d = 0; d < D; ++d) acc[d] = fmaf(y[k][d], w, acc[d]);
+  }
+}
+
 // Joins the splits of a (row, head): one wave each.
 template <int HD, bool QF16>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
@@ -762,22 +781,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     // (a split without visible keys has the maximum -inf and the sum 0)
     const float f = v.x == -INFINITY ? (v.y == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(v.x - mm);
     ll += wave_sum(v.y * f);
-    for (int x = 0; x < n; x += 8) {  // eight splits' sums in flight
-      float y[8][D];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float* p = po + (size_t)(x0 + min(x + k, n - 1)) * HD + lane * D;
-#pragma unroll
-        for (int d = 0; d < D; ++d) y[k][d] = p[d];
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float w = x + k < n ? lane_f32(f, min(x + k, n - 1)) : 0.f;
-#pragma unroll
-        for (int d = 0; d < D; ++d)
-          if (x + k < n) acc[d] = fmaf(y[k][d], w, acc[d]);
-      }
-    }
+    int x = 0;
+    for (; x + 32 <= n; x += 32) add_splits<HD, 32>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
+    for (; x + 8 <= n; x += 8) add_splits<HD, 8>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
+    for (; x + 2 <= n; x += 2) add_splits<HD, 2>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
+    if (x < n) add_splits<HD, 1>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
   }
   const bool none = pos0 + i < 0;
   const float inv = 1.f / ll;
@@ -803,7 +811,7 @@ struct PagedPlan {
     const int64_t units = std::max<int64_t>(1, S * tiles * KVH);
     const int64_t blocks = std::max<int64_t>(1, ceil_div(max_tokens, kBlock));
     const int64_t want = std::max<int64_t>(1, ceil_div(tile == kRows16 ? 1024 : 512, units));
-    cb = (int)(ceil_div(std::max<int64_t>(16, ceil_div(blocks, want)), 16) * 16);
+    cb = (int)(ceil_div(std::max<int64_t>(32, ceil_div(blocks, want)), 16) * 16);
     nsplit = (int)ceil_div(blocks, cb);
     wgs = tile == kRows16 ? S * tiles * KVH * nsplit
                           : PrefillMap((uint32_t)(S * KVH * nsplit), (uint32_t)tiles).workgroups();

@@ -212,7 +212,7 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_table: torch.Ten
     if max_tokens is None:
         max_tokens = min(cols * cache.page_tokens, 0x7fffffff)
     nbytes, ws = 0, None
-    if max_tokens > 256:  # (none for fewer)
+    if max_tokens > 512:  # (none for fewer)
         nbytes = _lib.lib().sm_paged_attention_workspace_bytes(S, rows, most, H, cache.kv_heads,
                                                                cache.head_dim, max_tokens)
         if nbytes < 0:
