@@ -1,5 +1,26 @@
 // Attention over a paged KV cache, 16-bit or 8-bit (e4m3 codes with a power-of-two
-// scale per 16 tokens of a head). See sm_paged_attention for the layouts.
+// scale per 16 tokens of a head); sm_paged_attention states the layouts.
+//
+//   MultiHeadAttention::forward_cached / sdpa (summa-llm/src/model/attention.rs:216-265,
+//   318-371): softmax(q . K^T / sqrt(hd)) . V over the keys up to the query's position.
+//
+// A row here is a (token, query head of a KV head's group) pair: the rows of a KV head see
+// the same keys, so its K and V are read once for G tokens' heads as for G heads of a token.
+//
+// Both kernels work on transposed scores, S^T = K Q^T, so that a lane owns one row and its
+// scores are, as they come out of the matrix cores, the B operand of O^T += V^T P^T: the sum
+// over keys may run in any order, and V is stored in that order. P never leaves the
+// registers, and nothing is transposed on the way.
+// - The softmax is one pass with a running maximum and sum in f32, in units of log2. The
+//   maximum is raised only when a score passes it by more than 8 (weights then reach 2^8, far
+//   from f16's 65504), so most steps neither reduce over lanes nor rescale O.
+// - An 8-bit block's K scale is a factor on its scores. Its V scale 2^e goes into the weights:
+//   t = score + e is what the running maximum is taken of, P' = 2^(t - max) multiplies the bare
+//   codes, and the sum gets 2^-e P' back. P' is at most 2^8 whatever the scales are, and a
+//   block with small values loses no accuracy to one with large ones.
+// - P' is rounded to f16 for 8-bit and f16 values (codes are exact in f16), to bf16 for bf16
+//   ones, whose range f16 does not hold: at most half a step (2^-11, 2^-8) of each weight,
+//   like the one rounding of the output. Scores, maxima, sums and O stay in f32.
 #include <algorithm>
 #include <cmath>
 
@@ -132,6 +153,16 @@ struct Blocks {
   }
 };
 
+// ---- up to 16 query rows a KV head: bound by reading K and V ----
+//
+// One workgroup per (split of the keys, KV head, sequence). Its four waves take steps of two
+// 16-key blocks in turn and meet in LDS at the end. K and V go from memory into the registers
+// as the matrix cores take them, 16 bytes a lane and load; 8-bit codes are converted there
+// (one instruction for two). v_mfma_f32_16x16x32: a score tile is 16 keys x 16 rows.
+// 256 sequences of 512-1023 tokens, 16 / 4 heads of 128, e4m3 (202 MB): 41 us, 4.9 TB/s; 4 of
+// 100-131 k (483 MB): 92 us, 5.2; 48 x 4 rows of 1-4 k, 16 heads, bf16 (1.08 GB): 204 us, 5.3,
+// where a copy on this card moves 4.9. Two blocks a step beside four: the same time with 40
+// registers fewer; four workgroups a unit (128 registers): no faster.
 constexpr int kRows16 = 16;  // query rows of a workgroup
 
 template <int HD, bool QF16, bool C8>
@@ -362,7 +393,18 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
     a.lse[at] = none ? -INFINITY : (mm + __log2f(ll)) * 0.69314718055994530942f;
 }
 
-// ---- many query rows: 128 of them a workgroup, keys staged through LDS ----
+// ---- more query rows: 128 of them a workgroup, keys staged through LDS ----
+//
+// Four waves x 32 rows (v_mfma_f32_32x32x16), two workgroups a unit. A tile of 64 keys, in
+// 16 bits, sits in one of two LDS buffers; the next tile's loads go out before this one's
+// products and are converted and stored after them, one barrier a tile.
+// 2 x 1024 tokens on 24-32 k keys, 16 / 4 heads of 128, f16 queries, e4m3: 0.56 ms, 0.92 PF/s,
+// 78 % of what a large f16 product reaches here; the clock is down to 1.9 GHz then, the matrix
+// cores work 41 % and the vector units 47 % of the cycles. Prefill of 32 prompts of 257-512:
+// 47 us: 1.75 us a tile and 5.6 us a workgroup for two round trips to memory and its output.
+// Tried and slower: scores of the next tile beside this one's softmax on 32-key tiles (670
+// beside 637 us at the time), three workgroups a unit (618 beside 583), workgroups that go
+// on to further row tiles with their first loads in flight (prefill 65 beside 50 us).
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <bool F16>
@@ -753,7 +795,7 @@ __device__ inline void add_splits(const float* po, float weight, int x, int lane
 
 // Joins the splits of a (row, head): one wave each.
 template <int HD, bool QF16>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, 8) void paged_join_kernel(PagedArgs a) {
   int s = (int)(blockIdx.x * 4 + threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const int head = a.H.mod(s), i = a.rows_each.mod(s);
@@ -782,7 +824,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     const float f = v.x == -INFINITY ? (v.y == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(v.x - mm);
     ll += wave_sum(v.y * f);
     int x = 0;
-    for (; x + 32 <= n; x += 32) add_splits<HD, 32>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
+    for (; x + 16 <= n; x += 16) add_splits<HD, 16>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
     for (; x + 8 <= n; x += 8) add_splits<HD, 8>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
     for (; x + 2 <= n; x += 2) add_splits<HD, 2>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
     if (x < n) add_splits<HD, 1>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
@@ -801,7 +843,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     a.lse[at] = none ? -INFINITY : (mm + __log2f(ll)) * 0.69314718055994530942f;
 }
 
-// How a call is split: rows of a tile, key blocks of a split and splits.
+// How a call is split: rows of a workgroup, key blocks of a split and splits.
+// - 16 rows or fewer a KV head take the 16-row kernel: 32 sequences of 2000 keys, 4 heads to
+//   each of 4 KV heads, e4m3, one token 17.2 us beside 21.1 on the 128-row kernel, 4 tokens 19.6
+//   beside 21.9; with 5, two 16-row workgroups 20.8 beside 22.5, but 8 tokens of 60000 keys 46.6
+//   beside 37.2.
+// - Keys are split where there are too few workgroups otherwise, to 1024 (four a unit) or 512
+//   (two): 256 sequences x 4 KV heads, already 1024, take 41 us whole and 50 in halves.
+// - A split has 512 keys at least, for its share of the join: 64 sequences of 300 keys take
+//   8.4 us whole and 13.4 in two (16 rows), 13 and 27 (64 rows).
 struct PagedPlan {
   int tile, cb, nsplit;
   int64_t tiles, wgs;
