@@ -457,7 +457,8 @@ int sm_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, const f
  *   with T = 4 (8-bit) or 2 (16-bit): four tokens' values of one dim lie together, as
  *   the matrix cores take them.
  * k_scales, v_scales (SM_F8E4M3; else ignored) [pages, kv_heads, page_tokens / 16]: the
- *   exponent + 127; a stored code c stands for c * 2^(scale - 127).
+ *   exponent + 127; a stored code c stands for c * 2^(scale - 127). The append writes 64 to
+ *   247; attention takes those.
  * dtype SM_BF16, SM_F16 or SM_F8E4M3; head_dim 64 or 128; page_tokens a multiple of 16;
  * k and v 16-byte aligned; fewer than 2^31 blocks in all.
  *
@@ -465,7 +466,7 @@ int sm_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, const f
  * the sequence's tokens j page_tokens ..; pos0 [S] the tokens it holds before the call;
  * its new rows are row_start[s] .. row_start[s + 1] - 1 (row_start [S + 1] int32), or,
  * with row_start NULL, max_rows each (rows = S * max_rows). Row i of a sequence is at
- * position pos0[s] + i. What a sequence has beyond max_rows rows is not processed, and
+ * position pos0[s] + i, below 2^31. What a sequence has beyond max_rows rows is not processed, and
  * rows that belong to no sequence are left as they are. The grid is sized for max_rows
  * rows of every sequence: it should be the longest's.
  *
@@ -474,7 +475,8 @@ int sm_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, const f
  *   rope_table [rope_rows, rot_dim / 2, 2] (as sm_rope; NULL with rot_dim 0: none), and q rows
  *   [rows, H, head_dim] (nullable) rotated into q_out [rows, H, head_dim] of q_dtype
  *   (SM_BF16 or SM_F16), which must not overlap q, k or v. Rotation in f32, one rounding
- *   to the cache's type; a position outside the table gives NaN. (project_qkv + slice_assign, attention.rs:142-177, 331-356.)
+ *   to the cache's type; a position outside the table gives NaN. (project_qkv +
+ *   slice_assign, attention.rs:142-177, 331-356.)
  *   8-bit: a block's scale is the least 2^e, e >= -63, with every finite value of the
  *   block within 448 * 2^e; it never falls while earlier tokens of the block stay, and
  *   where a later token raises it their codes are scaled down and rounded again, which
@@ -486,11 +488,11 @@ int sm_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, const f
  * sm_paged_attention: out [rows, H, head_dim] of `dtype` (SM_BF16 or SM_F16; a 16-bit
  *   cache must have the same): softmax(q . K / sqrt(head_dim)) . V over keys 0 .. position
  *   of the row, query head h reading KV head h / (H / kv_heads); q rows ldq values apart,
- *   16-byte aligned; lse (nullable) [rows, H] f32, the log-sum-exp of the scaled scores.
+ *   16-byte aligned, not overlapping out; lse (nullable) [rows, H] f32, the log-sum-exp of the scaled scores.
  *   A row at a negative position sees no key: out 0, lse -inf. A row that sees a token
  *   without a page gives NaN. What the pages hold behind a sequence's last token, and
  *   values that a row does not see, do not enter its result, NaN and infinities among
- *   them. (forward_cached / sdpa, attention.rs:216-265, 318-371.)
+ *   them; an infinity that it sees makes its sum infinite, whatever its weight. (forward_cached / sdpa, attention.rs:216-265, 318-371.)
  *   max_tokens: the tokens of the longest sequence, new rows included; it only decides
  *   how the keys are split, a longer sequence is still attended to in full.
  *   workspace: sm_paged_attention_workspace_bytes(...) bytes (-1 for a bad shape; 0 where

@@ -437,8 +437,10 @@ extern "C" int sm_paged_append(const sm_paged_cache* cache, const int32_t* block
   SM_REQUIRE(row_start || rows == S * max_rows,
              "%s: without row_start, rows must be S * max_rows", me);
   const int64_t each = dtype == SM_F32 ? 4 : 8;  // values of 16 bytes
+  const int64_t wide = (int64_t)1 << 31;
   SM_REQUIRE(ldk >= KVH * hd && ldv >= KVH * hd && ldk % each == 0 && ldv % each == 0 &&
-                 (!q || (ldq >= H * hd && ldq % each == 0)),
+                 ldk < wide && ldv < wide &&
+                 (!q || (ldq >= H * hd && ldq % each == 0 && ldq < wide)),
              "%s: rows must be 16-byte aligned and hold their heads", me);
   if (q) {
     const size_t size = 16 / each;

@@ -46,6 +46,7 @@ struct PagedArgs {
   PagedMap map;                  // of paged_tile_kernel
   Divide H, KVH, G, bpp, nsplit, tiles, rows_each, tile;
   int S, rows, max_rows, pages, cols, cb;
+  int most;                      // blocks that a table row holds, and one
   float c2;                      // log2(e) / sqrt(hd)
 };
 
@@ -97,18 +98,23 @@ __device__ inline uint32_t finite_only(uint32_t w) {
   }
 }
 
-// Values that some of a tile's rows see and some do not go into the products only where
-// they are finite (a weight of zero would turn an infinity into a NaN for the rows that do
-// not see it). The others come here, after the sweep and only where there are any: each is
-// added to the rows that see it, whose sums it makes infinite or NaN as its weight, which
-// is positive, would. dim(i): the dims of this lane's sums.
-template <int HD, bool C8, bool F16, int N, typename Dim>
-__device__ inline void add_odd(const PagedArgs& a, const int32_t* trow, int kvh, int first_block,
-                               int end_block, int keys, int qpos, Dim dim, float (&sum)[N]) {
+// Values that are not finite. Those that some of a tile's rows see and some do not are kept
+// out of the products (a weight of zero would turn an infinity into a NaN for the rows that
+// do not see it); those that all see go in, and leave a NaN where a weight, or what 16 bits
+// leave of one, is rounded to zero. So where there are any, each row's sums are put right
+// after the sweep: a weight is positive, however small, and one infinity or NaN decides a
+// sum. mine(block): it is the caller's; dim(i): the dims of this lane's sums.
+template <int HD, bool C8, bool F16, int N, typename Mine, typename Dim>
+__device__ inline void fix_odd(const PagedArgs& a, const int32_t* trow, int kvh, int first_block,
+                               int end_block, int keys, int qpos, Mine mine, Dim dim,
+                               float (&sum)[N]) {
   constexpr int T = C8 ? 4 : 2;
+  float x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = 0.f;
   for (int blk = first_block; blk < end_block; ++blk) {
     const int bi = paged_block(trow, a.cols, a.pages, (int)a.KVH.d, kvh, a.bpp, blk);
-    if (bi < 0) continue;
+    if (bi < 0 || !mine(blk)) continue;
     const size_t base = (size_t)bi * (kBlock * HD);
     for (int t = 0; t < kBlock; ++t) {
       const int key = blk * kBlock + t;
@@ -125,10 +131,21 @@ __device__ inline void add_odd(const PagedArgs& a, const int32_t* trow, int kvh,
           v = F16 ? (float)__builtin_bit_cast(_Float16, w) : bf16_to_f32(w);
           if (fabsf(v) < INFINITY) v = 0.f;
         }
-        if (key <= qpos) sum[i] += v;
+        if (key <= qpos) x[i] += v;
       }
     }
   }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (!(x[i] == 0.f)) sum[i] = x[i];
+}
+
+// Weight of a partial sum with the maximum m and the sum l of weights among those whose
+// maximum is mm: zero without keys (m -inf, l 0), else positive, so that what it has of an
+// infinity stays.
+__device__ inline float join_weight(float m, float l, float mm) {
+  return m == -INFINITY ? (l == 0.f ? 0.f : NAN)
+                        : fmaxf(__builtin_amdgcn_exp2f(m - mm), 1.1754943508e-38f);
 }
 
 // Where 64 blocks of a sequence lie, one to a lane, and their scales.
@@ -191,7 +208,7 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
   const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
   const int pos0 = a.pos0[s];
   const int row0 = tile * kRows16, all = pr.n * (int)a.G.d;
-  const PagedKeys pk(pos0, pr.n, a.G, row0, kRows16, a.cb, (int)a.nsplit.d);
+  const PagedKeys pk(pos0, pr.n, a.G, row0, kRows16, a.cb, (int)a.nsplit.d, a.most);
   const bool idle = row0 >= all || split >= max(pk.splits, 1);
   const int b0 = split * a.cb, b1 = idle || pk.keys <= 0 ? b0 : pk.end(split, a.cb);
 
@@ -333,22 +350,26 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
       }
     }
   }
-  if (odd) {  // (uniform per wave)
-    // the blocks of this wave's steps among those that not all rows see
-    for (int st = b0 + wave * NB; st < b1; st += 4 * NB) {
-      const int from = max(st, (pos_first + 1) / kBlock);
-      float x[4 * NT];
+  l += __shfl_xor(l, 16, kWave);
+  l += __shfl_xor(l, 32, kWave);
+  float zero = 0.f;  // NaN where a sum is not finite
 #pragma unroll
-      for (int i = 0; i < 4 * NT; ++i) x[i] = o[i / 4][i % 4];
-      add_odd<HD, C8, QF16>(a, trow, kvh, from, min(st + NB, b1), pk.keys, qpos,
-                            [&](int i) { return 16 * (i / 4) + 4 * g + i % 4; }, x);
+  for (int i = 0; i < 4 * NT; ++i) zero = fmaf(o[i / 4][i % 4], 0.f, zero);
+  const bool all_see = __ballot(zero != zero && l == l) != 0;
+  if (odd || all_see) {  // (uniform per wave)
+    // this wave's steps, or those among them that not all rows see
+    const int from = all_see ? b0 : max(b0, (pos_first + 1) / kBlock);
 #pragma unroll
-      for (int i = 0; i < 4 * NT; ++i) o[i / 4][i % 4] = x[i];
+    for (int n = 0; n < NT; ++n) {
+      float x[4] = {o[n][0], o[n][1], o[n][2], o[n][3]};
+      fix_odd<HD, C8, QF16>(a, trow, kvh, from, b1, pk.keys, qpos,
+                            [&](int blk) { return (blk - b0) % (4 * NB) / NB == wave; },
+                            [&](int i) { return 16 * n + 4 * g + i; }, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[n][i] = x[i];
     }
   }
   if (idle) return;  // (uniform)
-  l += __shfl_xor(l, 16, kWave);
-  l += __shfl_xor(l, 32, kWave);
   if (g == 0) {
     sm_m[wave][r] = m;
     sm_l[wave][r] = l;
@@ -368,9 +389,7 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
   float ll = 0.f, f[4];
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    // (a wave without keys has an empty sum, whatever its partner's maximum)
-    f[w] = sm_m[w][y] == -INFINITY ? (sm_l[w][y] == 0.f ? 0.f : NAN)
-                                   : __builtin_amdgcn_exp2f(sm_m[w][y] - mm);
+    f[w] = join_weight(sm_m[w][y], sm_l[w][y], mm);
     ll = fmaf(sm_l[w][y], f[w], ll);
   }
   float acc[HD / 16];
@@ -570,15 +589,27 @@ struct TileSweep {
       if (more) store_tile(blk + NB, buf ^ 1, cur);  // last read before the previous barrier
       __syncthreads();
     }
-    if (s.odd) {
-      float x[16 * DB];
+    // (the sums end here for the compiler: it copies them in every tile otherwise)
 #pragma unroll
-      for (int i = 0; i < 16 * DB; ++i) x[i] = o[i / 16][i % 16];
-      add_odd<HD, C8, QF16>(
-          a, trow, kvh, max(b0, (pos_first + 1) / kBlock), b1, keys, qpos,
-          [&](int i) { return 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * hf + i % 4; }, x);
+    for (int d = 0; d < DB; ++d) asm volatile("" : "+v"(o[d]));
+    l += __shfl_xor(l, 32, kWave);
+    float zero = 0.f;  // NaN where a sum is not finite
 #pragma unroll
-      for (int i = 0; i < 16 * DB; ++i) o[i / 16][i % 16] = x[i];
+    for (int i = 0; i < 16 * DB; ++i) zero = fmaf(o[i / 16][i % 16], 0.f, zero);
+    const bool all_see = __ballot(zero != zero && l == l) != 0;
+    if (s.odd || all_see) {  // (uniform per wave)
+      const int from = all_see ? b0 : max(b0, (pos_first + 1) / kBlock);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = o[d][e];
+        fix_odd<HD, C8, QF16>(
+            a, trow, kvh, from, b1, keys, qpos, [](int) { return true; },
+            [&](int e) { return 32 * d + 8 * (e / 4) + 4 * hf + e % 4; }, x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = x[e];
+      }
     }
   }
 
@@ -714,7 +745,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
   const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
   const int pos0 = a.pos0[s];
   const int row0 = tile * kRowsTile, all = pr.n * (int)a.G.d;
-  const PagedKeys pk(pos0, pr.n, a.G, row0, kRowsTile, a.cb, (int)a.nsplit.d);
+  const PagedKeys pk(pos0, pr.n, a.G, row0, kRowsTile, a.cb, (int)a.nsplit.d, a.most);
   const bool idle = row0 >= all || split >= max(pk.splits, 1);
   const int j = t.j = t.lane % 32, hf = t.hf = t.lane / 32;
   t.b0 = split * a.cb;
@@ -734,7 +765,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
   if (idle) return;  // (uniform)
   f32x16(&o)[T::DB] = t.o;
   constexpr int DB = T::DB;
-  const float l = t.l + __shfl_xor(t.l, 32, kWave), m = t.m;
+  const float l = t.l, m = t.m;
   const int row = r0 + j;
   int tok = row;
   const int head = kvh * (int)a.G.d + a.G.mod(tok);
@@ -815,7 +846,7 @@ __global__ __launch_bounds__(256, 8) void paged_join_kernel(PagedArgs a) {
   int x = head;
   const int pos0 = a.pos0[s], row = i * (int)a.G.d + a.G.mod(x);
   const PagedKeys pk(pos0, pr.n, a.G, a.tile.div(row) * (int)a.tile.d, (int)a.tile.d, a.cb,
-                     (int)a.nsplit.d);
+                     (int)a.nsplit.d, a.most);
   if (pk.splits <= 1) return;  // written already
   const size_t at = (size_t)(pr.first + i) * a.H.d + head;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at * a.nsplit.d;
@@ -830,8 +861,7 @@ __global__ __launch_bounds__(256, 8) void paged_join_kernel(PagedArgs a) {
   for (int x0 = 0; x0 < pk.splits; x0 += kWave) {
     const int n = min(kWave, pk.splits - x0);
     const float2 v = lane < n ? ml[x0 + lane] : float2{-INFINITY, 0.f};
-    // (a split without visible keys has the maximum -inf and the sum 0)
-    const float f = v.x == -INFINITY ? (v.y == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(v.x - mm);
+    const float f = join_weight(v.x, v.y, mm);
     ll += wave_sum(v.y * f);
     int x = 0;
     for (; x + 16 <= n; x += 16) add_splits<HD, 16>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
@@ -893,7 +923,8 @@ int check_shape(const char* who, int64_t S, int64_t rows, int64_t max_rows, int6
   // (the grid holds less than 2^24 workgroups of 256 threads, and 32 bits index a row)
   if (max_rows * (H / KVH) >= most ||
       (double)S * (double)ceil_div(max_rows * (H / KVH), 16) * (double)KVH >= (double)(1 << 24) ||
-      (double)S * (double)max_rows * (double)H >= (double)(1 << 26)) {
+      (double)S * (double)max_rows * (double)H >= (double)(1 << 26) ||
+      (double)rows * (double)H >= (double)((int64_t)1 << 40)) {  // (bytes: below 2^60)
     set_error("%s: problem too large", who);
     return SM_ERR_UNSUPPORTED;
   }
@@ -955,15 +986,19 @@ extern "C" int sm_paged_attention(const sm_paged_cache* cache, const int32_t* bl
   SM_REQUIRE(table_cols > 0 && table_cols <= 0x7fffffff, "%s: table_cols must be positive", me);
   SM_REQUIRE(row_start || rows == S * max_rows,
              "%s: without row_start, rows must be S * max_rows", me);
-  SM_REQUIRE(ldq >= H * hd && ldq % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
-                 reinterpret_cast<uintptr_t>(out) % 16 == 0,
-             "%s: q rows and out must be 16-byte aligned, ldq >= H * head_dim", me);
+  const uintptr_t qa = reinterpret_cast<uintptr_t>(q), oa = reinterpret_cast<uintptr_t>(out);
+  SM_REQUIRE(ldq >= H * hd && ldq < ((int64_t)1 << 31) && ldq % 8 == 0 && qa % 16 == 0 &&
+                 oa % 16 == 0,
+             "%s: q rows and out must be 16-byte aligned, ldq >= H * head_dim and ldq < 2^31", me);
   const PagedPlan plan(S, max_rows, H / KVH, KVH, max_tokens);
   const int64_t need = plan.bytes(rows, H, hd);
   SM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need &&
                            reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
              "%s: workspace of %lld bytes, %lld needed, 16-byte aligned", me,
              (long long)workspace_bytes, (long long)need);
+  SM_REQUIRE(qa + (size_t)((rows - 1) * ldq + H * hd) * 2 <= oa ||
+                 oa + (size_t)(rows * H * hd) * 2 <= qa,
+             "%s: out must not overlap q", me);
   const int64_t joins = ceil_div(S * max_rows * H, 4);
   if (plan.wgs >= (1 << 24) || joins >= (1 << 24)) {
     set_error("%s: problem too large", me);
@@ -995,6 +1030,7 @@ extern "C" int sm_paged_attention(const sm_paged_cache* cache, const int32_t* bl
   a.bpp = Divide((int)(cache->page_tokens / kBlock));
   a.cols = (int)table_cols;
   a.cb = plan.cb;
+  a.most = (int)std::min<int64_t>(table_cols * a.bpp.d + 1, 1 << 27);
   a.nsplit = Divide(plan.nsplit);
   a.tile = Divide(plan.tile);
   a.tiles = Divide((int)plan.tiles);

@@ -72,18 +72,21 @@ __host__ __device__ inline int64_t paged_touched(int64_t n) { return (n + kBlock
 // Keys of one tile of `tile` query rows and their split. A row is a (token, head of
 // the KV head's group) pair, G heads to a token, so the tile's last row sees the most
 // keys. Split i of `nsplit` takes blocks [i cb, (i + 1) cb); the last one takes what is
-// left, so that no key is dropped however long the sequence is.
+// left, so that no key is dropped however long the sequence is. `most`: blocks that a table
+// row holds, and one: the first without a page, for all the keys behind it that have none,
+// so that a wrong length costs no more than a full table.
 struct PagedKeys {
   int keys;    // keys that the tile's last row sees (<= 0: none)
   int blocks;  // blocks that hold them
   int splits;  // splits that have work (0 without keys)
   __host__ __device__ PagedKeys(int pos0, int n, const Divide& G, int first_row, int tile,
-                                int cb, int nsplit) {
+                                int cb, int nsplit, int most = 1 << 27) {
     const int all = n * (int)G.d;
     int last = first_row + tile - 1;
     if (last > all - 1) last = all - 1;
     const int64_t k = last < 0 ? 0 : (int64_t)pos0 + G.div(last) + 1;
-    keys = k < 0 ? 0 : k > 0x7fffffff ? 0x7fffffff : (int)k;
+    const int64_t held = (int64_t)most * kBlock, in = k > held ? held : k;
+    keys = in < 0 ? 0 : in > 0x7fffffff ? 0x7fffffff : (int)in;
     blocks = (int)(((int64_t)keys + kBlock - 1) / kBlock);
     const int64_t want = ((int64_t)blocks + cb - 1) / cb;
     splits = want < nsplit ? (int)want : nsplit;

@@ -82,7 +82,7 @@ class PagedKVCache:
                 raise ValueError(f"{name} must be a device tensor, all on one device")
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
-        self.k, self.v, self.k_scales, self.v_scales = k, v, ks, vs
+        self._tensors = k, v, ks, vs  # (the descriptor below holds their addresses)
         self.pages, self.kv_heads, self.page_tokens, self.head_dim = k.shape
         self.dtype, self.device, self.index = k.dtype, k.device, k.get_device()
         self._c = _lib.PagedCache(k.data_ptr(), v.data_ptr(), ks.data_ptr() if ks is not None else 0,
@@ -91,11 +91,14 @@ class PagedKVCache:
                                   _CACHE[k.dtype])
         self._at = C.addressof(self._c)
 
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_scales = property(lambda self: self._tensors[2])
+    v_scales = property(lambda self: self._tensors[3])
+
     @property
     def nbytes(self) -> int:
-        tensors = [self.k, self.v] + ([self.k_scales, self.v_scales] if self.k_scales is not None
-                                      else [])
-        return sum(t.numel() * t.element_size() for t in tensors)
+        return sum(t.numel() * t.element_size() for t in self._tensors if t is not None)
 
 
 def _rows(cache, t: torch.Tensor, name: str):

@@ -388,6 +388,52 @@ def test_values_a_row_does_not_see(dev, dtype, cdt, n):
     assert not bool(fin.all()) and bool(fin[0].all())
 
 
+@pytest.mark.parametrize("dtype,cdt", [(F16, F8), (BF16, BF16), (F16, F16)])
+@pytest.mark.parametrize("pos0,n", [(40, 1), (40, 60), (1400, 3), (1400, 90)])
+def test_infinite_values_that_rows_see(dev, pos0, n, dtype, cdt):
+    """An infinity has a positive weight in every row that sees it, however small: the sum is
+    infinite, of both signs or with a NaN it is NaN, and other dims are left alone. (8 bits:
+    an infinity is stored as NaN.)"""
+    b = Batch(dev, [0], [pos0 + n], 1, 64, 32, cdt)
+    k, v = torch.randn(2, pos0 + n, 1, 64)
+    k[:pos0 * 2 // 5] = -60.0  # weights that 32 bits round to zero: whole splits, or steps
+    v[0, 0, 1], v[pos0 - 1, 0, 2], v[pos0 // 2, 0, 3] = math.inf, -math.inf, math.inf
+    v[1, 0, 4], v[pos0 - 2, 0, 4] = math.inf, -math.inf
+    v[2, 0, 5], v[pos0 // 2, 0, 6], v[pos0 + n // 2, 0, 7] = math.nan, math.nan, math.inf
+    v[3, 0, 8] = v[pos0 + n - 1, 0, 8] = math.inf
+    b.append(k.to(dev), v.to(dev))
+    b.pos0, b.n, b.starts, b.rows, b.most = [pos0], [n], [0, n], n, n
+    b.p = torch.tensor([pos0], dtype=torch.int32, device=dev)
+    q = torch.randn(n, 4, 64).abs().to(dtype)
+    got = b.attention(q.to(dev)).cpu().double()
+    ref, _, mag, err, unit = P.attend(q, b.store(), b.table, b.pos0, b.starts, b.page)
+    assert bool((ref[..., 1].isnan() if cdt == F8 else ref[..., 1] == math.inf).all())
+    odd = ~torch.isfinite(ref)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    inf = torch.isinf(ref)
+    assert torch.equal(got[inf], ref[inf]) and bool(torch.isfinite(got[~odd]).all())
+    tol = tolerance(dtype, cdt, ref, mag, err, unit, 64)
+    assert bool(((got - ref).abs() <= tol)[~odd].all())
+
+
+@pytest.mark.parametrize("cdt", [F8, F16])
+def test_lengths_beyond_the_table(dev, cdt):
+    """A length that no table row holds is read no further than the first token without a
+    page: its rows are NaN, and the call ends as soon as one over a full table."""
+    from summa_amd import paged
+    cache = paged.PagedKVCache(4, 2, 64, 32, cdt, dev)
+    t = torch.tensor([[0, 1], [2, 3], [1, 0]], dtype=torch.int32, device=dev)
+    k = torch.randn(3 * 64, 2, 64, device=dev)
+    paged.paged_append(cache, k, k, t, torch.zeros(3, dtype=torch.int32, device=dev))
+    for n in (1, 40):
+        pos0 = torch.tensor([1 << 30, 64 - n, 2 ** 31 - 50], dtype=torch.int32, device=dev)
+        q = torch.randn(3 * n, 4, 64, device=dev).half()
+        out = paged.paged_attention(cache, q, t, pos0, max_tokens=4096)
+        assert bool(out[:n].isnan().all()) and bool(out[2 * n:].isnan().all())
+        assert torch.equal(out[n:2 * n], paged.paged_attention(cache, q[n:2 * n], t[1:2], pos0[1:2],
+                                                               max_tokens=4096))
+
+
 @pytest.mark.parametrize("cdt", [F8, F16])
 def test_rows_without_keys_or_pages(dev, cdt):
     """Negative positions: zero and -inf. A row that needs a page that is none: NaN, the rows
@@ -560,6 +606,16 @@ def test_two_calls_at_once(dev):
             c = b.attention(q2)
         torch.cuda.synchronize()
         assert torch.equal(a, want[0]) and torch.equal(c, want[1])
+
+
+def test_a_cache_keeps_its_storage(dev):
+    """The descriptor holds addresses: the tensors behind it cannot be exchanged."""
+    from summa_amd import paged
+    c = paged.PagedKVCache(4, 2, 64, 32, F8, dev)
+    with pytest.raises(AttributeError):
+        c.k = torch.zeros_like(c.v)
+    again = paged.PagedKVCache.from_tensors(c.k, c.v, c.k_scales, c.v_scales)
+    assert again.nbytes == c.nbytes == 4 * 2 * 32 * 64 * 2 + 2 * 4 * 2 * 2
 
 
 def test_python_refusals(dev):

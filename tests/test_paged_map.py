@@ -109,6 +109,12 @@ int main() {
       at = k.end(i, cb);
     }
     CHECK(at == k.blocks);
+    // no more blocks than a table row holds and one
+    const int most = 1 + rnd() % 200;
+    const PagedKeys c(pos0, n, G, row0, tile, cb, nsplit, most);
+    CHECK(c.blocks == (k.blocks < most ? k.blocks : most) && c.keys <= k.keys);
+    CHECK(c.keys == (k.blocks <= most ? k.keys : most * 16) && c.splits <= k.splits);
+    CHECK(c.splits == 0 || c.end(c.splits - 1, cb) == c.blocks);
   }
   printf("ok\n");
   return 0;
@@ -208,6 +214,19 @@ def test_append_refusals(kw, msg):
 def test_attention_refusals(kw, msg):
     st, err = attention(cache(), **kw)
     assert st == -1 and msg in err, err
+
+
+def test_more_refusals():
+    for kw in (dict(out=D), dict(out=D + 512), dict(out=D - 512), dict(q=D + 256, ldq=512)):
+        st, err = attention(cache(), **kw)
+        assert st == -1 and "out must not overlap q" in err, err
+    st, err = attention(cache(), ldq=1 << 31)
+    assert st == -1 and "ldq < 2^31" in err
+    for kw in (dict(ldk=1 << 31), dict(ldv=1 << 40), dict(q=D, ldq=1 << 62, H=4, out=4 * D)):
+        st, err = append(cache(), **kw)
+        assert st == -1 and "hold their heads" in err
+    # workspace bytes that no card holds, and no 64-bit sum
+    assert _lib.lib().sm_paged_attention_workspace_bytes(1, (1 << 31) - 2, 1, 65535, 1, 128, 1 << 30) == -1
 
 
 def test_attention_types_have_to_agree():
