@@ -179,8 +179,8 @@ struct Blocks {
 // 16-key blocks in turn and meet in LDS at the end. K and V go from memory into the registers
 // as the matrix cores take them, 16 bytes a lane and load; 8-bit codes are converted there
 // (one instruction for two). v_mfma_f32_16x16x32: a score tile is 16 keys x 16 rows.
-// 256 sequences of 512-1023 tokens, 16 / 4 heads of 128, e4m3 (202 MB): 41 us, 4.9 TB/s; 4 of
-// 100-131 k (483 MB): 92 us, 5.2; 48 x 4 rows of 1-4 k, 16 heads, bf16 (1.08 GB): 204 us, 5.3,
+// 256 sequences of 512-1023 tokens, 16 / 4 heads of 128, e4m3 (202 MB): 42 us, 4.8 TB/s; 4 of
+// 100-131 k (483 MB): 94 us, 5.1; 48 x 4 rows of 1-4 k, 16 heads, bf16 (1.08 GB): 205 us, 5.3,
 // where a copy on this card moves 4.9. Two blocks a step beside four: the same time with 40
 // registers fewer; four workgroups a unit (128 registers): no faster.
 constexpr int kRows16 = 16;  // query rows of a workgroup
@@ -427,13 +427,15 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
 // Four waves x 32 rows (v_mfma_f32_32x32x16), two workgroups a unit. A tile of 64 keys, in
 // 16 bits, sits in one of two LDS buffers; the next tile's loads go out before this one's
 // products and are converted and stored after them, one barrier a tile.
-// 2 x 1024 tokens on 24-32 k keys, 16 / 4 heads of 128, f16 queries, e4m3: 0.56 ms, 0.92 PF/s,
-// 78 % of what a large f16 product reaches here; the clock is down to 1.9 GHz then, the matrix
-// cores work 41 % and the vector units 47 % of the cycles. Prefill of 32 prompts of 257-512:
-// 47 us: 1.75 us a tile and 5.6 us a workgroup for two round trips to memory and its output.
+// 2 x 1024 tokens on 24-32 k keys, 16 / 4 heads of 128, f16 queries, e4m3: 0.57-0.60 ms from
+// card to card, 0.86-0.90 PF/s, three quarters of what a large f16 product reaches; the clock is
+// down to 1.9 GHz then, the matrix cores work 41 % and the vector units 46 % of the cycles.
+// Prefill of 32 prompts of 257-512: 48 us: 1.75 us a tile and 5.6 us a workgroup for two round
+// trips to memory and its output.
 // Tried and slower: scores of the next tile beside this one's softmax on 32-key tiles (670
 // beside 637 us at the time), three workgroups a unit (618 beside 583), workgroups that go
-// on to further row tiles with their first loads in flight (prefill 65 beside 50 us).
+// on to further row tiles with their first loads in flight (prefill 65 beside 50 us), output and
+// query rows kept out of the L2 (60 beside 53; the output alone: the same).
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <bool F16>
