@@ -483,8 +483,8 @@ int sm_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, const f
  *   is exact except among e4m3's subnormals. An infinity or NaN is stored as NaN (0x7f)
  *   and does not enter the scale.
  *   Tokens at a negative position, or for which the table names no page in [0, pages),
- *   are not stored (nor is q of a negative position). Pages that several sequences hold
- *   must not be written by two of them in one call.
+ *   are not stored (nor is q of a negative position). A page is written for one of its
+ *   sequences and at one of its table entries in a call, whoever else reads it.
  * sm_paged_attention: out [rows, H, head_dim] of `dtype` (SM_BF16 or SM_F16; a 16-bit
  *   cache must have the same): softmax(q . K / sqrt(head_dim)) . V over keys 0 .. position
  *   of the row, query head h reading KV head h / (H / kv_heads); q rows ldq values apart,
@@ -492,7 +492,9 @@ int sm_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, const f
  *   A row at a negative position sees no key: out 0, lse -inf. A row that sees a token
  *   without a page gives NaN. What the pages hold behind a sequence's last token, and
  *   values that a row does not see, do not enter its result, NaN and infinities among
- *   them; an infinity that it sees makes its sum infinite, whatever its weight. (forward_cached / sdpa, attention.rs:216-265, 318-371.)
+ *   them; an infinity that it sees makes its sum infinite, whatever its weight (so do sums
+ *   that pass f32: bf16 values beyond 2^88 may). (forward_cached / sdpa,
+ *   attention.rs:216-265, 318-371.)
  *   max_tokens: the tokens of the longest sequence, new rows included; it only decides
  *   how the keys are split, a longer sequence is still attended to in full.
  *   workspace: sm_paged_attention_workspace_bytes(...) bytes (-1 for a bad shape; 0 where

@@ -100,21 +100,45 @@ __device__ inline uint32_t finite_only(uint32_t w) {
 
 // Values that are not finite. Those that some of a tile's rows see and some do not are kept
 // out of the products (a weight of zero would turn an infinity into a NaN for the rows that
-// do not see it); those that all see go in, and leave a NaN where a weight, or what 16 bits
-// leave of one, is rounded to zero. So where there are any, each row's sums are put right
-// after the sweep: a weight is positive, however small, and one infinity or NaN decides a
-// sum. mine(block): it is the caller's; dim(i): the dims of this lane's sums.
-template <int HD, bool C8, bool F16, int N, typename Mine, typename Dim>
-__device__ inline void fix_odd(const PagedArgs& a, const int32_t* trow, int kvh, int first_block,
-                               int end_block, int keys, int qpos, Mine mine, Dim dim,
-                               float (&sum)[N]) {
+// do not see it); those that all see go in, and in 16 bits leave a NaN where a weight, or
+// what its rounding leaves, is zero. So where there are any, each row's sums are put right
+// after the sweep: a weight is positive, however small, and one infinity or NaN decides a sum.
+//
+// Blocks first, first + 1, .. below end, 64 at most, that have such values and are the
+// caller's: mine(block).
+template <int HD, bool C8, bool F16, typename Mine>
+__device__ inline uint64_t odd_blocks(const PagedArgs& a, const int32_t* trow, int kvh, int first,
+                                      int end, int lane, Mine mine) {
+  constexpr int BB = kBlock * HD * (C8 ? 1 : 2);
+  uint64_t mask = 0;
+  for (int i = 0; i < min(kWave, end - first); ++i) {
+    if (!mine(first + i)) continue;
+    const int bi = paged_block(trow, a.cols, a.pages, (int)a.KVH.d, kvh, a.bpp, first + i);
+    if (bi < 0) continue;
+    bool odd = false;
+#pragma unroll
+    for (int c = 0; c < BB / 1024; ++c) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(a.v + (size_t)bi * BB + c * 1024 + lane * 16);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) odd |= finite_only<C8, F16>(w[k]) != w[k];
+    }
+    if (__ballot(odd)) mask |= (uint64_t)1 << i;
+  }
+  return mask;
+}
+// sum[i], of dim(i): what the blocks of `mask` have that is not finite and this lane's row
+// sees, in place of the sum at first (its bit of `done` is clear), with it from then on.
+template <int HD, bool C8, bool F16, int N, typename Dim>
+__device__ inline void fix_odd(const PagedArgs& a, const int32_t* trow, int kvh, int first,
+                               uint64_t mask, int keys, int qpos, Dim dim, uint32_t& done,
+                               int bit, float (&sum)[N]) {
   constexpr int T = C8 ? 4 : 2;
   float x[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = 0.f;
-  for (int blk = first_block; blk < end_block; ++blk) {
+  for (; mask; mask &= mask - 1) {
+    const int blk = first + __builtin_ctzll(mask);
     const int bi = paged_block(trow, a.cols, a.pages, (int)a.KVH.d, kvh, a.bpp, blk);
-    if (bi < 0 || !mine(blk)) continue;
     const size_t base = (size_t)bi * (kBlock * HD);
     for (int t = 0; t < kBlock; ++t) {
       const int key = blk * kBlock + t;
@@ -137,7 +161,10 @@ __device__ inline void fix_odd(const PagedArgs& a, const int32_t* trow, int kvh,
   }
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (!(x[i] == 0.f)) sum[i] = x[i];
+    if (!(x[i] == 0.f)) {
+      sum[i] = done >> (bit + i) & 1 ? sum[i] + x[i] : x[i];
+      done |= 1u << (bit + i);
+    }
 }
 
 // Weight of a partial sum with the maximum m and the sum l of weights among those whose
@@ -352,21 +379,27 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
   }
   l += __shfl_xor(l, 16, kWave);
   l += __shfl_xor(l, 32, kWave);
-  float zero = 0.f;  // NaN where a sum is not finite
+  bool all_see = false;  // values that are not finite among the others
+  if constexpr (!C8) {   // (a code is finite or NaN, which any weight leaves a NaN)
+    float zero = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4 * NT; ++i) zero = fmaf(o[i / 4][i % 4], 0.f, zero);
-  const bool all_see = __ballot(zero != zero && l == l) != 0;
+    for (int i = 0; i < 4 * NT; ++i) zero = fmaf(o[i / 4][i % 4], 0.f, zero);
+    all_see = __ballot(zero != zero && l == l) != 0;
+  }
   if (odd || all_see) {  // (uniform per wave)
-    // this wave's steps, or those among them that not all rows see
-    const int from = all_see ? b0 : max(b0, (pos_first + 1) / kBlock);
+    uint32_t done = 0;
+    for (int seg = all_see ? b0 : max(b0, (pos_first + 1) / kBlock); seg < b1; seg += kWave) {
+      const uint64_t mask = odd_blocks<HD, C8, QF16>(
+          a, trow, kvh, seg, b1, lane, [&](int blk) { return (blk - b0) % (4 * NB) / NB == wave; });
+      if (!mask) continue;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float x[4] = {o[n][0], o[n][1], o[n][2], o[n][3]};
-      fix_odd<HD, C8, QF16>(a, trow, kvh, from, b1, pk.keys, qpos,
-                            [&](int blk) { return (blk - b0) % (4 * NB) / NB == wave; },
-                            [&](int i) { return 16 * n + 4 * g + i; }, x);
+      for (int n = 0; n < NT; ++n) {
+        float x[4] = {o[n][0], o[n][1], o[n][2], o[n][3]};
+        fix_odd<HD, C8, QF16>(a, trow, kvh, seg, mask, pk.keys, qpos,
+                              [&](int i) { return 16 * n + 4 * g + i; }, done, 4 * n, x);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[n][i] = x[i];
+        for (int i = 0; i < 4; ++i) o[n][i] = x[i];
+      }
     }
   }
   if (idle) return;  // (uniform)
@@ -595,22 +628,31 @@ struct TileSweep {
 #pragma unroll
     for (int d = 0; d < DB; ++d) asm volatile("" : "+v"(o[d]));
     l += __shfl_xor(l, 32, kWave);
-    float zero = 0.f;  // NaN where a sum is not finite
+    bool all_see = false;  // (as in paged_split_kernel)
+    if constexpr (!C8) {
+      float zero = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16 * DB; ++i) zero = fmaf(o[i / 16][i % 16], 0.f, zero);
-    const bool all_see = __ballot(zero != zero && l == l) != 0;
+      for (int i = 0; i < 16 * DB; ++i) zero = fmaf(o[i / 16][i % 16], 0.f, zero);
+      all_see = __ballot(zero != zero && l == l) != 0;
+    }
     if (s.odd || all_see) {  // (uniform per wave)
-      const int from = all_see ? b0 : max(b0, (pos_first + 1) / kBlock);
+      uint32_t done[(DB + 1) / 2] = {};
+      for (int seg = all_see ? b0 : max(b0, (pos_first + 1) / kBlock); seg < b1; seg += kWave) {
+        const uint64_t mask =
+            odd_blocks<HD, C8, QF16>(a, trow, kvh, seg, b1, lane, [](int) { return true; });
+        if (!mask) continue;
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        float x[16];
+        for (int d = 0; d < DB; ++d) {
+          float x[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = o[d][e];
-        fix_odd<HD, C8, QF16>(
-            a, trow, kvh, from, b1, keys, qpos, [](int) { return true; },
-            [&](int e) { return 32 * d + 8 * (e / 4) + 4 * hf + e % 4; }, x);
+          for (int e = 0; e < 16; ++e) x[e] = o[d][e];
+          fix_odd<HD, C8, QF16>(
+              a, trow, kvh, seg, mask, keys, qpos,
+              [&](int e) { return 32 * d + 8 * (e / 4) + 4 * hf + e % 4; }, done[d / 2],
+              d % 2 * 16, x);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[d][e] = x[e];
+          for (int e = 0; e < 16; ++e) o[d][e] = x[e];
+        }
       }
     }
   }
