@@ -457,16 +457,16 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
 
 // ---- more query rows: 128 of them a workgroup, keys staged through LDS ----
 //
-// Four waves x 32 rows (v_mfma_f32_32x32x16), two workgroups a unit. A tile of 64 keys, in
-// 16 bits, sits in one of two LDS buffers; the next tile's loads go out before this one's
-// products and are converted and stored after them, one barrier a tile.
-// 2 x 1024 tokens on 24-32 k keys, 16 / 4 heads of 128, f16 queries, e4m3: 0.57-0.60 ms from
-// card to card, 0.86-0.90 PF/s, three quarters of what a large f16 product reaches; the clock is
-// down to 1.9 GHz then, the matrix cores work 41 % and the vector units 46 % of the cycles.
-// Prefill of 32 prompts of 257-512: 48 us: 1.75 us a tile and 5.6 us a workgroup for two round
-// trips to memory and its output.
+// Four or eight waves x 32 rows (v_mfma_f32_32x32x16), two waves a SIMD. A tile of 64 keys, in
+// 16 bits, sits in one of two LDS buffers; the next tiles' loads are on their way during this
+// one's products and are converted and stored before the barrier that ends it.
+// 2 x 1024 tokens on 24-32 k keys, 16 / 4 heads of 128, f16 queries, e4m3 (eight waves): 0.51 ms,
+// 1.01 PF/s, 85 % of what a large f16 product reaches; the clock is down to 1.9 GHz then.
+// Of four waves' 563 us, staging took 91, the barriers 10, the exponentials 44, the sums 16.
+// Prefill of 32 prompts of 257-512 (four waves): 48 us: 1.75 us a tile and 5.6 us a workgroup
+// for two round trips to memory and its output.
 // Tried and slower: scores of the next tile beside this one's softmax on 32-key tiles (670
-// beside 637 us at the time), three workgroups a unit (618 beside 583), workgroups that go
+// beside 637 us at the time), three workgroups a unit (618 beside 583), four times and twice the splits (the join's bytes), workgroups that go
 // on to further row tiles with their first loads in flight (prefill 65 beside 50 us), output and
 // query rows kept out of the L2 (60 beside 53; the output alone: the same).
 
@@ -488,10 +488,9 @@ __device__ inline float max3(float a, float b, float c) {
   return r;
 }
 
-constexpr int kRowsTile = 128;  // query rows of a workgroup, 32 a wave
-constexpr int kTile = 64;       // keys of a tile
+constexpr int kTile = 64;  // keys of a tile
 
-template <int HD, bool QF16, bool C8>
+template <int HD, bool QF16, bool C8, int W>  // W waves, 32 query rows each
 struct TileSweep {
   static constexpr int ES = C8 ? 1 : 2;
   static constexpr bool PF16 = C8 || QF16;
@@ -499,7 +498,7 @@ struct TileSweep {
   static constexpr int KP = HD + 8, VP = kTile + 8; // padded LDS rows (elements)
   static constexpr int NB = kTile / kBlock;         // blocks of a tile
   static constexpr int NC = HD * ES / 64;           // kilobytes of a block, each one wave's load
-  static constexpr int PER = (NB * NC + 3) / 4;     // of a tile's K, and of its V, for each wave
+  static constexpr int PER = (NB * NC + W - 1) / W; // of a tile's K, and of its V, for each wave
   static constexpr int BB = kBlock * HD * ES;
   struct Lds {
     __attribute__((aligned(16))) uint16_t ks[2][kTile * KP];
@@ -518,6 +517,7 @@ struct TileSweep {
   float m, l;
 
   Blocks cur, next;  // of the 64 blocks at hand, and of the next
+  bool missing;      // any of those at hand has keys and no page
   u32x4 kr[PER], vr[PER];
 
   __device__ TileSweep(const PagedArgs& a_, Lds& s_) : a(a_), s(s_) {}
@@ -527,7 +527,7 @@ struct TileSweep {
     const int x = wave * PER + n;
     block = x / NC;
     c = x % NC;
-    return 4 * PER == NB * NC || x < NB * NC;
+    return W * PER == NB * NC || x < NB * NC;
   }
   __device__ inline void load_tile(int blk) {  // first block of the tile
 #pragma unroll
@@ -540,9 +540,14 @@ struct TileSweep {
       vr[n] = *reinterpret_cast<const u32x4*>(a.v + at + lane * 16);
     }
   }
-  __device__ inline void store_tile(int blk, int buf, const Blocks& of) {
-    const int g = lane / 16, r = lane % 16;
-    const float kscale = of.template kscale<C8>(a.c2), vexp = of.template vexp<C8>();
+  // Whether blocks with keys have no page, of the 64 from `first` on (uniform).
+  __device__ inline bool any_missing(const Blocks& of, int first) const {
+    return __ballot(of.none && (first + lane) * kBlock < keys) != 0;
+  }
+  // Values that are not the cache's, or that only some rows see, out of what is staged.
+  __device__ inline void mask_tile(int blk, const Blocks& of) {
+    const int g = lane / 16;
+    const float kscale = of.template kscale<C8>(a.c2);
 #pragma unroll
     for (int n = 0; n < PER; ++n) {
       int block, c;
@@ -569,6 +574,16 @@ struct TileSweep {
         }
         if (x) s.odd = 1;
       }
+    }
+  }
+  __device__ inline void store_tile(int blk, int buf, const Blocks& of) {
+    const int g = lane / 16, r = lane % 16;
+    if (missing || (blk + NB) * kBlock > min(keys, pos_first + 1)) mask_tile(blk, of);
+    const float kscale = of.template kscale<C8>(a.c2), vexp = of.template vexp<C8>();
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      int block, c;
+      if (!part(n, block, c)) continue;
       const int at = (c * 64 + lane) * (16 / ES);  // element of the block
       uint16_t* kp = &s.ks[buf][(block * kBlock + at / HD) * KP + at % HD];
       if constexpr (C8) {
@@ -593,6 +608,18 @@ struct TileSweep {
     if (i < NB) *reinterpret_cast<float2*>(s.info[buf][i]) = float2{kscale, vexp};
   }
 
+  // The next tile, on its way, to LDS, and the one after it on its way.
+  __device__ inline void stage(int blk, int buf) {
+    store_tile(blk + NB, buf, cur);  // last read before the previous barrier
+    const int to = blk + 2 * NB;
+    if (to >= b1) return;
+    if ((to - b0) % kWave == 0) {
+      cur = next;
+      missing = any_missing(cur, to);
+      if (to + kWave < b1) next.find(a, trow, kvh, to + kWave + lane);
+    }
+    load_tile(to);
+  }
   // One pass over the keys.
   __device__ inline void sweep() {
 #pragma unroll
@@ -608,21 +635,41 @@ struct TileSweep {
     if (threadIdx.x == 0) s.odd = 0;
     __syncthreads();
     load_tile(b0);
+    missing = any_missing(cur, b0);
     store_tile(b0, 0, cur);
     __syncthreads();
     int buf = 0;
-    for (int blk = b0; blk < b1; blk += NB, buf ^= 1) {
-      const bool more = blk + NB < b1;
-      if ((blk - b0) % kWave == 0 && blk + kWave < b1)
-        next.find(a, trow, kvh, blk + kWave + lane);
-      if (more) {
-        if ((blk + NB - b0) % kWave == 0) cur = next;
-        load_tile(blk + NB);
+    if constexpr (W > 4) {
+      // Half of the waves stage the next tile before this one's products and half after them,
+      // so that the two waves of a SIMD are not in the same part of their work.
+      const bool early = wave >= W / 2;
+      if (b0 + kWave < b1) next.find(a, trow, kvh, b0 + kWave + lane);
+      if (b0 + NB < b1) load_tile(b0 + NB);
+      for (int blk = b0; blk < b1; blk += NB, buf ^= 1) {
+        const bool more = blk + NB < b1;
+        const int key0 = blk * kBlock;
+        if (early && more) stage(blk, buf ^ 1);
+        if (key0 <= wave_last) tile(buf, key0);  // (uniform per wave) later keys: no row sees them
+        if (!early && more) stage(blk, buf ^ 1);
+        __syncthreads();
       }
-      const int key0 = blk * kBlock;
-      if (key0 <= wave_last) tile(buf, key0);  // (uniform per wave) later keys: no row sees them
-      if (more) store_tile(blk + NB, buf ^ 1, cur);  // last read before the previous barrier
-      __syncthreads();
+    } else {
+      for (int blk = b0; blk < b1; blk += NB, buf ^= 1) {
+        const bool more = blk + NB < b1;
+        if ((blk - b0) % kWave == 0 && blk + kWave < b1)
+          next.find(a, trow, kvh, blk + kWave + lane);
+        if (more) {
+          if ((blk + NB - b0) % kWave == 0) {
+            cur = next;
+            missing = any_missing(cur, blk + NB);
+          }
+          load_tile(blk + NB);
+        }
+        const int key0 = blk * kBlock;
+        if (key0 <= wave_last) tile(buf, key0);
+        if (more) store_tile(blk + NB, buf ^ 1, cur);  // last read before the previous barrier
+        __syncthreads();
+      }
     }
     // (the sums end here for the compiler: it copies them in every tile otherwise)
 #pragma unroll
@@ -770,9 +817,10 @@ struct TileSweep {
   }
 };
 
-template <int HD, bool QF16, bool C8>
-__global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
-  typedef TileSweep<HD, QF16, C8> T;
+template <int HD, bool QF16, bool C8, int W>
+__global__ __launch_bounds__(64 * W, 2) void paged_tile_kernel(PagedArgs a) {
+  typedef TileSweep<HD, QF16, C8, W> T;
+  constexpr int kRowsTile = 32 * W;  // query rows of a workgroup
   __shared__ typename T::Lds lds;
   uint32_t grp, place;
   if (!a.map.at(blockIdx.x, grp, place)) return;  // (uniform)
@@ -832,8 +880,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
   const float inv = 1.f / l;
   const bool none = pos0 + tok < 0;  // a row without keys
   constexpr int OP = HD + 8;
-  uint16_t* lo = &lds.ks[0][0] + t.wave * 32 * OP;  // (the buffers are free: 4 x 32 x OP fit)
-  static_assert(4 * 32 * OP <= 2 * kTile * T::KP, "the rows of O fit the keys' buffers");
+  uint16_t* lo = &lds.ks[0][0] + t.wave * 32 * OP;  // (the buffers are free)
+  static_assert(2 * W * 32 * OP <= sizeof(lds.ks) + sizeof(lds.vts), "the rows of O fit K and V");
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -932,23 +980,42 @@ __global__ __launch_bounds__(256, 8) void paged_join_kernel(PagedArgs a) {
 //   each of 4 KV heads, e4m3, one token 17.2 us beside 21.1 on the 128-row kernel, 4 tokens 19.6
 //   beside 21.9; with 5, two 16-row workgroups 20.8 beside 22.5, but 8 tokens of 60000 keys 46.6
 //   beside 37.2.
-// - Keys are split where there are too few workgroups otherwise, to 1024 (four a unit) or 512
-//   (two): 256 sequences x 4 KV heads, already 1024, take 41 us whole and 50 in halves.
+// - Keys are split where there are too few workgroups otherwise, to 1024 (four a unit), 512
+//   (two) or 256 (one of 256 rows): 256 sequences x 4 KV heads, already 1024, take 41 us whole
+//   and 50 in halves; 32 x 128 rows on 1024 keys, 512 workgroups, 52 whole and 95 in halves.
 // - A split has 512 keys at least, for its share of the join: 64 sequences of 300 keys take
 //   8.4 us whole and 13.4 in two (16 rows), 13 and 27 (64 rows).
+// - 256 rows a workgroup, which stage a tile's keys once for twice the rows (16 % of the time of
+//   128), take heads of 128 where sequences are long and workgroups enough: 2 x 1024 rows on
+//   24-32 k keys 511 beside 566 us, 8 x 2048 without a context 143 beside 146; but 32 x 512 65
+//   beside 56 (one workgroup a unit, whose first loads nothing covers), 1 x 4096 (256
+//   workgroups of unequal length) 109 beside 98, 1 x 64 on 4000 (32 of them) 27 beside 21.
+//   Heads of 64 have the registers for more than two workgroups of 128: 16 x 512 on 2048 110
+//   beside 115, 8 x 2048 117 beside 160.
 struct PagedPlan {
   int tile, cb, nsplit;
   int64_t tiles, wgs;
-  PagedPlan(int64_t S, int64_t max_rows, int64_t G, int64_t KVH, int64_t max_tokens) {
-    tile = max_rows * G <= kRows16 ? kRows16 : kRowsTile;
-    tiles = ceil_div(max_rows * G, tile);
-    const int64_t units = std::max<int64_t>(1, S * tiles * KVH);
+  PagedPlan(int64_t S, int64_t max_rows, int64_t G, int64_t KVH, int64_t hd, int64_t max_tokens) {
+    const int64_t all = max_rows * G, units = S * KVH;
+    split(all <= kRows16 ? kRows16 : 128, all, units, max_tokens);
+    if (tile == 128 && hd == 128 && tiles > 1 && max_tokens > 1024) {
+      const PagedPlan narrow = *this;
+      split(256, all, units, max_tokens);
+      const int64_t least = max_tokens < 2 * max_rows ? 512 : 192;
+      if (units * tiles * nsplit < least || 20 * tiles > 11 * narrow.tiles) *this = narrow;
+    }
+    wgs = tile == kRows16 ? units * tiles * nsplit
+                          : PrefillMap((uint32_t)(units * nsplit), (uint32_t)tiles).workgroups();
+  }
+  void split(int tile_, int64_t all, int64_t units, int64_t max_tokens) {
+    tile = tile_;
+    tiles = ceil_div(all, tile);
     const int64_t blocks = std::max<int64_t>(1, ceil_div(max_tokens, kBlock));
-    const int64_t want = std::max<int64_t>(1, ceil_div(tile == kRows16 ? 1024 : 512, units));
+    const int64_t fill = tile == kRows16 ? 1024 : tile == 128 ? 512 : 256;  // workgroups
+    const int64_t want =
+        std::max<int64_t>(1, ceil_div(fill, std::max<int64_t>(1, units * tiles)));
     cb = (int)(ceil_div(std::max<int64_t>(32, ceil_div(blocks, want)), 16) * 16);
     nsplit = (int)ceil_div(blocks, cb);
-    wgs = tile == kRows16 ? S * tiles * KVH * nsplit
-                          : PrefillMap((uint32_t)(S * KVH * nsplit), (uint32_t)tiles).workgroups();
   }
   int64_t bytes(int64_t rows, int64_t H, int64_t hd) const {
     return nsplit > 1 ? rows * H * nsplit * (hd + 2) * 4 : 0;
@@ -1008,7 +1075,7 @@ extern "C" int64_t sm_paged_attention_workspace_bytes(int64_t S, int64_t rows, i
                       max_tokens) != SM_OK)
     return -1;
   if (S == 0 || max_rows == 0) return 0;
-  return sm::PagedPlan(S, max_rows, H / KVH, KVH, max_tokens).bytes(rows, H, head_dim);
+  return sm::PagedPlan(S, max_rows, H / KVH, KVH, head_dim, max_tokens).bytes(rows, H, head_dim);
 }
 
 extern "C" int sm_paged_attention(const sm_paged_cache* cache, const int32_t* block_table,
@@ -1034,7 +1101,7 @@ extern "C" int sm_paged_attention(const sm_paged_cache* cache, const int32_t* bl
   SM_REQUIRE(ldq >= H * hd && ldq < ((int64_t)1 << 31) && ldq % 8 == 0 && qa % 16 == 0 &&
                  oa % 16 == 0,
              "%s: q rows and out must be 16-byte aligned, ldq >= H * head_dim and ldq < 2^31", me);
-  const PagedPlan plan(S, max_rows, H / KVH, KVH, max_tokens);
+  const PagedPlan plan(S, max_rows, H / KVH, KVH, hd, max_tokens);
   const int64_t need = plan.bytes(rows, H, hd);
   SM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need &&
                            reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
@@ -1089,8 +1156,10 @@ extern "C" int sm_paged_attention(const sm_paged_cache* cache, const int32_t* bl
   do {                                                                           \
     if (plan.tile == kRows16)                                                    \
       paged_split_kernel<HD, F, C><<<(unsigned)plan.wgs, 256, 0, st>>>(a);       \
-    else                                                                         \
-      paged_tile_kernel<HD, F, C><<<(unsigned)plan.wgs, 256, 0, st>>>(a);        \
+    else if (HD < 128 || plan.tile == 128)                                       \
+      paged_tile_kernel<HD, F, C, 4><<<(unsigned)plan.wgs, 256, 0, st>>>(a);     \
+    else if constexpr (HD == 128)                                                \
+      paged_tile_kernel<HD, F, C, 8><<<(unsigned)plan.wgs, 512, 0, st>>>(a);     \
     if (plan.nsplit > 1)                                                         \
       paged_join_kernel<HD, F><<<(unsigned)joins, 256, 0, st>>>(a);              \
   } while (0)

@@ -343,6 +343,48 @@ def test_attention(dev, case, dtype, cdt):
         check_attention(b, q, out, lse)
 
 
+@pytest.mark.parametrize("dtype,cdt", [(F16, F8), (BF16, F8), (F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("pos0,n", [
+    ([1200, 900], [200, 131]),                          # keys in two splits
+    ([1100, -40, 0, 1024, 77], [200, 131, 256, 190, 0]),  # whole
+    ([2100, 1000], [130, 256])])
+def test_attention_of_many_heads_and_long_sequences(dev, pos0, n, dtype, cdt):
+    """Enough heads, rows and keys for the largest workgroups (256 rows, heads of 128), the
+    definition checked for some heads: ragged rows, rows without keys, a page that is none,
+    values that are not finite among those that all rows, some or none see."""
+    KVH = 64
+    b = Batch(dev, pos0, n, KVH, 128, 32, cdt, pad_rows=3)
+    b.fill()
+    k, v = torch.randn(2, b.rows, KVH, 128)
+    heads = torch.tensor([0, 1, 31, 63])
+    v[0, 1, 5], v[100, 31, 127], v[b.starts[1] + 5, 63, 64] = math.inf, math.nan, -math.inf
+    b.append(k.to(dev), v.to(dev))
+    if cdt != F8:  # seen by all rows of sequence 0; and behind sequence 1, seen by none
+        b.cache.v[b.table[0][0], 31, 0, 0, 0, 3, 0, 2] = math.inf
+    if len(n) == 2:
+        b.t[1, -(-(pos0[1] + 60) // 32)] = -1
+        b.table[1][-(-(pos0[1] + 60) // 32)] = -1
+    q = torch.randn(b.rows, KVH, 128).to(dtype)
+    out = torch.full((b.rows, KVH, 128), 5.0, dtype=dtype, device=dev)
+    _, lse = b.attention(q.to(dev), want_lse=True, out=out)
+    assert bool((out[b.starts[-1]:] == 5).all())
+    cached = tuple(x if x is None else x[:, heads] for x in b.store())
+    m = b.starts[-1]
+    ref, rl, mag, err, unit = (x[:m] for x in P.attend(q[:, heads], cached, b.table, b.pos0,
+                                                       b.starts, b.page))
+    got, lse = (x[:, heads].cpu().double()[:m] for x in (out, lse))
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    inf = torch.isinf(ref)
+    assert torch.equal(got[inf], ref[inf])
+    fin = torch.isfinite(ref)
+    tol = tolerance(dtype, cdt, ref, mag, err, unit, 128)
+    assert bool(((got - ref).abs() <= tol)[fin].all())
+    assert torch.equal(torch.isneginf(lse), torch.isneginf(rl))
+    f = torch.isfinite(rl)
+    t = err.double() * (128 + 6) * 2.0 ** -24 + 2.0 ** -21 + 2.0 ** -22 * rl.abs()
+    assert torch.equal(torch.isnan(lse), torch.isnan(rl)) and bool(((lse - rl).abs() <= t)[f].all())
+
+
 @pytest.mark.parametrize("dtype,cdt", [(F16, F8), (BF16, BF16)])
 @pytest.mark.parametrize("H,KVH,n", [(4, 1, 1), (2, 1, 24), (4, 2, 200)])
 def test_attention_split_over_many_keys(dev, dtype, cdt, H, KVH, n):
