@@ -741,9 +741,10 @@ def _stream_on(index: int) -> int:
 
 def _head_rows(t: torch.Tensor, name: str):
     """(rows, heads, head_dim, row stride) of rows whose heads lie side by side."""
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [rows, heads, head_dim]")
-    (rows, heads, hd), (ld, step, unit) = t.shape, t.stride()
+    try:
+        (rows, heads, hd), (ld, step, unit) = t.shape, t.stride()
+    except ValueError:
+        raise ValueError(f"{name} must be [rows, heads, head_dim]") from None
     if unit != 1 or (step != hd and heads > 1):
         raise ValueError(f"{name} must be [rows, heads, head_dim] with contiguous heads")
     return rows, heads, hd, ld if rows > 1 else heads * hd
@@ -753,12 +754,13 @@ def _rope_angles(table: torch.Tensor | None, index: int):
     """(pointer, rows, rot_dim) of a checked rotary table; None: no rotation."""
     if table is None:
         return None, 0, 0
-    if table.dtype is not torch.float32 or table.dim() != 3 or table.shape[2] != 2 or \
+    shape = table.shape
+    if len(shape) != 3 or shape[2] != 2 or table.dtype is not torch.float32 or \
             not table.is_contiguous():
         raise ValueError("a rotary table is contiguous float32 [positions, rot_dim / 2, 2]")
     if table.get_device() != index:
         raise ValueError("the rotary table must be on the tensors' device")
-    rows, half, _ = table.shape
+    rows, half, _ = shape
     if rows == 0 or half == 0:
         raise ValueError("the rotary table is empty")
     return table.data_ptr(), rows, 2 * half

@@ -127,9 +127,10 @@ def _batch(cache, rows, block_table, pos0, row_start, max_rows):
     """(stream, sequences, columns, row_start pointer, max_rows) of a checked batch."""
     index = cache.index
     stream = _stream_on(index)
-    if block_table.dim() != 2 or not block_table.is_contiguous():
+    shape = block_table.shape
+    if len(shape) != 2 or not block_table.is_contiguous():
         raise ValueError("block_table must be contiguous [sequences, columns]")
-    S, cols = block_table.shape
+    S, cols = shape
     if pos0.shape != (S,) or not pos0.is_contiguous():
         raise ValueError("pos0 must be contiguous [sequences]")
     if block_table.dtype is not torch.int32 or pos0.dtype is not torch.int32:
@@ -162,8 +163,8 @@ def paged_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
     sequence are not written. (project_qkv + slice_assign,
     summa-llm/src/model/attention.rs:142-177, 331-356.)"""
     rows, heads, ldk = _rows(cache, k, "k")
-    _, _, ldv = _rows(cache, v, "v")
-    if heads != cache.kv_heads or v.shape != k.shape:
+    v_rows, v_heads, ldv = _rows(cache, v, "v")
+    if heads != cache.kv_heads or v_heads != heads or v_rows != rows:
         raise ValueError(f"k and v must be [rows, {cache.kv_heads}, {cache.head_dim}]")
     dt = _ROWS.get(k.dtype)
     if dt is None or v.dtype is not k.dtype or (q is not None and q.dtype is not k.dtype):
