@@ -460,8 +460,9 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
 // Four or eight waves x 32 rows (v_mfma_f32_32x32x16), two waves a SIMD. A tile of 64 keys, in
 // 16 bits, sits in one of two LDS buffers; the next tiles' loads are on their way during this
 // one's products and are converted and stored before the barrier that ends it.
-// 2 x 1024 tokens on 24-32 k keys, 16 / 4 heads of 128, f16 queries, e4m3 (eight waves): 0.51 ms,
-// 1.01 PF/s, 85 % of what a large f16 product reaches; the clock is down to 1.9 GHz then.
+// 2 x 1024 tokens on 24-32 k keys, 16 / 4 heads of 128, f16 queries, e4m3 (eight waves): 0.51-0.53
+// ms from card to card, 0.98-1.01 PF/s, 84 % of what a large f16 product reaches; the clock is
+// down to 1.84 GHz, the matrix cores work 47 % and the vector units 49 % of the cycles.
 // Of four waves' 563 us, staging took 91, the barriers 10, the exponentials 44, the sums 16.
 // Prefill of 32 prompts of 257-512 (four waves): 48 us: 1.75 us a tile and 5.6 us a workgroup
 // for two round trips to memory and its output.
