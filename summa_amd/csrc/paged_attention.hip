@@ -467,9 +467,10 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
 // Prefill of 32 prompts of 257-512 (four waves): 48 us: 1.75 us a tile and 5.6 us a workgroup
 // for two round trips to memory and its output.
 // Tried and slower: scores of the next tile beside this one's softmax on 32-key tiles (670
-// beside 637 us at the time), three workgroups a unit (618 beside 583), four times and twice the splits (the join's bytes), workgroups that go
-// on to further row tiles with their first loads in flight (prefill 65 beside 50 us), output and
-// query rows kept out of the L2 (60 beside 53; the output alone: the same).
+// beside 637 us at the time), three workgroups a unit (618 beside 583), two and four times the
+// splits (the join's bytes), workgroups that go on to further row tiles with their first loads
+// in flight (prefill 65 beside 50 us), half a last tile left out (spills), output and query
+// rows kept out of the L2 (60 beside 53; the output alone: the same).
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <bool F16>
@@ -742,7 +743,8 @@ struct TileSweep {
 #pragma unroll
         for (int e = 0; e < 16; ++e) sc[g / 2][e] = 0.f;
 #pragma unroll
-      for (int i = 0; i < KG; ++i) sc[g / 2] = mfma32<QF16>(kfr[g % 2][i], qa[g % 2 * KG + i], sc[g / 2]);
+      for (int i = 0; i < KG; ++i)
+        sc[g / 2] = mfma32<QF16>(kfr[g % 2][i], qa[g % 2 * KG + i], sc[g / 2]);
       __builtin_amdgcn_sched_barrier(0);
       if (g + 2 < NB) read_k(g + 2);
       else read_v(g + 2 - NB);
