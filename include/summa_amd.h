@@ -428,8 +428,8 @@ int sm_attention_backward(const float* q, const float* k, const float* v, const 
  *   rotated where they lie; y == x (with ldy == ldx) is allowed, other overlaps are
  *   not. dtype SM_F32, SM_BF16 or SM_F16 (f32 arithmetic, one rounding); head_dim a
  *   multiple of 16 up to 1024, rot_dim a multiple of 16 up to head_dim; rows, x, y and
- *   table 16-byte aligned. A position outside [0, table_rows) gives NaN;
- *   table_rows > 0.
+ *   table 16-byte aligned, rows below 2^26 - 4. A position outside [0, table_rows) gives
+ *   NaN; table_rows > 0.
  */
 enum { SM_ROPE_INTERLEAVED = 0, SM_ROPE_HALF = 1 };
 enum {
@@ -500,6 +500,7 @@ int sm_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, const f
  *   workspace: sm_paged_attention_workspace_bytes(...) bytes (-1 for a bad shape; 0 where
  *   the keys are not split, so always for max_tokens <= 512), 16-byte aligned, for the
  *   partial sums of the splits; calls that share one must not overlap.
+ * Both return SM_ERR_UNSUPPORTED where a grid of 2^24 workgroups does not hold the batch.
  * Every length is read on the device, so a captured call may be replayed with other
  * contents of the batch's arrays, up to max_rows.
  */
