@@ -12,15 +12,18 @@
 // over keys may run in any order, and V is stored in that order. P never leaves the
 // registers, and nothing is transposed on the way.
 // - The softmax is one pass with a running maximum and sum in f32, in units of log2. The
-//   maximum is raised only when a score passes it by more than 8 (weights then reach 2^8, far
-//   from f16's 65504), so most steps neither reduce over lanes nor rescale O.
+//   reference that weights are taken from is raised only when a score passes it by more than
+//   kWeightMost, so most steps neither reduce over lanes nor rescale O.
 // - An 8-bit block's K scale is a factor on its scores. Its V scale 2^e goes into the weights:
 //   t = score + e is what the running maximum is taken of, P' = 2^(t - max) multiplies the bare
 //   codes, and the sum gets 2^-e P' back. P' is at most 2^8 whatever the scales are, and a
 //   block with small values loses no accuracy to one with large ones.
 // - P' is rounded to f16 for 8-bit and f16 values (codes are exact in f16), to bf16 for bf16
 //   ones, whose range f16 does not hold: at most half a step (2^-11, 2^-8) of each weight,
-//   like the one rounding of the output. The 16-row kernel multiplies the rest of each weight
+//   like the one rounding of the output. In f16 weights fill the type's range: the largest is
+//   2^11 to 2^15 (f16 ends at 65504), so that only those 25 binary orders below it lose bits
+//   and those 36 below it all. (131 k keys 26 orders below one dominant key have 0.2 % of the
+//   sum; with the largest weight at 1 all of that would be lost.) The 16-row kernel multiplies the rest of each weight
 //   too, in 16 bits again, which costs it 1-2 % (its matrix cores wait for memory) and leaves
 //   the output's rounding: error of a rollout step in f16 2.1e-4 with it, 2.6e-4 without.
 //   Scores, maxima, sums and O stay in f32.
@@ -74,6 +77,13 @@ __device__ inline f4 mfma16(u32x4 a, u32x4 b, f4 c) {
   return Op8<F16>::mfma(__builtin_bit_cast(typename Op8<F16>::T, a),
                         __builtin_bit_cast(typename Op8<F16>::T, b), c);
 }
+// log2 of what the largest weight is where the reference is raised, and of what it may reach
+// before the next time. (2 x 1024 rows on 24-32 k keys 536 us, prefill of 32 prompts 50.7; with
+// 0 and 8 532 and 49.3, with 7 and 15 533 and 49.5, with 13 and 15 539 and 50.9, each with its
+// share of weights lost.) bf16 weights have f32's range and stay at 1, for sums of large values.
+__device__ constexpr float kWeight(bool f16) { return f16 ? 11.f : 0.f; }
+__device__ constexpr float kWeightMost(bool f16) { return f16 ? 15.f : 8.f; }
+
 template <bool F16>
 __device__ inline uint32_t pack2(float a, float b) {
   if constexpr (F16) {
@@ -332,10 +342,10 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
           odd |= __ballot(x) != 0;
         }
       }
-      if (__ballot(mx > m + 8.f)) {
+      if (__ballot(mx > m + kWeightMost(PF16))) {
         mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
         mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-        const float mn = fmaxf(m, mx);
+        const float mn = fmaxf(m, mx - kWeight(PF16));
         const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
         m = mn;
         l *= f;
@@ -773,9 +783,9 @@ struct TileSweep {
                            fmaxf(z[e + 6], z[e + 7]));
       mx = fmaxf(mx, C8 ? fmaf(x, kf[b], vf[b]) : x * kf[b]);
     }
-    if (__ballot(mx > m + 8.f)) {
+    if (__ballot(mx > m + kWeightMost(PF16))) {
       mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-      const float mn = fmaxf(m, mx);
+      const float mn = fmaxf(m, mx - kWeight(PF16));
       const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= f;
