@@ -16,8 +16,15 @@
 //   kWeightMost, so most steps neither reduce over lanes nor rescale O.
 // - An 8-bit block's K scale is a factor on its scores. Its V scale 2^e goes into the weights:
 //   t = score + e is what the running maximum is taken of, P' = 2^(t - max) multiplies the bare
-//   codes, and the sum gets 2^-e P' back. P' is at most 2^8 whatever the scales are, and a
-//   block with small values loses no accuracy to one with large ones.
+//   codes, and P' stays in its type's range whatever the scales are. A value's error is that of
+//   its weight, relative to the largest |weight x scale| that the row has.
+// - The sum of the weights, without their scales, is 2^-e P' block by block while every scale
+//   so far is at most 2^kScaleSmall: a P' that f32 rounds to zero then has a weight of less
+//   than 2^-50 of the largest. Behind a larger scale it is taken of the scores themselves, with
+//   exponentials of its own. It is held kSumShift binary orders up, where the 183 orders between
+//   the least and the largest scale lie inside f32 (weights 33 orders below the largest may still
+//   be left out, where all values of that one pass 2^120), and moved in two factors that f32
+//   holds where the product of both is less than it does.
 // - P' is rounded to f16 for 8-bit and f16 values (codes are exact in f16), to bf16 for bf16
 //   ones, whose range f16 does not hold: at most half a step (2^-11, 2^-8) of each weight,
 //   like the one rounding of the output. In f16 weights fill the type's range: the largest is
@@ -83,6 +90,26 @@ __device__ inline f4 mfma16(u32x4 a, u32x4 b, f4 c) {
 // share of weights lost.) bf16 weights have f32's range and stay at 1, for sums of large values.
 __device__ constexpr float kWeight(bool f16) { return f16 ? 11.f : 0.f; }
 __device__ constexpr float kWeightMost(bool f16) { return f16 ? 15.f : 8.f; }
+
+constexpr int kScaleSmall = 17;  // (8-bit) values up to 5.9e7 need no care in the sum
+__device__ constexpr float kSumShift(bool c8) { return c8 ? 20.f : 0.f; }
+// Factor of a block's sum of P' in the sum of weights; zero: taken of the scores. (A block behind
+// the last key may have any scale byte: its P' are zero, the factor has to be finite.)
+template <bool C8>
+__device__ inline float sum_factor(float vexp, bool large) {
+  return !C8 ? 1.f : large ? 0.f : __builtin_amdgcn_exp2f(fminf(kSumShift(true) - vexp, 100.f));
+}
+// log2 and reciprocal of a sum that is held up
+template <bool C8>
+__device__ inline float sum_log2(float m, float l) {
+  return m + ((float)__builtin_amdgcn_frexp_expf(l) - kSumShift(C8)) +
+         __log2f(__builtin_amdgcn_frexp_mantf(l));
+}
+template <bool C8>
+__device__ inline float sum_inverse(float l) {
+  return (C8 ? 1048576.f : 1.f) / l;
+}
+static_assert(kSumShift(true) == 20.f, "2^20 is sum_inverse's");
 
 template <bool F16>
 __device__ inline uint32_t pack2(float a, float b) {
@@ -177,12 +204,19 @@ __device__ inline void fix_odd(const PagedArgs& a, const int32_t* trow, int kvh,
     }
 }
 
-// Weight of a partial sum with the maximum m and the sum l of weights among those whose
-// maximum is mm: zero without keys (m -inf, l 0), else positive, so that what it has of an
-// infinity stays.
-__device__ inline float join_weight(float m, float l, float mm) {
-  return m == -INFINITY ? (l == 0.f ? 0.f : NAN)
-                        : fmaxf(__builtin_amdgcn_exp2f(m - mm), 1.1754943508e-38f);
+// Partial sums (m, l, o) of one row join as sum l f and sum o f, f = 2^(m - mm) with the largest
+// m of them: half of f's exponent is kept, so that l, which scales may hold far up or down, is
+// multiplied by two factors that f32 holds. Without keys (m -inf, l 0) it is zero.
+struct Join {
+  float half;
+  __device__ inline Join(float m, float l, float mm)
+      : half(m == -INFINITY ? (l == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(0.5f * (m - mm))) {}
+  __device__ inline float sum(float l) const { return l * half * half; }
+  __device__ inline float weight() const { return half * half; }
+};
+// A part of O times its weight; one that is not finite stays what it is, as a weight is positive.
+__device__ inline float join_o(float o, float weight, float acc) {
+  return fabsf(o) < INFINITY ? fmaf(o, weight, acc) : acc + o;
 }
 
 // Where 64 blocks of a sequence lie, one to a lane, and their scales.
@@ -207,6 +241,11 @@ struct Blocks {
   template <bool C8>
   __device__ inline float vexp() const {
     return C8 ? (float)(ve - 127) : 0.f;
+  }
+  // Whether any of the first n of these blocks has a scale above 2^kScaleSmall (uniform).
+  template <bool C8>
+  __device__ inline bool large(int n) const {
+    return C8 && __ballot((int)(threadIdx.x % kWave) < n && !none && ve > 127 + kScaleSmall) != 0;
   }
 };
 
@@ -267,14 +306,16 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
 #pragma unroll
   for (int n = 0; n < NT; ++n) o[n] = f4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
-  bool odd = false;  // values that are not finite, among keys that not all rows see
+  bool odd = false;    // values that are not finite, among keys that not all rows see
+  bool large = false;  // scales of V above 2^kScaleSmall, up to here
 
   for (int seg = b0; seg < b1; seg += kWave, cur = next) {
     const int nb = min(kWave, b1 - seg);
     if (seg + kWave < b1) next.find(a, trow, kvh, seg + kWave + lane);
+    large |= cur.template large<C8>(nb);
     for (int st = wave * NB; st < nb; st += 4 * NB) {
       u32x4 kr[NB][NC], vr[NB][NC];
-      float ksc[NB], vex[NB];
+      float ksc[NB], vex[NB], lf[NB];
 #pragma unroll
       for (int u = 0; u < NB; ++u) {
         const size_t at = (size_t)__builtin_amdgcn_readlane(cur.at, min(st + u, nb - 1)) * BB;
@@ -287,10 +328,12 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
       }
       __builtin_amdgcn_sched_barrier(0);  // (the scales are waited for behind these loads)
       const float kscale = cur.template kscale<C8>(a.c2), vexp = cur.template vexp<C8>();
+      const float factor = sum_factor<C8>(vexp, large);
 #pragma unroll
       for (int u = 0; u < NB; ++u) {
         ksc[u] = lane_f32(kscale, min(st + u, nb - 1));
         vex[u] = lane_f32(vexp, min(st + u, nb - 1));
+        lf[u] = lane_f32(factor, min(st + u, nb - 1));
       }
       // scores, in units of log2 and raised by the exponent of V's scale
       float t[NB][4];
@@ -346,13 +389,20 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
         mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
         mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
         const float mn = fmaxf(m, mx - kWeight(PF16));
-        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        const Join j(m, l, mn);
         m = mn;
-        l *= f;
+        l = j.sum(l);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) o[n] *= f;
+        for (int n = 0; n < NT; ++n) o[n] *= j.weight();
       }
       const float ms = m == -INFINITY ? 0.f : m;
+      if (C8 && large) {  // (uniform)
+#pragma unroll
+        for (int u = 0; u < NB; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            l += __builtin_amdgcn_exp2f(t[u][i] - vex[u] - (ms - kSumShift(C8)));
+      }
       u32x4 p[NB / 2], rest[NB / 2];  // rest: what 16 bits leave of the weights
 #pragma unroll
       for (int u = 0; u < NB; ++u) {
@@ -360,7 +410,7 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(t[u][i] - ms);
         sum = (e[0] + e[1]) + (e[2] + e[3]);
-        l = C8 ? fmaf(sum, __builtin_amdgcn_exp2f(-vex[u]), l) : l + sum;
+        l = C8 ? fmaf(sum, lf[u], l) : l + sum;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t w = pack2<PF16>(e[2 * i], e[2 * i + 1]);
@@ -432,15 +482,16 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
   float ll = 0.f, f[4];
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    f[w] = join_weight(sm_m[w][y], sm_l[w][y], mm);
-    ll = fmaf(sm_l[w][y], f[w], ll);
+    const Join j(sm_m[w][y], sm_l[w][y], mm);
+    f[w] = j.weight();
+    ll += j.sum(sm_l[w][y]);
   }
   float acc[HD / 16];
 #pragma unroll
   for (int i = 0; i < HD / 16; ++i) {
     acc[i] = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) acc[i] = fmaf(sm_o[w][y][d0 + i], f[w], acc[i]);
+    for (int w = 0; w < 4; ++w) acc[i] = join_o(sm_o[w][y][d0 + i], f[w], acc[i]);
   }
   const size_t at = (size_t)(pr.first + tok) * a.H.d + head;
   if (pk.splits > 1) {
@@ -453,7 +504,7 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
     return;
   }
   const bool none = pos0 + tok < 0;  // a row without keys
-  const float inv = 1.f / ll;
+  const float inv = sum_inverse<C8>(ll);
   uint32_t w2[HD / 32];
 #pragma unroll
   for (int i = 0; i < HD / 32; ++i)
@@ -462,7 +513,7 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
 #pragma unroll
   for (int i = 0; i < HD / 32; ++i) op[i] = w2[i];
   if (a.lse && d0 == 0)
-    a.lse[at] = none ? -INFINITY : (mm + __log2f(ll)) * 0.69314718055994530942f;
+    a.lse[at] = none ? -INFINITY : sum_log2<C8>(mm, ll) * 0.69314718055994530942f;
 }
 
 // ---- more query rows: 128 of them a workgroup, keys staged through LDS ----
@@ -515,7 +566,8 @@ struct TileSweep {
   struct Lds {
     __attribute__((aligned(16))) uint16_t ks[2][kTile * KP];
     __attribute__((aligned(16))) uint16_t vts[2][HD * VP];
-    __attribute__((aligned(16))) float info[2][NB][2];  // a block's score factor and V exponent
+    // a block's score factor, V exponent and factor of its weights' sum
+    __attribute__((aligned(16))) float info[2][NB][4];
     int odd;
   };
 
@@ -530,6 +582,7 @@ struct TileSweep {
 
   Blocks cur, next;  // of the 64 blocks at hand, and of the next
   bool missing;      // any of those at hand has keys and no page
+  bool large;        // scales of V above 2^kScaleSmall, up to those at hand
   u32x4 kr[PER], vr[PER];
 
   __device__ TileSweep(const PagedArgs& a_, Lds& s_) : a(a_), s(s_) {}
@@ -555,6 +608,11 @@ struct TileSweep {
   // Whether blocks with keys have no page, of the 64 from `first` on (uniform).
   __device__ inline bool any_missing(const Blocks& of, int first) const {
     return __ballot(of.none && (first + lane) * kBlock < keys) != 0;
+  }
+  // `cur` is the 64 blocks from `first` on.
+  __device__ inline void at_hand(int first) {
+    missing = any_missing(cur, first);
+    large |= cur.template large<C8>(b1 - first);
   }
   // Values that are not the cache's, or that only some rows see, out of what is staged.
   __device__ inline void mask_tile(int blk, const Blocks& of) {
@@ -617,7 +675,8 @@ struct TileSweep {
     }
     // (wave 0's lanes that hold the tile's blocks)
     const unsigned i = (unsigned)(threadIdx.x - (blk - b0) % kWave);
-    if (i < NB) *reinterpret_cast<float2*>(s.info[buf][i]) = float2{kscale, vexp};
+    if (i < NB)
+      *reinterpret_cast<f4*>(s.info[buf][i]) = f4{kscale, vexp, sum_factor<C8>(vexp, large), 0.f};
   }
 
   // The next tile, on its way, to LDS, and the one after it on its way.
@@ -627,7 +686,7 @@ struct TileSweep {
     if (to >= b1) return;
     if ((to - b0) % kWave == 0) {
       cur = next;
-      missing = any_missing(cur, to);
+      at_hand(to);
       if (to + kWave < b1) next.find(a, trow, kvh, to + kWave + lane);
     }
     load_tile(to);
@@ -647,7 +706,8 @@ struct TileSweep {
     if (threadIdx.x == 0) s.odd = 0;
     __syncthreads();
     load_tile(b0);
-    missing = any_missing(cur, b0);
+    large = false;
+    at_hand(b0);
     store_tile(b0, 0, cur);
     __syncthreads();
     int buf = 0;
@@ -673,7 +733,7 @@ struct TileSweep {
         if (more) {
           if ((blk + NB - b0) % kWave == 0) {
             cur = next;
-            missing = any_missing(cur, blk + NB);
+            at_hand(blk + NB);
           }
           load_tile(blk + NB);
         }
@@ -718,12 +778,13 @@ struct TileSweep {
 
   __device__ inline void tile(int buf, int key0) {
     f32x16 sc[kTile / 32];
-    float kf[NB], vf[NB];
+    float kf[NB], vf[NB], lf[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const float2 x = *reinterpret_cast<const float2*>(s.info[buf][b]);
-      kf[b] = x.x;
-      vf[b] = x.y;
+      const f4 x = *reinterpret_cast<const f4*>(s.info[buf][b]);
+      kf[b] = x[0];
+      vf[b] = x[1];
+      lf[b] = x[2];
     }
     constexpr int KG = KS / 2;  // steps of a group of key fragments; two groups in flight
     u32x4 kfr[2][KG];
@@ -786,15 +847,22 @@ struct TileSweep {
     if (__ballot(mx > m + kWeightMost(PF16))) {
       mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
       const float mn = fmaxf(m, mx - kWeight(PF16));
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      const Join j(m, l, mn);
       m = mn;
-      l *= f;
+      l = j.sum(l);
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[d][e] *= f;
+        for (int e = 0; e < 16; ++e) o[d][e] *= j.weight();
     }
     const float ms = m == -INFINITY ? 0.f : m;
+    if (C8 && __builtin_amdgcn_readfirstlane(__float_as_int(lf[0])) == 0) {  // (of all blocks)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          l += __builtin_amdgcn_exp2f(fmaf(sc[b / 2][8 * (b % 2) + e], kf[b], kSumShift(C8) - ms));
+    }
     u32x4 p[NB];  // P^T of a block's 16 keys
 #pragma unroll
     for (int b = 0; b < NB + 1; ++b) {
@@ -811,7 +879,7 @@ struct TileSweep {
           sum += y;
           p[b][e] = pack2<PF16>(x, y);
         }
-        l = C8 ? fmaf(sum, __builtin_amdgcn_exp2f(-vf[b]), l) : l + sum;
+        l = C8 ? fmaf(sum, lf[b], l) : l + sum;
       }
       if (b > 0) {
 #pragma unroll
@@ -890,7 +958,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_tile_kernel(PagedArgs a) {
   }
   // Through LDS, so that a store instruction writes whole rows: a lane holds 8 bytes of its
   // row at a time, and 16-byte pieces of 32 rows reach the L2 as as many requests.
-  const float inv = 1.f / l;
+  const float inv = sum_inverse<C8>(l);
   const bool none = pos0 + tok < 0;  // a row without keys
   constexpr int OP = HD + 8;
   uint16_t* lo = &lds.ks[0][0] + t.wave * 32 * OP;  // (the buffers are free)
@@ -904,7 +972,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_tile_kernel(PagedArgs a) {
       *reinterpret_cast<u32x2*>(lo + j * OP + d * 32 + 8 * i + 4 * hf) = none ? u32x2{0u, 0u} : w;
     }
   if (a.lse && hf == 0 && row < all)
-    a.lse[at] = none ? -INFINITY : (m + __log2f(l)) * 0.69314718055994530942f;
+    a.lse[at] = none ? -INFINITY : sum_log2<C8>(m, l) * 0.69314718055994530942f;
   __builtin_amdgcn_wave_barrier();  // (one wave's rows: its LDS accesses are in order)
   constexpr int LR = HD / 8;        // lanes of a row
 #pragma unroll
@@ -935,12 +1003,12 @@ __device__ inline void add_splits(const float* po, float weight, int x, int lane
   for (int k = 0; k < N; ++k) {
     const float w = lane_f32(weight, x + k);
 #pragma unroll
-    for (int d = 0; d < D; ++d) acc[d] = fmaf(y[k][d], w, acc[d]);
+    for (int d = 0; d < D; ++d) acc[d] = join_o(y[k][d], w, acc[d]);
   }
 }
 
 // Joins the splits of a (row, head): one wave each.
-template <int HD, bool QF16>
+template <int HD, bool QF16, bool C8>
 __global__ __launch_bounds__(256, 8) void paged_join_kernel(PagedArgs a) {
   int s = (int)(blockIdx.x * 4 + threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
@@ -966,8 +1034,9 @@ __global__ __launch_bounds__(256, 8) void paged_join_kernel(PagedArgs a) {
   for (int x0 = 0; x0 < pk.splits; x0 += kWave) {
     const int n = min(kWave, pk.splits - x0);
     const float2 v = lane < n ? ml[x0 + lane] : float2{-INFINITY, 0.f};
-    const float f = join_weight(v.x, v.y, mm);
-    ll += wave_sum(v.y * f);
+    const Join j(v.x, v.y, mm);
+    const float f = j.weight();
+    ll += wave_sum(j.sum(v.y));
     int x = 0;
     for (; x + 16 <= n; x += 16) add_splits<HD, 16>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
     for (; x + 8 <= n; x += 8) add_splits<HD, 8>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
@@ -975,7 +1044,7 @@ __global__ __launch_bounds__(256, 8) void paged_join_kernel(PagedArgs a) {
     if (x < n) add_splits<HD, 1>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
   }
   const bool none = pos0 + i < 0;
-  const float inv = 1.f / ll;
+  const float inv = sum_inverse<C8>(ll);
 #pragma unroll
   for (int d = 0; d < D; ++d) {
     const float v = none ? 0.f : acc[d] * inv;
@@ -985,7 +1054,7 @@ __global__ __launch_bounds__(256, 8) void paged_join_kernel(PagedArgs a) {
       static_cast<uint16_t*>(a.out)[at * HD + lane * D + d] = f32_to_bf16(v);
   }
   if (a.lse && lane == 0)
-    a.lse[at] = none ? -INFINITY : (mm + __log2f(ll)) * 0.69314718055994530942f;
+    a.lse[at] = none ? -INFINITY : sum_log2<C8>(mm, ll) * 0.69314718055994530942f;
 }
 
 // How a call is split: rows of a workgroup, key blocks of a split and splits.
@@ -1174,7 +1243,7 @@ extern "C" int sm_paged_attention(const sm_paged_cache* cache, const int32_t* bl
     else if constexpr (HD == 128)                                                \
       paged_tile_kernel<HD, F, C, 8><<<(unsigned)plan.wgs, 512, 0, st>>>(a);     \
     if (plan.nsplit > 1)                                                         \
-      paged_join_kernel<HD, F><<<(unsigned)joins, 256, 0, st>>>(a);              \
+      paged_join_kernel<HD, F, C><<<(unsigned)joins, 256, 0, st>>>(a);              \
   } while (0)
 #define SM_PAGED(HD)                             \
   do {                                           \
