@@ -500,7 +500,9 @@ int sm_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, const f
  *   workspace: sm_paged_attention_workspace_bytes(...) bytes (-1 for a bad shape; 0 where
  *   the keys are not split, so always for max_tokens <= 512), 16-byte aligned, for the
  *   partial sums of the splits; calls that share one must not overlap.
- * Both return SM_ERR_UNSUPPORTED where a grid of 2^24 workgroups does not hold the batch.
+ * Both return SM_ERR_UNSUPPORTED where a grid of 2^24 workgroups does not hold the batch
+ * (attention: S * kv_heads tiles of 128 rows each, of max_rows * H / kv_heads rows), for 2^31 and
+ * more rows of a KV head or 2^40 of all heads.
  * Every length is read on the device, so a captured call may be replayed with other
  * contents of the batch's arrays, up to max_rows.
  */

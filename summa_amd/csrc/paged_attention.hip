@@ -1099,6 +1099,7 @@ struct PagedPlan {
     cb = (int)(ceil_div(std::max<int64_t>(32, ceil_div(blocks, want)), 16) * 16);
     nsplit = (int)ceil_div(blocks, cb);
   }
+  int64_t threads() const { return wgs * (tile == 256 ? 512 : 256); }
   int64_t bytes(int64_t rows, int64_t H, int64_t hd) const {
     return nsplit > 1 ? rows * H * nsplit * (hd + 2) * 4 : 0;
   }
@@ -1113,11 +1114,15 @@ int check_shape(const char* who, int64_t S, int64_t rows, int64_t max_rows, int6
              "%s: H must be a multiple of KVH, at most 65535", who);
   SM_REQUIRE(hd == 64 || hd == 128, "%s: head_dim must be 64 or 128", who);
   SM_REQUIRE(max_tokens >= 0 && max_tokens <= most, "%s: max_tokens must be in 0..2^31 - 1", who);
-  // (the grid holds less than 2^24 workgroups of 256 threads, and 32 bits index a row)
-  if (max_rows * (H / KVH) >= most ||
-      (double)S * (double)ceil_div(max_rows * (H / KVH), 16) * (double)KVH >= (double)(1 << 24) ||
-      (double)S * (double)max_rows * (double)H >= (double)(1 << 26) ||
-      (double)rows * (double)H >= (double)((int64_t)1 << 40)) {  // (bytes: below 2^60)
+  if (S == 0 || max_rows == 0) return SM_OK;
+  const int64_t all = max_rows * (H / KVH);
+  // 32 bits index a row of a KV head; the workspace's bytes stay below 2^60; and a grid holds less
+  // than 2^32 threads. (The plan's counts fit 64 bits behind the test before it: a workgroup
+  // takes 256 rows at most. Keys are split where there are at most 2^16 rows, a wave of the join
+  // each.)
+  if (all >= most || (double)rows * (double)H >= (double)((int64_t)1 << 40) ||
+      (double)S * (double)KVH * (double)ceil_div(all, 256) >= (double)(1 << 24) ||
+      PagedPlan(S, max_rows, H / KVH, KVH, hd, max_tokens).threads() >= (int64_t)1 << 32) {
     set_error("%s: problem too large", who);
     return SM_ERR_UNSUPPORTED;
   }
@@ -1193,10 +1198,6 @@ extern "C" int sm_paged_attention(const sm_paged_cache* cache, const int32_t* bl
                  oa + (size_t)(rows * H * hd) * 2 <= qa,
              "%s: out must not overlap q", me);
   const int64_t joins = ceil_div(S * max_rows * H, 4);
-  if (plan.wgs >= (1 << 24) || joins >= (1 << 24)) {
-    set_error("%s: problem too large", me);
-    return SM_ERR_UNSUPPORTED;
-  }
   hipStream_t st = as_stream(stream);
   PagedArgs a;
   a.k = static_cast<const uint8_t*>(cache->k);
