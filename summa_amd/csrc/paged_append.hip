@@ -66,14 +66,6 @@ __device__ inline void load_dims(const T* p, float (&f)[D]) {
     }
   }
 }
-template <typename T, int D>
-__device__ inline void store_dims(T* p, const float (&f)[D]) {
-  if constexpr (D == 8) {
-    store8<T>(p, f);
-  } else {
-    *reinterpret_cast<u32x2*>(p) = u32x2{round2<T>(f[0], f[1]), round2<T>(f[2], f[3])};
-  }
-}
 
 // Four f32 -> e4m3 codes (nearest even), the first in the low byte.
 __device__ inline uint32_t pack_e4m3(float a, float b, float c, float d) {
