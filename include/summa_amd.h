@@ -495,6 +495,13 @@ int sm_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int dtype, const f
  *   them; an infinity that it sees makes its sum infinite, whatever its weight (so do sums
  *   that pass f32: bf16 values beyond 2^88 may). (forward_cached / sdpa,
  *   attention.rs:216-265, 318-371.)
+ *   Scores, the softmax's maximum and sum, and O are f32. The products with V take weights in
+ *   16 bits: f16 for 8-bit and f16 caches (those 25 and more binary orders below a row's largest
+ *   weight times scale keep fewer bits, those 36 below none), bf16 for bf16 ones. With up to 16
+ *   rows a KV head (max_rows * H / kv_heads) what that rounding leaves is multiplied as well, and
+ *   the error is the output's rounding; with more it is not: half a step of each weight, 2^-11
+ *   of it in f16 and 2^-8 in bf16, comes on top (over random keys about as much
+ *   as the output's own rounding to the same type).
  *   max_tokens: the tokens of the longest sequence, new rows included; it only decides
  *   how the keys are split, a longer sequence is still attended to in full.
  *   workspace: sm_paged_attention_workspace_bytes(...) bytes (-1 for a bad shape; 0 where

@@ -206,7 +206,9 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_table: torch.Ten
     head_dim] (``out`` where given; rows of no sequence are not written) and, with
     ``want_lse``, lse [rows, H] f32. ``max_tokens``: the longest sequence, new rows
     included (default: what the block table can hold); it decides how the keys are
-    split, not which are read. (forward_cached / sdpa,
+    split, not which are read. With more than 16 rows a KV head (``max_rows * H / kv_heads``)
+    softmax weights are rounded once to 16 bits, bf16 for a bf16 cache and f16 else; with up to
+    16 the error is the output's rounding alone. (forward_cached / sdpa,
     summa-llm/src/model/attention.rs:216-265, 318-371.)"""
     rows, H, ldq = _rows(cache, q, "q")
     dt = _ROWS.get(q.dtype)
