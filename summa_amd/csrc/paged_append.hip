@@ -15,8 +15,10 @@
 // or two of the stored block a dim; the block goes through LDS to be stored as it lies.
 // Bound by memory: 12.6 k bf16 rows of 16 + 2 x 4 heads of 128 into an e4m3 cache (146 MB read
 // and written) 33 us, 4.5 TB/s; 4.6 k f16 rows of 36 heads of 64 into an f16 cache (48 MB)
-// 11.3 us. A step of 256 sequences, one token each, is 8 us of three round trips (lengths,
-// page, scale) in 9.7 us of the host's call.
+// 11.3 us. A step of 256 sequences, one token each, is 8 us of round trips to memory, one behind
+// the other - a key's wave waits for the lengths, its rows and angles, the page and the block's
+// scale, a value's for the lengths, the page, its rows, the scale and the block as it was - in
+// 9.7 us of the host's call.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

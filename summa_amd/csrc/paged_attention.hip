@@ -259,8 +259,8 @@ struct Blocks {
 // as the matrix cores take them, 16 bytes a lane and load; 8-bit codes are converted there
 // (one instruction for two). v_mfma_f32_16x16x32: a score tile is 16 keys x 16 rows.
 // 256 sequences of 512-1023 tokens, 16 / 4 heads of 128, e4m3 (202 MB): 42 us, 4.8 TB/s; 4 of
-// 100-131 k (483 MB): 94 us, 5.1; 48 x 4 rows of 1-4 k, 16 heads, bf16 (1.08 GB): 205 us, 5.3,
-// where a copy on this card moves 4.9. Two blocks a step beside four: the same time with 40
+// 100-131 k (483 MB): 96-98 us, 5.0; 48 x 4 rows of 1-4 k, 16 heads, bf16 (1.08 GB): 206-216 us,
+// 5.0-5.3, where a copy on this card moves 4.8. Two blocks a step beside four: the same time with 40
 // registers fewer; four workgroups a unit (128 registers): no faster.
 constexpr int kRows16 = 16;  // query rows of a workgroup
 
@@ -525,11 +525,16 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
 // 16 bits, sits in one of two LDS buffers; the next tiles' loads are on their way during this
 // one's products and are converted and stored before the barrier that ends it.
 // 2 x 1024 tokens on 24-32 k keys, 16 / 4 heads of 128, f16 queries, e4m3 (eight waves): 0.51-0.53
-// ms from card to card, 0.98-1.01 PF/s, 84 % of what a large f16 product reaches; the clock is
-// down to 1.84 GHz, the matrix cores work 47 % and the vector units 49 % of the cycles.
+// ms from card to card, 0.98-1.02 PF/s, 84 % of what a large f16 product reaches; the clock is
+// down to 1.88 GHz, the matrix cores work 46 % and the vector units 48 % of the cycles. With V
+// scales above 2^kScaleSmall, whose sum has exponentials of its own, 491 us where it is 434
+// (1024 rows on 28 k keys).
 // Of four waves' 563 us, staging took 91, the barriers 10, the exponentials 44, the sums 16.
-// Prefill of 32 prompts of 257-512 (four waves): 48 us: 1.75 us a tile and 5.6 us a workgroup
+// Prefill of 32 prompts of 257-512 (four waves): 50 us: 1.75 us a tile and 5.6 us a workgroup
 // for two round trips to memory and its output.
+// bf16 cache: 2 x 1024 tokens on 28 k keys 484-497 us (0.97 PF/s), 16 x 512 on 2 k 192 (0.81); f16
+// cache: 8 x 512 on 4 k 163 (0.90), e4m3 there 154. Heads of 64, where a product has half the
+// work beside the same softmax: 8 x 1024 on 1 k, 12 heads, bf16 71 us (0.55), e4m3 66.
 // Tried and slower: scores of the next tile beside this one's softmax on 32-key tiles (670
 // beside 637 us at the time), three workgroups a unit (618 beside 583), two and four times the
 // splits (the join's bytes), workgroups that go on to further row tiles with their first loads
@@ -1062,14 +1067,18 @@ __global__ __launch_bounds__(256, 8) void paged_join_kernel(PagedArgs a) {
 
 // How a call is split: rows of a workgroup, key blocks of a split and splits.
 // - 16 rows or fewer a KV head take the 16-row kernel: 32 sequences of 2000 keys, 4 heads to
-//   each of 4 KV heads, e4m3, one token 17.2 us beside 21.1 on the 128-row kernel, 4 tokens 19.6
-//   beside 21.9; with 5, two 16-row workgroups 20.8 beside 22.5, but 8 tokens of 60000 keys 46.6
-//   beside 37.2.
+//   each of 4 KV heads, e4m3, one token 17.3 us beside 20.9 on the 128-row kernel, 4 tokens 18.0
+//   beside 22.0. With 5 and 8 tokens two 16-row workgroups are no faster there (21.9, 22.5 beside
+//   21.8, 22.7) and slower on 60000 keys: 8 tokens of one sequence 29.5 beside 26.6, of two 46.1
+//   beside 35.1, of eight 117 beside 103. (17 to 64 rows leave waves of the 128-row kernel without
+//   rows: they stage keys only, and these calls take 1.4 times their bytes' time or more.)
 // - Keys are split where there are too few workgroups otherwise, to 1024 (four a unit), 512
 //   (two) or 256 (one of 256 rows): 256 sequences x 4 KV heads, already 1024, take 41 us whole
 //   and 50 in halves; 32 x 128 rows on 1024 keys, 512 workgroups, 52 whole and 95 in halves.
-// - A split has 512 keys at least, for its share of the join: 64 sequences of 300 keys take
-//   8.4 us whole and 13.4 in two (16 rows), 13 and 27 (64 rows).
+// - A split has 512 keys at least, for its share of the join: 64 sequences of 300 keys, 256
+//   workgroups, take 8.4 us whole and 13.4 in two (16 rows), 13 and 27 (64 rows). (Measured where
+//   workgroups fill the chip. Calls with few, as 1 x 64 rows on 4000 keys with 64 of them,
+//   21 us, would gain from shorter splits, which this rule does not give them.)
 // - 256 rows a workgroup, which stage a tile's keys once for twice the rows (16 % of the time of
 //   128), take heads of 128 where sequences are long and workgroups enough: 2 x 1024 rows on
 //   24-32 k keys 511 beside 566 us, 8 x 2048 without a context 143 beside 146; but 32 x 512 65
