@@ -22,8 +22,8 @@
 //   so far is at most 2^kScaleSmall: a P' that f32 rounds to zero then has a weight of less
 //   than 2^-50 of the largest. Behind a larger scale it is taken of the scores themselves, with
 //   exponentials of its own. It is held kSumShift binary orders up, where the 183 orders between
-//   the least and the largest scale lie inside f32 (weights 33 orders below the largest may still
-//   be left out, where all values of that one pass 2^120), and moved in two factors that f32
+//   the least and the largest scale lie inside f32 (where a scale of 2^120 sets the reference,
+//   weights 33 orders below the largest are still left out), and moved in two factors that f32
 //   holds where the product of both is less than it does.
 // - P' is rounded to f16 for 8-bit and f16 values (codes are exact in f16), to bf16 for bf16
 //   ones, whose range f16 does not hold: at most half a step (2^-11, 2^-8) of each weight,
