@@ -535,6 +535,93 @@ int sm_paged_attention(const sm_paged_cache* cache, const int32_t* block_table,
                        const void* q, int dtype, int64_t ldq, int64_t H, void* out, float* lse,
                        void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Attention of a tree of drafted tokens: sm_paged_attention where row i of a sequence sees its
+ * context, the keys before pos0[s], and those of its n rows' own keys pos0[s] + j that have their
+ * bit set in mask row i: bit j % 32 of word j / 32, mask [rows, words] uint32, words >= max_rows / 32
+ * (sm_tree_masks; any mask is taken, a row that does not see itself or sees later ones among
+ * them). Bits from n on are ignored, keys at negative positions seen by no row; a row that sees
+ * no key gives 0 and lse -inf. Everything else, the workspace among it
+ * (sm_paged_attention_workspace_bytes), as sm_paged_attention; max_tokens counts the rows. */
+int sm_paged_tree_attention(const sm_paged_cache* cache, const int32_t* block_table,
+                            int64_t table_cols, const int32_t* pos0, const int32_t* row_start,
+                            int64_t S, int64_t rows, int64_t max_rows, int64_t max_tokens,
+                            const int32_t* mask, int64_t words, const void* q, int dtype,
+                            int64_t ldq, int64_t H, void* out, float* lse, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/* Trees of drafted tokens (TextGenerator::generate, generate.rs:68-124, several tokens a
+ * forward). A sequence's rows as in a paged batch (row_start or max_rows each), at most 1024:
+ * row 0 is the last chosen token, not yet in the cache; row i > 0 continues row parents[i] < i
+ * (any other value: the context alone). Appended at pos0 .. pos0 + n - 1 and rotated by their
+ * depth (sm_rope at `positions`, then sm_paged_append without a table).
+ * sm_tree_masks: mask [rows, words] (words >= max_rows / 32): row i's ancestors and itself;
+ *   positions (nullable) [rows] = pos0 + depth (pos0 [S]; NULL without positions).
+ * sm_tree_accept: from row 0 on to the first (lowest) row that continues the current one and
+ *   whose drafted token is the one sampled behind the current, while there is one: path
+ *   [S, max_rows] the rows walked, emitted (nullable) [S, max_rows] the tokens sampled behind
+ *   them, -1 behind count [S] of each. emitted[count - 1] is the next tree's row 0. A sequence
+ *   without rows has count 0.
+ * sm_paged_keep: in every cache (all of one geometry) token pos0 + path[j] to pos0 + j, for
+ *   j < count (path and count as above; max_rows the path's stride): the sequence then holds
+ *   pos0 + count tokens. Entries rise; the first that does not, or that names a token without a
+ *   page, ends the path. 16-bit values move as they are. 8-bit: a block's scale becomes the largest of its own
+ *   and those of the blocks that its tokens come from; codes of a smaller scale are scaled down
+ *   and rounded again, the block's other tokens among them (as in sm_paged_append a scale never
+ *   falls while tokens of its block stay; NaN codes stay). Several caches (a model's layers)
+ *   in one launch of up to 32. A page is written for one of its sequences in a call. */
+int sm_tree_masks(const int32_t* parents, const int32_t* pos0, const int32_t* row_start,
+                  int64_t S, int64_t rows, int64_t max_rows, int32_t* mask, int64_t words,
+                  int32_t* positions, void* stream);
+int sm_tree_accept(const int32_t* parents, const int32_t* tokens, const int32_t* sampled,
+                   const int32_t* row_start, int64_t S, int64_t rows, int64_t max_rows,
+                   int32_t* path, int32_t* count, int32_t* emitted, void* stream);
+int sm_paged_keep(const sm_paged_cache* caches, int64_t ncaches, const int32_t* path,
+                  const int32_t* count, int64_t S, int64_t max_rows, const int32_t* block_table,
+                  int64_t table_cols, const int32_t* pos0, void* stream);
+
+/* The pages of a paged cache (no counterpart in the reference, whose AttnCache has one sequence;
+ * GRPO's groups share a prompt, posttrain.rs:1206-1216). refs [pages] int32: how many table
+ * entries hold each page, 0 a free one (all zero at first); it is all the state there is, kept
+ * once for the caches of all layers. Pages are given lowest free one first, so every result is a
+ * function of the arguments. Block tables [S, table_cols] as above, rows filled from the front,
+ * -1 behind. Calls on one refs must be ordered, as on one stream.
+ * sm_page_reserve: pages for tokens[s] tokens of each sequence, from the first entry that names
+ *   none on, sequences in order.
+ * sm_page_fork: child c, of prompt source[c], whose tokens[source[c]] tokens it shares: row c of
+ *   out [C, table_cols] gets the prompt's full pages (one holder more) and, where the prompt's last page
+ *   is unfinished, a page of its own, to be copied from src[c] to dst[c] (sm_paged_copy; both -1
+ *   where nothing is to be copied). out may be the last batch's table, freed, but not overlap
+ *   block_table. A source outside [0, P) gives an empty row.
+ * sm_page_free: entries behind those of the first tokens[s] tokens (NULL: all) leave their
+ *   pages and become -1. A page that nothing holds is free; its contents stay until it is given.
+ * missing (nullable) [1]: how many pages were not there (those entries stay -1, and tokens
+ *   behind them are not stored by sm_paged_append), columns and prompts that the table does not have included.
+ * sm_page_compact: the L live pages to the front: refs_out (may be refs) and page_map [pages],
+ *   where each page is then (-1: free); the i-th live page from L on goes to the i-th free page
+ *   below L, src[i] to dst[i] (arrays of pages / 2; -1 behind the last). Pages from L on are
+ *   free after the copy.
+ * sm_page_remap: out[i] = page_map[block_table[i]] for n entries, -1 for those that name no
+ *   page; out may be block_table.
+ * sm_paged_copy: page src[i] to page dst[i], values and scales, for n pairs in every cache (all
+ *   of one geometry; up to 32 a launch); a pair with a page outside [0, pages) is left out. No
+ *   page may be the destination of two pairs, nor of one and the source of another (those of the
+ *   calls above are not). */
+int sm_page_reserve(int32_t* refs, int64_t pages, int32_t* block_table, int64_t S,
+                    int64_t table_cols, const int32_t* tokens, int64_t page_tokens,
+                    int32_t* missing, void* stream);
+int sm_page_fork(int32_t* refs, int64_t pages, const int32_t* block_table, int64_t P,
+                 int64_t table_cols, const int32_t* tokens, const int32_t* source, int64_t C,
+                 int64_t page_tokens, int32_t* out, int32_t* src, int32_t* dst, int32_t* missing,
+                 void* stream);
+int sm_page_free(int32_t* refs, int64_t pages, int32_t* block_table, int64_t S,
+                 int64_t table_cols, const int32_t* tokens, int64_t page_tokens, void* stream);
+int sm_page_compact(const int32_t* refs, int64_t pages, int32_t* refs_out, int32_t* page_map,
+                    int32_t* src, int32_t* dst, void* stream);
+int sm_page_remap(const int32_t* block_table, int64_t n, const int32_t* page_map, int64_t pages,
+                  int32_t* out, void* stream);
+int sm_paged_copy(const sm_paged_cache* caches, int64_t ncaches, const int32_t* src,
+                  const int32_t* dst, int64_t n, void* stream);
+
 /* Next-token selection for `rows` logits rows (select_next_token /
  * sample_from_logits, summa-llm/src/generate.rs:127-202). temperature <= 0:
  * greedy, first max wins ties; otherwise Gumbel-max sampling from
@@ -579,6 +666,38 @@ int sm_sample_ex(const float* logits, int64_t rows, int64_t ld, int64_t vocab,
                  int64_t seen_ld, int32_t* done, int32_t* lengths, int32_t* tokens,
                  int64_t tok_stride, float* logprobs, int64_t lp_stride, int32_t* next_ids,
                  void* stream);
+/* Next tokens from given random numbers, each row with options of its own (a batch of requests,
+ * the nodes of drafted trees, rollouts that are drawn again from stored numbers; select_next_token
+ * / sample_from_values, generate.rs:127-250, with the nucleus of RolloutSampling and min-p).
+ * logits [rows, vocab] of dtype (SM_F32, SM_BF16, SM_F16), rows ld values apart; uniforms [rows]
+ * f32 in [0, 1). Per row, with m the largest logit and w_i = exp((x_i - m) / temperature):
+ *   temperature <= 0 or NaN: the first of the largest logits;
+ *   else the top_k largest (by value, then lowest index; < 1 or >= vocab: all), of these the
+ *   smallest prefix in that order with at least top_p of their weight (>= 1 or NaN: all; the largest
+ *   always), of these those with w_i >= min_p (<= 0 or NaN: all; the largest always), and of
+ *   these, in the order of the vocabulary, the first at which their running sum of weights passes
+ *   uniforms[r] times their whole.
+ * A logit of -inf or NaN is never chosen; with logits of +inf, those weigh 1 and all others
+ * nothing. A row without any other logit than -inf and NaN gives token -1 and log-prob -inf.
+ * Options: arrays [rows] on the device, or where NULL the one value for all rows (which is
+ * checked: "temperature must not be NaN", "top_p must be in (0, 1]", "min_p must be in [0, 1]").
+ * tokens [rows]; logprobs (nullable) [rows] f32: log_softmax(logits)[token] of the raw logits.
+ * Weights are held to 2^-46 of the row's largest and summed exactly (as whole numbers), so a
+ * token depends on nothing but its row. vocab <= 2^17 ... see sm_sample_rows_workspace_bytes: the
+ * device bytes (16-byte aligned) that a call needs, 0 for most, -1 for a bad shape. */
+typedef struct sm_row_sampling {
+  const float* temperatures;
+  const int32_t* top_ks;
+  const float* top_ps;
+  const float* min_ps;
+  float temperature; /* for all rows, where the array above is NULL */
+  int32_t top_k;
+  float top_p, min_p;
+} sm_row_sampling;
+int64_t sm_sample_rows_workspace_bytes(int64_t rows, int64_t vocab, int dtype);
+int sm_sample_rows(const void* logits, int dtype, int64_t rows, int64_t ld, int64_t vocab,
+                   const float* uniforms, const sm_row_sampling* options, int32_t* tokens,
+                   float* logprobs, void* workspace, int64_t workspace_bytes, void* stream);
 /* seen[r] |= {ids[r, 0..n)} (ids [rows, ids_ld] int32; ids outside [0, vocab)
  * mark nothing); clear != 0 zeroes the rows first. The prior_tokens set of
  * apply_repetition_penalty (generate.rs:155-182). */

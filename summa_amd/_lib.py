@@ -87,9 +87,22 @@ SIGNATURES: dict[str, tuple] = {
     "sm_paged_attention_workspace_bytes": (i64, [i64, i64, i64, i64, i64, i64, i64]),
     "sm_paged_attention": (i32, [vp, vp, i64, vp, vp, i64, i64, i64, i64, vp, i32, i64, i64, vp,
                                  vp, vp, i64, vp]),
+    "sm_paged_tree_attention": (i32, [vp, vp, i64, vp, vp, i64, i64, i64, i64, vp, i64, vp, i32,
+                                      i64, i64, vp, vp, vp, i64, vp]),
+    "sm_tree_masks": (i32, [vp, vp, vp, i64, i64, i64, vp, i64, vp, vp]),
+    "sm_tree_accept": (i32, [vp, vp, vp, vp, i64, i64, i64, vp, vp, vp, vp]),
+    "sm_paged_keep": (i32, [vp, i64, vp, vp, i64, i64, vp, i64, vp, vp]),
+    "sm_page_reserve": (i32, [vp, i64, vp, i64, i64, vp, i64, vp, vp]),
+    "sm_page_fork": (i32, [vp, i64, vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, vp, vp]),
+    "sm_page_free": (i32, [vp, i64, vp, i64, i64, vp, i64, vp]),
+    "sm_page_compact": (i32, [vp, i64, vp, vp, vp, vp, vp]),
+    "sm_page_remap": (i32, [vp, i64, vp, i64, vp, vp]),
+    "sm_paged_copy": (i32, [vp, i64, vp, vp, i64, vp]),
     "sm_sample": (i32, [vp, i64, i64, i64, f32, u64, i64, vp, i64, vp, i64, vp, vp]),
     "sm_sample_ex": (i32, [vp, i64, i64, i64, vp, u64, i64, vp, i64, vp, vp, vp, i64, vp, i64, vp,
                            vp]),
+    "sm_sample_rows_workspace_bytes": (i64, [i64, i64, i32]),
+    "sm_sample_rows": (i32, [vp, i32, i64, i64, i64, vp, vp, vp, vp, vp, i64, vp]),
     "sm_seen_tokens": (i32, [vp, i64, i64, i64, i64, vp, i64, i32, vp]),
     "sm_moe_plan_words": (i64, [i64, i64, i64]),
     "sm_moe_router_top2": (i32, [vp, i32, vp, i64, i64, i64, vp, vp, vp, vp]),

@@ -3,7 +3,9 @@
 The cache of ``AttnCache`` (summa-llm/src/model/attention.rs:20-40) in pages that any
 sequence may hold, so rollouts of unequal length take what they use. Calls mirror
 ``sm_paged_append`` / ``sm_paged_attention`` (include/summa_amd.h, which states the
-layouts and what each call leaves alone). A batch is described by device tensors:
+layouts and what each call leaves alone); ``paged_tree_attention``, ``paged_keep`` and
+``paged_copy`` are for trees of drafted tokens (``tree``) and for pages that change hands
+(``pages``). A batch is described by device tensors:
 
 - ``block_table`` int32 [S, columns]: entry j of a row is the page of the sequence's
   tokens ``j * page_tokens ..``;
@@ -210,6 +212,28 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_table: torch.Ten
     softmax weights are rounded once to 16 bits, bf16 for a bf16 cache and f16 else; with up to
     16 the error is the output's rounding alone. (forward_cached / sdpa,
     summa-llm/src/model/attention.rs:216-265, 318-371.)"""
+    return _attention("sm_paged_attention", cache, q, block_table, pos0, row_start, max_rows,
+                      max_tokens, want_lse, out, None)
+
+
+def paged_tree_attention(cache: PagedKVCache, q: torch.Tensor, mask: torch.Tensor,
+                         block_table: torch.Tensor, pos0: torch.Tensor,
+                         row_start: torch.Tensor | None = None, *, max_rows: int | None = None,
+                         max_tokens: int | None = None, want_lse: bool = False,
+                         out: torch.Tensor | None = None):
+    """``paged_attention`` of trees of drafted tokens: row i of a sequence sees the keys before
+    ``pos0`` and those of the sequence's own rows j (keys ``pos0 + j``) that have bit j of
+    ``mask`` [rows, words] int32 set in row i (``tree.tree_masks``; any mask is taken). A row
+    that sees no key gives 0 and lse -inf."""
+    if mask.dtype is not torch.int32 or mask.dim() != 2 or mask.shape[0] != q.shape[0] or \
+            not mask.is_contiguous() or mask.get_device() != cache.index:
+        raise ValueError("mask must be contiguous int32 [rows, words] on the cache's device")
+    return _attention("sm_paged_tree_attention", cache, q, block_table, pos0, row_start, max_rows,
+                      max_tokens, want_lse, out, mask)
+
+
+def _attention(name, cache, q, block_table, pos0, row_start, max_rows, max_tokens, want_lse, out,
+               mask):
     rows, H, ldq = _rows(cache, q, "q")
     dt = _ROWS.get(q.dtype)
     if dt is None or dt == SM_F32:
@@ -227,8 +251,61 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_table: torch.Ten
             ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device)
     out = _out(cache, out, rows, H, q.dtype)
     lse = torch.empty((rows, H), dtype=torch.float32, device=cache.device) if want_lse else None
-    call("sm_paged_attention", cache._at, block_table.data_ptr(), cols, pos0.data_ptr(), starts,
-         S, rows, most, max_tokens, q.data_ptr(), dt, ldq, H, out.data_ptr(),
+    masks = () if mask is None else (mask.data_ptr(), mask.shape[1])
+    call(name, cache._at, block_table.data_ptr(), cols, pos0.data_ptr(), starts, S, rows, most,
+         max_tokens, *masks, q.data_ptr(), dt, ldq, H, out.data_ptr(),
          None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
          stream)
     return (out, lse) if want_lse else out
+
+
+def _layers(caches):
+    """(array of descriptors, how many, the first) of one cache or several of one geometry."""
+    caches = (caches,) if isinstance(caches, PagedKVCache) else tuple(caches)
+    if not caches:
+        raise ValueError("need at least one cache")
+    index = caches[0].index
+    if any(c.index != index for c in caches):
+        raise ValueError("the caches must be on one device")
+    return (_lib.PagedCache * len(caches))(*[c._c for c in caches]), len(caches), caches[0]
+
+
+def _int32(t: torch.Tensor, name: str, index: int, dims: int = 1) -> None:
+    if t.dtype is not torch.int32 or t.dim() != dims or not t.is_contiguous() or \
+            t.get_device() != index:
+        raise ValueError(f"{name} must be contiguous int32 of {dims} dimension"
+                         f"{'s' if dims > 1 else ''} on the device of the others")
+
+
+def paged_keep(caches, path: torch.Tensor, count: torch.Tensor, block_table: torch.Tensor,
+               pos0: torch.Tensor) -> None:
+    """Token ``pos0 + path[s, j]`` to ``pos0 + j`` for j < ``count[s]``, in one cache or in those
+    of all layers at once (path [S, max_rows], count [S] of ``tree.tree_accept``): the sequences
+    then hold ``pos0 + count`` tokens. Entries of a path rise; the first that does not, or that
+    has no page, ends it. In 8 bits a block's scale becomes the largest of its own and those
+    of the blocks that its tokens come from."""
+    array, n, first = _layers(caches)
+    index = first.index
+    _int32(path, "path", index, 2)
+    _int32(block_table, "block_table", index, 2)
+    _int32(count, "count", index)
+    _int32(pos0, "pos0", index)
+    S = path.shape[0]
+    if count.shape[0] != S or pos0.shape[0] != S or block_table.shape[0] != S:
+        raise ValueError("path, count, block_table and pos0 must have one row a sequence")
+    call("sm_paged_keep", array, n, path.data_ptr(), count.data_ptr(), S, path.shape[1],
+         block_table.data_ptr(), block_table.shape[1], pos0.data_ptr(), _stream_on(index))
+
+
+def paged_copy(caches, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Page ``src[i]`` to page ``dst[i]`` (int32; a pair with a page outside the cache, as -1, is
+    left out) in one cache or in those of all layers. No page may be the destination of two
+    pairs, nor of one and the source of another; ``pages.page_fork`` and ``pages.page_compact``
+    give no such pairs."""
+    array, n, first = _layers(caches)
+    _int32(src, "src", first.index)
+    _int32(dst, "dst", first.index)
+    if src.shape != dst.shape:
+        raise ValueError("src and dst must have one length")
+    call("sm_paged_copy", array, n, src.data_ptr(), dst.data_ptr(), src.shape[0],
+         _stream_on(first.index))

@@ -14,7 +14,8 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import call
+from ._lib import SM_BF16, SM_F16, SM_F32, call
+from .ops import _stream_on
 
 MAX_POST_TRAINING_SEQUENCE_TOKENS = 1_048_576  # posttrain.rs:54
 
@@ -110,3 +111,75 @@ def sample(logits: torch.Tensor, cfg: SamplingConfig, seed: int, step: int, *,
          None if lengths is None else lengths.data_ptr(), tok.data_ptr(), 1, lp.data_ptr(), 1,
          None, torch.cuda.current_stream(logits.device).cuda_stream)
     return tok, lp
+
+
+class RowSamplingC(C.Structure):
+    """``sm_row_sampling`` of include/summa_amd.h."""
+    _fields_ = [("temperatures", C.c_void_p), ("top_ks", C.c_void_p), ("top_ps", C.c_void_p),
+                ("min_ps", C.c_void_p), ("temperature", C.c_float), ("top_k", C.c_int32),
+                ("top_p", C.c_float), ("min_p", C.c_float)]
+
+
+_LOGITS = {torch.float32: SM_F32, torch.bfloat16: SM_BF16, torch.float16: SM_F16}
+
+
+def sample_rows(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0,
+                top_k: int | torch.Tensor | None = None, top_p=1.0, min_p=0.0,
+                want_logprobs: bool = True):
+    """(tokens int32 [rows], log-probs f32 [rows]) drawn with the given ``uniforms`` (float32
+    [rows], in [0, 1)) from logits [rows, vocab] (float32, bfloat16 or float16; rows may be
+    strided); without ``want_logprobs`` the tokens alone. Every option is one value or a
+    tensor of one a row (float32; ``top_k`` int32). In this order: the ``top_k`` largest logits
+    (None, or less than 1 in a tensor: all), of them the smallest value-ordered prefix with
+    ``top_p`` of their weight exp(logit / temperature), of them those with at least ``min_p`` of the
+    largest's weight; of these, in the vocabulary's order, the token at which the running sum
+    of weights passes u times their whole. ``temperature`` <= 0 takes the first of the largest
+    logits. Log-probs are log_softmax(logits)[token]. Logits of -inf and NaN are never chosen; a row
+    of nothing else gives token -1 and log-prob -inf (``sm_sample_rows``; select_next_token,
+    summa-llm/src/generate.rs:127-250)."""
+    dt = _LOGITS.get(logits.dtype)
+    if dt is None:
+        raise TypeError("logits must be float32, bfloat16 or float16")
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be [rows, vocab] with contiguous rows")
+    index = logits.get_device()
+    stream = _stream_on(index)
+    rows, vocab = logits.shape
+    ld = logits.stride(0) if rows > 1 else vocab
+
+    def row_values(t, name, dtype):
+        if t.dtype is not dtype or t.shape != (rows,) or not t.is_contiguous() or \
+                t.get_device() != index:
+            raise ValueError(f"{name} must be contiguous {dtype} [rows] on the device of logits")
+        return t.data_ptr()
+
+    at = row_values(uniforms, "uniforms", torch.float32)
+    o = RowSamplingC(None, None, None, None, 1.0, -1, 1.0, 0.0)
+    if torch.is_tensor(temperature):
+        o.temperatures = row_values(temperature, "temperature", torch.float32)
+    else:
+        o.temperature = temperature
+    if torch.is_tensor(top_k):
+        o.top_ks = row_values(top_k, "top_k", torch.int32)
+    elif top_k is not None:
+        if top_k == 0:
+            raise ValueError("top_k must be >= 1 (got 0)")
+        o.top_k = top_k
+    if torch.is_tensor(top_p):
+        o.top_ps = row_values(top_p, "top_p", torch.float32)
+    else:
+        o.top_p = top_p
+    if torch.is_tensor(min_p):
+        o.min_ps = row_values(min_p, "min_p", torch.float32)
+    else:
+        o.min_p = min_p
+    tok = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    lp = torch.empty(rows, dtype=torch.float32, device=logits.device) if want_logprobs else None
+    nbytes = _lib.lib().sm_sample_rows_workspace_bytes(rows, vocab, dt)
+    if nbytes < 0:
+        raise _lib.SummaError(-1, _lib.lib().sm_last_error().decode())
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+    call("sm_sample_rows", logits.data_ptr(), dt, rows, ld, vocab, at, C.addressof(o),
+         tok.data_ptr(), None if lp is None else lp.data_ptr(), None if ws is None else ws.data_ptr(),
+         nbytes, stream)
+    return (tok, lp) if want_logprobs else tok
