@@ -230,8 +230,21 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(RowsArgs a) {
     const double u = fmin(fmax((double)a.uniforms[r], 0.0), 1.0 - 0x1p-53);
     const unsigned long long u64 = (unsigned long long)(u * 0x1p64);
     const unsigned long long aim = __umul64hi(w, u64);
-    if (tid == 0) sh.last = first;
+    if (tid == 0) sh.last = a.uniforms[r] > 0.f ? first : 0x7fffffff;
     unsigned long long before = 0;
+    if (!(a.uniforms[r] > 0.f)) {
+      // u = 0: the first of any weight, also of one that rounds to no 2^-46 (the least u above
+      // it, 2^-24, is past the sum of all of those)
+      __syncthreads();
+      for (int v = tid; v < a.vocab; v += kThreads) {
+        const float x = row.at(v);
+        const uint32_t key = key_of(x);
+        if (!ck.keeps(key, v) || !cp.keeps(key, v)) continue;
+        const double y = row.weight(x);
+        if (y > 0.0 && y >= least) atomicMin(&sh.last, v);
+      }
+      before = ~0ull;
+    }
     for (int v0 = 0; v0 < a.vocab && before <= aim; v0 += kThreads) {
       const int v = v0 + tid;
       const unsigned long long x = v < a.vocab ? kept(v, row.at(v)) : 0ull;
