@@ -13,8 +13,6 @@
 namespace sm {
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / kWave;
-
 struct RowsArgs {
   const void* logits;
   int64_t ld;
@@ -23,11 +21,16 @@ struct RowsArgs {
   int32_t* tokens;
   float* logprobs;
   int vocab, bits;
+  int steps;  // slots of a wave
 };
 
 __device__ inline uint32_t key_of(float f) {
   const uint32_t u = __float_as_uint(f + 0.f);  // (-0 is 0)
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+__device__ inline float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
 }
 
 struct Cut {  // keys above T are kept, and those at T up to index `last`
@@ -38,26 +41,29 @@ struct Cut {  // keys above T are kept, and those at T up to index `last`
   }
 };
 
+template <int THREADS>
 struct Shared {
-  unsigned long long hist[256], total;
-  unsigned long long part[kWaves];
-  float f[kWaves];
-  int i[kWaves];
+  unsigned long long hist[256];
+  unsigned long long part[THREADS / kWave];
+  float f[THREADS / kWave];
+  int i[THREADS / kWave];
   int bin, last;
   unsigned long long left;
 };
 
-__device__ inline unsigned long long block_sum(unsigned long long x, Shared& sh) {
+template <int THREADS>
+__device__ inline unsigned long long block_sum(unsigned long long x, Shared<THREADS>& sh) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, kWave);
   if (threadIdx.x % kWave == 0) sh.part[threadIdx.x / kWave] = x;
   __syncthreads();
   unsigned long long s = 0;
-  for (int i = 0; i < kWaves; ++i) s += sh.part[i];
+  for (int i = 0; i < THREADS / kWave; ++i) s += sh.part[i];
   __syncthreads();
   return s;
 }
-__device__ inline unsigned long long block_before(unsigned long long x, Shared& sh,
+template <int THREADS>
+__device__ inline unsigned long long block_before(unsigned long long x, Shared<THREADS>& sh,
                                                   unsigned long long& total) {
   const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
   unsigned long long inc = x;
@@ -70,7 +76,7 @@ __device__ inline unsigned long long block_before(unsigned long long x, Shared& 
   __syncthreads();
   unsigned long long base = 0;
   total = 0;
-  for (int i = 0; i < kWaves; ++i) {
+  for (int i = 0; i < THREADS / kWave; ++i) {
     if (i < w) base += sh.part[i];
     total += sh.part[i];
   }
@@ -102,13 +108,14 @@ struct Row {
 
 // The place in (value, index) order up to which the elements kept by `outer` amount to
 // `target`, counted or weighed.
-template <bool MASS, typename T>
-__device__ Cut select(const Row<T>& row, const Cut& outer, unsigned long long target, Shared& sh) {
+template <bool MASS, int THREADS, typename T>
+__device__ Cut select(const Row<T>& row, const Cut& outer, unsigned long long target,
+                      Shared<THREADS>& sh) {
   uint32_t prefix = 0, mask = 0;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kThreads) sh.hist[i] = 0;
+    for (int i = threadIdx.x; i < 256; i += THREADS) sh.hist[i] = 0;
     __syncthreads();
-    for (int v = threadIdx.x; v < row.vocab; v += kThreads) {
+    for (int v = threadIdx.x; v < row.vocab; v += THREADS) {
       const float x = row.at(v);
       const uint32_t key = key_of(x);
       if ((key & mask) != prefix || !outer.keeps(key, v)) continue;
@@ -134,7 +141,7 @@ __device__ Cut select(const Row<T>& row, const Cut& outer, unsigned long long ta
   if (threadIdx.x == 0) sh.last = 0x7fffffff;
   __syncthreads();
   unsigned long long before = 0;  // of the elements at the value, by index
-  for (int v0 = 0; v0 < row.vocab; v0 += kThreads) {
+  for (int v0 = 0; v0 < row.vocab; v0 += THREADS) {
     const int v = v0 + threadIdx.x;
     unsigned long long w = 0;
     if (v < row.vocab) {
@@ -153,40 +160,18 @@ __device__ Cut select(const Row<T>& row, const Cut& outer, unsigned long long ta
   return c;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_rows_kernel(RowsArgs a) {
-  __shared__ Shared sh;
-  const int r = (int)blockIdx.x, tid = threadIdx.x;
-  Row<T> row;
-  row.p = static_cast<const T*>(a.logits) + r * a.ld;
-  row.vocab = a.vocab;
-  row.bits = a.bits;
-  const float temperature = a.o.temperatures ? a.o.temperatures[r] : a.o.temperature;
-  const int top_k = a.o.top_ks ? a.o.top_ks[r] : a.o.top_k;
-  const float top_p = a.o.top_ps ? a.o.top_ps[r] : a.o.top_p;
-  const float min_p = a.o.min_ps ? a.o.min_ps[r] : a.o.min_p;
-  // the largest, and the first place of it
-  float m = -INFINITY;
-  for (int v = tid; v < a.vocab; v += kThreads) m = fmaxf(m, row.at(v));
-  m = wave_max(m);
-  if (tid % kWave == 0) sh.f[tid / kWave] = m;
-  __syncthreads();
-  for (int i = 0; i < kWaves; ++i) m = fmaxf(m, sh.f[i]);
-  __syncthreads();
-  row.m = m;
-  if (m == -INFINITY) {
-    if (tid == 0) {
-      a.tokens[r] = -1;
-      if (a.logprobs) a.logprobs[r] = -INFINITY;
-    }
-    return;
-  }
-  float s = 0.f;
+// One row by passes over memory: takes every row, and is what rows that the kernel below does not
+// hold in its lists come to. Whole-number weights here: sums by atomics.
+template <int THREADS, typename T>
+__device__ void by_passes(const RowsArgs& a, int r, const Row<T>& row, int top_k, float top_p,
+                          float min_p, Shared<THREADS>& sh) {
+  const int tid = threadIdx.x;
   int first = 0x7fffffff;
-  for (int v = tid; v < a.vocab; v += kThreads) {
+  float s = 0.f;
+  for (int v = tid; v < a.vocab; v += THREADS) {
     const float x = row.at(v);
-    s += x == m ? 1.f : m == INFINITY ? 0.f : __expf(x - m);
-    if (x == m) first = min(first, v);
+    s += x == row.m ? 1.f : row.m == INFINITY ? 0.f : __expf(x - row.m);
+    if (x == row.m) first = min(first, v);
   }
   s = wave_sum(s);
 #pragma unroll
@@ -197,25 +182,25 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(RowsArgs a) {
   }
   __syncthreads();
   s = 0.f;
-  for (int i = 0; i < kWaves; ++i) {
+  for (int i = 0; i < THREADS / kWave; ++i) {
     s += sh.f[i];
     first = min(first, sh.i[i]);
   }
   __syncthreads();
   int token = first;
-  if (temperature > 0.f) {
-    row.inv = 1.0 / (double)temperature;
+  if (row.inv > 0.0 || row.inv == 0.0) {  // (not greedy: NaN)
     Cut ck, cp;
-    if (top_k >= 1 && top_k < a.vocab) ck = select<false>(row, Cut{}, (unsigned long long)top_k, sh);
+    if (top_k >= 1 && top_k < a.vocab)
+      ck = select<false, THREADS>(row, Cut{}, (unsigned long long)top_k, sh);
     if (top_p < 1.f) {
       unsigned long long w = 0;
-      for (int v = tid; v < a.vocab; v += kThreads) {
+      for (int v = tid; v < a.vocab; v += THREADS) {
         const float x = row.at(v);
         if (ck.keeps(key_of(x), v)) w += row.whole(x);
       }
       w = block_sum(w, sh);
       const double t = ceil((double)w * (double)top_p);
-      cp = select<true>(row, ck, t < 1.0 ? 1ull : (unsigned long long)t, sh);
+      cp = select<true, THREADS>(row, ck, t < 1.0 ? 1ull : (unsigned long long)t, sh);
     }
     const double least = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0;
     auto kept = [&](int v, float x) {
@@ -224,19 +209,19 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(RowsArgs a) {
       return least > 0.0 && row.weight(x) < least ? 0ull : row.whole(x);
     };
     unsigned long long w = 0;
-    for (int v = tid; v < a.vocab; v += kThreads) w += kept(v, row.at(v));
+    for (int v = tid; v < a.vocab; v += THREADS) w += kept(v, row.at(v));
     w = block_sum(w, sh);
     // whole numbers: the sum passes u w where it passes floor(u w)
     const double u = fmin(fmax((double)a.uniforms[r], 0.0), 1.0 - 0x1p-53);
     const unsigned long long u64 = (unsigned long long)(u * 0x1p64);
     const unsigned long long aim = __umul64hi(w, u64);
-    if (tid == 0) sh.last = a.uniforms[r] > 0.f ? first : 0x7fffffff;
+    if (tid == 0) sh.last = u > 0.0 ? first : 0x7fffffff;
     unsigned long long before = 0;
-    if (!(a.uniforms[r] > 0.f)) {
-      // u = 0: the first of any weight, also of one that rounds to no 2^-46 (the least u above
-      // it, 2^-24, is past the sum of all of those)
-      __syncthreads();
-      for (int v = tid; v < a.vocab; v += kThreads) {
+    __syncthreads();
+    if (u == 0.0) {
+      // the first of any weight, also of one that rounds to no 2^-46 (the least u above
+      // zero, 2^-24, is past the sum of all of those)
+      for (int v = tid; v < a.vocab; v += THREADS) {
         const float x = row.at(v);
         const uint32_t key = key_of(x);
         if (!ck.keeps(key, v) || !cp.keeps(key, v)) continue;
@@ -245,7 +230,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(RowsArgs a) {
       }
       before = ~0ull;
     }
-    for (int v0 = 0; v0 < a.vocab && before <= aim; v0 += kThreads) {
+    for (int v0 = 0; v0 < a.vocab && before <= aim; v0 += THREADS) {
       const int v = v0 + tid;
       const unsigned long long x = v < a.vocab ? kept(v, row.at(v)) : 0ull;
       unsigned long long total;
@@ -258,8 +243,597 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(RowsArgs a) {
   }
   if (tid == 0) {
     a.tokens[r] = token;
-    if (a.logprobs) a.logprobs[r] = (m == INFINITY ? 0.f : row.at(token) - m) - __logf(s);
+    if (a.logprobs)
+      a.logprobs[r] = (row.m == INFINITY ? 0.f : row.at(token) - row.m) - __logf(s);
   }
+}
+
+// 2^y, y <= 0, within 2^-45: a polynomial of degree 9 on the half octave to either side of a whole one
+// (interpolated at the Chebyshev nodes).
+__device__ inline double exp2_f64(double y) {
+  y = fmax(y, -1100.0);  // (and -inf: zero)
+  const double magic = 0x1.8p52, t = y + magic;
+  const double r = y - (t - magic);
+  double p = 0x1.b6571e229927fp-24;
+  p = fma(p, r, 0x1.63ef9699120e2p-20);
+  p = fma(p, r, 0x1.ffcb767842e11p-17);
+  p = fma(p, r, 0x1.43088e2580989p-13);
+  p = fma(p, r, 0x1.5d87fe908fb19p-10);
+  p = fma(p, r, 0x1.3b2ab72b175e1p-7);
+  p = fma(p, r, 0x1.c6b08d7044117p-5);
+  p = fma(p, r, 0x1.ebfbdff8149f2p-3);
+  p = fma(p, r, 0x1.62e42fefa39f7p-1);
+  p = fma(p, r, 1.0);
+  return __builtin_amdgcn_ldexp(p, (int)(uint32_t)__builtin_bit_cast(uint64_t, t));
+}
+
+template <int CTRL>
+__device__ inline double dpp_f64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ inline double lane_f64(double v, int l) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, l);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), l);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ inline double wave_add(double v) {  // (as wave_sum)
+  v += dpp_f64<kDppXor1>(v);
+  v += dpp_f64<kDppXor2>(v);
+  v += dpp_f64<kDppHalfMirror>(v);
+  v += dpp_f64<kDppMirror>(v);
+  return (lane_f64(v, 0) + lane_f64(v, 16)) + (lane_f64(v, 32) + lane_f64(v, 48));
+}
+__device__ inline double wave_inclusive(double v) {
+  const int lane = threadIdx.x % kWave;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const double t = __shfl_up(v, o, kWave);
+    if (lane >= o) v += t;
+  }
+  return v;
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kSlot = 512;   // consecutive logits, a wave's share of a step: a sum of its own
+constexpr int kSlots = 1024;
+constexpr float kOctaves = 40.f;  // that the bins cover
+
+template <int THREADS>
+struct RowLds {
+  static constexpr int BINS = THREADS == 1024 ? 4096 : 1024;
+  static constexpr int CAP = THREADS == 1024 ? 1024 : 512;  // candidates held
+  union {
+    unsigned long long mass[BINS];
+    uint32_t count[BINS];
+    struct {
+      unsigned long long key[CAP];  // by index: order key, ~index
+      double w[CAP];
+      int order[CAP];               // by value
+      int rank[CAP];
+    } c;
+    Shared<THREADS> passes;
+  };
+  double slot[THREADS == 1024 ? kSlots : 64];
+  double all[THREADS / kWave], above[THREADS / kWave];
+  float m[THREADS / kWave], s[THREADS / kWave], low[THREADS / kWave];
+  int n[THREADS / kWave];
+  unsigned long long part[THREADS / kWave];
+  int lo, hi;
+};
+
+// A row in the registers of a workgroup: wave w has its slots w steps .., lane l of a step
+// eight consecutive logits of the slot. Steps past STEPS are read again at each use.
+template <typename T, int THREADS, int STEPS>
+struct Held {
+  static constexpr int W = sizeof(T) == 4 ? 2 : 1;  // 16-byte loads of eight logits
+  const T* p;
+  int vocab, steps, first;  // first: of this wave
+  u32x4 raw[STEPS][W];
+
+  struct __attribute__((packed, aligned(2))) Piece {
+    u32x4 w;
+  };
+  // Where the lane's eight of a step lie: the last eight of the row where they would pass its
+  // end; `skip` of them are then others'.
+  __device__ inline int place(int step, int& skip) const {
+    const int base = first + step * kSlot + (int)(threadIdx.x % kWave) * 8;
+    const int at = min(base, vocab - 8);
+    skip = base - at;
+    return at;
+  }
+  __device__ inline void read(int step, u32x4 (&w)[W]) const {
+    int skip;
+    const T* q = p + place(step, skip);
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = reinterpret_cast<const Piece*>(q + 4 * i)->w;
+  }
+  __device__ inline void load() {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+      if (i < steps) read(i, raw[i]);
+  }
+  // The values of a step; what is not the lane's, and NaN, -inf.
+  __device__ inline void values(const u32x4 (&w)[W], int step, float (&x)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (W == 2)
+        x[e] = __uint_as_float(w[e / 4][e % 4]);
+      else if constexpr (std::is_same<T, uint16_t>::value)
+        x[e] = e % 2 ? bf16hi(w[0][e / 2]) : bf16lo(w[0][e / 2]);
+      else
+        x[e] = (float)as_h2(w[0][e / 2])[e % 2];
+      x[e] = fmaxf(x[e], -INFINITY);
+    }
+    if (first + (step + 1) * kSlot > vocab) {  // (uniform per wave)
+      int skip;
+      place(step, skip);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < skip) x[e] = -INFINITY;
+    }
+  }
+  template <typename F>
+  __device__ inline void each(F f) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      if (i < steps) {  // (uniform)
+        // (so that the compiler keeps the row and nothing made of it from one use to the next)
+#pragma unroll
+        for (int j = 0; j < W; ++j) asm volatile("" : "+v"(raw[i][j]));
+        float x[8];
+        values(raw[i], i, x);
+        f(i, x);
+      }
+    }
+    for (int i = STEPS; i < steps; ++i) {
+      u32x4 w[W];
+      read(i, w);
+      float x[8];
+      values(w, i, x);
+      f(i, x);
+    }
+  }
+};
+
+// ---- the kernel ----
+//
+// A workgroup holds a row in registers (up to 65536 f32 or 131072 16-bit logits of 1024
+// threads), so that memory is read once and each step below works on registers and LDS:
+// - the largest logit, and the sum of exponentials for the log-prob, as the loads arrive;
+// - top-k (up to half of the list): the k-th largest of the threads' own maxima has at least k
+//   logits at or above it and seldom many more. These go to a list in LDS, in the vocabulary's
+//   order, are ranked by counting, and everything else is done on them;
+// - top-p without that: the weights, in f32, are added up in bins of a hundredth of an octave. The
+//   bins around p times the sum, within what f32 may be off, go to the list; one pass with 64-bit weights gives
+//   the sums of all and of those above the list, and the exact border is found in the list;
+// - the draw: sums of 512 consecutive logits are kept by the 64-bit pass; the one that u falls in
+//   is read again.
+// Every sum has a fixed order. Rows that the list does not hold (hundreds of equal logits at
+// the border, top-k above half of it), and those with +inf, go by passes.
+template <typename T, int THREADS, int STEPS>
+__global__ __launch_bounds__(THREADS) void sample_rows_kernel(RowsArgs a) {
+  typedef RowLds<THREADS> L;
+  constexpr int NW = THREADS / kWave;
+  __shared__ L sh;
+  const int r = (int)blockIdx.x, tid = threadIdx.x, lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  Row<T> row;
+  row.p = static_cast<const T*>(a.logits) + r * a.ld;
+  row.vocab = a.vocab;
+  row.bits = a.bits;
+  const float temperature = a.o.temperatures ? a.o.temperatures[r] : a.o.temperature;
+  const int top_k = a.o.top_ks ? a.o.top_ks[r] : a.o.top_k;
+  const float top_p = a.o.top_ps ? a.o.top_ps[r] : a.o.top_p;
+  const float min_p = a.o.min_ps ? a.o.min_ps[r] : a.o.min_p;
+  const bool small = a.vocab < 8;
+  Held<T, THREADS, STEPS> held;
+  held.p = row.p;
+  held.vocab = a.vocab;
+  held.steps = small ? 0 : a.steps;
+  held.first = wave * a.steps * kSlot;
+  if (!small) held.load();
+
+  // maximum; sum of exp(x - maximum) in f32
+  float tm = -INFINITY, ts = 0.f;
+  held.each([&](int, const float(&x)[8]) {
+    float g = x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) g = fmaxf(g, x[e]);
+    if (a.logprobs) {  // (uniform)
+      const float n = fmaxf(tm, g), ref = n == -INFINITY ? 0.f : n;
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += __builtin_amdgcn_exp2f((x[e] - ref) * kLog2e);
+      ts = fmaf(ts, __builtin_amdgcn_exp2f((tm - ref) * kLog2e), s);
+    }
+    tm = fmaxf(tm, g);
+  });
+  if (small)
+    for (int v = tid; v < a.vocab; v += THREADS) tm = fmaxf(tm, row.at(v));
+  float m = wave_max(tm);
+  {
+    const float s = wave_sum(tm == -INFINITY ? 0.f : ts * __builtin_amdgcn_exp2f((tm - m) * kLog2e));
+    if (lane == 0) {
+      sh.m[wave] = m;
+      sh.s[wave] = s;
+    }
+  }
+  __syncthreads();
+  const float wm = lane < NW ? sh.m[lane] : -INFINITY;
+  m = wave_max(wm);
+  const float sum =
+      wave_sum(wm == -INFINITY ? 0.f : sh.s[lane < NW ? lane : 0] * __builtin_amdgcn_exp2f((wm - m) * kLog2e));
+  row.m = m;
+  if (m == -INFINITY) {
+    if (tid == 0) {
+      a.tokens[r] = -1;
+      if (a.logprobs) a.logprobs[r] = -INFINITY;
+    }
+    return;
+  }
+  const bool greedy = !(temperature > 0.f);
+  row.inv = greedy ? NAN : 1.0 / (double)temperature;
+  const bool plain = !small && m < INFINITY && temperature <= 1e30f && (greedy || temperature >= 1e-30f) &&
+                     NW * a.steps <= kSlots;
+  const bool by_k = top_k >= 1 && top_k < a.vocab, by_p = top_p < 1.f;
+  auto log_prob = [&](float x) { return (x - m) - __logf(sum); };
+  if (plain && greedy) {
+    int first = 0x7fffffff;
+    held.each([&](int i, const float(&x)[8]) {
+      int skip;
+      const int at = held.place(i, skip);
+#pragma unroll
+      for (int e = 7; e >= 0; --e)
+        if (x[e] == m) first = min(first, at + e);
+    });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, kWave));
+    if (lane == 0) sh.n[wave] = first;
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+      for (int i = 0; i < NW; ++i) first = min(first, sh.n[i]);
+      a.tokens[r] = first;
+      if (a.logprobs) a.logprobs[r] = log_prob(m);
+    }
+    return;
+  }
+  const double c2 = row.inv * 1.4426950408889634074, m64 = (double)m;
+  const float c = (float)c2;
+  auto weight = [&](float x) { return exp2_f64(((double)x - m64) * c2); };  // (1 for the largest)
+  // weights below 2^-1000 of the largest are none
+  const float live = m - 1000.f / c;
+  const double least = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0;
+  bool fits = plain && !(by_k && top_k > L::CAP / 2);  // (uniform from here on)
+  int lo = 0, hi = -1;   // bins that the list holds
+  float scale = 0.f;     // bins to a unit of logit
+  int n = 0;             // of the list
+  auto bin = [&](float x) { return (int)fminf((m - x) * scale, (float)(L::BINS - 1)); };
+  if (fits && (by_k || by_p)) {
+    if (by_k) {
+      // bins between the least and the largest of the threads' maxima
+      float low = tm >= live ? tm : m;
+      low = -wave_max(-low);
+      if (lane == 0) sh.low[wave] = low;
+      for (int i = tid; i < L::BINS; i += THREADS) sh.count[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NW; ++i) low = fminf(low, sh.low[i]);
+      scale = m > low ? (float)L::BINS * 0.999f / (m - low) : 0.f;
+      if (!(scale < 1e30f)) scale = 1e30f;
+      if (tm >= live) atomicAdd(&sh.count[bin(tm)], 1u);
+    } else {
+      scale = c * ((float)L::BINS / kOctaves);
+      for (int i = tid; i < L::BINS; i += THREADS) sh.mass[i] = 0;
+      __syncthreads();
+      held.each([&](int, const float(&x)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float d = (m - x[e]) * scale;
+          const float y = __builtin_amdgcn_exp2f(fmaf(d, -kOctaves / (float)L::BINS, 31.f));
+          const uint32_t w = (uint32_t)y;
+          if (w) atomicAdd(&sh.mass[(int)fminf(d, (float)(L::BINS - 1))], (unsigned long long)w);
+        }
+      });
+    }
+    __syncthreads();
+    // the bins where the running sum reaches the border, and what f32 may be off
+    constexpr int PER = L::BINS / THREADS;
+    unsigned long long v[PER], mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      v[i] = by_k ? sh.count[tid * PER + i] : sh.mass[tid * PER + i];
+      mine += v[i];
+    }
+    unsigned long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const unsigned long long t = __shfl_up(inc, o, kWave);
+      if (lane >= o) inc += t;
+    }
+    if (lane == kWave - 1) sh.part[wave] = inc;
+    if (tid == 0) {
+      sh.lo = 0;
+      sh.hi = L::BINS - 1;
+    }
+    __syncthreads();
+    unsigned long long before = 0, total = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      if (i < wave) before += sh.part[i];
+      total += sh.part[i];
+    }
+    before += inc - mine;
+    unsigned long long from, to;
+    if (by_k) {
+      from = 0;
+      to = (unsigned long long)top_k;
+    } else {
+      const double t = (double)total * (double)fmaxf(top_p, 0.f);
+      const double off = (double)total * 0x1p-17 + (double)a.vocab;
+      from = t > off ? (unsigned long long)(t - off) : 0ull;
+      to = (unsigned long long)(t + off) + 1;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const unsigned long long after = before + v[i];
+      if (before < from && after >= from) sh.lo = tid * PER + i;
+      if (before < to && after >= to) sh.hi = tid * PER + i;
+      before = after;
+    }
+    __syncthreads();
+    lo = sh.lo;
+    hi = sh.hi;
+    // the list, in the vocabulary's order
+    auto listed = [&](float x) {
+      if (!(x >= live)) return false;
+      const int b = bin(x);
+      return b >= lo && b <= hi;
+    };
+    int have = 0;
+    held.each([&](int, const float(&x)[8]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) have += listed(x[e]);
+    });
+    int upto = have;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const int t = __shfl_up(upto, o, kWave);
+      if (lane >= o) upto += t;
+    }
+    if (lane == kWave - 1) sh.n[wave] = upto;
+    __syncthreads();
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      if (i < wave) at += sh.n[i];
+      n += sh.n[i];
+    }
+    fits = n <= L::CAP;
+    if (fits) {
+      for (int i = tid; i < n; i += THREADS) sh.c.rank[i] = 0;
+      held.each([&](int i, const float(&x)[8]) {
+        int k = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) k += listed(x[e]);
+        if (!__ballot(k > 0)) return;
+        int inc = k;
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+          const int t = __shfl_up(inc, o, kWave);
+          if (lane >= o) inc += t;
+        }
+        int skip, to = at + inc - k;
+        const int place = held.place(i, skip);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (listed(x[e])) {
+            sh.c.key[to] = (unsigned long long)key_of(x[e]) << 32 | (uint32_t)~(place + e);
+            sh.c.w[to] = weight(x[e]);
+            ++to;
+          }
+        at += __builtin_amdgcn_readlane(inc, kWave - 1);
+      });
+    }
+    __syncthreads();
+  }
+  if (!fits) {
+    __syncthreads();
+    by_passes<THREADS, T>(a, r, row, top_k, top_p, min_p, sh.passes);
+    return;
+  }
+  if (!by_k) {
+    // sums in 64 bits: of all (top-p), of those above the list, and of those that are kept, by slots
+    double all = 0.0, above = 0.0;
+    // in f32, what may pass min-p
+    const float bar = min_p > 0.f ? fmaxf(live, m + (__log2f(fminf(min_p, 1.f)) - 0.01f) / c) : live;
+    held.each([&](int i, const float(&x)[8]) {
+      double k = 0.0;
+      bool any = by_p;
+      if (!by_p) {
+        float g = x[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) g = fmaxf(g, x[e]);
+        any = __ballot(g >= bar) != 0;
+      }
+      if (any) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const double w = weight(x[e]);
+          if (by_p) {
+            const bool over = bin(x[e]) < lo;
+            all += w;
+            if (over) above += w;
+            if (over && w >= least) k += w;
+          } else if (w >= least) {
+            k += w;
+          }
+        }
+        k = wave_add(k);
+      }
+      if (lane == 0) sh.slot[wave * a.steps + i] = k;
+    });
+    if (by_p) {
+      all = wave_add(all);
+      above = wave_add(above);
+      if (lane == 0) {
+        sh.all[wave] = all;
+        sh.above[wave] = above;
+      }
+    }
+  }
+  // ranks of the list: how many come before
+  if (n > 0) {
+    int wide = 64;
+    while (wide < n) wide *= 2;
+    const int parts = max(1, THREADS / wide);
+    for (int i = tid % wide; i < n; i += THREADS) {
+      const unsigned long long key = sh.c.key[i];
+      int before = 0;
+      for (int j = tid / wide; j < n; j += parts) before += sh.c.key[j] > key;
+      if (before) atomicAdd(&sh.c.rank[i], before);
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += THREADS) sh.c.order[sh.c.rank[i]] = i;
+  }
+  __syncthreads();
+  if (wave > 0) return;
+
+  // one wave from here on
+  const double u = fmin(fmax((double)a.uniforms[r], 0.0), 1.0 - 0x1p-53);
+  unsigned long long cut = ~0ull;  // the last key of the list that is kept
+  double all = 0.0, above = 0.0;
+  if (n > 0) {
+    if (!by_k) {
+      all = lane < NW ? sh.all[lane] : 0.0;
+      above = lane < NW ? sh.above[lane] : 0.0;
+      all = wave_add(all);
+      above = wave_add(above);
+    }
+    const int per = (n + kWave - 1) / kWave, q0 = lane * per;
+    const int most = by_k ? min(n, top_k) : n;
+    double mine = 0.0;
+    for (int q = q0; q < min(q0 + per, most); ++q) mine += sh.c.w[sh.c.order[q]];
+    const double inc = wave_inclusive(mine);
+    if (by_k) all = lane_f64(inc, kWave - 1);
+    double before = above + (inc - mine);
+    const double border = by_p ? (double)fmaxf(top_p, 0.f) * all : INFINITY;
+    int kept = 0;
+    for (int q = q0; q < min(q0 + per, most); ++q) {
+      const double w = sh.c.w[sh.c.order[q]];
+      if ((before < border || (q == 0 && lo == 0)) && w >= least) kept = q + 1;
+      before += w;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) kept = max(kept, __shfl_xor(kept, o, kWave));
+    if (kept > 0) cut = sh.c.key[sh.c.order[kept - 1]];
+  }
+  if (by_k) {
+    // the draw among the list, in the vocabulary's order
+    const int per = (n + kWave - 1) / kWave, i0 = lane * per;
+    double mine = 0.0;
+    for (int i = i0; i < min(i0 + per, n); ++i)
+      if (sh.c.key[i] >= cut) mine += sh.c.w[i];
+    const double inc = wave_inclusive(mine);
+    const double aim = u * lane_f64(inc, kWave - 1);
+    const uint64_t pass = __ballot(inc > aim);
+    const int who = pass ? (int)__builtin_ctzll(pass) : kWave - 1;
+    if (lane != who) return;
+    double at = inc - mine;
+    int got = -1;
+    for (int i = i0; i < min(i0 + per, n); ++i)
+      if (sh.c.key[i] >= cut) {
+        at += sh.c.w[i];
+        got = i;
+        if (at > aim) break;
+      }
+    if (got < 0) got = sh.c.order[0];
+    const unsigned long long key = sh.c.key[got];
+    a.tokens[r] = (int)~(uint32_t)key;
+    if (a.logprobs) a.logprobs[r] = log_prob(key_value((uint32_t)(key >> 32)));
+    return;
+  }
+  // the draw among the slots, the kept of the list in theirs
+  const int slots = (a.vocab + kSlot - 1) / kSlot, per = (slots + kWave - 1) / kWave, s0 = lane * per;
+  double mine = 0.0;
+  int i = 0;
+  if (n > 0) {  // the list's first entry of this lane's slots
+    int top = n;
+    while (i < top) {
+      const int mid = (i + top) / 2;
+      if ((int)~(uint32_t)sh.c.key[mid] < s0 * kSlot) i = mid + 1;
+      else top = mid;
+    }
+  }
+  for (int s = s0; s < min(s0 + per, slots); ++s) {
+    double k = sh.slot[s];
+    for (; i < n && (int)~(uint32_t)sh.c.key[i] < (s + 1) * kSlot; ++i)
+      if (sh.c.key[i] >= cut) k += sh.c.w[i];
+    sh.slot[s] = k;
+    mine += k;
+  }
+  const double inc = wave_inclusive(mine);
+  const double aim = u * lane_f64(inc, kWave - 1);
+  const uint64_t pass = __ballot(inc > aim);
+  int who = pass ? (int)__builtin_ctzll(pass) : kWave - 1;
+  double left = 0.0;  // of the slot that u falls in
+  int slot = 0;
+  if (lane == who) {
+    double at = inc - mine;
+    for (int s = s0; s < min(s0 + per, slots); ++s) {
+      const double k = sh.slot[s];
+      if (k > 0.0) {
+        slot = s;
+        left = aim - at;
+      }
+      at += k;
+      if (at > aim) break;
+    }
+  }
+  slot = __builtin_amdgcn_readlane(slot, who);
+  left = lane_f64(left, who);
+  const int base = slot * kSlot + lane * 8;
+  double w[8];
+  float x[8];
+  mine = 0.0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    x[e] = base + e < a.vocab ? row.at(base + e) : -INFINITY;
+    w[e] = weight(x[e]);
+    bool keep = w[e] >= least;
+    if (by_p && keep) {
+      const int b = bin(x[e]);
+      const unsigned long long key = (unsigned long long)key_of(x[e]) << 32 | (uint32_t)~(base + e);
+      keep = b < lo || (b <= hi && key >= cut);
+    }
+    if (!keep) w[e] = 0.0;
+    mine += w[e];
+  }
+  const double in = wave_inclusive(mine);
+  uint64_t hit = __ballot(in > left && mine > 0.0);
+  if (!hit) {
+    hit = __ballot(mine > 0.0);
+    hit = hit ? (uint64_t)1 << (63 - __builtin_clzll(hit)) : 1;
+  }
+  who = (int)__builtin_ctzll(hit);
+  if (lane != who) return;
+  double at = in - mine;
+  int got = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (w[e] > 0.0 && at <= left) got = e;
+    at += w[e];
+  }
+  float chosen = x[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e)
+    if (e == got) chosen = x[e];
+  a.tokens[r] = base + got;
+  if (a.logprobs) a.logprobs[r] = log_prob(chosen);
 }
 
 int check_rows(const char* who, int64_t rows, int64_t vocab, int dtype) {
@@ -306,10 +880,25 @@ extern "C" int sm_sample_rows(const void* logits, int dtype, int64_t rows, int64
   a.vocab = (int)vocab;
   a.bits = 46;
   while (((int64_t)1 << (63 - a.bits)) < vocab) --a.bits;
+  // 256 threads hold rows of up to 16384 logits, so that several are in flight on a unit
+  const int threads = vocab <= 16384 ? 256 : 1024;
+  a.steps = (int)ceil_div(vocab, kSlot * (threads / kWave));
   hipStream_t st = as_stream(stream);
-  if (dtype == SM_F32) sample_rows_kernel<float><<<(unsigned)rows, kThreads, 0, st>>>(a);
-  else if (dtype == SM_BF16) sample_rows_kernel<uint16_t><<<(unsigned)rows, kThreads, 0, st>>>(a);
-  else sample_rows_kernel<_Float16><<<(unsigned)rows, kThreads, 0, st>>>(a);
+#define SM_ROWS(T, THREADS, STEPS) \
+  sample_rows_kernel<T, THREADS, STEPS><<<(unsigned)rows, THREADS, 0, st>>>(a)
+#define SM_ROWS_OF(T, MOST)                                  \
+  do {                                                       \
+    if (threads == 256 && a.steps <= 2) SM_ROWS(T, 256, 2);  \
+    else if (threads == 256) SM_ROWS(T, 256, 8);             \
+    else if (a.steps <= 4) SM_ROWS(T, 1024, 4);              \
+    else if (a.steps <= 8) SM_ROWS(T, 1024, 8);              \
+    else SM_ROWS(T, 1024, MOST);                             \
+  } while (0)
+  if (dtype == SM_F32) SM_ROWS_OF(float, 8);
+  else if (dtype == SM_BF16) SM_ROWS_OF(uint16_t, 16);
+  else SM_ROWS_OF(_Float16, 16);
+#undef SM_ROWS_OF
+#undef SM_ROWS
   SM_LAUNCH_CHECK();
   return SM_OK;
 }
