@@ -248,24 +248,52 @@ __device__ void by_passes(const RowsArgs& a, int r, const Row<T>& row, int top_k
   }
 }
 
-// 2^y, y <= 0, within 2^-45: a polynomial of degree 9 on the half octave to either side of a whole one
-// (interpolated at the Chebyshev nodes).
-__device__ inline double exp2_f64(double y) {
-  y = fmax(y, -1100.0);  // (and -inf: zero)
-  const double magic = 0x1.8p52, t = y + magic;
-  const double r = y - (t - magic);
-  double p = 0x1.b6571e229927fp-24;
-  p = fma(p, r, 0x1.63ef9699120e2p-20);
-  p = fma(p, r, 0x1.ffcb767842e11p-17);
-  p = fma(p, r, 0x1.43088e2580989p-13);
-  p = fma(p, r, 0x1.5d87fe908fb19p-10);
-  p = fma(p, r, 0x1.3b2ab72b175e1p-7);
-  p = fma(p, r, 0x1.c6b08d7044117p-5);
-  p = fma(p, r, 0x1.ebfbdff8149f2p-3);
-  p = fma(p, r, 0x1.62e42fefa39f7p-1);
-  p = fma(p, r, 1.0);
-  return __builtin_amdgcn_ldexp(p, (int)(uint32_t)__builtin_bit_cast(uint64_t, t));
+// (what is called for every step is not left to the compiler's measure of size)
+#define SM_INLINE __attribute__((always_inline)) inline
+
+// Four at a time, step by step: one after the other, as the compiler orders them by itself, each
+// operation waits for the one before it (65536 weights of a row 33 us, so 14).
+__device__ SM_INLINE void side_by_side(double (&x)[4]) {
+  asm volatile("" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
 }
+// 2^(d c), d <= 0, d c >= -1022, within 2^-45: a polynomial of degree 9 on the half octave to either
+// side of a whole one (interpolated at the Chebyshev nodes).
+__device__ SM_INLINE void exp2_f64(const double (&d)[4], double c, double (&p)[4]) {
+  constexpr double magic = 0x1.8p52;
+  constexpr double co[] = {0x1.63ef9699120e2p-20, 0x1.ffcb767842e11p-17, 0x1.43088e2580989p-13,
+                           0x1.5d87fe908fb19p-10, 0x1.3b2ab72b175e1p-7,  0x1.c6b08d7044117p-5,
+                           0x1.ebfbdff8149f2p-3,  0x1.62e42fefa39f7p-1,  1.0};
+  double t[4], r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[i] = fma(d[i], c, magic);
+  side_by_side(t);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = t[i] - magic;
+  side_by_side(r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = fma(d[i], c, -r[i]);
+  side_by_side(r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = fma(r[i], 0x1.b6571e229927fp-24, co[0]);
+#pragma unroll
+  for (int k = 1; k < 9; ++k) {
+    side_by_side(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = fma(p[i], r[i], co[k]);
+  }
+  side_by_side(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    p[i] = __builtin_amdgcn_ldexp(p[i], (int)(uint32_t)__builtin_bit_cast(uint64_t, t[i]));
+}
+__device__ inline double exp2_f64(double d, double c) {
+  const double x[4] = {d, d, d, d};
+  double p[4];
+  exp2_f64(x, c, p);
+  return p[0];
+}
+
+__device__ inline uint64_t ballot(bool x) { return __builtin_amdgcn_ballot_w64(x); }
 
 template <int CTRL>
 __device__ inline double dpp_f64(double v) {
@@ -299,16 +327,15 @@ __device__ inline double wave_inclusive(double v) {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kSlot = 512;   // consecutive logits, a wave's share of a step: a sum of its own
-constexpr int kSlots = 1024;
+constexpr int kSlots = 512;   // sums held: 64 steps of eight waves
 constexpr float kOctaves = 40.f;  // that the bins cover
 
 template <int THREADS>
 struct RowLds {
-  static constexpr int BINS = THREADS == 1024 ? 4096 : 1024;
-  static constexpr int CAP = THREADS == 1024 ? 1024 : 512;  // candidates held
+  static constexpr int BINS = THREADS == 512 ? 4096 : 1024;
+  static constexpr int CAP = THREADS == 512 ? 1024 : 512;  // candidates held
   union {
-    unsigned long long mass[BINS];
-    uint32_t count[BINS];
+    uint32_t bin[BINS];
     struct {
       unsigned long long key[CAP];  // by index: order key, ~index
       double w[CAP];
@@ -317,47 +344,59 @@ struct RowLds {
     } c;
     Shared<THREADS> passes;
   };
-  double slot[THREADS == 1024 ? kSlots : 64];
+  double slot[THREADS == 512 ? kSlots : 64];
   double all[THREADS / kWave], above[THREADS / kWave];
-  float m[THREADS / kWave], s[THREADS / kWave], low[THREADS / kWave];
+  float m[THREADS / kWave], s[THREADS / kWave], w[THREADS / kWave], low[THREADS / kWave];
   int n[THREADS / kWave];
-  unsigned long long part[THREADS / kWave];
+  uint32_t part[THREADS / kWave];
   int lo, hi;
 };
 
-// A row in the registers of a workgroup: wave w has its slots w steps .., lane l of a step
-// eight consecutive logits of the slot. Steps past STEPS are read again at each use.
+// A row in the registers of a workgroup: wave w has the slots w steps .., a slot a step; of each
+// quarter (f32) or all (16 bits) of 1 KB of it lane l has 16 bytes. Steps past STEPS are read again at each use.
 template <typename T, int THREADS, int STEPS>
 struct Held {
-  static constexpr int W = sizeof(T) == 4 ? 2 : 1;  // 16-byte loads of eight logits
+  static constexpr int G = 16 / sizeof(T);   // logits of a lane's 16 bytes
+  static constexpr int W = 8 / G;            // 16-byte pieces of a step
   const T* p;
   int vocab, steps, first;  // first: of this wave
-  u32x4 raw[STEPS][W];
+  // The row as vectors of registers that a uniform index reaches: a loop over the steps is a loop
+  // in the code too. (Unrolled, a pass over 64-bit weights is 12 KB of it, and fetching the code
+  // took most of the kernel's time.)
+  static constexpr int R = STEPS * W * 4 < 32 ? 16 : 32, V = (STEPS * W * 4 + R - 1) / R;
+  typedef uint32_t Vec __attribute__((ext_vector_type(R)));
+  Vec reg[V];
 
   struct __attribute__((packed, aligned(2))) Piece {
     u32x4 w;
   };
-  // Where the lane's eight of a step lie: the last eight of the row where they would pass its
-  // end; `skip` of them are then others'.
-  __device__ inline int place(int step, int& skip) const {
-    const int base = first + step * kSlot + (int)(threadIdx.x % kWave) * 8;
-    const int at = min(base, vocab - 8);
+  // Where a piece lies: at the row's end, where it would pass that, and the first `skip` of it are
+  // then others'.
+  __device__ inline int place(int step, int i, int& skip) const {
+    const int base = first + step * kSlot + (i * kWave + (int)(threadIdx.x % kWave)) * G;
+    const int at = min(base, vocab - G);
     skip = base - at;
     return at;
   }
   __device__ inline void read(int step, u32x4 (&w)[W]) const {
-    int skip;
-    const T* q = p + place(step, skip);
 #pragma unroll
-    for (int i = 0; i < W; ++i) w[i] = reinterpret_cast<const Piece*>(q + 4 * i)->w;
+    for (int i = 0; i < W; ++i) {
+      int skip;
+      w[i] = reinterpret_cast<const Piece*>(p + place(step, i, skip))->w;
+    }
   }
   __device__ inline void load() {
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i)
-      if (i < steps) read(i, raw[i]);
+    for (int i = 0; i < STEPS; ++i) {
+      u32x4 w[W] = {};
+      if (i < steps) read(i, w);
+#pragma unroll
+      for (int j = 0; j < 4 * W; ++j) reg[(i * 4 * W + j) / R][(i * 4 * W + j) % R] = w[j / 4][j % 4];
+    }
   }
-  // The values of a step; what is not the lane's, and NaN, -inf.
-  __device__ inline void values(const u32x4 (&w)[W], int step, float (&x)[8]) const {
+  // The values of a step, eight a lane, piece after piece; what is less than `floor`, not the lane's, or NaN
+  // is `floor`.
+  __device__ SM_INLINE void values(const u32x4 (&w)[W], int step, float floor, float (&x)[8]) const {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if constexpr (W == 2)
@@ -366,34 +405,60 @@ struct Held {
         x[e] = e % 2 ? bf16hi(w[0][e / 2]) : bf16lo(w[0][e / 2]);
       else
         x[e] = (float)as_h2(w[0][e / 2])[e % 2];
-      x[e] = fmaxf(x[e], -INFINITY);
+      x[e] = fmaxf(x[e], floor);
     }
     if (first + (step + 1) * kSlot > vocab) {  // (uniform per wave)
-      int skip;
-      place(step, skip);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < skip) x[e] = -INFINITY;
+      for (int e = 0; e < 8; ++e) {
+        int skip;
+        place(step, e / G, skip);
+        if (e % G < skip) x[e] = floor;
+      }
     }
   }
   template <typename F>
-  __device__ inline void each(F f) {
+  __device__ SM_INLINE void step_again(int i, float floor, F f) const {
+    u32x4 w[W];
+    read(i, w);
+    float x[8];
+    values(w, i, floor, x);
+    f(i, x);
+  }
+  // f(step, values) of every step; the first time through, as the loads arrive
+  template <typename F>
+  __device__ SM_INLINE void each_arriving(float floor, F f) {
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
-      if (i < steps) {  // (uniform)
-        // (so that the compiler keeps the row and nothing made of it from one use to the next)
-#pragma unroll
-        for (int j = 0; j < W; ++j) asm volatile("" : "+v"(raw[i][j]));
-        float x[8];
-        values(raw[i], i, x);
-        f(i, x);
-      }
-    }
-    for (int i = STEPS; i < steps; ++i) {
+      if (i >= steps) continue;  // (uniform)
       u32x4 w[W];
-      read(i, w);
+#pragma unroll
+      for (int j = 0; j < 4 * W; ++j) w[j / 4][j % 4] = reg[(i * 4 * W + j) / R][(i * 4 * W + j) % R];
       float x[8];
-      values(w, i, x);
+      values(w, i, floor, x);
+      f(i, x);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll 1
+    for (int i = STEPS; i < steps; ++i) step_again(i, floor, f);
+  }
+  template <typename F>
+  __device__ SM_INLINE void each(float floor, F f) {
+#pragma unroll 1
+    for (int i = 0; i < steps; ++i) {
+      u32x4 w[W];
+      if (i < STEPS) {
+        const int at = i * 4 * W % R;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (i * 4 * W / R == v) {
+#pragma unroll
+            for (int j = 0; j < 4 * W; ++j) w[j / 4][j % 4] = reg[v][at + j];
+          }
+      } else {
+        read(i, w);
+      }
+      float x[8];
+      values(w, i, floor, x);
       f(i, x);
     }
   }
@@ -415,7 +480,7 @@ struct Held {
 // Every sum has a fixed order. Rows that the list does not hold (hundreds of equal logits at
 // the border, top-k above half of it), and those with +inf, go by passes.
 template <typename T, int THREADS, int STEPS>
-__global__ __launch_bounds__(THREADS) void sample_rows_kernel(RowsArgs a) {
+__global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void sample_rows_kernel(RowsArgs a) {
   typedef RowLds<THREADS> L;
   constexpr int NW = THREADS / kWave;
   __shared__ L sh;
@@ -430,43 +495,62 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(RowsArgs a) {
   const float top_p = a.o.top_ps ? a.o.top_ps[r] : a.o.top_p;
   const float min_p = a.o.min_ps ? a.o.min_ps[r] : a.o.min_p;
   const bool small = a.vocab < 8;
-  Held<T, THREADS, STEPS> held;
+  typedef Held<T, THREADS, STEPS> H;
+  H held;
   held.p = row.p;
   held.vocab = a.vocab;
   held.steps = small ? 0 : a.steps;
   held.first = wave * a.steps * kSlot;
   if (!small) held.load();
 
-  // maximum; sum of exp(x - maximum) in f32
-  float tm = -INFINITY, ts = 0.f;
-  held.each([&](int, const float(&x)[8]) {
+  // maximum; sums of exp(x - maximum) for the log-prob and of the weights, in f32
+  const bool greedy = !(temperature > 0.f);
+  const bool by_k = top_k >= 1 && top_k < a.vocab, by_p = top_p < 1.f;
+  const bool weigh = by_p && !by_k && !greedy;
+  const float ct = weigh ? lane_f32(kLog2e / temperature, 0) : 0.f;
+  float tm = -INFINITY, ts = 0.f, tw = 0.f;
+  held.each_arriving(-INFINITY, [&](int, const float(&x)[8]) __attribute__((always_inline)) {
     float g = x[0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) g = fmaxf(g, x[e]);
+    const float n = fmaxf(tm, g), ref = n == -INFINITY ? 0.f : n;
     if (a.logprobs) {  // (uniform)
-      const float n = fmaxf(tm, g), ref = n == -INFINITY ? 0.f : n;
       float s = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) s += __builtin_amdgcn_exp2f((x[e] - ref) * kLog2e);
       ts = fmaf(ts, __builtin_amdgcn_exp2f((tm - ref) * kLog2e), s);
     }
-    tm = fmaxf(tm, g);
+    if (weigh) {  // (uniform)
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += __builtin_amdgcn_exp2f((x[e] - ref) * ct);
+      tw = fmaf(tw, __builtin_amdgcn_exp2f((tm - ref) * ct), s);
+    }
+    tm = n;
   });
   if (small)
     for (int v = tid; v < a.vocab; v += THREADS) tm = fmaxf(tm, row.at(v));
   float m = wave_max(tm);
   {
-    const float s = wave_sum(tm == -INFINITY ? 0.f : ts * __builtin_amdgcn_exp2f((tm - m) * kLog2e));
+    const float d = tm - m;  // (not a number for a wave without logits, whose sums are not used)
+    const float s = wave_sum(tm == -INFINITY ? 0.f : ts * __builtin_amdgcn_exp2f(d * kLog2e));
+    const float w = wave_sum(tm == -INFINITY ? 0.f : tw * __builtin_amdgcn_exp2f(d * ct));
     if (lane == 0) {
       sh.m[wave] = m;
       sh.s[wave] = s;
+      sh.w[wave] = w;
     }
   }
   __syncthreads();
+  // (uniform values are read to scalar registers)
   const float wm = lane < NW ? sh.m[lane] : -INFINITY;
-  m = wave_max(wm);
-  const float sum =
-      wave_sum(wm == -INFINITY ? 0.f : sh.s[lane < NW ? lane : 0] * __builtin_amdgcn_exp2f((wm - m) * kLog2e));
+  m = lane_f32(wave_max(wm), 0);
+  const int from_wave = lane < NW ? lane : 0;
+  const bool empty = wm == -INFINITY;
+  const float sum = lane_f32(
+      wave_sum(empty ? 0.f : sh.s[from_wave] * __builtin_amdgcn_exp2f((wm - m) * kLog2e)), 0);
+  const float whole = lane_f32(
+      wave_sum(empty ? 0.f : sh.w[from_wave] * __builtin_amdgcn_exp2f((wm - m) * ct)), 0);
   row.m = m;
   if (m == -INFINITY) {
     if (tid == 0) {
@@ -475,20 +559,25 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(RowsArgs a) {
     }
     return;
   }
-  const bool greedy = !(temperature > 0.f);
   row.inv = greedy ? NAN : 1.0 / (double)temperature;
-  const bool plain = !small && m < INFINITY && temperature <= 1e30f && (greedy || temperature >= 1e-30f) &&
-                     NW * a.steps <= kSlots;
-  const bool by_k = top_k >= 1 && top_k < a.vocab, by_p = top_p < 1.f;
+  const double c2 = lane_f64(row.inv * 1.4426950408889634074, 0), m64 = lane_f64((double)m, 0);
+  const float c = lane_f32((float)c2, 0);
+  // Weights of 2^-1000 of the largest and less are none: logits below `live` are raised to it, and the
+  // draw does not take them.
+  const float live = lane_f32(m - 1000.f / c, 0);
+  const bool plain = !small && m < INFINITY && a.steps <= 64 &&
+                     (greedy || (temperature <= 1e30f && temperature >= 1e-30f &&
+                                 (m - live) * c > 980.f && (m - live) * c < 1020.f));
   auto log_prob = [&](float x) { return (x - m) - __logf(sum); };
   if (plain && greedy) {
     int first = 0x7fffffff;
-    held.each([&](int i, const float(&x)[8]) {
-      int skip;
-      const int at = held.place(i, skip);
+    held.each(-INFINITY, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 7; e >= 0; --e)
-        if (x[e] == m) first = min(first, at + e);
+      for (int e = 7; e >= 0; --e) {
+        int skip;
+        const int at = held.place(i, e / H::G, skip);
+        if (x[e] == m) first = min(first, at + e % H::G);
+      }
     });
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, kWave));
@@ -502,57 +591,66 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(RowsArgs a) {
     }
     return;
   }
-  const double c2 = row.inv * 1.4426950408889634074, m64 = (double)m;
-  const float c = (float)c2;
-  auto weight = [&](float x) { return exp2_f64(((double)x - m64) * c2); };  // (1 for the largest)
-  // weights below 2^-1000 of the largest are none
-  const float live = m - 1000.f / c;
-  const double least = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0;
+  auto weights = [&](const float* x, double(&w)[4]) __attribute__((always_inline)) {
+    double d[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = (double)x[i] - m64;
+    side_by_side(d);
+    exp2_f64(d, c2, w);
+  };
+  auto weight = [&](float x) __attribute__((always_inline)) { return exp2_f64((double)x - m64, c2); };  // (1 for the largest)
+  const double least = lane_f64(min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0, 0);
   bool fits = plain && !(by_k && top_k > L::CAP / 2);  // (uniform from here on)
-  int lo = 0, hi = -1;   // bins that the list holds
-  float scale = 0.f;     // bins to a unit of logit
-  int n = 0;             // of the list
-  auto bin = [&](float x) { return (int)fminf((m - x) * scale, (float)(L::BINS - 1)); };
+  // places below the largest logit, in bins: the list holds [from, to)
+  float scale = 0.f, from = 0.f, to = 0.f;
+  auto depth = [&](float x) __attribute__((always_inline)) { return (m - x) * scale; };
+  int n = 0;           // of the list
+  uint64_t some = 0;   // steps of this wave with a part of the list
+  int mine = 0;        // this wave's part of it
   if (fits && (by_k || by_p)) {
     if (by_k) {
       // bins between the least and the largest of the threads' maxima
-      float low = tm >= live ? tm : m;
+      float low = tm > live ? tm : m;
       low = -wave_max(-low);
       if (lane == 0) sh.low[wave] = low;
-      for (int i = tid; i < L::BINS; i += THREADS) sh.count[i] = 0;
+      for (int i = tid; i < L::BINS; i += THREADS) sh.bin[i] = 0;
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < NW; ++i) low = fminf(low, sh.low[i]);
       scale = m > low ? (float)L::BINS * 0.999f / (m - low) : 0.f;
       if (!(scale < 1e30f)) scale = 1e30f;
-      if (tm >= live) atomicAdd(&sh.count[bin(tm)], 1u);
+      scale = lane_f32(scale, 0);
+      if (tm > live) atomicAdd(&sh.bin[(int)fminf(depth(tm), (float)(L::BINS - 1))], 1u);
     } else {
-      scale = c * ((float)L::BINS / kOctaves);
-      for (int i = tid; i < L::BINS; i += THREADS) sh.mass[i] = 0;
+      scale = lane_f32(c * ((float)L::BINS / kOctaves), 0);
+      for (int i = tid; i < L::BINS; i += THREADS) sh.bin[i] = 0;
       __syncthreads();
-      held.each([&](int, const float(&x)[8]) {
+      // in units of 2^-30 of the whole, so that a bin's sum fits 32 bits
+      const float unit = lane_f32(30.f - __log2f(whole), 0);
+      held.each(live, [&](int, const float(&x)[8]) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float d = (m - x[e]) * scale;
-          const float y = __builtin_amdgcn_exp2f(fmaf(d, -kOctaves / (float)L::BINS, 31.f));
-          const uint32_t w = (uint32_t)y;
-          if (w) atomicAdd(&sh.mass[(int)fminf(d, (float)(L::BINS - 1))], (unsigned long long)w);
+          if (e % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+          const float d = depth(x[e]);
+          const uint32_t w = (uint32_t)__builtin_rintf(
+              __builtin_amdgcn_exp2f(fmaf(d, -kOctaves / (float)L::BINS, unit)));
+          if (w) atomicAdd(&sh.bin[(int)fminf(d, (float)(L::BINS - 1))], w);
         }
       });
     }
     __syncthreads();
     // the bins where the running sum reaches the border, and what f32 may be off
     constexpr int PER = L::BINS / THREADS;
-    unsigned long long v[PER], mine = 0;
+    uint32_t v[PER], sum_v = 0;  // (all are 2^30 and a bit, or as many as threads)
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      v[i] = by_k ? sh.count[tid * PER + i] : sh.mass[tid * PER + i];
-      mine += v[i];
+      v[i] = sh.bin[tid * PER + i];
+      sum_v += v[i];
     }
-    unsigned long long inc = mine;
+    uint32_t inc = sum_v;
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {
-      const unsigned long long t = __shfl_up(inc, o, kWave);
+      const uint32_t t = __shfl_up(inc, o, kWave);
       if (lane >= o) inc += t;
     }
     if (lane == kWave - 1) sh.part[wave] = inc;
@@ -561,51 +659,106 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(RowsArgs a) {
       sh.hi = L::BINS - 1;
     }
     __syncthreads();
-    unsigned long long before = 0, total = 0;
+    uint32_t before = 0, total = 0;
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
       if (i < wave) before += sh.part[i];
       total += sh.part[i];
     }
-    before += inc - mine;
-    unsigned long long from, to;
-    if (by_k) {
-      from = 0;
-      to = (unsigned long long)top_k;
-    } else {
-      const double t = (double)total * (double)fmaxf(top_p, 0.f);
-      const double off = (double)total * 0x1p-17 + (double)a.vocab;
-      from = t > off ? (unsigned long long)(t - off) : 0ull;
-      to = (unsigned long long)(t + off) + 1;
+    before += inc - sum_v;
+    uint32_t first = 0, last = (uint32_t)top_k;
+    if (!by_k) {
+      // half a unit a logit, f32's exponentials (of up to kOctaves octaves: 2^-18) and its sum
+      const float t = (float)total * fmaxf(top_p, 0.f), off = (float)total * 0x1p-16f + (float)a.vocab;
+      first = (uint32_t)fmaxf(t - off, 0.f);
+      last = (uint32_t)(t + off) + 1;
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const unsigned long long after = before + v[i];
-      if (before < from && after >= from) sh.lo = tid * PER + i;
-      if (before < to && after >= to) sh.hi = tid * PER + i;
+      const uint32_t after = before + v[i];
+      if (before < first && after >= first) sh.lo = tid * PER + i;
+      if (before < last && after >= last) sh.hi = tid * PER + i;
       before = after;
     }
     __syncthreads();
-    lo = sh.lo;
-    hi = sh.hi;
-    // the list, in the vocabulary's order
-    auto listed = [&](float x) {
-      if (!(x >= live)) return false;
-      const int b = bin(x);
-      return b >= lo && b <= hi;
-    };
-    int have = 0;
-    held.each([&](int, const float(&x)[8]) {
+    from = lane_f32((float)sh.lo, 0);
+    to = lane_f32(sh.hi < L::BINS - 1 ? (float)(sh.hi + 1) : INFINITY, 0);
+    if (by_k) {  // few reach it: none in most steps
+      held.each(live, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
+        float g = x[0];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) have += listed(x[e]);
-    });
-    int upto = have;
+        for (int e = 1; e < 8; ++e) g = fmaxf(g, x[e]);
+        if (!ballot(depth(g) < to && g > live)) return;
+        int k = 0;
 #pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const int t = __shfl_up(upto, o, kWave);
-      if (lane >= o) upto += t;
+        for (int e = 0; e < 8; ++e)
+          k += (int)__builtin_popcountll(ballot(depth(x[e]) < to && x[e] > live));
+        some |= (uint64_t)1 << i;
+        mine += k;
+      });
     }
-    if (lane == kWave - 1) sh.n[wave] = upto;
+  }
+  if (fits && !by_k) {
+    // sums in 64 bits: of all (top-p), of those above the list, and of those that are kept, by slots
+    double all = 0.0, above = 0.0;
+    if (by_p) {
+      held.each(live, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
+        double k = 0.0, z = 0.0;
+        int c = 0;
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) {
+          __builtin_amdgcn_sched_barrier(0);
+          double w[4];
+          weights(x + h, w);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float d = depth(x[h + e]);
+            const bool over = d < from;
+            all += w[e];
+            k = fma(w[e], over ? 1.0 : 0.0, k);
+            if (least > 0.0) z = fma(w[e], over && w[e] >= least ? 1.0 : 0.0, z);  // (uniform)
+            c += (int)__builtin_popcountll(ballot(d < to && x[h + e] > live)) -
+                 (int)__builtin_popcountll(ballot(over));
+          }
+        }
+        above += k;
+        k = wave_add(least > 0.0 ? z : k);
+        if (lane == 0) sh.slot[wave * a.steps + i] = k;
+        if (c > 0) some |= (uint64_t)1 << i;
+        mine += c;
+      });
+      all = wave_add(all);
+      above = wave_add(above);
+      if (lane == 0) {
+        sh.all[wave] = all;
+        sh.above[wave] = above;
+      }
+    } else {
+      // in f32, what may pass min-p
+      const float bar = min_p > 0.f ? fmaxf(live, m + (__log2f(fminf(min_p, 1.f)) - 0.01f) / c) : live;
+      held.each(live, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
+        float g = x[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) g = fmaxf(g, x[e]);
+        double k = 0.0;
+        if (ballot(g > bar || g == m)) {
+#pragma unroll
+          for (int h = 0; h < 8; h += 4) {
+            __builtin_amdgcn_sched_barrier(0);
+            double w[4];
+            weights(x + h, w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k = fma(w[e], w[e] >= least ? 1.0 : 0.0, k);
+          }
+          k = wave_add(k);
+        }
+        if (lane == 0) sh.slot[wave * a.steps + i] = k;
+      });
+    }
+  }
+  if (fits && (by_k || by_p)) {
+    // the list, in the vocabulary's order
+    if (lane == 0) sh.n[wave] = mine;
     __syncthreads();
     int at = 0;
 #pragma unroll
@@ -616,27 +769,30 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(RowsArgs a) {
     fits = n <= L::CAP;
     if (fits) {
       for (int i = tid; i < n; i += THREADS) sh.c.rank[i] = 0;
-      held.each([&](int i, const float(&x)[8]) {
-        int k = 0;
+      held.each(live, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
+        if (!(some >> i & 1)) return;  // (uniform)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) k += listed(x[e]);
-        if (!__ballot(k > 0)) return;
-        int inc = k;
+        for (int j = 0; j < H::W; ++j) {
+          bool hit[H::G];
+          int put = at, hits = 0;  // lanes before this one, then this lane's
 #pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-          const int t = __shfl_up(inc, o, kWave);
-          if (lane >= o) inc += t;
-        }
-        int skip, to = at + inc - k;
-        const int place = held.place(i, skip);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (listed(x[e])) {
-            sh.c.key[to] = (unsigned long long)key_of(x[e]) << 32 | (uint32_t)~(place + e);
-            sh.c.w[to] = weight(x[e]);
-            ++to;
+          for (int e = 0; e < H::G; ++e) {
+            const float y = x[j * H::G + e], d = depth(y);
+            hit[e] = d >= from && d < to && y > live;
+            const uint64_t b = ballot(hit[e]);
+            hits += (int)__builtin_popcountll(b);
+            put = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32),
+                                                 __builtin_amdgcn_mbcnt_lo((uint32_t)b, put));
           }
-        at += __builtin_amdgcn_readlane(inc, kWave - 1);
+          int skip;
+          const int place = held.place(i, j, skip);
+#pragma unroll
+          for (int e = 0; e < H::G; ++e)
+            if (hit[e])
+              sh.c.key[put++] =
+                  (unsigned long long)key_of(x[j * H::G + e]) << 32 | (uint32_t)~(place + e);
+          at += hits;
+        }
       });
     }
     __syncthreads();
@@ -645,46 +801,6 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(RowsArgs a) {
     __syncthreads();
     by_passes<THREADS, T>(a, r, row, top_k, top_p, min_p, sh.passes);
     return;
-  }
-  if (!by_k) {
-    // sums in 64 bits: of all (top-p), of those above the list, and of those that are kept, by slots
-    double all = 0.0, above = 0.0;
-    // in f32, what may pass min-p
-    const float bar = min_p > 0.f ? fmaxf(live, m + (__log2f(fminf(min_p, 1.f)) - 0.01f) / c) : live;
-    held.each([&](int i, const float(&x)[8]) {
-      double k = 0.0;
-      bool any = by_p;
-      if (!by_p) {
-        float g = x[0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) g = fmaxf(g, x[e]);
-        any = __ballot(g >= bar) != 0;
-      }
-      if (any) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const double w = weight(x[e]);
-          if (by_p) {
-            const bool over = bin(x[e]) < lo;
-            all += w;
-            if (over) above += w;
-            if (over && w >= least) k += w;
-          } else if (w >= least) {
-            k += w;
-          }
-        }
-        k = wave_add(k);
-      }
-      if (lane == 0) sh.slot[wave * a.steps + i] = k;
-    });
-    if (by_p) {
-      all = wave_add(all);
-      above = wave_add(above);
-      if (lane == 0) {
-        sh.all[wave] = all;
-        sh.above[wave] = above;
-      }
-    }
   }
   // ranks of the list: how many come before
   if (n > 0) {
@@ -698,7 +814,10 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(RowsArgs a) {
       if (before) atomicAdd(&sh.c.rank[i], before);
     }
     __syncthreads();
-    for (int i = tid; i < n; i += THREADS) sh.c.order[sh.c.rank[i]] = i;
+    for (int i = tid; i < n; i += THREADS) {
+      sh.c.order[sh.c.rank[i]] = i;
+      sh.c.w[i] = weight(key_value((uint32_t)(sh.c.key[i] >> 32)));
+    }
   }
   __syncthreads();
   if (wave > 0) return;
@@ -716,16 +835,16 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(RowsArgs a) {
     }
     const int per = (n + kWave - 1) / kWave, q0 = lane * per;
     const int most = by_k ? min(n, top_k) : n;
-    double mine = 0.0;
-    for (int q = q0; q < min(q0 + per, most); ++q) mine += sh.c.w[sh.c.order[q]];
-    const double inc = wave_inclusive(mine);
+    double part = 0.0;
+    for (int q = q0; q < min(q0 + per, most); ++q) part += sh.c.w[sh.c.order[q]];
+    const double inc = wave_inclusive(part);
     if (by_k) all = lane_f64(inc, kWave - 1);
-    double before = above + (inc - mine);
+    double before = above + (inc - part);
     const double border = by_p ? (double)fmaxf(top_p, 0.f) * all : INFINITY;
     int kept = 0;
     for (int q = q0; q < min(q0 + per, most); ++q) {
       const double w = sh.c.w[sh.c.order[q]];
-      if ((before < border || (q == 0 && lo == 0)) && w >= least) kept = q + 1;
+      if ((before < border || (q == 0 && from == 0.f)) && w >= least) kept = q + 1;
       before += w;
     }
 #pragma unroll
@@ -735,15 +854,15 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(RowsArgs a) {
   if (by_k) {
     // the draw among the list, in the vocabulary's order
     const int per = (n + kWave - 1) / kWave, i0 = lane * per;
-    double mine = 0.0;
+    double part = 0.0;
     for (int i = i0; i < min(i0 + per, n); ++i)
-      if (sh.c.key[i] >= cut) mine += sh.c.w[i];
-    const double inc = wave_inclusive(mine);
-    const double aim = u * lane_f64(inc, kWave - 1);
-    const uint64_t pass = __ballot(inc > aim);
+      if (sh.c.key[i] >= cut) part += sh.c.w[i];
+    const double inc = wave_inclusive(part);
+    const double aim = fmax(u * lane_f64(inc, kWave - 1), 0x1p-900);
+    const uint64_t pass = ballot(inc > aim);
     const int who = pass ? (int)__builtin_ctzll(pass) : kWave - 1;
     if (lane != who) return;
-    double at = inc - mine;
+    double at = inc - part;
     int got = -1;
     for (int i = i0; i < min(i0 + per, n); ++i)
       if (sh.c.key[i] >= cut) {
@@ -759,7 +878,7 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(RowsArgs a) {
   }
   // the draw among the slots, the kept of the list in theirs
   const int slots = (a.vocab + kSlot - 1) / kSlot, per = (slots + kWave - 1) / kWave, s0 = lane * per;
-  double mine = 0.0;
+  double part = 0.0;
   int i = 0;
   if (n > 0) {  // the list's first entry of this lane's slots
     int top = n;
@@ -774,16 +893,16 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(RowsArgs a) {
     for (; i < n && (int)~(uint32_t)sh.c.key[i] < (s + 1) * kSlot; ++i)
       if (sh.c.key[i] >= cut) k += sh.c.w[i];
     sh.slot[s] = k;
-    mine += k;
+    part += k;
   }
-  const double inc = wave_inclusive(mine);
-  const double aim = u * lane_f64(inc, kWave - 1);
-  const uint64_t pass = __ballot(inc > aim);
+  const double inc = wave_inclusive(part);
+  const double aim = fmax(u * lane_f64(inc, kWave - 1), 0x1p-900);
+  const uint64_t pass = ballot(inc > aim);
   int who = pass ? (int)__builtin_ctzll(pass) : kWave - 1;
   double left = 0.0;  // of the slot that u falls in
   int slot = 0;
   if (lane == who) {
-    double at = inc - mine;
+    double at = inc - part;
     for (int s = s0; s < min(s0 + per, slots); ++s) {
       const double k = sh.slot[s];
       if (k > 0.0) {
@@ -799,29 +918,30 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(RowsArgs a) {
   const int base = slot * kSlot + lane * 8;
   double w[8];
   float x[8];
-  mine = 0.0;
+  part = 0.0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    x[e] = base + e < a.vocab ? row.at(base + e) : -INFINITY;
+    x[e] = fmaxf(base + e < a.vocab ? row.at(base + e) : -INFINITY, live);
     w[e] = weight(x[e]);
     bool keep = w[e] >= least;
     if (by_p && keep) {
-      const int b = bin(x[e]);
+      const float d = depth(x[e]);
       const unsigned long long key = (unsigned long long)key_of(x[e]) << 32 | (uint32_t)~(base + e);
-      keep = b < lo || (b <= hi && key >= cut);
+      keep = d < from || (d < to && key >= cut);
     }
+    keep &= x[e] > live;
     if (!keep) w[e] = 0.0;
-    mine += w[e];
+    part += w[e];
   }
-  const double in = wave_inclusive(mine);
-  uint64_t hit = __ballot(in > left && mine > 0.0);
+  const double in = wave_inclusive(part);
+  uint64_t hit = ballot(in > left && part > 0.0);
   if (!hit) {
-    hit = __ballot(mine > 0.0);
+    hit = ballot(part > 0.0);
     hit = hit ? (uint64_t)1 << (63 - __builtin_clzll(hit)) : 1;
   }
   who = (int)__builtin_ctzll(hit);
   if (lane != who) return;
-  double at = in - mine;
+  double at = in - part;
   int got = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -881,7 +1001,7 @@ extern "C" int sm_sample_rows(const void* logits, int dtype, int64_t rows, int64
   a.bits = 46;
   while (((int64_t)1 << (63 - a.bits)) < vocab) --a.bits;
   // 256 threads hold rows of up to 16384 logits, so that several are in flight on a unit
-  const int threads = vocab <= 16384 ? 256 : 1024;
+  const int threads = vocab <= 16384 ? 256 : 512;
   a.steps = (int)ceil_div(vocab, kSlot * (threads / kWave));
   hipStream_t st = as_stream(stream);
 #define SM_ROWS(T, THREADS, STEPS) \
@@ -890,13 +1010,13 @@ extern "C" int sm_sample_rows(const void* logits, int dtype, int64_t rows, int64
   do {                                                       \
     if (threads == 256 && a.steps <= 2) SM_ROWS(T, 256, 2);  \
     else if (threads == 256) SM_ROWS(T, 256, 8);             \
-    else if (a.steps <= 4) SM_ROWS(T, 1024, 4);              \
-    else if (a.steps <= 8) SM_ROWS(T, 1024, 8);              \
-    else SM_ROWS(T, 1024, MOST);                             \
+    else if (a.steps <= 8) SM_ROWS(T, 512, 8);               \
+    else if (a.steps <= 16) SM_ROWS(T, 512, 16);             \
+    else SM_ROWS(T, 512, MOST);                              \
   } while (0)
-  if (dtype == SM_F32) SM_ROWS_OF(float, 8);
-  else if (dtype == SM_BF16) SM_ROWS_OF(uint16_t, 16);
-  else SM_ROWS_OF(_Float16, 16);
+  if (dtype == SM_F32) SM_ROWS_OF(float, 16);
+  else if (dtype == SM_BF16) SM_ROWS_OF(uint16_t, 32);
+  else SM_ROWS_OF(_Float16, 32);
 #undef SM_ROWS_OF
 #undef SM_ROWS
   SM_LAUNCH_CHECK();
