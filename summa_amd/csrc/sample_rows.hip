@@ -251,8 +251,8 @@ __device__ void by_passes(const RowsArgs& a, int r, const Row<T>& row, int top_k
 // (what is called for every step is not left to the compiler's measure of size)
 #define SM_INLINE __attribute__((always_inline)) inline
 
-// Four at a time, step by step: one after the other, as the compiler orders them by itself, each
-// operation waits for the one before it (65536 weights of a row 33 us, so 14).
+// Four at a time, step by step: left to itself the compiler makes one after the other, and each
+// operation waits for the one before it.
 __device__ SM_INLINE void side_by_side(double (&x)[4]) {
   asm volatile("" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
 }
@@ -332,24 +332,25 @@ constexpr float kOctaves = 40.f;  // that the bins cover
 
 template <int THREADS>
 struct RowLds {
-  static constexpr int BINS = THREADS == 512 ? 4096 : 1024;
-  static constexpr int CAP = THREADS == 512 ? 1024 : 512;  // candidates held
+  static constexpr int BINS = THREADS >= 512 ? 4096 : 1024;
+  static constexpr int CAP = THREADS >= 512 ? 1024 : 512;  // candidates held
+  uint32_t bin[BINS + kWave];
+  unsigned long long own[THREADS / kWave][CAP / (THREADS / kWave)];
   union {
-    uint32_t bin[BINS];
     struct {
-      unsigned long long key[CAP];  // by index: order key, ~index
+      unsigned long long key[CAP];  // order key, ~index
       double w[CAP];
-      int order[CAP];               // by value
-      int rank[CAP];
+      int rank[CAP];                // how many come before: by value, and by index (high half)
+      uint16_t order[CAP], place[CAP];  // the list by value, by index
     } c;
     Shared<THREADS> passes;
   };
-  double slot[THREADS == 512 ? kSlots : 64];
+  double slot[THREADS >= 512 ? kSlots : 64];
   double all[THREADS / kWave], above[THREADS / kWave];
   float m[THREADS / kWave], s[THREADS / kWave], w[THREADS / kWave], low[THREADS / kWave];
   int n[THREADS / kWave];
   uint32_t part[THREADS / kWave];
-  int lo, hi;
+  int lo, hi, listed;
 };
 
 // A row in the registers of a workgroup: wave w has the slots w steps .., a slot a step; of each
@@ -395,7 +396,8 @@ struct Held {
     }
   }
   // The values of a step, eight a lane, piece after piece; what is less than `floor`, not the lane's, or NaN
-  // is `floor`.
+  // is `floor`. CLEAN: without NaN.
+  template <bool CLEAN>
   __device__ SM_INLINE void values(const u32x4 (&w)[W], int step, float floor, float (&x)[8]) const {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -405,7 +407,9 @@ struct Held {
         x[e] = e % 2 ? bf16hi(w[0][e / 2]) : bf16lo(w[0][e / 2]);
       else
         x[e] = (float)as_h2(w[0][e / 2])[e % 2];
-      x[e] = fmaxf(x[e], floor);
+      // (fmaxf is two instructions: the first for signalling NaN)
+      if constexpr (CLEAN) asm("v_max_f32 %0, %1, %0" : "+v"(x[e]) : "s"(floor));
+      else x[e] = fmaxf(x[e], floor);
     }
     if (first + (step + 1) * kSlot > vocab) {  // (uniform per wave)
 #pragma unroll
@@ -416,17 +420,28 @@ struct Held {
       }
     }
   }
+  __device__ SM_INLINE void clean(const float (&x)[8], u32x4 (&w)[W]) const {
+#pragma unroll
+    for (int j = 0; j < 4 * W; ++j) {
+      if constexpr (W == 2)
+        w[j / 4][j % 4] = __float_as_uint(x[j]);
+      else if constexpr (std::is_same<T, uint16_t>::value)
+        w[0][j] = __float_as_uint(x[2 * j]) >> 16 | (__float_as_uint(x[2 * j + 1]) & 0xffff0000u);
+      else
+        w[0][j] = __builtin_bit_cast(uint32_t, h2{(_Float16)x[2 * j], (_Float16)x[2 * j + 1]});
+    }
+  }
   template <typename F>
   __device__ SM_INLINE void step_again(int i, float floor, F f) const {
     u32x4 w[W];
     read(i, w);
     float x[8];
-    values(w, i, floor, x);
+    values<false>(w, i, floor, x);
     f(i, x);
   }
   // f(step, values) of every step; the first time through, as the loads arrive
   template <typename F>
-  __device__ SM_INLINE void each_arriving(float floor, F f) {
+  __device__ SM_INLINE void each_arriving(F f) {
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       if (i >= steps) continue;  // (uniform)
@@ -434,17 +449,42 @@ struct Held {
 #pragma unroll
       for (int j = 0; j < 4 * W; ++j) w[j / 4][j % 4] = reg[(i * 4 * W + j) / R][(i * 4 * W + j) % R];
       float x[8];
-      values(w, i, floor, x);
+      values<false>(w, i, -INFINITY, x);
       f(i, x);
+      clean(x, w);
+#pragma unroll
+      for (int j = 0; j < 4 * W; ++j) reg[(i * 4 * W + j) / R][(i * 4 * W + j) % R] = w[j / 4][j % 4];
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll 1
-    for (int i = STEPS; i < steps; ++i) step_again(i, floor, f);
+    for (int i = STEPS; i < steps; ++i) step_again(i, -INFINITY, f);
+  }
+  // Steps of which this wave has a value above `bar` (those past STEPS without a look), a bit each.
+  __device__ SM_INLINE uint64_t above(float bar) const {
+    uint64_t m = 0;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      if (i >= steps) continue;
+      u32x4 w[W];
+#pragma unroll
+      for (int j = 0; j < 4 * W; ++j) w[j / 4][j % 4] = reg[(i * 4 * W + j) / R][(i * 4 * W + j) % R];
+      float g = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4 * W; ++j) {
+        if constexpr (W == 2) g = fmaxf(g, __uint_as_float(w[j / 4][j % 4]));
+        else if constexpr (std::is_same<T, uint16_t>::value) g = fmaxf(fmaxf(g, bf16lo(w[0][j])), bf16hi(w[0][j]));
+        else g = fmaxf(fmaxf(g, (float)as_h2(w[0][j])[0]), (float)as_h2(w[0][j])[1]);
+      }
+      if (__builtin_amdgcn_ballot_w64(g > bar)) m |= (uint64_t)1 << i;
+    }
+    if (steps > STEPS) m |= ~(uint64_t)0 << STEPS;
+    return m;
   }
   template <typename F>
-  __device__ SM_INLINE void each(float floor, F f) {
+  __device__ SM_INLINE void each(float floor, F f, uint64_t which = ~(uint64_t)0) {
 #pragma unroll 1
     for (int i = 0; i < steps; ++i) {
+      if (!(which >> i & 1)) continue;
       u32x4 w[W];
       if (i < STEPS) {
         const int at = i * 4 * W % R;
@@ -454,12 +494,12 @@ struct Held {
 #pragma unroll
             for (int j = 0; j < 4 * W; ++j) w[j / 4][j % 4] = reg[v][at + j];
           }
+        float x[8];
+        values<true>(w, i, floor, x);
+        f(i, x);
       } else {
-        read(i, w);
+        step_again(i, floor, f);
       }
-      float x[8];
-      values(w, i, floor, x);
-      f(i, x);
     }
   }
 };
@@ -508,12 +548,13 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
   const bool by_k = top_k >= 1 && top_k < a.vocab, by_p = top_p < 1.f;
   const bool weigh = by_p && !by_k && !greedy;
   const float ct = weigh ? lane_f32(kLog2e / temperature, 0) : 0.f;
-  float tm = -INFINITY, ts = 0.f, tw = 0.f;
-  held.each_arriving(-INFINITY, [&](int, const float(&x)[8]) __attribute__((always_inline)) {
-    float g = x[0];
+  // (four maxima a thread, for top-k)
+  float four[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, tm = -INFINITY, ts = 0.f, tw = 0.f;
+  held.each_arriving([&](int, const float(&x)[8]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 1; e < 8; ++e) g = fmaxf(g, x[e]);
-    const float n = fmaxf(tm, g), ref = n == -INFINITY ? 0.f : n;
+    for (int e = 0; e < 4; ++e) four[e] = fmaxf(four[e], fmaxf(x[2 * e], x[2 * e + 1]));
+    const float n = fmaxf(fmaxf(four[0], four[1]), fmaxf(four[2], four[3]));
+    const float ref = n == -INFINITY ? 0.f : n;
     if (a.logprobs) {  // (uniform)
       float s = 0.f;
 #pragma unroll
@@ -601,47 +642,91 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
   auto weight = [&](float x) __attribute__((always_inline)) { return exp2_f64((double)x - m64, c2); };  // (1 for the largest)
   const double least = lane_f64(min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0, 0);
   bool fits = plain && !(by_k && top_k > L::CAP / 2);  // (uniform from here on)
-  // places below the largest logit, in bins: the list holds [from, to)
-  float scale = 0.f, from = 0.f, to = 0.f;
-  auto depth = [&](float x) __attribute__((always_inline)) { return (m - x) * scale; };
-  int n = 0;           // of the list
-  uint64_t some = 0;   // steps of this wave with a part of the list
-  int mine = 0;        // this wave's part of it
+  float list_lo = m, list_hi = m;  // the list: logits from list_lo to list_hi
+  int n = 0;
+  // Adds what piece j of a step has of it, in no order: with top-k, where few pieces have any, to the
+  // list; else to the wave's part of it, which needs no answer from LDS.
+  int mine = 0;
+  auto to_list = [&](int i, int j, const float* x) __attribute__((always_inline)) {
+    bool hit[H::G];
+    int put = 0, hits = 0;  // hits of the lanes before this one; of all
+#pragma unroll
+    for (int e = 0; e < H::G; ++e) {
+      hit[e] = x[e] >= list_lo && x[e] <= list_hi;
+      const uint64_t b = ballot(hit[e]);
+      hits += (int)__builtin_popcountll(b);
+      put = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32),
+                                           __builtin_amdgcn_mbcnt_lo((uint32_t)b, put));
+    }
+    if (hits == 0) return;  // (uniform)
+    int end = L::CAP;
+    unsigned long long* to = sh.c.key;
+    if (by_k) {
+      int base = 0;
+      if (lane == 0) base = atomicAdd(&sh.listed, hits);
+      put += __builtin_amdgcn_readfirstlane(base);
+    } else {
+      to = sh.own[wave];
+      end = L::CAP / NW;
+      put += mine;
+      mine += hits;
+    }
+    int skip;
+    const int place = held.place(i, j, skip);
+#pragma unroll
+    for (int e = 0; e < H::G; ++e)
+      if (hit[e]) {
+        if (put < end) to[put] = (unsigned long long)key_of(x[e]) << 32 | (uint32_t)~(place + e);
+        ++put;
+      }
+  };
   if (fits && (by_k || by_p)) {
+    float scale;  // bins to a unit of logit
+    for (int i = tid; i < L::BINS; i += THREADS) sh.bin[i] = 0;
+    if (tid == 0) {
+      sh.lo = 0;
+      sh.hi = L::BINS - 1;
+      sh.listed = 0;
+    }
     if (by_k) {
       // bins between the least and the largest of the threads' maxima
-      float low = tm > live ? tm : m;
+      float low = m;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) low = four[e] > live ? fminf(low, four[e]) : low;
       low = -wave_max(-low);
       if (lane == 0) sh.low[wave] = low;
-      for (int i = tid; i < L::BINS; i += THREADS) sh.bin[i] = 0;
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < NW; ++i) low = fminf(low, sh.low[i]);
       scale = m > low ? (float)L::BINS * 0.999f / (m - low) : 0.f;
-      if (!(scale < 1e30f)) scale = 1e30f;
-      scale = lane_f32(scale, 0);
-      if (tm > live) atomicAdd(&sh.bin[(int)fminf(depth(tm), (float)(L::BINS - 1))], 1u);
+      scale = lane_f32(scale < 1e30f ? scale : 1e30f, 0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (four[e] > live) atomicAdd(&sh.bin[(int)fminf((m - four[e]) * scale, (float)(L::BINS - 1))], 1u);
     } else {
+      // the weights in f32, in units of 2^-30 of their sum, so that a bin's sum fits 32 bits
       scale = lane_f32(c * ((float)L::BINS / kOctaves), 0);
-      for (int i = tid; i < L::BINS; i += THREADS) sh.bin[i] = 0;
-      __syncthreads();
-      // in units of 2^-30 of the whole, so that a bin's sum fits 32 bits
       const float unit = lane_f32(30.f - __log2f(whole), 0);
+      const float top = lane_f32(m * scale, 0), rest = (float)(L::BINS + lane);
+      __syncthreads();
       held.each(live, [&](int, const float(&x)[8]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (e % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-          const float d = depth(x[e]);
-          const uint32_t w = (uint32_t)__builtin_rintf(
-              __builtin_amdgcn_exp2f(fmaf(d, -kOctaves / (float)L::BINS, unit)));
-          if (w) atomicAdd(&sh.bin[(int)fminf(d, (float)(L::BINS - 1))], w);
+        for (int h = 0; h < 8; h += 4) {
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int e = h; e < h + 4; ++e) {
+            const float d = fmaf(-scale, x[e], top);
+            const float w = __builtin_amdgcn_exp2f(fmaf(d, -kOctaves / (float)L::BINS, unit));
+            // (what lies behind the bins goes to one of the lane's own, where it meets nobody)
+            atomicAdd(&sh.bin[(int)__builtin_amdgcn_fmed3f(d, 0.f, rest)], (uint32_t)w);
+          }
         }
       });
     }
     __syncthreads();
     // the bins where the running sum reaches the border, and what f32 may be off
     constexpr int PER = L::BINS / THREADS;
-    uint32_t v[PER], sum_v = 0;  // (all are 2^30 and a bit, or as many as threads)
+    uint32_t v[PER], sum_v = 0;  // (all are 2^30 and a bit, or four a thread)
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       v[i] = sh.bin[tid * PER + i];
@@ -654,10 +739,6 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
       if (lane >= o) inc += t;
     }
     if (lane == kWave - 1) sh.part[wave] = inc;
-    if (tid == 0) {
-      sh.lo = 0;
-      sh.hi = L::BINS - 1;
-    }
     __syncthreads();
     uint32_t before = 0, total = 0;
 #pragma unroll
@@ -668,7 +749,7 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
     before += inc - sum_v;
     uint32_t first = 0, last = (uint32_t)top_k;
     if (!by_k) {
-      // half a unit a logit, f32's exponentials (of up to kOctaves octaves: 2^-18) and its sum
+      // a unit a logit, f32's exponentials (of up to kOctaves octaves: 2^-18) and its sums
       const float t = (float)total * fmaxf(top_p, 0.f), off = (float)total * 0x1p-16f + (float)a.vocab;
       first = (uint32_t)fmaxf(t - off, 0.f);
       last = (uint32_t)(t + off) + 1;
@@ -681,120 +762,95 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
       before = after;
     }
     __syncthreads();
-    from = lane_f32((float)sh.lo, 0);
-    to = lane_f32(sh.hi < L::BINS - 1 ? (float)(sh.hi + 1) : INFINITY, 0);
-    if (by_k) {  // few reach it: none in most steps
+    // The logits of these bins, and what rounding may take for them: d is off by three roundings of
+    // up to |m| scale + BINS.
+    const float guard = (fabsf(m) + (float)L::BINS / fmaxf(scale, 1e-30f)) * 0x1p-21f;
+    list_hi = lane_f32(sh.lo > 0 ? m - (float)sh.lo / scale + guard : m, 0);
+    list_lo = lane_f32(sh.hi < L::BINS - 1 && scale > 0.f ? m - (float)(sh.hi + 1) / scale - guard
+                                                         : -INFINITY, 0);
+    // (above `live`: the next f32)
+    const float next = key_value(key_of(live) + 1);
+    list_lo = fmaxf(list_lo, next);
+    if (by_k)  // few reach it: none in most steps
       held.each(live, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
-        float g = x[0];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) g = fmaxf(g, x[e]);
-        if (!ballot(depth(g) < to && g > live)) return;
-        int k = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          k += (int)__builtin_popcountll(ballot(depth(x[e]) < to && x[e] > live));
-        some |= (uint64_t)1 << i;
-        mine += k;
-      });
-    }
+        for (int j = 0; j < H::W; ++j) to_list(i, j, x + j * H::G);
+      }, held.above(key_value(key_of(list_lo) - 1)));
   }
   if (fits && !by_k) {
     // sums in 64 bits: of all (top-p), of those above the list, and of those that are kept, by slots
-    double all = 0.0, above = 0.0;
     if (by_p) {
-      held.each(live, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
-        double k = 0.0, z = 0.0;
-        int c = 0;
-#pragma unroll
-        for (int h = 0; h < 8; h += 4) {
-          __builtin_amdgcn_sched_barrier(0);
-          double w[4];
-          weights(x + h, w);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float d = depth(x[h + e]);
-            const bool over = d < from;
-            all += w[e];
-            k = fma(w[e], over ? 1.0 : 0.0, k);
-            if (least > 0.0) z = fma(w[e], over && w[e] >= least ? 1.0 : 0.0, z);  // (uniform)
-            c += (int)__builtin_popcountll(ballot(d < to && x[h + e] > live)) -
-                 (int)__builtin_popcountll(ballot(over));
-          }
-        }
-        above += k;
-        k = wave_add(least > 0.0 ? z : k);
-        if (lane == 0) sh.slot[wave * a.steps + i] = k;
-        if (c > 0) some |= (uint64_t)1 << i;
-        mine += c;
-      });
-      all = wave_add(all);
-      above = wave_add(above);
-      if (lane == 0) {
-        sh.all[wave] = all;
-        sh.above[wave] = above;
-      }
-    } else {
-      // in f32, what may pass min-p
-      const float bar = min_p > 0.f ? fmaxf(live, m + (__log2f(fminf(min_p, 1.f)) - 0.01f) / c) : live;
-      held.each(live, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
-        float g = x[0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) g = fmaxf(g, x[e]);
-        double k = 0.0;
-        if (ballot(g > bar || g == m)) {
+      double all = 0.0, above = 0.0;
+      auto sums = [&](auto MIN_P) __attribute__((always_inline)) {
+        held.each(live, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
+          double k = 0.0, z = 0.0;
+          uint64_t some = 0;  // lanes with a part of the list
 #pragma unroll
           for (int h = 0; h < 8; h += 4) {
             __builtin_amdgcn_sched_barrier(0);
             double w[4];
             weights(x + h, w);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) k = fma(w[e], w[e] >= least ? 1.0 : 0.0, k);
+            for (int e = 0; e < 4; ++e) {
+              const bool over = x[h + e] > list_hi;
+              all += w[e];
+              k = fma(w[e], over ? 1.0 : 0.0, k);
+              if constexpr (MIN_P.value) z = fma(w[e], over && w[e] >= least ? 1.0 : 0.0, z);
+              some |= ballot(x[h + e] >= list_lo) & ~ballot(over);
+            }
+            if ((h + 4) % H::G == 0) {  // a piece
+              if (some) to_list(i, h / H::G, x + h / H::G * H::G);
+              some = 0;
+            }
           }
-          k = wave_add(k);
+          above += k;
+          k = wave_add(MIN_P.value ? z : k);
+          if (lane == 0) sh.slot[wave * a.steps + i] = k;
+        });
+      };
+      if (least > 0.0) sums(std::true_type{});
+      else sums(std::false_type{});
+      all = wave_add(all);
+      above = wave_add(above);
+      if (lane == 0) {
+        sh.all[wave] = all;
+        sh.above[wave] = above;
+        sh.n[wave] = mine;
+      }
+    } else {
+      for (int i = lane; i < a.steps; i += kWave) sh.slot[wave * a.steps + i] = 0.0;
+      // in f32, what may pass min-p
+      const float bar = min_p > 0.f ? fmaxf(live, m + (__log2f(fminf(min_p, 1.f)) - 0.01f) / c) : live;
+      held.each(live, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
+        double k = 0.0;
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) {
+          __builtin_amdgcn_sched_barrier(0);
+          double w[4];
+          weights(x + h, w);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) k = fma(w[e], w[e] >= least ? 1.0 : 0.0, k);
         }
+        k = wave_add(k);
         if (lane == 0) sh.slot[wave * a.steps + i] = k;
-      });
+      }, min_p > 0.f ? held.above(key_value(key_of(lane_f32(bar, 0)) - 1)) : ~(uint64_t)0);
     }
   }
-  if (fits && (by_k || by_p)) {
-    // the list, in the vocabulary's order
-    if (lane == 0) sh.n[wave] = mine;
-    __syncthreads();
-    int at = 0;
+  __syncthreads();
+  if (fits && by_k) {
+    n = sh.listed;
+    fits = n <= L::CAP;
+  } else if (fits && by_p) {  // the waves' parts, one behind the other
+    int most = 0, at = 0;
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
       if (i < wave) at += sh.n[i];
       n += sh.n[i];
+      most = max(most, sh.n[i]);
     }
-    fits = n <= L::CAP;
-    if (fits) {
-      for (int i = tid; i < n; i += THREADS) sh.c.rank[i] = 0;
-      held.each(live, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
-        if (!(some >> i & 1)) return;  // (uniform)
-#pragma unroll
-        for (int j = 0; j < H::W; ++j) {
-          bool hit[H::G];
-          int put = at, hits = 0;  // lanes before this one, then this lane's
-#pragma unroll
-          for (int e = 0; e < H::G; ++e) {
-            const float y = x[j * H::G + e], d = depth(y);
-            hit[e] = d >= from && d < to && y > live;
-            const uint64_t b = ballot(hit[e]);
-            hits += (int)__builtin_popcountll(b);
-            put = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32),
-                                                 __builtin_amdgcn_mbcnt_lo((uint32_t)b, put));
-          }
-          int skip;
-          const int place = held.place(i, j, skip);
-#pragma unroll
-          for (int e = 0; e < H::G; ++e)
-            if (hit[e])
-              sh.c.key[put++] =
-                  (unsigned long long)key_of(x[j * H::G + e]) << 32 | (uint32_t)~(place + e);
-          at += hits;
-        }
-      });
-    }
+    fits = most <= L::CAP / NW;
+    if (fits)
+      for (int i = lane; i < mine; i += kWave) sh.c.key[at + i] = sh.own[wave][i];
     __syncthreads();
   }
   if (!fits) {
@@ -802,21 +858,30 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
     by_passes<THREADS, T>(a, r, row, top_k, top_p, min_p, sh.passes);
     return;
   }
-  // ranks of the list: how many come before
+  // the list's orders, by value and by place: how many come before
   if (n > 0) {
+    for (int i = tid; i < n; i += THREADS) {
+      sh.c.rank[i] = 0;
+      sh.c.w[i] = weight(key_value((uint32_t)(sh.c.key[i] >> 32)));
+    }
+    __syncthreads();
     int wide = 64;
     while (wide < n) wide *= 2;
     const int parts = max(1, THREADS / wide);
     for (int i = tid % wide; i < n; i += THREADS) {
       const unsigned long long key = sh.c.key[i];
       int before = 0;
-      for (int j = tid / wide; j < n; j += parts) before += sh.c.key[j] > key;
+#pragma unroll 4
+      for (int j = tid / wide; j < n; j += parts) {
+        const unsigned long long other = sh.c.key[j];
+        before += (other > key) + ((uint32_t)other > (uint32_t)key ? 1 << 16 : 0);
+      }
       if (before) atomicAdd(&sh.c.rank[i], before);
     }
     __syncthreads();
     for (int i = tid; i < n; i += THREADS) {
-      sh.c.order[sh.c.rank[i]] = i;
-      sh.c.w[i] = weight(key_value((uint32_t)(sh.c.key[i] >> 32)));
+      sh.c.order[sh.c.rank[i] & 0xffff] = (uint16_t)i;
+      sh.c.place[sh.c.rank[i] >> 16] = (uint16_t)i;
     }
   }
   __syncthreads();
@@ -844,7 +909,7 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
     int kept = 0;
     for (int q = q0; q < min(q0 + per, most); ++q) {
       const double w = sh.c.w[sh.c.order[q]];
-      if ((before < border || (q == 0 && from == 0.f)) && w >= least) kept = q + 1;
+      if ((before < border || (q == 0 && list_hi == m)) && w >= least) kept = q + 1;
       before += w;
     }
 #pragma unroll
@@ -855,8 +920,10 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
     // the draw among the list, in the vocabulary's order
     const int per = (n + kWave - 1) / kWave, i0 = lane * per;
     double part = 0.0;
-    for (int i = i0; i < min(i0 + per, n); ++i)
+    for (int q = i0; q < min(i0 + per, n); ++q) {
+      const int i = sh.c.place[q];
       if (sh.c.key[i] >= cut) part += sh.c.w[i];
+    }
     const double inc = wave_inclusive(part);
     const double aim = fmax(u * lane_f64(inc, kWave - 1), 0x1p-900);
     const uint64_t pass = ballot(inc > aim);
@@ -864,12 +931,14 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
     if (lane != who) return;
     double at = inc - part;
     int got = -1;
-    for (int i = i0; i < min(i0 + per, n); ++i)
+    for (int q = i0; q < min(i0 + per, n); ++q) {
+      const int i = sh.c.place[q];
       if (sh.c.key[i] >= cut) {
         at += sh.c.w[i];
         got = i;
         if (at > aim) break;
       }
+    }
     if (got < 0) got = sh.c.order[0];
     const unsigned long long key = sh.c.key[got];
     a.tokens[r] = (int)~(uint32_t)key;
@@ -884,14 +953,17 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
     int top = n;
     while (i < top) {
       const int mid = (i + top) / 2;
-      if ((int)~(uint32_t)sh.c.key[mid] < s0 * kSlot) i = mid + 1;
+      if ((int)~(uint32_t)sh.c.key[sh.c.place[mid]] < s0 * kSlot) i = mid + 1;
       else top = mid;
     }
   }
   for (int s = s0; s < min(s0 + per, slots); ++s) {
     double k = sh.slot[s];
-    for (; i < n && (int)~(uint32_t)sh.c.key[i] < (s + 1) * kSlot; ++i)
-      if (sh.c.key[i] >= cut) k += sh.c.w[i];
+    for (; i < n; ++i) {
+      const int at = sh.c.place[i];
+      if ((int)~(uint32_t)sh.c.key[at] >= (s + 1) * kSlot) break;
+      if (sh.c.key[at] >= cut) k += sh.c.w[at];
+    }
     sh.slot[s] = k;
     part += k;
   }
@@ -920,16 +992,25 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
   float x[8];
   part = 0.0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < 8; ++e)
     x[e] = fmaxf(base + e < a.vocab ? row.at(base + e) : -INFINITY, live);
-    w[e] = weight(x[e]);
-    bool keep = w[e] >= least;
-    if (by_p && keep) {
-      const float d = depth(x[e]);
-      const unsigned long long key = (unsigned long long)key_of(x[e]) << 32 | (uint32_t)~(base + e);
-      keep = d < from || (d < to && key >= cut);
+  {
+    double lo[4], hi[4];
+    weights(x, lo);
+    weights(x + 4, hi);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] = lo[e];
+      w[4 + e] = hi[e];
     }
-    keep &= x[e] > live;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    bool keep = w[e] >= least && x[e] > live;
+    if (by_p) {
+      const unsigned long long key = (unsigned long long)key_of(x[e]) << 32 | (uint32_t)~(base + e);
+      keep &= x[e] > list_hi || (x[e] >= list_lo && key >= cut);
+    }
     if (!keep) w[e] = 0.0;
     part += w[e];
   }
@@ -1001,7 +1082,7 @@ extern "C" int sm_sample_rows(const void* logits, int dtype, int64_t rows, int64
   a.bits = 46;
   while (((int64_t)1 << (63 - a.bits)) < vocab) --a.bits;
   // 256 threads hold rows of up to 16384 logits, so that several are in flight on a unit
-  const int threads = vocab <= 16384 ? 256 : 512;
+  const int threads = vocab <= 16384 ? 256 : vocab > 32768 ? 1024 : 512;
   a.steps = (int)ceil_div(vocab, kSlot * (threads / kWave));
   hipStream_t st = as_stream(stream);
 #define SM_ROWS(T, THREADS, STEPS) \
@@ -1010,6 +1091,7 @@ extern "C" int sm_sample_rows(const void* logits, int dtype, int64_t rows, int64
   do {                                                       \
     if (threads == 256 && a.steps <= 2) SM_ROWS(T, 256, 2);  \
     else if (threads == 256) SM_ROWS(T, 256, 8);             \
+    else if (threads == 1024) SM_ROWS(T, 1024, 8);  \
     else if (a.steps <= 8) SM_ROWS(T, 512, 8);               \
     else if (a.steps <= 16) SM_ROWS(T, 512, 16);             \
     else SM_ROWS(T, 512, MOST);                              \
