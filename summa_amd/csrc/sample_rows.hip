@@ -5,6 +5,7 @@
 // vocabularies past 2^17, so that a row's sum fits 63 bits). Sums of whole numbers do not
 // depend on their order, so neither does which token the sum passes u at; in f32 one sum in a
 // few hundred rows would fall on the other side of its border.
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -22,6 +23,8 @@ struct RowsArgs {
   float* logprobs;
   int vocab, bits;
   int steps;  // slots of a wave
+  int parts;  // workgroups of a row
+  uint8_t* ws;
 };
 
 __device__ inline uint32_t key_of(float f) {
@@ -504,6 +507,18 @@ struct Held {
   }
 };
 
+// What the kernels of a row in parts leave each other.
+struct RowShare {
+  static constexpr int PARTS = 64, WAVES = 512, KEYS = 1024;
+  int listed, first;       // the list's entries; the largest logit's first place
+  float list_lo, list_hi;
+  float m[PARTS], s[PARTS], w[PARTS], low[PARTS];
+  double all[WAVES], above[WAVES];
+  double slot[kSlots];
+  unsigned long long key[KEYS];
+  uint32_t bin[4096];
+};
+
 // ---- the kernel ----
 //
 // A workgroup holds a row in registers (up to 65536 f32 or 131072 16-bit logits of 1024
@@ -519,13 +534,24 @@ struct Held {
 //   is read again.
 // Every sum has a fixed order. Rows that the list does not hold (hundreds of equal logits at
 // the border, top-k above half of it), and those with +inf, go by passes.
-template <typename T, int THREADS, int STEPS>
+//
+// PHASE 0: all of it, a workgroup a row. 1 to 4: a few large rows in `parts` workgroups each, whose parts
+// meet in memory between four kernels: 1 maxima and f32 sums, 2 bins, 3 the list and the 64-bit
+// sums, 4 the draw, a workgroup a row again.
+template <typename T, int THREADS, int STEPS, int PHASE>
 __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void sample_rows_kernel(RowsArgs a) {
   typedef RowLds<THREADS> L;
   constexpr int NW = THREADS / kWave;
+  constexpr bool PARTS = PHASE > 0;
   __shared__ L sh;
-  const int r = (int)blockIdx.x, tid = threadIdx.x, lane = tid % kWave;
+  const int tid = threadIdx.x, lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  int r = (int)blockIdx.x, nth = 0;
+  if constexpr (PHASE >= 1 && PHASE <= 3) {
+    nth = r % a.parts;
+    r /= a.parts;
+  }
+  RowShare* const rs = PARTS ? reinterpret_cast<RowShare*>(a.ws) + r : nullptr;
   Row<T> row;
   row.p = static_cast<const T*>(a.logits) + r * a.ld;
   row.vocab = a.vocab;
@@ -539,9 +565,9 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
   H held;
   held.p = row.p;
   held.vocab = a.vocab;
-  held.steps = small ? 0 : a.steps;
-  held.first = wave * a.steps * kSlot;
-  if (!small) held.load();
+  held.steps = small || PHASE == 4 ? 0 : a.steps;
+  held.first = (nth * NW + wave) * a.steps * kSlot;
+  if (!small && PHASE != 4) held.load();
 
   // maximum; sums of exp(x - maximum) for the log-prob and of the weights, in f32
   const bool greedy = !(temperature > 0.f);
@@ -555,13 +581,13 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
     for (int e = 0; e < 4; ++e) four[e] = fmaxf(four[e], fmaxf(x[2 * e], x[2 * e + 1]));
     const float n = fmaxf(fmaxf(four[0], four[1]), fmaxf(four[2], four[3]));
     const float ref = n == -INFINITY ? 0.f : n;
-    if (a.logprobs) {  // (uniform)
+    if (PHASE < 2 && a.logprobs) {  // (uniform)
       float s = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) s += __builtin_amdgcn_exp2f((x[e] - ref) * kLog2e);
       ts = fmaf(ts, __builtin_amdgcn_exp2f((tm - ref) * kLog2e), s);
     }
-    if (weigh) {  // (uniform)
+    if (PHASE < 2 && weigh) {  // (uniform)
       float s = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) s += __builtin_amdgcn_exp2f((x[e] - ref) * ct);
@@ -571,30 +597,57 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
   });
   if (small)
     for (int v = tid; v < a.vocab; v += THREADS) tm = fmaxf(tm, row.at(v));
-  float m = wave_max(tm);
+  float m, sum, whole, low_of_parts = INFINITY;
   {
-    const float d = tm - m;  // (not a number for a wave without logits, whose sums are not used)
-    const float s = wave_sum(tm == -INFINITY ? 0.f : ts * __builtin_amdgcn_exp2f(d * kLog2e));
-    const float w = wave_sum(tm == -INFINITY ? 0.f : tw * __builtin_amdgcn_exp2f(d * ct));
-    if (lane == 0) {
-      sh.m[wave] = m;
-      sh.s[wave] = s;
-      sh.w[wave] = w;
+    // of this wave, of the workgroup, of the parts; uniform values are read to scalar registers
+    auto merge = [&](float wm, float ws, float ww) __attribute__((always_inline)) {
+      m = lane_f32(wave_max(wm), 0);
+      const bool none = wm == -INFINITY;
+      const float d = none ? 0.f : wm - m;
+      sum = lane_f32(wave_sum(none ? 0.f : ws * __builtin_amdgcn_exp2f(d * kLog2e)), 0);
+      whole = lane_f32(wave_sum(none ? 0.f : ww * __builtin_amdgcn_exp2f(d * ct)), 0);
+    };
+    if constexpr (PHASE < 2) {
+      merge(tm, ts, tw);
+      float low = INFINITY;
+      if constexpr (PHASE == 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) low = four[e] > -INFINITY ? fminf(low, four[e]) : low;
+        low = -wave_max(-low);
+      }
+      if (lane == 0) {
+        sh.m[wave] = m;
+        sh.s[wave] = sum;
+        sh.w[wave] = whole;
+        sh.low[wave] = low;
+      }
+      __syncthreads();
+      const int of = lane < NW ? lane : 0;
+      merge(lane < NW ? sh.m[of] : -INFINITY, sh.s[of], sh.w[of]);
+      if constexpr (PHASE == 1) {
+        low = -wave_max(-sh.low[of]);
+        if (tid == 0) {
+          rs->m[nth] = m;
+          rs->s[nth] = sum;
+          rs->w[nth] = whole;
+          rs->low[nth] = low;
+          if (nth == 0) {
+            rs->listed = 0;
+            rs->first = 0x7fffffff;
+          }
+        }
+        for (int i = nth * THREADS + tid; i < L::BINS; i += a.parts * THREADS) rs->bin[i] = 0;
+        return;
+      }
+    } else {
+      const int of = lane < a.parts ? lane : 0;
+      merge(lane < a.parts ? rs->m[of] : -INFINITY, rs->s[of], rs->w[of]);
+      low_of_parts = lane_f32(-wave_max(-rs->low[of]), 0);
     }
   }
-  __syncthreads();
-  // (uniform values are read to scalar registers)
-  const float wm = lane < NW ? sh.m[lane] : -INFINITY;
-  m = lane_f32(wave_max(wm), 0);
-  const int from_wave = lane < NW ? lane : 0;
-  const bool empty = wm == -INFINITY;
-  const float sum = lane_f32(
-      wave_sum(empty ? 0.f : sh.s[from_wave] * __builtin_amdgcn_exp2f((wm - m) * kLog2e)), 0);
-  const float whole = lane_f32(
-      wave_sum(empty ? 0.f : sh.w[from_wave] * __builtin_amdgcn_exp2f((wm - m) * ct)), 0);
   row.m = m;
   if (m == -INFINITY) {
-    if (tid == 0) {
+    if (tid == 0 && (PHASE == 0 || PHASE == 4)) {
       a.tokens[r] = -1;
       if (a.logprobs) a.logprobs[r] = -INFINITY;
     }
@@ -611,7 +664,8 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
                                  (m - live) * c > 980.f && (m - live) * c < 1020.f));
   auto log_prob = [&](float x) { return (x - m) - __logf(sum); };
   if (plain && greedy) {
-    int first = 0x7fffffff;
+    if constexpr (PHASE == 2) return;
+    int first = PHASE == 4 ? rs->first : 0x7fffffff;
     held.each(-INFINITY, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 7; e >= 0; --e) {
@@ -627,8 +681,12 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
     if (tid == 0) {
 #pragma unroll
       for (int i = 0; i < NW; ++i) first = min(first, sh.n[i]);
-      a.tokens[r] = first;
-      if (a.logprobs) a.logprobs[r] = log_prob(m);
+      if constexpr (PHASE == 3) {
+        atomicMin(&rs->first, first);
+      } else {
+        a.tokens[r] = first;
+        if (a.logprobs) a.logprobs[r] = log_prob(m);
+      }
     }
     return;
   }
@@ -660,10 +718,10 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
     }
     if (hits == 0) return;  // (uniform)
     int end = L::CAP;
-    unsigned long long* to = sh.c.key;
-    if (by_k) {
+    unsigned long long* to = PARTS ? rs->key : sh.c.key;
+    if (PARTS || by_k) {
       int base = 0;
-      if (lane == 0) base = atomicAdd(&sh.listed, hits);
+      if (lane == 0) base = atomicAdd(PARTS ? &rs->listed : &sh.listed, hits);
       put += __builtin_amdgcn_readfirstlane(base);
     } else {
       to = sh.own[wave];
@@ -680,9 +738,13 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
         ++put;
       }
   };
-  if (fits && (by_k || by_p)) {
+  if constexpr (PHASE == 4) {
+    list_lo = lane_f32(rs->list_lo, 0);
+    list_hi = lane_f32(rs->list_hi, 0);
+  }
+  if (PHASE != 4 && fits && (by_k || by_p)) {
     float scale;  // bins to a unit of logit
-    for (int i = tid; i < L::BINS; i += THREADS) sh.bin[i] = 0;
+    for (int i = tid; i < L::BINS; i += THREADS) sh.bin[i] = PHASE == 3 ? rs->bin[i] : 0;
     if (tid == 0) {
       sh.lo = 0;
       sh.hi = L::BINS - 1;
@@ -691,24 +753,31 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
     if (by_k) {
       // bins between the least and the largest of the threads' maxima
       float low = m;
+      if constexpr (PARTS) {
+        low = fmaxf(low_of_parts, live);
+        __syncthreads();
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) low = four[e] > live ? fminf(low, four[e]) : low;
-      low = -wave_max(-low);
-      if (lane == 0) sh.low[wave] = low;
-      __syncthreads();
+        for (int e = 0; e < 4; ++e) low = four[e] > live ? fminf(low, four[e]) : low;
+        low = -wave_max(-low);
+        if (lane == 0) sh.low[wave] = low;
+        __syncthreads();
 #pragma unroll
-      for (int i = 0; i < NW; ++i) low = fminf(low, sh.low[i]);
+        for (int i = 0; i < NW; ++i) low = fminf(low, sh.low[i]);
+      }
       scale = m > low ? (float)L::BINS * 0.999f / (m - low) : 0.f;
       scale = lane_f32(scale < 1e30f ? scale : 1e30f, 0);
+      if constexpr (PHASE != 3)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (four[e] > live) atomicAdd(&sh.bin[(int)fminf((m - four[e]) * scale, (float)(L::BINS - 1))], 1u);
     } else {
-      // the weights in f32, in units of 2^-30 of their sum, so that a bin's sum fits 32 bits
+      // the weights in f32, in units of 2^-31 of their sum, so that a bin's sum fits 32 bits
       scale = lane_f32(c * ((float)L::BINS / kOctaves), 0);
-      const float unit = lane_f32(30.f - __log2f(whole), 0);
+      const float unit = lane_f32(31.f - __log2f(whole), 0);
       const float top = lane_f32(m * scale, 0), rest = (float)(L::BINS + lane);
       __syncthreads();
+      if constexpr (PHASE != 3)
       held.each(live, [&](int, const float(&x)[8]) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 8; h += 4) {
@@ -718,15 +787,21 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
             const float d = fmaf(-scale, x[e], top);
             const float w = __builtin_amdgcn_exp2f(fmaf(d, -kOctaves / (float)L::BINS, unit));
             // (what lies behind the bins goes to one of the lane's own, where it meets nobody)
-            atomicAdd(&sh.bin[(int)__builtin_amdgcn_fmed3f(d, 0.f, rest)], (uint32_t)w);
+            atomicAdd(&sh.bin[(int)__builtin_amdgcn_fmed3f(d, 0.f, rest)], (uint32_t)(w + 0.5f));
           }
         }
       });
     }
+    if constexpr (PHASE == 2) {
+      __syncthreads();
+      for (int i = tid; i < L::BINS; i += THREADS)
+        if (sh.bin[i]) atomicAdd(&rs->bin[i], sh.bin[i]);
+      return;
+    }
     __syncthreads();
     // the bins where the running sum reaches the border, and what f32 may be off
     constexpr int PER = L::BINS / THREADS;
-    uint32_t v[PER], sum_v = 0;  // (all are 2^30 and a bit, or four a thread)
+    uint32_t v[PER], sum_v = 0;  // (all are 2^31 and a bit, or four a thread)
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       v[i] = sh.bin[tid * PER + i];
@@ -749,9 +824,10 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
     before += inc - sum_v;
     uint32_t first = 0, last = (uint32_t)top_k;
     if (!by_k) {
-      // a unit a logit, f32's exponentials (of up to kOctaves octaves: 2^-18) and its sums
-      const float t = (float)total * fmaxf(top_p, 0.f), off = (float)total * 0x1p-16f + (float)a.vocab;
-      first = (uint32_t)fmaxf(t - off, 0.f);
+      // half a unit a logit, f32's exponentials (of up to kOctaves octaves: 2^-18) and this product
+      const double t = (double)total * (double)fmaxf(top_p, 0.f),
+                   off = (double)total * 0x1p-17 + 0.5 * (double)a.vocab;
+      first = (uint32_t)fmax(t - off, 0.0);
       last = (uint32_t)(t + off) + 1;
     }
 #pragma unroll
@@ -771,13 +847,20 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
     // (above `live`: the next f32)
     const float next = key_value(key_of(live) + 1);
     list_lo = fmaxf(list_lo, next);
+    if constexpr (PHASE == 3)
+      if (tid == 0 && nth == 0) {
+        rs->list_lo = list_lo;
+        rs->list_hi = list_hi;
+      }
     if (by_k)  // few reach it: none in most steps
       held.each(live, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < H::W; ++j) to_list(i, j, x + j * H::G);
       }, held.above(key_value(key_of(list_lo) - 1)));
   }
-  if (fits && !by_k) {
+  if constexpr (PHASE == 2) return;
+  double* const slots_of_row = PARTS ? rs->slot : sh.slot;
+  if (PHASE != 4 && fits && !by_k) {
     // sums in 64 bits: of all (top-p), of those above the list, and of those that are kept, by slots
     if (by_p) {
       double all = 0.0, above = 0.0;
@@ -805,7 +888,7 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
           }
           above += k;
           k = wave_add(MIN_P.value ? z : k);
-          if (lane == 0) sh.slot[wave * a.steps + i] = k;
+          if (lane == 0) slots_of_row[held.first / kSlot + i] = k;
         });
       };
       if (least > 0.0) sums(std::true_type{});
@@ -813,12 +896,12 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
       all = wave_add(all);
       above = wave_add(above);
       if (lane == 0) {
-        sh.all[wave] = all;
-        sh.above[wave] = above;
+        (PARTS ? rs->all : sh.all)[nth * NW + wave] = all;
+        (PARTS ? rs->above : sh.above)[nth * NW + wave] = above;
         sh.n[wave] = mine;
       }
     } else {
-      for (int i = lane; i < a.steps; i += kWave) sh.slot[wave * a.steps + i] = 0.0;
+      for (int i = lane; i < a.steps; i += kWave) slots_of_row[held.first / kSlot + i] = 0.0;
       // in f32, what may pass min-p
       const float bar = min_p > 0.f ? fmaxf(live, m + (__log2f(fminf(min_p, 1.f)) - 0.01f) / c) : live;
       held.each(live, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
@@ -832,12 +915,36 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
           for (int e = 0; e < 4; ++e) k = fma(w[e], w[e] >= least ? 1.0 : 0.0, k);
         }
         k = wave_add(k);
-        if (lane == 0) sh.slot[wave * a.steps + i] = k;
+        if (lane == 0) slots_of_row[held.first / kSlot + i] = k;
       }, min_p > 0.f ? held.above(key_value(key_of(lane_f32(bar, 0)) - 1)) : ~(uint64_t)0);
     }
   }
+  if constexpr (PHASE == 3) return;
   __syncthreads();
-  if (fits && by_k) {
+  if constexpr (PHASE == 4) {
+    if (fits && !by_k) {  // (loads that do not wait for the list's length)
+      for (int i = tid; i < (a.vocab + kSlot - 1) / kSlot; i += THREADS) sh.slot[i] = rs->slot[i];
+      double all = 0.0, above = 0.0;
+      if (by_p)
+        for (int i = tid; i < a.parts * (512 / kWave); i += THREADS) {
+          all += rs->all[i];
+          above += rs->above[i];
+        }
+      all = wave_add(all);
+      above = wave_add(above);
+      if (lane == 0) {
+        sh.all[wave] = all;
+        sh.above[wave] = above;
+      }
+    }
+    if (fits && (by_k || by_p)) {
+      n = rs->listed;
+      fits = n <= L::CAP;
+      if (fits)
+        for (int i = tid; i < n; i += THREADS) sh.c.key[i] = rs->key[i];
+      __syncthreads();
+    }
+  } else if (fits && by_k) {
     n = sh.listed;
     fits = n <= L::CAP;
   } else if (fits && by_p) {  // the waves' parts, one behind the other
@@ -1045,6 +1152,14 @@ int check_rows(const char* who, int64_t rows, int64_t vocab, int dtype) {
   return SM_OK;
 }
 
+// Workgroups of a row: as many as a call's rows leave units for.
+int row_parts(int64_t rows, int64_t vocab) {
+  const int64_t parts = std::min<int64_t>({256 / std::max<int64_t>(1, rows), ceil_div(vocab, 4096),
+                                           RowShare::PARTS});
+  return vocab <= kSlots * kSlot && ((vocab > 49152 && parts >= 8) || (vocab > 98304 && parts >= 4))
+             ? (int)parts : 1;
+}
+
 }  // namespace
 }  // namespace sm
 
@@ -1052,7 +1167,7 @@ using namespace sm;
 
 extern "C" int64_t sm_sample_rows_workspace_bytes(int64_t rows, int64_t vocab, int dtype) {
   if (check_rows("sm_sample_rows_workspace_bytes", rows, vocab, dtype) != SM_OK) return -1;
-  return 0;
+  return row_parts(rows, vocab) > 1 ? rows * (int64_t)sizeof(RowShare) : 0;
 }
 
 extern "C" int sm_sample_rows(const void* logits, int dtype, int64_t rows, int64_t ld,
@@ -1081,24 +1196,51 @@ extern "C" int sm_sample_rows(const void* logits, int dtype, int64_t rows, int64
   a.vocab = (int)vocab;
   a.bits = 46;
   while (((int64_t)1 << (63 - a.bits)) < vocab) --a.bits;
+  hipStream_t st = as_stream(stream);
+  a.parts = row_parts(rows, vocab);
+  a.ws = static_cast<uint8_t*>(workspace);
+#define SM_ROWS(T, THREADS, STEPS, PHASE, GRID) \
+  sample_rows_kernel<T, THREADS, STEPS, PHASE><<<(unsigned)(GRID), THREADS, 0, st>>>(a)
+  if (a.parts > 1) {
+    const int64_t need = rows * (int64_t)sizeof(RowShare);
+    SM_REQUIRE(workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+               "%s: workspace of %lld bytes, %lld needed, 16-byte aligned", me,
+               (long long)workspace_bytes, (long long)need);
+    a.steps = (int)ceil_div(vocab, (int64_t)a.parts * 8 * kSlot);
+#define SM_ROWS_PARTS(T, STEPS)                 \
+  do {                                          \
+    SM_ROWS(T, 512, STEPS, 1, rows * a.parts);  \
+    SM_ROWS(T, 512, STEPS, 2, rows * a.parts);  \
+    SM_ROWS(T, 512, STEPS, 3, rows * a.parts);  \
+  } while (0)
+#define SM_ROWS_OF(T)                           \
+  do {                                          \
+    if (a.steps <= 2) SM_ROWS_PARTS(T, 2);      \
+    else SM_ROWS_PARTS(T, 8);                   \
+    SM_ROWS(T, 512, 2, 4, rows);                \
+  } while (0)
+    if (dtype == SM_F32) SM_ROWS_OF(float);
+    else if (dtype == SM_BF16) SM_ROWS_OF(uint16_t);
+    else SM_ROWS_OF(_Float16);
+#undef SM_ROWS_OF
+#undef SM_ROWS_PARTS
+    SM_LAUNCH_CHECK();
+    return SM_OK;
+  }
   // 256 threads hold rows of up to 16384 logits, so that several are in flight on a unit
   const int threads = vocab <= 16384 ? 256 : vocab > 32768 ? 1024 : 512;
   a.steps = (int)ceil_div(vocab, kSlot * (threads / kWave));
-  hipStream_t st = as_stream(stream);
-#define SM_ROWS(T, THREADS, STEPS) \
-  sample_rows_kernel<T, THREADS, STEPS><<<(unsigned)rows, THREADS, 0, st>>>(a)
-#define SM_ROWS_OF(T, MOST)                                  \
-  do {                                                       \
-    if (threads == 256 && a.steps <= 2) SM_ROWS(T, 256, 2);  \
-    else if (threads == 256) SM_ROWS(T, 256, 8);             \
-    else if (threads == 1024) SM_ROWS(T, 1024, 8);  \
-    else if (a.steps <= 8) SM_ROWS(T, 512, 8);               \
-    else if (a.steps <= 16) SM_ROWS(T, 512, 16);             \
-    else SM_ROWS(T, 512, MOST);                              \
+#define SM_ROWS_OF(T, MOST)                                            \
+  do {                                                                 \
+    if (threads == 256 && a.steps <= 2) SM_ROWS(T, 256, 2, 0, rows);   \
+    else if (threads == 256) SM_ROWS(T, 256, 8, 0, rows);              \
+    else if (threads == 512) SM_ROWS(T, 512, 8, 0, rows);              \
+    else if (a.steps <= 8) SM_ROWS(T, 1024, 8, 0, rows);               \
+    else SM_ROWS(T, 1024, MOST, 0, rows);                              \
   } while (0)
-  if (dtype == SM_F32) SM_ROWS_OF(float, 16);
-  else if (dtype == SM_BF16) SM_ROWS_OF(uint16_t, 32);
-  else SM_ROWS_OF(_Float16, 32);
+  if (dtype == SM_F32) SM_ROWS_OF(float, 8);
+  else if (dtype == SM_BF16) SM_ROWS_OF(uint16_t, 16);
+  else SM_ROWS_OF(_Float16, 16);
 #undef SM_ROWS_OF
 #undef SM_ROWS
   SM_LAUNCH_CHECK();
