@@ -682,9 +682,14 @@ int sm_sample_ex(const float* logits, int64_t rows, int64_t ld, int64_t vocab,
  * Options: arrays [rows] on the device, or where NULL the one value for all rows (which is
  * checked: "temperature must not be NaN", "top_p must be in (0, 1]", "min_p must be in [0, 1]").
  * tokens [rows]; logprobs (nullable) [rows] f32: log_softmax(logits)[token] of the raw logits.
- * Weights are held to 2^-46 of the row's largest and summed exactly (as whole numbers), so a
- * token depends on nothing but its row. vocab <= 2^17 ... see sm_sample_rows_workspace_bytes: the
- * device bytes (16-byte aligned) that a call needs, 0 for most, -1 for a bad shape. */
+ * Weights and their sums are held in 64 bits, relative to each other within 2^-44 (weights below
+ * 2^-1000 of the row's largest are none); a row's token does not depend on the others. Rows with
+ * more equal logits at the border of a filter than a list of 1024 holds (512 up to 16384 logits), with
+ * top_k above half of that, with +inf, or with a temperature outside 1e-30 .. 1e30, take several
+ * passes over the row, 3 to 10 times as long.
+ * workspace: sm_sample_rows_workspace_bytes(...) bytes (0 but for a few rows of a large vocabulary, which
+ * are shared out over the chip; -1 for a bad shape), 16-byte aligned; calls that share one must
+ * not overlap. rows below 2^22, vocab below 2^30. */
 typedef struct sm_row_sampling {
   const float* temperatures;
   const int32_t* top_ks;

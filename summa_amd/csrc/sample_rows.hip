@@ -330,7 +330,7 @@ __device__ inline double wave_inclusive(double v) {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kSlot = 512;   // consecutive logits, a wave's share of a step: a sum of its own
-constexpr int kSlots = 512;   // sums held: 64 steps of eight waves
+constexpr int kSlots = 512;  // sums held: rows of up to 262144 logits
 constexpr float kOctaves = 40.f;  // that the bins cover
 
 template <int THREADS>
@@ -659,7 +659,7 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
   // Weights of 2^-1000 of the largest and less are none: logits below `live` are raised to it, and the
   // draw does not take them.
   const float live = lane_f32(m - 1000.f / c, 0);
-  const bool plain = !small && m < INFINITY && a.steps <= 64 &&
+  const bool plain = !small && m < INFINITY && a.vocab <= kSlots * kSlot &&
                      (greedy || (temperature <= 1e30f && temperature >= 1e-30f &&
                                  (m - live) * c > 980.f && (m - live) * c < 1020.f));
   auto log_prob = [&](float x) { return (x - m) - __logf(sum); };
@@ -888,7 +888,7 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
           }
           above += k;
           k = wave_add(MIN_P.value ? z : k);
-          if (lane == 0) slots_of_row[held.first / kSlot + i] = k;
+          if (lane == 0 && held.first + i * kSlot < a.vocab) slots_of_row[held.first / kSlot + i] = k;
         });
       };
       if (least > 0.0) sums(std::true_type{});
@@ -901,7 +901,8 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
         sh.n[wave] = mine;
       }
     } else {
-      for (int i = lane; i < a.steps; i += kWave) slots_of_row[held.first / kSlot + i] = 0.0;
+      for (int i = lane; i < a.steps; i += kWave)
+        if (held.first + i * kSlot < a.vocab) slots_of_row[held.first / kSlot + i] = 0.0;
       // in f32, what may pass min-p
       const float bar = min_p > 0.f ? fmaxf(live, m + (__log2f(fminf(min_p, 1.f)) - 0.01f) / c) : live;
       held.each(live, [&](int i, const float(&x)[8]) __attribute__((always_inline)) {
@@ -915,7 +916,7 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
           for (int e = 0; e < 4; ++e) k = fma(w[e], w[e] >= least ? 1.0 : 0.0, k);
         }
         k = wave_add(k);
-        if (lane == 0) slots_of_row[held.first / kSlot + i] = k;
+        if (lane == 0 && held.first + i * kSlot < a.vocab) slots_of_row[held.first / kSlot + i] = k;
       }, min_p > 0.f ? held.above(key_value(key_of(lane_f32(bar, 0)) - 1)) : ~(uint64_t)0);
     }
   }

@@ -82,10 +82,10 @@ def page_fork(refs: torch.Tensor, block_table: torch.Tensor, tokens: torch.Tenso
     _rows(tokens, "tokens", block_table)
     (P, cols), C = block_table.shape, source.shape[0]
     if out is None:
-        out = torch.empty((C, cols), dtype=torch.int32, device=refs.device)
+        out = refs.new_empty((C, cols))
     elif out.shape != (C, cols):
         raise ValueError("out must have a row a child and the columns of block_table")
-    src, dst = (torch.empty((C,), dtype=torch.int32, device=refs.device) for _ in range(2))
+    src, dst = torch.empty_like(source), torch.empty_like(source)
     call("sm_page_fork", refs.data_ptr(), refs.shape[0], block_table.data_ptr(), P, cols,
          tokens.data_ptr(), source.data_ptr(), C, int(page_tokens), out.data_ptr(),
          src.data_ptr(), dst.data_ptr(), _p(missing), stream)
@@ -115,8 +115,7 @@ def page_compact(refs: torch.Tensor, out: torch.Tensor | None = None):
     elif out.shape != refs.shape:
         raise ValueError("out must have the shape of refs")
     page_map = torch.empty_like(refs)
-    src, dst = (torch.empty((pages // 2,), dtype=torch.int32, device=refs.device)
-                for _ in range(2))
+    src, dst = refs.new_empty(pages // 2), refs.new_empty(pages // 2)
     call("sm_page_compact", refs.data_ptr(), pages, out.data_ptr(), page_map.data_ptr(),
          src.data_ptr(), dst.data_ptr(), stream)
     return out, page_map, src, dst

@@ -164,7 +164,7 @@ def sample_rows(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0
     elif top_k is not None:
         if top_k == 0:
             raise ValueError("top_k must be >= 1 (got 0)")
-        o.top_k = top_k
+        o.top_k = min(int(top_k), 0x7fffffff)
     if torch.is_tensor(top_p):
         o.top_ps = row_values(top_p, "top_p", torch.float32)
     else:
@@ -173,8 +173,8 @@ def sample_rows(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0
         o.min_ps = row_values(min_p, "min_p", torch.float32)
     else:
         o.min_p = min_p
-    tok = torch.empty(rows, dtype=torch.int32, device=logits.device)
-    lp = torch.empty(rows, dtype=torch.float32, device=logits.device) if want_logprobs else None
+    tok = torch.empty_like(uniforms, dtype=torch.int32)
+    lp = torch.empty_like(uniforms) if want_logprobs else None
     nbytes = _lib.lib().sm_sample_rows_workspace_bytes(rows, vocab, dt)
     if nbytes < 0:
         raise _lib.SummaError(-1, _lib.lib().sm_last_error().decode())

@@ -48,16 +48,14 @@ def _tree(t: torch.Tensor, name: str, row_start, max_rows):
 def tree_masks(parents: torch.Tensor, pos0: torch.Tensor, row_start: torch.Tensor | None = None,
                *, max_rows: int | None = None):
     """(mask int32 [rows, words], positions int32 [rows]) of every row: the rows that it sees, its
-    ancestors and itself, a bit each, and ``pos0`` plus its depth."""
+    ancestors and itself, a bit each, and ``pos0`` plus its depth. Rows of no sequence are not
+    written."""
     stream, S, rows, most, starts = _tree(parents, "parents", row_start, max_rows)
     if pos0.dtype is not torch.int32 or pos0.shape != (S,) or not pos0.is_contiguous() or \
             pos0.get_device() != parents.get_device():
         raise ValueError("pos0 must be contiguous int32 [sequences] on the device of parents")
     words = max(1, (most + 31) // 32)
-    # (rows of no sequence are not written)
-    new = torch.zeros if starts is not None else torch.empty
-    mask = new((rows, words), dtype=torch.int32, device=parents.device)
-    positions = new((rows,), dtype=torch.int32, device=parents.device)
+    mask, positions = parents.new_empty((rows, words)), parents.new_empty(rows)
     call("sm_tree_masks", parents.data_ptr(), pos0.data_ptr(), starts, S, rows, most,
          mask.data_ptr(), words, positions.data_ptr(), stream)
     return mask, positions
@@ -74,9 +72,8 @@ def tree_accept(parents: torch.Tensor, tokens: torch.Tensor, sampled: torch.Tens
         if t.dtype is not torch.int32 or t.shape != parents.shape or not t.is_contiguous() or \
                 t.get_device() != parents.get_device():
             raise ValueError(f"{name} must be contiguous int32 of parents' shape, on its device")
-    path, emitted = (torch.empty((S, most), dtype=torch.int32, device=parents.device)
-                     for _ in range(2))
-    count = torch.empty((S,), dtype=torch.int32, device=parents.device)
+    path = torch.empty_like(parents) if starts is None else parents.new_empty((S, most))
+    emitted, count = torch.empty_like(path), parents.new_empty(S)
     call("sm_tree_accept", parents.data_ptr(), tokens.data_ptr(), sampled.data_ptr(), starts, S,
          rows, most, path.data_ptr(), count.data_ptr(), emitted.data_ptr(), stream)
     return path, count, emitted

@@ -59,6 +59,36 @@ def test_sizes_and_filters(dev, vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(3, 262144), (5, 262143), (3, 262145), (2, 700001)])
+def test_the_largest_vocabularies(dev, rows, vocab, dtype):
+    """Where the sums of 512 logits fill their place, and past it."""
+    print(f"case sample {rows} {vocab} {dtype}", flush=True)
+    x = (torch.randn(rows, vocab) * 2.5).to(dtype)
+    x[:, 7] += 8
+    u = torch.rand(rows)
+    for kw in (dict(), dict(k=40), dict(p=0.9), dict(m=0.01), dict(T=0.0), dict(k=700, p=0.8)):
+        check(x, u, **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 3, 8, 31, 32, 33, 64, 65])
+@pytest.mark.parametrize("vocab", [49153, 98305, 131071])
+def test_rows_shared_out_over_the_chip(dev, rows, vocab, dtype):
+    """Every number of parts to a row and its neighbours, filters mixed over the rows."""
+    print(f"case sample {rows} {vocab} {dtype}", flush=True)
+    x = (torch.randn(rows, vocab) * 2).to(dtype)
+    u = torch.rand(rows)
+    T = torch.tensor([1.0, 0.0, 0.7, 1.3])[torch.arange(rows) % 4]
+    k = torch.tensor([-1, 50, 1, -1, 400, 600])[torch.arange(rows) % 6].to(torch.int32)
+    p = torch.tensor([0.95, 1.0, 0.5, 0.99, 1.0])[torch.arange(rows) % 5]
+    m = torch.tensor([0.0, 0.05, 0.0])[torch.arange(rows) % 3]
+    x[rows // 2, 5:] = -math.inf
+    if rows > 4:
+        x[4], x[3, 9], x[2, 100:90000] = -math.inf, math.inf, torch.finfo(dtype).min
+    check(x, u, T, k, p, m)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("rows,vocab", [(1, 151), (700, 61), (300, 4097), (37, 32768)])
 def test_many_rows_one_setting(dev, rows, vocab, dtype):
     x = (torch.randn(rows, vocab) * 3).to(dtype)
