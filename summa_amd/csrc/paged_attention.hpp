@@ -59,7 +59,7 @@ struct PagedArgs {
   float *part_o, *part_ml;       // per (row, head, split): unnormalised O; (max, sum)
   int64_t ldq;
   PagedMap map;                  // of paged_tile_kernel
-  Divide H, KVH, G, bpp, nsplit, tiles, rows_each, tile;
+  Divide H, KVH, G, bpp, nsplit, tiles, rows_each, tile, seqs;
   int S, rows, max_rows, pages, cols, cb;
   int most;                      // blocks that a table row holds, and one
   const uint32_t* mask;          // tree form: [rows, words], who sees which of its sequence's rows
@@ -103,6 +103,13 @@ struct Sees<true> {
     return true;
   }
 };
+
+// Whether row `row` < pr.n sees no key at all.
+template <bool TREE>
+__device__ inline bool no_keys(const PagedArgs& a, const PagedRows& pr, int pos0, int row) {
+  if (pos0 > 0) return false;
+  return Sees<TREE>(a, pr, pos0, row).none();
+}
 
 // Four / eight cache codes of one packed word -> the MFMA operand's 16-bit values.
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
@@ -558,7 +565,7 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
       *reinterpret_cast<float2*>(a.part_ml + (at * a.nsplit.d + split) * 2) = float2{mm, ll};
     return;
   }
-  const bool none = Sees<TREE>(a, pr, pos0, tok).none();  // a row without keys
+  const bool none = no_keys<TREE>(a, pr, pos0, tok);
   const float inv = sum_inverse<C8>(ll);
   uint32_t w2[HD / 32];
 #pragma unroll
@@ -978,8 +985,18 @@ __global__ __launch_bounds__(64 * W, 2) void paged_tile_kernel(PagedArgs a) {
   __shared__ typename T::Lds lds;
   uint32_t grp, place;
   if (!a.map.at(blockIdx.x, grp, place)) return;  // (uniform)
-  int s = (int)grp;
-  const int split = a.nsplit.mod(s), kvh = a.KVH.mod(s);
+  int s = (int)grp, split, kvh;
+  if constexpr (TREE) {
+    // The first splits of all sequences first: those that the shorter sequences do not have come
+    // last, and the units share what there is.
+    kvh = a.KVH.mod(s);
+    const int seq = a.seqs.mod(s);
+    split = s;
+    s = seq;
+  } else {
+    split = a.nsplit.mod(s);
+    kvh = a.KVH.mod(s);
+  }
   const int tile = (int)a.tiles.d - 1 - (int)place;  // the rows with the most keys first
   T t(a, lds);
   // (as in paged_split_kernel: the first loads do not wait for the lengths)
@@ -1038,7 +1055,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_tile_kernel(PagedArgs a) {
   // Through LDS, so that a store instruction writes whole rows: a lane holds 8 bytes of its
   // row at a time, and 16-byte pieces of 32 rows reach the L2 as as many requests.
   const float inv = sum_inverse<C8>(l);
-  const bool none = Sees<TREE>(a, pr, pos0, min(tok, max(0, pr.n - 1))).none();  // no keys
+  const bool none = no_keys<TREE>(a, pr, pos0, min(tok, pr.n - 1));
   constexpr int OP = HD + 8;
   uint16_t* lo = &lds.ks[0][0] + t.wave * 32 * OP;  // (the buffers are free)
   static_assert(2 * W * 32 * OP <= sizeof(lds.ks) + sizeof(lds.vts), "the rows of O fit K and V");
@@ -1122,7 +1139,7 @@ __global__ __launch_bounds__(256, 8) void paged_join_kernel(PagedArgs a) {
     for (; x + 2 <= n; x += 2) add_splits<HD, 2>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
     if (x < n) add_splits<HD, 1>(po + (size_t)(x0 + x) * HD, f, x, lane, acc);
   }
-  const bool none = Sees<TREE>(a, pr, pos0, i).none();
+  const bool none = no_keys<TREE>(a, pr, pos0, i);
   const float inv = sum_inverse<C8>(ll);
 #pragma unroll
   for (int d = 0; d < D; ++d) {
@@ -1282,6 +1299,7 @@ int paged_attention(const char* me, const sm_paged_cache* cache, const int32_t* 
   a.words = (int)words;
   a.most = (int)std::min<int64_t>(table_cols * a.bpp.d + 1, 1 << 27);
   a.nsplit = Divide(plan.nsplit);
+  a.seqs = Divide((int)S);
   a.tile = Divide(plan.tile);
   a.tiles = Divide((int)plan.tiles);
   // the keys of a group, and whether an XCD's groups leave a quarter of its 4 MiB L2
