@@ -1,10 +1,10 @@
 // Next tokens from given random numbers, each row with its own temperature, top-k, top-p and
 // min-p (sm_sample_rows; select_next_token / sample_from_values, summa-llm/src/generate.rs:127-250).
 //
-// w_i = exp((x_i - max) / T) in 64 bits, rounded to a whole number of 2^-46 (fewer for
-// vocabularies past 2^17, so that a row's sum fits 63 bits). Sums of whole numbers do not
-// depend on their order, so neither does which token the sum passes u at; in f32 one sum in a
-// few hundred rows would fall on the other side of its border.
+// The token is decided by where u falls among running sums of w_i = exp((x_i - max) / T): with
+// sums in f32 (2^-20 of the whole off) one row in a few hundred of a flat distribution over 65536
+// logits would take a neighbour. Weights and sums are held in 64 bits where they decide, in a fixed order,
+// and in f32 where they only say where to look.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -521,23 +521,36 @@ struct RowShare {
 
 // ---- the kernel ----
 //
-// A workgroup holds a row in registers (up to 65536 f32 or 131072 16-bit logits of 1024
-// threads), so that memory is read once and each step below works on registers and LDS:
-// - the largest logit, and the sum of exponentials for the log-prob, as the loads arrive;
-// - top-k (up to half of the list): the k-th largest of the threads' own maxima has at least k
-//   logits at or above it and seldom many more. These go to a list in LDS, in the vocabulary's
-//   order, are ranked by counting, and everything else is done on them;
-// - top-p without that: the weights, in f32, are added up in bins of a hundredth of an octave. The
-//   bins around p times the sum, within what f32 may be off, go to the list; one pass with 64-bit weights gives
-//   the sums of all and of those above the list, and the exact border is found in the list;
-// - the draw: sums of 512 consecutive logits are kept by the 64-bit pass; the one that u falls in
-//   is read again.
-// Every sum has a fixed order. Rows that the list does not hold (hundreds of equal logits at
-// the border, top-k above half of it), and those with +inf, go by passes.
+// A workgroup holds a row in registers (up to 65536 f32 or 131072 16-bit logits of 1024 threads), so
+// that memory is read once, and what follows works on registers and LDS:
+// - the largest logit, and in f32 the sums of the exponentials (for the log-prob) and of the
+//   weights, as the loads arrive;
+// - top-k up to half of the list: the k-th largest of the threads' own maxima, four each, has at least k
+//   logits at or above it and seldom twice as many. These go to a list in LDS, are put in order by
+//   counting, and everything else is done on them;
+// - top-p without that: the weights in f32 are added up in bins of a hundredth of an octave (LDS
+//   atomics on whole numbers: any order gives the same). The logits of the bins around p times the
+//   sum, within what f32 may be off, go to the list; one pass with 64-bit weights gives the sums of all
+//   and of those above the list, and the exact border is found in the list;
+// - the draw: sums of 512 consecutive logits are kept by the 64-bit pass; those that u falls in are
+//   read again. One wave does it.
+// Rows that the list does not hold (hundreds of equal logits at a border, a larger top-k), and those
+// with +inf, go by passes.
+//
+// Bound by instructions, not by memory. 256 rows of 65536 f32 with top-p 54 us (1.24 TB/s; the logits are 14
+// us of HBM): 13 us until the row is there, 8 for the bins, 22 for the 64-bit pass (an f64
+// operation takes 4.9 clocks of a SIMD with four waves, of which a weight needs 16 and its sums 3
+// and a logit's share of the rest 14 of 3.3), 8 for list and draw. Without a filter 25 us for 128 rows, with top-k 22.
+// 768 rows of 50001 bf16 with options of all kinds 98 us: 17 us a row with top-k, most of it eight
+// barriers' waits with one workgroup a unit, 36 with top-p.
+// Tried: 512 threads with twice the registers (54 us -> 66: two waves a SIMD issue 5.7 clocks apart), two
+// workgroups of 64 registers a thread a unit (16 bits: spills, 98 -> 466), loops unrolled over the
+// row's registers (code of 120 KB, fetched anew by every phase: 87), 64-bit bins (8 -> 12).
 //
 // PHASE 0: all of it, a workgroup a row. 1 to 4: a few large rows in `parts` workgroups each, whose parts
 // meet in memory between four kernels: 1 maxima and f32 sums, 2 bins, 3 the list and the 64-bit
-// sums, 4 the draw, a workgroup a row again.
+// sums, 4 the draw, a workgroup a row again. 6 rows of 131072 f32 with top-p and min-p 83 -> 31 us (3.5,
+// 4.6, 8.2 and 13 in the kernels).
 template <typename T, int THREADS, int STEPS, int PHASE>
 __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void sample_rows_kernel(RowsArgs a) {
   typedef RowLds<THREADS> L;
@@ -1153,7 +1166,10 @@ int check_rows(const char* who, int64_t rows, int64_t vocab, int dtype) {
   return SM_OK;
 }
 
-// Workgroups of a row: as many as a call's rows leave units for.
+// Workgroups of a row: as many as a call's rows leave units for, where that is faster than one. The
+// four launches take 18 us of the host. f32, us in parts / whole: 32 rows of 65536 with top-p 33 / 49,
+// no filter 19 / 23, top-k 23 / 20; 64 rows 44 / 49, 22 / 24, 28 / 20. 64 rows of 131072 69 / 95, 28 / 44, 33 / 34; 128
+// rows 110 / 100. 16 rows of 32768 25 / 31, 19 / 16, 20 / 16.
 int row_parts(int64_t rows, int64_t vocab) {
   const int64_t parts = std::min<int64_t>({256 / std::max<int64_t>(1, rows), ceil_div(vocab, 4096),
                                            RowShare::PARTS});
