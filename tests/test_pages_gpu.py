@@ -287,3 +287,73 @@ def test_drafted_rollouts_as_they_run(dev, cdt):
     pg.page_free(new, moved, page)
     pg.page_free(new, table, page)
     assert not new.any()
+
+
+def test_graph_of_the_page_calls(dev):
+    """A batch's turn captured once - the old rollouts freed, prompts forked, pages copied, room
+    reserved, the pool compacted - and replayed with other prompts and lengths, eager work between."""
+    from summa_amd import paged, pages as pg
+    pages, page, P, group, cols = 200, 16, 3, 4, 12
+    cache = paged.PagedKVCache(pages, 2, 64, page, F16, dev)
+    cache.k.normal_(generator=torch.Generator(device=dev).manual_seed(1))
+    cache.v.copy_(cache.k.view(cache.v.shape))
+    refs = pg.page_refs(pages, dev)
+    prompts = torch.full((P, cols), -1, dtype=torch.int32, device=dev)
+    kids = torch.full((P * group, cols), -1, dtype=torch.int32, device=dev)
+    source = torch.arange(P, dtype=torch.int32, device=dev).repeat_interleave(group)
+    tokens, room = (torch.zeros(n, dtype=torch.int32, device=dev) for n in (P, P * group))
+    new = torch.empty_like(refs)
+
+    def turn():
+        pg.page_free(refs, kids, page)
+        pg.page_free(refs, prompts, page)
+        pg.page_reserve(refs, prompts, tokens, page)
+        _, src, dst = pg.page_fork(refs, prompts, tokens, source, page, out=kids)
+        paged.paged_copy(cache, src, dst)
+        pg.page_reserve(refs, kids, room, page)
+        _, where, a, b = pg.page_compact(refs, new)
+        paged.paged_copy(cache, a, b)
+        return pg.page_remap(kids, where), src, dst, where
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        turn()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = turn()
+    gen = torch.Generator().manual_seed(5)
+    for _ in range(5):
+        tokens.copy_(torch.randint(0, 6 * page, (P,), generator=gen))
+        room.copy_(tokens[source.long()] + torch.randint(0, 5 * page, (P * group,), generator=gen).to(dev))
+        state = [x.clone() for x in (refs, prompts, kids, cache.k, cache.v)]
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in (*out, refs, prompts, kids, new, cache.k, cache.v)]
+        for x, y in zip((refs, prompts, kids, cache.k, cache.v), state):
+            x.copy_(y)
+        again = turn()
+        for x, y in zip(got, (*again, refs, prompts, kids, new, cache.k, cache.v)):
+            assert torch.equal(x, y)
+        used = -(-room // page)
+        assert torch.equal((kids >= 0).sum(1), used.clamp(max=cols).long())
+
+
+def test_two_streams_at_once(dev):
+    """Calls on two streams share nothing: sampling in parts, trees and attention."""
+    from summa_amd import sampling
+    xs = [torch.randn(4, 131072, device=dev) for _ in range(2)]
+    us = [torch.rand(4, device=dev) for _ in range(2)]
+    alone = [sampling.sample_rows(x, u, top_p=0.9) for x, u in zip(xs, us)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(sampling.sample_rows(xs[i], us[i], top_p=0.9))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for tok, lp in outs[i]:
+            assert torch.equal(tok, alone[i][0]) and torch.equal(lp, alone[i][1])
