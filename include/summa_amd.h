@@ -540,8 +540,12 @@ int sm_paged_attention(const sm_paged_cache* cache, const int32_t* block_table,
  * bit set in mask row i: bit j % 32 of word j / 32, mask [rows, words] uint32, words >= max_rows / 32
  * (sm_tree_masks; any mask is taken, a row that does not see itself or sees later ones among
  * them). Bits from n on are ignored, keys at negative positions seen by no row; a row that sees
- * no key gives 0 and lse -inf. Everything else, the workspace among it
- * (sm_paged_attention_workspace_bytes), as sm_paged_attention; max_tokens counts the rows. */
+ * no key gives 0 and lse -inf. Everything else as sm_paged_attention; the workspace's size is
+ * sm_paged_tree_attention_workspace_bytes, max_tokens counts the rows, and of up to 256 sequences
+ * the keys are split by each one's own length. */
+int64_t sm_paged_tree_attention_workspace_bytes(int64_t S, int64_t rows, int64_t max_rows,
+                                                int64_t H, int64_t KVH, int64_t head_dim,
+                                                int64_t max_tokens);
 int sm_paged_tree_attention(const sm_paged_cache* cache, const int32_t* block_table,
                             int64_t table_cols, const int32_t* pos0, const int32_t* row_start,
                             int64_t S, int64_t rows, int64_t max_rows, int64_t max_tokens,

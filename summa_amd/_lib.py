@@ -85,6 +85,7 @@ SIGNATURES: dict[str, tuple] = {
     "sm_paged_append": (i32, [vp, vp, i64, vp, vp, i64, i64, i64, vp, i64, vp, i64, vp, i64, i32,
                               i64, vp, i64, i64, i32, vp, i32, vp]),
     "sm_paged_attention_workspace_bytes": (i64, [i64, i64, i64, i64, i64, i64, i64]),
+    "sm_paged_tree_attention_workspace_bytes": (i64, [i64, i64, i64, i64, i64, i64, i64]),
     "sm_paged_attention": (i32, [vp, vp, i64, vp, vp, i64, i64, i64, i64, vp, i32, i64, i64, vp,
                                  vp, vp, i64, vp]),
     "sm_paged_tree_attention": (i32, [vp, vp, i64, vp, vp, i64, i64, i64, i64, vp, i64, vp, i32,

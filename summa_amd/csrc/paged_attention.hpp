@@ -64,6 +64,8 @@ struct PagedArgs {
   int most;                      // blocks that a table row holds, and one
   const uint32_t* mask;          // tree form: [rows, words], who sees which of its sequence's rows
   int words;
+  int share;                     // splits of all sequences together; 0: nsplit each
+  int32_t* counts;               // [S], the splits that each sequence was given
   float c2;                      // log2(e) / sqrt(hd)
 };
 
@@ -72,7 +74,7 @@ struct PagedArgs {
 // words are read in the last blocks or tiles of the keys alone, which are the only ones that have such keys;
 // held in registers from the start they make the tile kernel spill (47 -> 640 us). The form costs what
 // the causal one does: 32 x 24 rows on 1-4 k e4m3 keys 49-51 us both, 2 x 48-64 rows on 90-131 k 134-147 beside
-// 130-142; ragged trees of up to 63 rows, 16 heads of their own, bf16, 56 beside 50.
+// 130-142; ragged trees of up to 63 rows, 16 heads of their own, bf16, 54 beside 50.
 template <bool TREE>
 struct Sees {
   int last;
@@ -114,6 +116,74 @@ __device__ inline bool no_keys(const PagedArgs& a, const PagedRows& pr, int pos0
   if (pos0 > 0) return false;
   return Sees<TREE>(a, pr, pos0, row).none();
 }
+
+// Split j of all the sequences' together, in the tree form: its calls are few rows on contexts that
+// differ, and the splits are as long as gives `share` of them, so that all units end together.
+// Every wave finds the length for itself, a sequence a lane (the bounds are close: one to three steps),
+// and then the sequence of j. 16 trees of 16 rows on 0.5-30 k e4m3 keys 93 us, 122 with the longest
+// sequence's splits for all; 32 x 4 rows on 1-4 k bf16 37 and 44; 17 ragged trees, 16 heads of their own,
+// 54 and 60; 2 x 48-64 rows on 90-131 k 139 and 142. Where all are alike, the lengths that the first loads
+// wait for cost 2-3 us: 32 x 24 rows on 4000 keys 53.5 and 51.
+constexpr int kShared = 256;  // sequences at most
+struct TreeSplit {
+  int s, split, splits, cb;  // s < 0: there is no such split
+  __device__ inline TreeSplit(const PagedArgs& a, int j) : s(-1), split(0), splits(1), cb(kUnit) {
+    const int lane = threadIdx.x % kWave;
+    constexpr int N = kShared / kWave;
+    uint32_t units[N];
+    float all = 0.f;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      units[c] = 0;
+      const int q = c * kWave + lane;
+      if (c * kWave < a.S && q < a.S) {
+        const PagedRows pr(a.row_start, q, a.rows, a.max_rows);
+        // (PagedKeys' of all of the sequence's rows)
+        const int64_t keys = pr.n > 0 ? (int64_t)a.pos0[q] + pr.n : 0;
+        const int64_t held = min((int64_t)a.most * kBlock, (int64_t)0x7fffffff);
+        units[c] = keys <= 0 ? 0 : ((uint32_t)min(keys, held) - 1) / (kBlock * kUnit) + 1;
+      }
+      all += (float)units[c];
+    }
+    all = wave_sum(all);
+    int lo, hi;
+    PagedShare::bounds(all, a.S, a.share, lo, hi);
+    while (lo < hi) {  // (uniform)
+      const int mid = lo + (hi - lo) / 2;
+      float n = 0.f;
+#pragma unroll
+      for (int c = 0; c < N; ++c)
+        if (c * kWave < a.S && c * kWave + lane < a.S)
+          n += (float)PagedShare::most(units[c], mid, a.nsplit.d);
+      if (wave_sum(n) <= (float)a.share) hi = mid;
+      else lo = mid + 1;
+    }
+    int before = 0;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      if (s >= 0 || c * kWave >= a.S) continue;  // (uniform)
+      const PagedShare ps(units[c], lo, a.nsplit.d);
+      const int n = c * kWave + lane < a.S ? ps.splits : 0;
+      int end = n;  // sums up to and with this lane's: in rows of 16 lanes, then of the rows
+      end += __builtin_amdgcn_update_dpp(0, end, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+      end += __builtin_amdgcn_update_dpp(0, end, 0x112, 0xF, 0xF, false);
+      end += __builtin_amdgcn_update_dpp(0, end, 0x114, 0xF, 0xF, false);
+      end += __builtin_amdgcn_update_dpp(0, end, 0x118, 0xF, 0xF, false);
+      const int r0 = __builtin_amdgcn_readlane(end, 15), r1 = __builtin_amdgcn_readlane(end, 31),
+                r2 = __builtin_amdgcn_readlane(end, 47);
+      end += lane >= 48 ? r0 + r1 + r2 : lane >= 32 ? r0 + r1 : lane >= 16 ? r0 : 0;
+      const uint64_t at = __ballot(j - before < end);
+      if (at) {
+        const int l = (int)__builtin_ctzll(at);
+        s = c * kWave + l;
+        splits = __builtin_amdgcn_readlane(n, l);
+        split = j - before - (__builtin_amdgcn_readlane(end, l) - splits);
+        cb = __builtin_amdgcn_readlane(ps.cb, l);
+      }
+      before += __builtin_amdgcn_readlane(end, kWave - 1);
+    }
+  }
+};
 
 // Four / eight cache codes of one packed word -> the MFMA operand's 16-bit values.
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
@@ -328,22 +398,36 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs a) {
   __shared__ float sm_m[4][kRows16], sm_l[4][kRows16];
   __shared__ __attribute__((aligned(16))) float sm_o[4][kRows16][HD + 4];
 
-  int s = (int)blockIdx.x;
-  const int split = a.nsplit.mod(s), kvh = a.KVH.mod(s), tile = a.tiles.mod(s);
+  int s = (int)blockIdx.x, split, kvh, tile, cb = a.cb, most_splits = (int)a.nsplit.d;
+  if (TREE && a.share) {  // (uniform)
+    kvh = a.KVH.mod(s);
+    tile = a.tiles.mod(s);
+    const TreeSplit ts(a, s);
+    if (ts.s < 0) return;
+    s = ts.s;
+    split = ts.split;
+    cb = ts.cb;
+    most_splits = ts.splits;
+    if (split + kvh + tile == 0 && threadIdx.x == 0) a.counts[s] = most_splits;
+  } else {
+    split = a.nsplit.mod(s);
+    kvh = a.KVH.mod(s);
+    tile = a.tiles.mod(s);
+  }
   // What the first loads need does not wait for the sequence's lengths: a workgroup without
   // work goes through them too (its rows and table row are there) and leaves after the loop.
   const int32_t* trow = a.table + (int64_t)s * a.cols;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int r = lane % 16, g = lane / 16;
   Blocks cur, next;
-  cur.find(a, trow, kvh, split * a.cb + lane);
+  cur.find(a, trow, kvh, split * cb + lane);
   const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
   const int pos0 = a.pos0[s];
   const int row0 = tile * kRows16, all = pr.n * (int)a.G.d;
-  const PagedKeys pk(pos0, pr.n, a.G, TREE ? 0 : row0, TREE ? all : kRows16, a.cb,
-                     (int)a.nsplit.d, a.most);
+  const PagedKeys pk(pos0, pr.n, a.G, TREE ? 0 : row0, TREE ? all : kRows16, cb, most_splits,
+                     a.most);
   const bool idle = row0 >= all || split >= max(pk.splits, 1);
-  const int b0 = split * a.cb, b1 = idle || pk.keys <= 0 ? b0 : pk.end(split, a.cb);
+  const int b0 = split * cb, b1 = idle || pk.keys <= 0 ? b0 : pk.end(split, cb);
 
   // this lane's query: row row0 + r
   const int qr = max(0, min(row0 + r, all - 1));
@@ -989,14 +1073,24 @@ __global__ __launch_bounds__(64 * W, 2) void paged_tile_kernel(PagedArgs a) {
   __shared__ typename T::Lds lds;
   uint32_t grp, place;
   if (!a.map.at(blockIdx.x, grp, place)) return;  // (uniform)
-  int s = (int)grp, split, kvh;
+  int s = (int)grp, split, kvh, cb = a.cb, most_splits = (int)a.nsplit.d;
   if constexpr (TREE) {
-    // The first splits of all sequences first: those that the shorter sequences do not have come
-    // last, and the units share what there is (17 trees on 0-3000 keys, 16 heads, bf16: 59 -> 56 us).
     kvh = a.KVH.mod(s);
-    const int seq = a.seqs.mod(s);
-    split = s;
-    s = seq;
+    if (a.share) {  // (uniform)
+      const TreeSplit ts(a, s);
+      if (ts.s < 0) return;
+      s = ts.s;
+      split = ts.split;
+      cb = ts.cb;
+      most_splits = ts.splits;
+      if (split + kvh + (int)place == 0 && threadIdx.x == 0) a.counts[s] = most_splits;
+    } else {
+      // The first splits of all sequences first: those that the shorter sequences do not have come
+      // last, and the units share what there is.
+      const int seq = a.seqs.mod(s);
+      split = s;
+      s = seq;
+    }
   } else {
     split = a.nsplit.mod(s);
     kvh = a.KVH.mod(s);
@@ -1008,16 +1102,16 @@ __global__ __launch_bounds__(64 * W, 2) void paged_tile_kernel(PagedArgs a) {
   t.kvh = kvh;
   t.wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   t.lane = threadIdx.x % kWave;
-  t.cur.find(a, t.trow, kvh, split * a.cb + t.lane);
+  t.cur.find(a, t.trow, kvh, split * cb + t.lane);
   const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
   const int pos0 = a.pos0[s];
   const int row0 = tile * kRowsTile, all = pr.n * (int)a.G.d;
-  const PagedKeys pk(pos0, pr.n, a.G, TREE ? 0 : row0, TREE ? all : kRowsTile, a.cb,
-                     (int)a.nsplit.d, a.most);
+  const PagedKeys pk(pos0, pr.n, a.G, TREE ? 0 : row0, TREE ? all : kRowsTile, cb, most_splits,
+                     a.most);
   const bool idle = row0 >= all || split >= max(pk.splits, 1);
   const int j = t.j = t.lane % 32, hf = t.hf = t.lane / 32;
-  t.b0 = split * a.cb;
-  t.b1 = idle || pk.keys <= 0 ? t.b0 : pk.end(split, a.cb);
+  t.b0 = split * cb;
+  t.b1 = idle || pk.keys <= 0 ? t.b0 : pk.end(split, cb);
   t.keys = pk.keys;
   const int r0 = row0 + t.wave * 32;  // first row of this wave
   const int qr = max(0, min(r0 + j, all - 1));
@@ -1114,25 +1208,27 @@ __global__ __launch_bounds__(256, 8) void paged_join_kernel(PagedArgs a) {
   const int lane = threadIdx.x % kWave;
   const int head = a.H.mod(s), i = a.rows_each.mod(s);
   if (s >= a.S) return;
+  const int given = TREE && a.share ? a.counts[s] : 0;
   const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
   if (i >= pr.n) return;
   int x = head;
   const int pos0 = a.pos0[s], row = i * (int)a.G.d + a.G.mod(x);
   const PagedKeys pk(pos0, pr.n, a.G, TREE ? 0 : a.tile.div(row) * (int)a.tile.d,
                      TREE ? pr.n * (int)a.G.d : (int)a.tile.d, a.cb, (int)a.nsplit.d, a.most);
-  if (pk.splits <= 1) return;  // written already
+  const int splits = TREE && a.share ? given : pk.splits;
+  if (splits <= 1) return;  // written already
   const size_t at = (size_t)(pr.first + i) * a.H.d + head;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at * a.nsplit.d;
   const float* po = a.part_o + at * a.nsplit.d * HD;
   constexpr int D = HD / kWave;
   float mm = -INFINITY;
-  for (int x = lane; x < pk.splits; x += kWave) mm = fmaxf(mm, ml[x].x);
+  for (int x = lane; x < splits; x += kWave) mm = fmaxf(mm, ml[x].x);
   mm = wave_max(mm);
   float ll = 0.f, acc[D];
 #pragma unroll
   for (int d = 0; d < D; ++d) acc[d] = 0.f;
-  for (int x0 = 0; x0 < pk.splits; x0 += kWave) {
-    const int n = min(kWave, pk.splits - x0);
+  for (int x0 = 0; x0 < splits; x0 += kWave) {
+    const int n = min(kWave, splits - x0);
     const float2 v = lane < n ? ml[x0 + lane] : float2{-INFINITY, 0.f};
     const Join j(v.x, v.y, mm);
     const float f = j.weight();
@@ -1207,6 +1303,21 @@ struct PagedPlan {
   int64_t bytes(int64_t rows, int64_t H, int64_t hd) const {
     return nsplit > 1 ? rows * H * nsplit * (hd + 2) * 4 : 0;
   }
+  // The tree form: where the longest sequence's keys are split, all sequences share `share` splits,
+  // as many as fill the units, of which one has four times its even share at most.
+  int share = 0;
+  void by_length(int64_t S, int64_t KVH, int64_t max_tokens) {
+    if (nsplit <= 1 || S > kShared) return;
+    const int64_t fill = tile == kRows16 ? 1024 : tile == 128 ? 512 : 256;
+    share = (int)ceil_div(fill, KVH * tiles);  // (more than S)
+    const int64_t blocks = ceil_div(max_tokens, kBlock);
+    nsplit = (int)std::min({ceil_div(blocks, kShare * kUnit), 4 * ceil_div(share, S),
+                            (int64_t)share - S + 1});
+    nsplit = std::max(nsplit, 2);
+    wgs = tile == kRows16 ? KVH * tiles * share
+                          : PrefillMap((uint32_t)(KVH * share), (uint32_t)tiles).workgroups();
+  }
+  int64_t counts(int64_t S) const { return share ? ceil_div(S, 4) * 16 : 0; }  // bytes
 };
 
 int check_shape(const char* who, int64_t S, int64_t rows, int64_t max_rows, int64_t H,
@@ -1263,8 +1374,9 @@ int paged_attention(const char* me, const sm_paged_cache* cache, const int32_t* 
   SM_REQUIRE(ldq >= H * hd && ldq < ((int64_t)1 << 31) && ldq % 8 == 0 && qa % 16 == 0 &&
                  oa % 16 == 0,
              "%s: q rows and out must be 16-byte aligned, ldq >= H * head_dim and ldq < 2^31", me);
-  const PagedPlan plan(S, max_rows, H / KVH, KVH, hd, max_tokens);
-  const int64_t need = plan.bytes(rows, H, hd);
+  PagedPlan plan(S, max_rows, H / KVH, KVH, hd, max_tokens);
+  if (TREE) plan.by_length(S, KVH, max_tokens);
+  const int64_t need = plan.bytes(rows, H, hd) + plan.counts(S);
   SM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need &&
                            reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
              "%s: workspace of %lld bytes, %lld needed, 16-byte aligned", me,
@@ -1285,7 +1397,9 @@ int paged_attention(const char* me, const sm_paged_cache* cache, const int32_t* 
   a.row_start = row_start;
   a.out = out;
   a.lse = lse;
-  a.part_o = static_cast<float*>(workspace);
+  a.share = plan.share;
+  a.counts = static_cast<int32_t*>(workspace);
+  a.part_o = need ? static_cast<float*>(workspace) + plan.counts(S) / 4 : nullptr;
   a.part_ml = need ? a.part_o + rows * H * plan.nsplit * hd : nullptr;
   a.ldq = ldq;
   a.S = (int)S;
@@ -1309,8 +1423,8 @@ int paged_attention(const char* me, const sm_paged_cache* cache, const int32_t* 
   // the keys of a group, and whether an XCD's groups leave a quarter of its 4 MiB L2
   const int64_t span = plan.nsplit > 1 ? (int64_t)plan.cb * kBlock : max_tokens;
   const int64_t kv = span * hd * (cache->dtype == SM_F8E4M3 ? 2 : 4);
-  a.map = PagedMap((uint32_t)(S * KVH * plan.nsplit), (uint32_t)plan.tiles,
-                   S * KVH * plan.nsplit / 8 * kv <= 3 << 20);
+  const int64_t groups = KVH * (plan.share ? plan.share : S * plan.nsplit);
+  a.map = PagedMap((uint32_t)groups, (uint32_t)plan.tiles, groups / 8 * kv <= 3 << 20);
   a.c2 = 1.44269504088896340736f / sqrtf((float)hd);
   const bool f16 = dtype == SM_F16, c8 = cache->dtype == SM_F8E4M3;
 #define SM_PAGED2(HD, F, C)                                                      \

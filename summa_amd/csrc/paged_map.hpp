@@ -97,6 +97,49 @@ struct PagedKeys {
   }
 };
 
+// Shares of a tree batch's sequences: splits by a sequence's own length, in units of kUnit
+// blocks. A split holds `cb` units at most where the `slots` of a row allow it; the sequence's
+// splits are alike but for the last. Without keys there is one, which writes zeros.
+constexpr int kUnit = 8;
+constexpr int kShare = 4;  // units of a split at least: 512 keys
+// x / by, rounded up. The quotient in f32 is off by less than 2^-22 of it, and so by less than the
+// 1 / by between it and the next whole number where x is below 2^21. (The compiler's own
+// division takes four times the instructions, and every workgroup waits for some.)
+__host__ __device__ inline uint32_t share_ceil(uint32_t x, uint32_t by) {
+  if (x >= 1u << 21) return (x - 1) / by + 1;
+#ifdef __HIP_DEVICE_COMPILE__
+  const float r = __builtin_amdgcn_rcpf((float)by);
+#else
+  const float r = 1.f / (float)by;
+#endif
+  const uint32_t q = (uint32_t)((float)x * r);
+  return q + (q * by < x);
+}
+struct PagedShare {
+  int cb;      // blocks of a split
+  int splits;  // 1 .. slots
+  // how many there are at most
+  __host__ __device__ static uint32_t most(uint32_t units, uint32_t cb_units, uint32_t slots) {
+    const uint32_t n = share_ceil(units, cb_units);
+    return n < 1 ? 1 : n > slots ? slots : n;
+  }
+  __host__ __device__ PagedShare(uint32_t units, uint32_t cb_units, uint32_t slots) {
+    const uint32_t each = units ? share_ceil(units, most(units, cb_units, slots)) : 1;
+    cb = (int)(each * kUnit);
+    splits = units ? (int)share_ceil(units, each) : 1;
+  }
+  // Lengths between which the shortest is that gives S < share sequences of `all` units together
+  // `share` splits at most. With hi it holds: units / hi rounded up, each, is at most one more each.
+  // (2^25 is more than a sequence has.)
+  __host__ __device__ static void bounds(float all, int S, int share, int& lo, int& hi) {
+    const float most = all / (float)(share - S) * 1.0001f;
+    lo = (int)(all / (float)share * 0.9999f);
+    if (lo < kShare) lo = kShare;
+    hi = most < 0x1p25f ? (int)most + 1 : 1 << 25;
+    if (hi < lo) hi = lo;
+  }
+};
+
 // Which workgroup takes which (KV head of a sequence's split) and row tile: PrefillMap's
 // share of groups for every XCD, whose L2 then reads a group's K and V once, but
 // - the eight groups of a set go to the XCDs in another turn in each set, so that a long

@@ -243,8 +243,8 @@ def _attention(name, cache, q, block_table, pos0, row_start, max_rows, max_token
         max_tokens = min(cols * cache.page_tokens, 0x7fffffff)
     nbytes, ws = 0, None
     if max_tokens > 512:  # (none for fewer)
-        nbytes = _lib.lib().sm_paged_attention_workspace_bytes(S, rows, most, H, cache.kv_heads,
-                                                               cache.head_dim, max_tokens)
+        size = getattr(_lib.lib(), name + "_workspace_bytes")
+        nbytes = size(S, rows, most, H, cache.kv_heads, cache.head_dim, max_tokens)
         if nbytes < 0:
             raise _lib.SummaError(-1, _lib.lib().sm_last_error().decode())
         if nbytes:

@@ -352,3 +352,42 @@ def test_graph_of_a_step(dev):
             assert torch.equal(x.view(bits), y.view(bits))
         for x, y in zip(moved, b.raw()):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("pos0,n,H,KVH,dtype,cdt", [
+    ([9000, 0, 700, 31, 4100], [3, 1, 2, 3, 3], 4, 2, F16, F8),          # 16 rows a KV head
+    ([20000, 0, -9, 513, 130], [40, 3, 9, 33, 64], 2, 1, BF16, BF16),    # 128
+    ([9000, 8000, 1], [150, 2, 70], 4, 2, F16, F16),                     # several tiles
+    ([60 * (i % 9) + (4000 if i == 70 else 0) for i in range(100)], [2] * 100, 2, 2, F16, F8),
+    ([40 * (i % 5) + 600 * (i % 64 == 63) for i in range(256)], [1] * 256, 2, 1, BF16, F8),
+    ([40 * (i % 5) + 600 * (i % 64 == 63) for i in range(257)], [1] * 257, 2, 1, F16, F16),
+])
+def test_unequal_contexts(dev, pos0, n, H, KVH, dtype, cdt):
+    """Splits shared by sequences of very different lengths, whatever max_tokens says, and captured
+    with other lengths than it is replayed with."""
+    print(f"case unequal {len(n)} {dtype} {cdt}", flush=True)
+    b = tree_batch(dev, pos0, n, KVH, 64, 32, cdt)
+    gen = torch.Generator().manual_seed(len(n))
+    sees = random_masks(b, gen, "tree")
+    mask = R.words(sees, (max(n) + 31) // 32).to(dev)
+    q = torch.randn(b.rows, H, 64).to(dtype)
+    qd = q.to(dev)
+    results = {}
+    for tokens in (None, max(pos0) + max(n), 513, 1, 2 ** 31 - 1):
+        got, lse = attention(b, qd, mask, want_lse=True, max_tokens=tokens)
+        check(b, q, sees, got, lse)
+        results[tokens] = got
+    out = torch.empty_like(results[None])
+    right = b.p.clone()
+    graph = torch.cuda.CUDAGraph()
+    b.p.zero_()
+    with torch.cuda.graph(graph):
+        attention(b, qd, mask, out=out)
+    for turn in range(4):
+        b.p.copy_(right if turn % 2 else torch.zeros_like(right))
+        graph.replay()
+        again = attention(b, qd, mask)
+        torch.cuda.synchronize()
+        # (bits: at position 0 a sequence without a page has NaN)
+        assert torch.equal(out.view(torch.int16), again.view(torch.int16))
+    assert torch.equal(out, results[None])
