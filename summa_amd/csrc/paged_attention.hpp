@@ -1208,7 +1208,7 @@ __global__ __launch_bounds__(256, 8) void paged_join_kernel(PagedArgs a) {
   const int lane = threadIdx.x % kWave;
   const int head = a.H.mod(s), i = a.rows_each.mod(s);
   if (s >= a.S) return;
-  const int given = TREE && a.share ? a.counts[s] : 0;
+  const int given = TREE && a.share ? min(a.counts[s], (int)a.nsplit.d) : 0;
   const PagedRows pr(a.row_start, s, a.rows, a.max_rows);
   if (i >= pr.n) return;
   int x = head;
