@@ -544,7 +544,8 @@ struct RowShare {
 // 768 rows of 50001 bf16 with options of all kinds 98 us: 17 us a row with top-k, most of it eight
 // barriers' waits with one workgroup a unit, 36 with top-p.
 // Tried: 512 threads with twice the registers (54 us -> 66: two waves a SIMD issue 5.7 clocks apart), two
-// workgroups of 64 registers a thread a unit (16 bits: spills, 98 -> 466), loops unrolled over the
+// workgroups of 64 registers a thread a unit (16 bits: spills, 98 -> 466) or of 512 threads (117: a row
+// takes twice as long), the rows in the order of their length (94, for a scan before the first load), loops unrolled over the
 // row's registers (code of 120 KB, fetched anew by every phase: 87), 64-bit bins (8 -> 12).
 //
 // PHASE 0: all of it, a workgroup a row. 1 to 4: a few large rows in `parts` workgroups each, whose parts
