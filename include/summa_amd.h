@@ -595,11 +595,13 @@ int sm_paged_keep(const sm_paged_cache* caches, int64_t ncaches, const int32_t* 
  *   out [C, table_cols] gets the prompt's full pages (one holder more) and, where the prompt's last page
  *   is unfinished, a page of its own, to be copied from src[c] to dst[c] (sm_paged_copy; both -1
  *   where nothing is to be copied). out may be the last batch's table, freed, but not overlap
- *   block_table. A source outside [0, P) gives an empty row.
+ *   block_table. A source outside [0, P) gives an empty row; a page that the prompt's row does not
+ *   hold, unfinished ones among them, is not the child's either (-1).
  * sm_page_free: entries behind those of the first tokens[s] tokens (NULL: all) leave their
  *   pages and become -1. A page that nothing holds is free; its contents stay until it is given.
  * missing (nullable) [1]: how many pages were not there (those entries stay -1, and tokens
- *   behind them are not stored by sm_paged_append), columns and prompts that the table does not have included.
+ *   behind them are not stored by sm_paged_append), columns that the table does not have and, of a
+ *   fork, pages that the prompt's row does not hold included; a prompt that there is not counts one.
  * sm_page_compact: the L live pages to the front: refs_out (may be refs) and page_map [pages],
  *   where each page is then (-1: free); the i-th live page from L on goes to the i-th free page
  *   below L, src[i] to dst[i] (arrays of pages / 2; -1 behind the last). Pages from L on are

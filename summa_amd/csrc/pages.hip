@@ -168,8 +168,20 @@ struct ForkArgs {
   int pages, P, C, cols;
 };
 
+__global__ void clear_missing_kernel(int32_t* missing) { *missing = 0; }
+
+// *to += n, 2^31 - 1 at most.
+__device__ inline void add_missing(int32_t* to, int64_t n) {
+  if (n <= 0) return;
+  int32_t old = *reinterpret_cast<volatile int32_t*>(to), seen;
+  while ((seen = atomicCAS(to, old, (int32_t)min((int64_t)old + n, (int64_t)0x7fffffff))) != old)
+    old = seen;
+}
+
 // Workgroup 0 gives each child a page of its own for its prompt's unfinished one; the others
-// share the full pages, a wave a child.
+// share the full pages, a wave a child. A page that the prompt's row does not hold is not the
+// child's either: nothing could be copied to one of its own, which would then show the tokens
+// of whoever had it last.
 __global__ __launch_bounds__(kScan) void fork_kernel(ForkArgs a) {
   if (blockIdx.x > 0) {
     const int64_t c = (int64_t)(blockIdx.x - 1) * kWaves + threadIdx.x / kWave;
@@ -178,16 +190,27 @@ __global__ __launch_bounds__(kScan) void fork_kernel(ForkArgs a) {
     const bool ok = p >= 0 && p < a.P;
     const int n = ok ? max(0, a.tokens[p]) : 0, full = a.page.div(n);
     const bool part = n - full * (int)a.page.d > 0;
+    int lacking = 0;  // of this lane's columns
     for (int j = lane; j < a.cols; j += kWave) {
       if (j == full && part) continue;  // workgroup 0's
       int page = -1;
       if (j < full) {
         page = a.table[(int64_t)p * a.cols + j];
-        if (page < 0 || page >= a.pages) page = -1;
-        else atomicAdd(a.refs + page, 1);
+        if (page < 0 || page >= a.pages) {
+          page = -1;
+          ++lacking;
+        } else {
+          atomicAdd(a.refs + page, 1);
+        }
       }
       a.out[c * a.cols + j] = page;
     }
+    if (!a.missing) return;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) lacking += __shfl_xor(lacking, o, kWave);
+    // and the columns that the table does not have
+    if (lane == 0)
+      add_missing(a.missing, !ok ? 1 : (int64_t)lacking + max(0, full + (part ? 1 : 0) - a.cols));
     return;
   }
   __shared__ Giver sh;
@@ -203,16 +226,13 @@ __global__ __launch_bounds__(kScan) void fork_kernel(ForkArgs a) {
       if (p >= 0 && p < a.P) {
         const int n = max(0, a.tokens[p]);
         full = a.page.div(n);
-        if (full >= a.cols) {
-          lacking += n - a.cols * (int64_t)a.page.d > 0;  // columns that the table does not have
-        } else if (n - full * (int)a.page.d > 0) {
-          want = 1;
+        if (full < a.cols && n - full * (int)a.page.d > 0) {
           from = a.table[(int64_t)p * a.cols + full];
           if (from >= a.pages) from = -1;
+          want = from >= 0;
+          lacking += from < 0;
           a.out[c * a.cols + full] = -1;
         }
-      } else {
-        lacking += 1;
       }
       a.src[c] = -1;
       a.dst[c] = -1;
@@ -230,7 +250,7 @@ __global__ __launch_bounds__(kScan) void fork_kernel(ForkArgs a) {
   }
   int total;
   sh.scan.exclusive(lacking, total);
-  if (a.missing && threadIdx.x == 0) *a.missing = total;
+  if (a.missing && threadIdx.x == 0) add_missing(a.missing, total);
 }
 
 // A wave a row: entries behind the first tokens[s] tokens' leave their pages.
@@ -422,6 +442,10 @@ extern "C" int sm_page_fork(int32_t* refs, int64_t pages, const int32_t* block_t
   a.P = (int)P;
   a.C = (int)C;
   a.cols = (int)table_cols;
+  if (missing) {  // (which all workgroups add to)
+    clear_missing_kernel<<<1, 1, 0, as_stream(stream)>>>(missing);
+    SM_LAUNCH_CHECK();
+  }
   fork_kernel<<<(unsigned)(1 + ceil_div(C, kWaves)), kScan, 0, as_stream(stream)>>>(a);
   SM_LAUNCH_CHECK();
   return SM_OK;

@@ -76,7 +76,8 @@ def page_fork(refs: torch.Tensor, block_table: torch.Tensor, tokens: torch.Tenso
     """(table [children, columns], src, dst [children]): child c shares the full pages that hold
     the ``tokens[source[c]]`` tokens of row ``source[c]`` of ``block_table``, and has a page of
     its own for an unfinished last one, to be copied with ``paged.paged_copy(caches, src, dst)``
-    (-1: none). ``out``: the table to write (what it held before is not freed)."""
+    (both -1: none). What the prompt's row does not hold, the child's does not either, and
+    ``missing`` counts it. ``out``: the table to write (what it held before is not freed)."""
     stream = _check(refs, (block_table, "block_table", 2), (tokens, "tokens", 1),
                     (source, "source", 1), (out, "out", 2), _missing(missing))
     _rows(tokens, "tokens", block_table)
