@@ -27,19 +27,20 @@ constexpr int kScan = 1024;        // threads of the workgroup that scans
 constexpr int kWaves = kScan / kWave;
 
 // Exclusive prefix sum of one value a thread over the workgroup, and the sum of all.
+template <typename T>
 struct Scan {
-  int part[kWaves];
-  __device__ inline int exclusive(int v, int& total) {
+  T part[kWaves];
+  __device__ inline T exclusive(T v, T& total) {
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
-    int inc = v;
+    T inc = v;
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {
-      const int t = __shfl_up(inc, o, kWave);
+      const T t = __shfl_up(inc, o, kWave);
       if (lane >= o) inc += t;
     }
     if (lane == kWave - 1) part[w] = inc;
     __syncthreads();
-    int base = 0;
+    T base = 0;
     total = 0;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
@@ -59,7 +60,8 @@ __device__ inline void load_refs(const int32_t* refs, int pages, int64_t p, int 
 
 // Gives pages to 1024 askers at a time, askers in order and pages from the lowest free one up.
 struct Giver {
-  Scan scan;
+  Scan<int> scan;
+  Scan<int64_t> sums;  // (1024 rows may ask for more than 2^31 pages together)
   int before[kScan];  // pages that the askers before this one get
   int first[kScan];   // column of the asker's first new page
   int row[kScan];     // its table row; -1: none
@@ -69,11 +71,12 @@ struct Giver {
 // Each thread asks for `want` pages from column `col` of table row `r` on. give(row, col, page,
 // asker) is called once for each page given. Returns how many were not there (uniform).
 template <typename Give>
-__device__ inline int give_pages(Giver& sh, int32_t* refs, int pages, int want, int r, int col,
-                                 Give give) {
-  int total;
-  const int at = sh.scan.exclusive(want, total);
-  sh.before[threadIdx.x] = at;
+__device__ inline int64_t give_pages(Giver& sh, int32_t* refs, int pages, int want, int r, int col,
+                                     Give give) {
+  int64_t asked;
+  const int64_t before = sh.sums.exclusive(want, asked);
+  const int total = (int)min(asked, (int64_t)pages);  // no more can be given
+  sh.before[threadIdx.x] = (int)min(before, (int64_t)pages);
   sh.first[threadIdx.x] = col;
   sh.row[threadIdx.x] = r;
   __syncthreads();
@@ -109,7 +112,7 @@ __device__ inline int give_pages(Giver& sh, int32_t* refs, int pages, int want, 
     given = min(total, given + found);
     __syncthreads();
   }
-  return total - given;
+  return asked - given;
 }
 
 __device__ inline int pages_of(int tokens, const Divide& page) {
@@ -125,7 +128,7 @@ __global__ __launch_bounds__(kScan) void reserve_kernel(int32_t* refs, int pages
   if (threadIdx.x == 0) sh.next = 0;
   __syncthreads();
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  int lacking = 0;
+  int64_t lacking = 0;
   for (int64_t s0 = 0; s0 < S; s0 += kScan) {
     // columns in use: a wave a row, 64 columns at a time
     for (int i = wave; i < kScan && s0 + i < S; i += kWaves) {
@@ -133,7 +136,7 @@ __global__ __launch_bounds__(kScan) void reserve_kernel(int32_t* refs, int pages
       const int need = min(cols, pages_of(tokens[s0 + i], page));
       int n = 0;
       while (n < need) {
-        const bool none = n + lane >= need || t[n + lane] < 0;
+        const bool none = n + (int64_t)lane >= need || t[n + lane] < 0;
         const uint64_t m = __ballot(none);
         if (m) {
           n = min(need, n + (int)__builtin_ctzll(m));
@@ -149,16 +152,16 @@ __global__ __launch_bounds__(kScan) void reserve_kernel(int32_t* refs, int pages
     const int col = s < S ? held[threadIdx.x] : 0;
     const int want = max(0, min(cols, asked) - col);
     lacking += max(0, asked - cols);  // columns that the table does not have
-    const int none = give_pages(sh, refs, pages, want, threadIdx.x, col,
-                                [&](int r, int c, int p, int) {
-                                  table[(s0 + r) * cols + c] = p;
-                                });
+    const int64_t none = give_pages(sh, refs, pages, want, threadIdx.x, col,
+                                    [&](int r, int c, int p, int) {
+                                      table[(s0 + r) * cols + c] = p;
+                                    });
     if (threadIdx.x == 0) lacking += none;
     __syncthreads();
   }
-  int total;
-  sh.scan.exclusive(lacking, total);
-  if (missing && threadIdx.x == 0) *missing = total;
+  int64_t total;
+  sh.sums.exclusive(lacking, total);
+  if (missing && threadIdx.x == 0) *missing = (int32_t)min(total, (int64_t)0x7fffffff);
 }
 
 struct ForkArgs {
@@ -216,7 +219,7 @@ __global__ __launch_bounds__(kScan) void fork_kernel(ForkArgs a) {
   __shared__ Giver sh;
   if (threadIdx.x == 0) sh.next = 0;
   __syncthreads();
-  int lacking = 0;
+  int64_t lacking = 0;
   for (int64_t c0 = 0; c0 < a.C; c0 += kScan) {
     const int64_t c = c0 + threadIdx.x;
     int full = 0, want = 0;
@@ -238,18 +241,18 @@ __global__ __launch_bounds__(kScan) void fork_kernel(ForkArgs a) {
       a.dst[c] = -1;
     }
     __syncthreads();
-    const int none = give_pages(sh, a.refs, a.pages, want, threadIdx.x, full,
-                                [&](int r, int col, int page, int) {
-                                  a.out[(c0 + r) * a.cols + col] = page;
-                                  a.dst[c0 + r] = page;
-                                });
+    const int64_t none = give_pages(sh, a.refs, a.pages, want, threadIdx.x, full,
+                                    [&](int r, int col, int page, int) {
+                                      a.out[(c0 + r) * a.cols + col] = page;
+                                      a.dst[c0 + r] = page;
+                                    });
     if (threadIdx.x == 0) lacking += none;
     __syncthreads();
     if (c < a.C && from >= 0 && a.dst[c] >= 0) a.src[c] = from;
     __syncthreads();
   }
-  int total;
-  sh.scan.exclusive(lacking, total);
+  int64_t total;
+  sh.sums.exclusive(lacking, total);
   if (a.missing && threadIdx.x == 0) add_missing(a.missing, total);
 }
 
@@ -275,7 +278,7 @@ __global__ __launch_bounds__(256) void free_kernel(int32_t* refs, int pages, int
 __global__ __launch_bounds__(kScan) void compact_kernel(const int32_t* refs, int pages,
                                                         int32_t* refs_out, int32_t* where,
                                                         int32_t* src, int32_t* dst) {
-  __shared__ Scan scan;
+  __shared__ Scan<int> scan;
   const int t = threadIdx.x;
   int live = 0;
   for (int64_t p = 4 * t; p < pages; p += 4 * kScan) {

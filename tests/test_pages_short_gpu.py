@@ -106,3 +106,18 @@ def test_missing_does_not_wrap(dev):
     assert int(missing) == 2 ** 31 - 1
     pg.page_fork(refs, table, most, i32([0, 9, 9], dev), 2 ** 20, missing=missing)
     assert int(missing) == 2 ** 11 + 2
+
+
+def test_missing_of_a_reserve_does_not_wrap(dev):
+    """Columns that narrow tables lack, past 2^31 together; the pages that there are are given all the same."""
+    from summa_amd import pages as pg
+    for S, page, most in ((3, 1, 2 ** 31 - 1), (1200, 16, 2 ** 31 - 1), (1, 16, 2 ** 27 - 2)):
+        refs = pg.page_refs(4, dev)
+        missing = torch.zeros(1, dtype=torch.int32, device=dev)
+        table = torch.full((S, 2), -1, dtype=torch.int32, device=dev)
+        pg.page_reserve(refs, table, torch.full((S,), 2 ** 31 - 1, dtype=torch.int32, device=dev), page,
+                        missing)
+        assert int(missing) == most
+        got = [p for row in table.tolist() for p in row]
+        given = min(4, 2 * S)
+        assert got == list(range(given)) + [-1] * (2 * S - given) and int(refs.sum()) == given
