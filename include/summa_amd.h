@@ -609,7 +609,8 @@ int sm_paged_keep(const sm_paged_cache* caches, int64_t ncaches, const int32_t* 
  * sm_page_remap: out[i] = page_map[block_table[i]] for n entries, -1 for those that name no
  *   page; out may be block_table.
  * sm_paged_copy: page src[i] to page dst[i], values and scales, for n pairs in every cache (all
- *   of one geometry; up to 32 a launch); a pair with a page outside [0, pages) is left out. No
+ *   of one geometry; up to 32 a launch, and launches of up to 2^24 pieces of 16 KB of a page's k or
+ *   v, below 2^31 in all); a pair with a page outside [0, pages) is left out. No
  *   page may be the destination of two pairs, nor of one and the source of another (those of the
  *   calls above are not). */
 int sm_page_reserve(int32_t* refs, int64_t pages, int32_t* block_table, int64_t S,

@@ -349,7 +349,7 @@ struct CopyArgs {
   const int32_t *src, *dst;
   Divide parts, layers;
   int64_t page_bytes;  // of k, and of v
-  int pages, n, scale_bytes;
+  int pages, scale_bytes;
 };
 constexpr int kPart = 16384;  // bytes of k or v that a workgroup copies
 
@@ -514,29 +514,34 @@ extern "C" int sm_paged_copy(const sm_paged_cache* caches, int64_t ncaches, cons
   SM_REQUIRE(src && dst, "%s: null buffer", me);
   const bool c8 = caches->dtype == SM_F8E4M3;
   CopyArgs a;
-  a.src = src;
-  a.dst = dst;
-  a.n = (int)n;
   a.pages = (int)caches->pages;
   a.page_bytes = caches->kv_heads * caches->page_tokens * caches->head_dim * (c8 ? 1 : 2);
   a.scale_bytes = (int)(caches->kv_heads * (caches->page_tokens / kBlock));
   const int64_t parts = 2 * ceil_div(a.page_bytes, kPart);
-  // (a grid holds less than 2^32 threads)
-  if (parts * std::min<int64_t>(ncaches, kLayers) > ((1 << 24) - 1) / n) {
+  // (a grid holds less than 2^32 threads: a launch takes the layers and pairs that fit)
+  constexpr int64_t most = (1 << 24) - 1;
+  if (parts > most || parts * ncaches > 0x7fffffff / n) {
     set_error("%s: problem too large", me);
     return SM_ERR_UNSUPPORTED;
   }
   a.parts = Divide((int)parts);
-  for (int64_t l0 = 0; l0 < ncaches; l0 += kLayers) {
-    const int64_t layers = std::min<int64_t>(kLayers, ncaches - l0);
+  const int64_t of_launch = std::min<int64_t>(kLayers, most / parts);
+  for (int64_t l0 = 0; l0 < ncaches; l0 += of_launch) {
+    const int64_t layers = std::min(of_launch, ncaches - l0);
     a.layers = Divide((int)layers);
     for (int64_t i = 0; i < layers; ++i) {
       const sm_paged_cache& c = caches[l0 + i];
       a.c[i] = {static_cast<uint8_t*>(c.k), static_cast<uint8_t*>(c.v),
                 c8 ? c.k_scales : nullptr, c8 ? c.v_scales : nullptr};
     }
-    copy_kernel<<<(unsigned)(parts * layers * n), 256, 0, as_stream(stream)>>>(a);
-    SM_LAUNCH_CHECK();
+    const int64_t each = most / (parts * layers);
+    for (int64_t i = 0; i < n; i += each) {
+      a.src = src + i;
+      a.dst = dst + i;
+      copy_kernel<<<(unsigned)(parts * layers * std::min(each, n - i)), 256, 0,
+                    as_stream(stream)>>>(a);
+      SM_LAUNCH_CHECK();
+    }
   }
   return SM_OK;
 }
