@@ -1423,7 +1423,10 @@ int paged_attention(const char* me, const sm_paged_cache* cache, const int32_t* 
   a.tile = Divide(plan.tile);
   a.tiles = Divide((int)plan.tiles);
   // the keys of a group, and whether an XCD's groups leave a quarter of its 4 MiB L2
-  const int64_t span = plan.nsplit > 1 ? (int64_t)plan.cb * kBlock : max_tokens;
+  // (shared splits: as long as they are where all sequences have max_tokens)
+  const int64_t span = plan.share ? std::max<int64_t>(kShare * kUnit * kBlock,
+                                                      ceil_div(S * max_tokens, plan.share))
+                       : plan.nsplit > 1 ? (int64_t)plan.cb * kBlock : max_tokens;
   const int64_t kv = span * hd * (cache->dtype == SM_F8E4M3 ? 2 : 4);
   const int64_t groups = KVH * (plan.share ? plan.share : S * plan.nsplit);
   a.map = PagedMap((uint32_t)groups, (uint32_t)plan.tiles, groups / 8 * kv <= 3 << 20);
