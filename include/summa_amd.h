@@ -689,8 +689,9 @@ int sm_sample_ex(const float* logits, int64_t rows, int64_t ld, int64_t vocab,
  * Options: arrays [rows] on the device, or where NULL the one value for all rows (which is
  * checked: "temperature must not be NaN", "top_p must be in (0, 1]", "min_p must be in [0, 1]").
  * tokens [rows]; logprobs (nullable) [rows] f32: log_softmax(logits)[token] of the raw logits.
- * Weights and their sums are held in 64 bits, relative to each other within 2^-44 (weights below
- * 2^-1000 of the row's largest are none); a row's token does not depend on the others. Rows with
+ * Weights and their sums are held in 64 bits, sums in a fixed order: a weight is within 2^-44 of
+ * itself down to 2^-80 of the row's largest and within 2^-42 below, and those under 2^-900 of the largest
+ * may count as none; a row's token does not depend on the others. Rows with
  * more equal logits at the border of a filter than a list of 1024 holds (512 up to 16384 logits), with
  * top_k above half of that, with +inf, or with a temperature outside 1e-30 .. 1e30, take several
  * passes over the row, 3 to 10 times as long.

@@ -21,7 +21,7 @@ struct RowsArgs {
   sm_row_sampling o;
   int32_t* tokens;
   float* logprobs;
-  int vocab, bits;
+  int vocab;
   int steps;  // slots of a wave
   int parts;  // workgroups of a row
   uint8_t* ws;
@@ -44,26 +44,83 @@ struct Cut {  // keys above T are kept, and those at T up to index `last`
   }
 };
 
-template <int THREADS>
-struct Shared {
-  unsigned long long hist[256];
-  unsigned long long part[THREADS / kWave];
-  float f[THREADS / kWave];
-  int i[THREADS / kWave];
-  int bin, last;
-  unsigned long long left;
+// Sums of weights by atomics, in any order: whole numbers of 128 bits, in units of 2^-96 of the
+// largest weight, so that the sums of 2^30 logits hold and are off by less than 2^-66 of it.
+struct Wide {
+  unsigned long long hi, lo;
+  __device__ inline bool less(const Wide& o) const { return hi < o.hi || (hi == o.hi && lo < o.lo); }
+  __device__ inline void add(const Wide& o) {
+    lo += o.lo;
+    hi += o.hi + (lo < o.lo);
+  }
+  __device__ inline void take(const Wide& o) {
+    hi -= o.hi + (lo < o.lo);
+    lo -= o.lo;
+  }
+  __device__ inline Wide times(unsigned long long c) const { return {hi * c + __umul64hi(lo, c), lo * c}; }
+  __device__ inline double value() const { return (double)hi * 0x1p64 + (double)lo; }
+  __device__ static inline Wide of(double x) {  // its whole part, x < 2^127
+    const unsigned long long hi = (unsigned long long)(x * 0x1p-64);
+    return {hi, (unsigned long long)(x - (double)hi * 0x1p64)};
+  }
+};
+
+// Sums of weights in a fixed order, in f64 with what each addition rounds off beside them: a row of
+// 2^30 logits is 2^20 additions a thread.
+struct Sum {
+  double s = 0.0, rest = 0.0;
+  __device__ inline void add(double x) {
+    const double t = s + x, y = t - s;
+    rest += (s - (t - y)) + (x - y);
+    s = t;
+  }
+  __device__ inline double value() const { return s + rest; }
 };
 
 template <int THREADS>
-__device__ inline unsigned long long block_sum(unsigned long long x, Shared<THREADS>& sh) {
+struct Shared {
+  unsigned long long hist[256], high[256];
+  unsigned long long part[THREADS / kWave];
+  double f[THREADS / kWave], rest[THREADS / kWave];
+  int i[THREADS / kWave];
+  int bin, last;
+  Wide left;
+};
+
+template <int THREADS>
+__device__ inline Wide block_sum(Wide x, Shared<THREADS>& sh) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, kWave);
-  if (threadIdx.x % kWave == 0) sh.part[threadIdx.x / kWave] = x;
+  for (int o = 32; o > 0; o >>= 1) x.add({__shfl_xor(x.hi, o, kWave), __shfl_xor(x.lo, o, kWave)});
+  if (threadIdx.x % kWave == 0) {
+    sh.hist[threadIdx.x / kWave] = x.lo;
+    sh.high[threadIdx.x / kWave] = x.hi;
+  }
   __syncthreads();
-  unsigned long long s = 0;
-  for (int i = 0; i < THREADS / kWave; ++i) s += sh.part[i];
+  Wide s{0, 0};
+  for (int i = 0; i < THREADS / kWave; ++i) s.add({sh.high[i], sh.hist[i]});
   __syncthreads();
   return s;
+}
+template <int THREADS>
+__device__ inline double block_sum(Sum x, Shared<THREADS>& sh) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const double rest = __shfl_xor(x.rest, o, kWave);
+    x.add(__shfl_xor(x.s, o, kWave));
+    x.rest += rest;
+  }
+  if (threadIdx.x % kWave == 0) {
+    sh.f[threadIdx.x / kWave] = x.s;
+    sh.rest[threadIdx.x / kWave] = x.rest;
+  }
+  __syncthreads();
+  Sum s;
+  for (int i = 0; i < THREADS / kWave; ++i) {
+    s.add(sh.f[i]);
+    s.rest += sh.rest[i];
+  }
+  __syncthreads();
+  return s.value();
 }
 template <int THREADS>
 __device__ inline unsigned long long block_before(unsigned long long x, Shared<THREADS>& sh,
@@ -86,11 +143,32 @@ __device__ inline unsigned long long block_before(unsigned long long x, Shared<T
   __syncthreads();
   return base + inc - x;
 }
+// Up to and with this thread's.
+template <int THREADS>
+__device__ inline double block_inclusive(double x, Shared<THREADS>& sh, double& total) {
+  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
+  double inc = x;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const double t = __shfl_up(inc, o, kWave);
+    if (lane >= o) inc += t;
+  }
+  if (lane == kWave - 1) sh.f[w] = inc;
+  __syncthreads();
+  double base = 0.0;
+  total = 0.0;
+  for (int i = 0; i < THREADS / kWave; ++i) {
+    if (i < w) base += sh.f[i];
+    total += sh.f[i];
+  }
+  __syncthreads();
+  return base + inc;
+}
 
 template <typename T>
 struct Row {
   const T* p;
-  int vocab, bits;
+  int vocab;
   float m;
   double inv;
   __device__ inline float at(int v) const {
@@ -104,32 +182,35 @@ struct Row {
     if (x == -INFINITY || m == INFINITY) return 0.0;
     return exp(((double)x - (double)m) * inv);
   }
-  __device__ inline unsigned long long whole(float x) const {
-    return (unsigned long long)rint(ldexp(weight(x), bits));
-  }
+  __device__ inline Wide whole(float x) const { return Wide::of(weight(x) * 0x1p96); }
 };
 
 // The place in (value, index) order up to which the elements kept by `outer` amount to
 // `target`, counted or weighed.
 template <bool MASS, int THREADS, typename T>
-__device__ Cut select(const Row<T>& row, const Cut& outer, unsigned long long target,
-                      Shared<THREADS>& sh) {
+__device__ Cut select(const Row<T>& row, const Cut& outer, Wide target, Shared<THREADS>& sh) {
   uint32_t prefix = 0, mask = 0;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += THREADS) sh.hist[i] = 0;
+    for (int i = threadIdx.x; i < 256; i += THREADS) sh.hist[i] = sh.high[i] = 0;
     __syncthreads();
     for (int v = threadIdx.x; v < row.vocab; v += THREADS) {
       const float x = row.at(v);
       const uint32_t key = key_of(x);
       if ((key & mask) != prefix || !outer.keeps(key, v)) continue;
-      const unsigned long long w = MASS ? row.whole(x) : 1ull;
-      if (w) atomicAdd(&sh.hist[key >> shift & 255u], w);
+      const uint32_t bin = key >> shift & 255u;
+      Wide w{0, 1};
+      if constexpr (MASS) w = row.whole(x);
+      if (w.lo) {
+        const unsigned long long old = atomicAdd(&sh.hist[bin], w.lo);
+        w.hi += old + w.lo < old;
+      }
+      if (w.hi) atomicAdd(&sh.high[bin], w.hi);
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-      unsigned long long left = target;
+      Wide left = target;
       int b = 255;
-      for (; b > 0 && sh.hist[b] < left; --b) left -= sh.hist[b];
+      for (; b > 0 && Wide{sh.high[b], sh.hist[b]}.less(left); --b) left.take({sh.high[b], sh.hist[b]});
       sh.bin = b;
       sh.left = left;
     }
@@ -141,20 +222,31 @@ __device__ Cut select(const Row<T>& row, const Cut& outer, unsigned long long ta
   }
   Cut c;
   c.T = prefix;
+  // of the elements at the value, which all weigh the same, the least count that amounts to it
+  unsigned long long need = target.lo;
+  if constexpr (MASS) {
+    const Wide w = row.whole(key_value(prefix));
+    unsigned long long lo = 1, hi = 1ull << 30;
+    while (lo < hi) {
+      const unsigned long long mid = (lo + hi) / 2;
+      if (w.times(mid).less(target)) lo = mid + 1;
+      else hi = mid;
+    }
+    need = lo;
+  }
   if (threadIdx.x == 0) sh.last = 0x7fffffff;
   __syncthreads();
   unsigned long long before = 0;  // of the elements at the value, by index
-  for (int v0 = 0; v0 < row.vocab; v0 += THREADS) {
+  for (int v0 = 0; v0 < row.vocab && before < need; v0 += THREADS) {
     const int v = v0 + threadIdx.x;
     unsigned long long w = 0;
     if (v < row.vocab) {
-      const float x = row.at(v);
-      const uint32_t key = key_of(x);
-      if (key == prefix && outer.keeps(key, v)) w = MASS ? row.whole(x) : 1ull;
+      const uint32_t key = key_of(row.at(v));
+      w = key == prefix && outer.keeps(key, v);
     }
     unsigned long long total;
     const unsigned long long at = before + block_before(w, sh, total);
-    if (w && at < target && at + w >= target) sh.last = v;
+    if (w && at + 1 == need) sh.last = v;
     before += total;
   }
   __syncthreads();
@@ -164,90 +256,99 @@ __device__ Cut select(const Row<T>& row, const Cut& outer, unsigned long long ta
 }
 
 // One row by passes over memory: takes every row, and is what rows that the kernel below does not
-// hold in its lists come to. Whole-number weights here: sums by atomics.
+// hold in its lists come to. Bound by its passes, each with an exponential in f64 for every logit.
 template <int THREADS, typename T>
 __device__ void by_passes(const RowsArgs& a, int r, const Row<T>& row, int top_k, float top_p,
                           float min_p, Shared<THREADS>& sh) {
   const int tid = threadIdx.x;
   int first = 0x7fffffff;
-  float s = 0.f;
+  Sum s;
   for (int v = tid; v < a.vocab; v += THREADS) {
     const float x = row.at(v);
-    s += x == row.m ? 1.f : row.m == INFINITY ? 0.f : __expf(x - row.m);
+    s.s += (double)(x == row.m ? 1.f : row.m == INFINITY ? 0.f : __expf(x - row.m));
     if (x == row.m) first = min(first, v);
   }
-  s = wave_sum(s);
+  const float exps = (float)block_sum(s, sh);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, kWave));
-  if (tid % kWave == 0) {
-    sh.f[tid / kWave] = s;
-    sh.i[tid / kWave] = first;
-  }
+  if (tid % kWave == 0) sh.i[tid / kWave] = first;
   __syncthreads();
-  s = 0.f;
-  for (int i = 0; i < THREADS / kWave; ++i) {
-    s += sh.f[i];
-    first = min(first, sh.i[i]);
-  }
+  for (int i = 0; i < THREADS / kWave; ++i) first = min(first, sh.i[i]);
   __syncthreads();
   int token = first;
   if (row.inv > 0.0 || row.inv == 0.0) {  // (not greedy: NaN)
     Cut ck, cp;
     if (top_k >= 1 && top_k < a.vocab)
-      ck = select<false, THREADS>(row, Cut{}, (unsigned long long)top_k, sh);
+      ck = select<false, THREADS>(row, Cut{}, Wide{0, (unsigned long long)top_k}, sh);
     if (top_p < 1.f) {
-      unsigned long long w = 0;
+      Wide w{0, 0};
       for (int v = tid; v < a.vocab; v += THREADS) {
         const float x = row.at(v);
-        if (ck.keeps(key_of(x), v)) w += row.whole(x);
+        if (ck.keeps(key_of(x), v)) w.add(row.whole(x));
       }
       w = block_sum(w, sh);
-      const double t = ceil((double)w * (double)top_p);
-      cp = select<true, THREADS>(row, ck, t < 1.0 ? 1ull : (unsigned long long)t, sh);
+      const double t = ceil(w.value() * (double)top_p);
+      cp = select<true, THREADS>(row, ck, t < 1.0 ? Wide{0, 1} : Wide::of(t), sh);
     }
     const double least = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0;
-    auto kept = [&](int v, float x) {
+    auto kept = [&](int v) {
+      const float x = row.at(v);
       const uint32_t key = key_of(x);
-      if (!ck.keeps(key, v) || !cp.keeps(key, v)) return 0ull;
-      return least > 0.0 && row.weight(x) < least ? 0ull : row.whole(x);
+      if (!ck.keeps(key, v) || !cp.keeps(key, v)) return 0.0;
+      const double w = row.weight(x);
+      return w < least ? 0.0 : w;
     };
-    unsigned long long w = 0;
-    for (int v = tid; v < a.vocab; v += THREADS) w += kept(v, row.at(v));
-    w = block_sum(w, sh);
-    // whole numbers: the sum passes u w where it passes floor(u w)
+    Sum w;
+    int last = -1;  // (where the sums below come to less than u = 1 - 2^-53 of this one)
+    for (int v = tid; v < a.vocab; v += THREADS) {
+      const double x = kept(v);
+      w.add(x);
+      if (x > 0.0) last = v;
+    }
     const double u = fmin(fmax((double)a.uniforms[r], 0.0), 1.0 - 0x1p-53);
-    const unsigned long long u64 = (unsigned long long)(u * 0x1p64);
-    const unsigned long long aim = __umul64hi(w, u64);
-    if (tid == 0) sh.last = u > 0.0 ? first : 0x7fffffff;
-    unsigned long long before = 0;
+    const double aim = fmax(u * block_sum(w, sh), 0x1p-900);
+    if (tid == 0) {
+      sh.last = 0x7fffffff;
+      sh.bin = -1;
+    }
     __syncthreads();
-    if (u == 0.0) {
-      // the first of any weight, also of one that rounds to no 2^-46 (the least u above
-      // zero, 2^-24, is past the sum of all of those)
-      for (int v = tid; v < a.vocab; v += THREADS) {
-        const float x = row.at(v);
-        const uint32_t key = key_of(x);
-        if (!ck.keeps(key, v) || !cp.keeps(key, v)) continue;
-        const double y = row.weight(x);
-        if (y > 0.0 && y >= least) atomicMin(&sh.last, v);
+    if (last >= 0) atomicMax(&sh.bin, last);
+    // four logits a thread and step: what passes is looked for in the first thread's that does
+    constexpr int PER = 4;
+    Sum before;
+    token = 0x7fffffff;
+    for (int v0 = 0; v0 < a.vocab && token == 0x7fffffff; v0 += PER * THREADS) {
+      double x[PER], part = 0.0, total;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const int v = v0 + tid * PER + e;
+        x[e] = v < a.vocab ? kept(v) : 0.0;
+        part += x[e];
       }
-      before = ~0ull;
+      const double inc = block_inclusive(part, sh, total);
+      const double left = (aim - before.s) - before.rest;
+      if (part > 0.0 && inc > left) {
+        double at = inc - part;
+        int got = -1;
+        bool passed = false;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          at += x[e];
+          if (x[e] > 0.0 && !passed) got = e;
+          passed |= x[e] > 0.0 && at > left;
+        }
+        atomicMin(&sh.last, v0 + tid * PER + got);
+      }
+      __syncthreads();
+      token = sh.last;
+      before.add(total);
     }
-    for (int v0 = 0; v0 < a.vocab && before <= aim; v0 += THREADS) {
-      const int v = v0 + tid;
-      const unsigned long long x = v < a.vocab ? kept(v, row.at(v)) : 0ull;
-      unsigned long long total;
-      const unsigned long long at = before + block_before(x, sh, total);
-      if (at <= aim && at + x > aim) sh.last = v;
-      before += total;
-    }
-    __syncthreads();
-    token = sh.last;
+    if (token == 0x7fffffff) token = sh.bin;
   }
   if (tid == 0) {
     a.tokens[r] = token;
     if (a.logprobs)
-      a.logprobs[r] = (row.m == INFINITY ? 0.f : row.at(token) - row.m) - __logf(s);
+      a.logprobs[r] = (row.m == INFINITY ? 0.f : row.at(token) - row.m) - __logf(exps);
   }
 }
 
@@ -259,8 +360,10 @@ __device__ void by_passes(const RowsArgs& a, int r, const Row<T>& row, int top_k
 __device__ SM_INLINE void side_by_side(double (&x)[4]) {
   asm volatile("" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
 }
-// 2^(d c), d <= 0, d c >= -1022, within 2^-45: a polynomial of degree 9 on the half octave to either
-// side of a whole one (interpolated at the Chebyshev nodes).
+// 2^(d c), d <= 0, d c >= -1022: a polynomial of degree 9 on the half octave to either side of a whole
+// one (interpolated at the Chebyshev nodes; 2^-44.59 off at its ends). Beside it c, a quotient and a
+// product that are rounded, is off by 2^-51.7 of itself, which every octave adds to: 2^-44 of the weight down
+// to 2^-80 of the largest, 2^-42 at the least.
 __device__ SM_INLINE void exp2_f64(const double (&d)[4], double c, double (&p)[4]) {
   constexpr double magic = 0x1.8p52;
   constexpr double co[] = {0x1.63ef9699120e2p-20, 0x1.ffcb767842e11p-17, 0x1.43088e2580989p-13,
@@ -569,7 +672,6 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
   Row<T> row;
   row.p = static_cast<const T*>(a.logits) + r * a.ld;
   row.vocab = a.vocab;
-  row.bits = a.bits;
   const float temperature = a.o.temperatures ? a.o.temperatures[r] : a.o.temperature;
   const int top_k = a.o.top_ks ? a.o.top_ks[r] : a.o.top_k;
   const float top_p = a.o.top_ps ? a.o.top_ps[r] : a.o.top_p;
@@ -1212,8 +1314,6 @@ extern "C" int sm_sample_rows(const void* logits, int dtype, int64_t rows, int64
   a.tokens = tokens;
   a.logprobs = logprobs;
   a.vocab = (int)vocab;
-  a.bits = 46;
-  while (((int64_t)1 << (63 - a.bits)) < vocab) --a.bits;
   hipStream_t st = as_stream(stream);
   a.parts = row_parts(rows, vocab);
   a.ws = static_cast<uint8_t*>(workspace);

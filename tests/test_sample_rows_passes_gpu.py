@@ -1,0 +1,89 @@
+"""Rows that the sampler does not hold in its lists: what many small weights together come to."""
+import math
+from fractions import Fraction
+
+import pytest
+import torch
+
+from test_sample_rows_gpu import BF16, F16, F32, check
+
+pytestmark = pytest.mark.gpu
+
+
+def peak_and_tail(vocab, octaves, at):
+    """One large logit and a flat rest, 2^-octaves of its weight each."""
+    x = torch.full((1, vocab), -octaves * math.log(2.0))
+    x[0, at] = 0.0
+    w = math.exp(float(x[0, at - 1 if at else 1]))
+    return x, w
+
+
+def behind_the_peak(n, w, u, p=1.0):
+    """Tokens that sampling may give where the first of n + 1 weighs 1 and the others w, in exact
+    arithmetic. (Running sums in f64 drift: 2^-53 at each of millions of additions to 1, against a w of
+    2^-42 to 2^-46.) The kernel's own sums may be off by what 36 additions of up to 1 and the product with u
+    round: of its first 4096 logits four in a thread, six over a wave, sixteen over the waves, for the
+    thread's sum and again for the step's, and four within the thread; what lies behind them adds up
+    small numbers. Its border is off by two roundings."""
+    w, u, p = Fraction(w), Fraction(u), Fraction(p)
+    whole = 1 + n * w
+    tokens = set()
+    for border in (p * whole * (1 - Fraction(2) ** -51), p * whole * (1 + Fraction(2) ** -51)):
+        kept = n if p >= 1 else min(n, max(0, math.ceil((border - 1) / w)))
+        aim = u * (1 + kept * w)
+        for off in (-37 * Fraction(2) ** -53, 37 * Fraction(2) ** -53):
+            tokens.add(0 if aim + off < 1 else min(kept, math.floor((aim + off - 1) / w) + 1))
+    return min(tokens), max(tokens)
+
+
+@pytest.mark.parametrize("vocab,octaves", [(2 ** 22, 42.1), (2 ** 20 + 7, 44.05), (300001, 46.3), (300001, 60.0)])
+def test_flat_tails_of_large_vocabularies(dev, vocab, octaves):
+    """Every weight of the tail is nothing beside the largest, and their sum is not."""
+    from summa_amd import sampling
+    print(f"case tail {vocab} {octaves}", flush=True)
+    # behind the peak: the last numbers below one (where the tail has 2^-24 of the whole)
+    x, w = peak_and_tail(vocab, octaves, 0)
+    tail, xd = w * (vocab - 1), x.to(dev)
+    for u in (1 - 2.0 ** -24, 1 - 2.0 ** -22, 1 - 2.0 ** -23):
+        for p in (1.0, 1 - 2.0 ** -24, 1 - 2.0 ** -22):
+            tok, lp = sampling.sample_rows(xd, torch.tensor([u], device=dev), top_p=p)
+            least, most = behind_the_peak(vocab - 1, w, u, p)
+            assert least <= int(tok) <= most and most - least <= 2, (u, p, int(tok), least, most)
+            assert abs(float(lp) - (float(x[0, int(tok)]) - math.log1p(tail))) <= 2.0 ** -16 + 2.0 ** -23 * 45
+            if p == 1:
+                assert (most > 0) == (1 - u < tail / (1 + tail))
+    # before it: small numbers
+    x, w = peak_and_tail(vocab, octaves, vocab - 1)
+    for j in (0, 1, 1000, vocab // 2):
+        u = torch.tensor([(j + 0.5) * w / (1 + tail)])
+        assert check(x, u) == [j]
+
+
+@pytest.mark.parametrize("vocab,k", [(7, 5), (20000, 9000), (65536, 60000), (131072, 1500)])
+@pytest.mark.parametrize("octaves", [47.5, 70.0, 200.0, 800.0])
+def test_small_numbers_of_rows_with_a_large_top_k(dev, vocab, k, octaves):
+    """A small u is an answer of its own, however small the weights are that it falls in."""
+    print(f"case small u {vocab} {k} {octaves}", flush=True)
+    x, w = peak_and_tail(vocab, octaves, vocab - 1)
+    for T in (1.0, 8.0):
+        y = x * T                                    # (exact: a power of two)
+        for j in (0, 2, k // 2):
+            u = (j + 0.5) * w
+            if u < 1e-45:                            # (below the least f32: u is zero)
+                u, j = 0.0, 0
+            got = check(y, torch.tensor([u]), T=T, k=k, where=(T, j))
+            if u == 0.0 or u > 1e-37:
+                assert got == [j]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("vocab", [65536, 131072, 262145, 1 << 20])
+def test_flat_rows(dev, vocab, dtype):
+    """Spreads from nothing to one: most logits are near the border."""
+    print(f"case flat {vocab} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(vocab)
+    spread = torch.tensor([0.0, 0.01, 0.1, 0.3, 1.0])
+    x = (torch.randn(5, vocab, generator=g) * spread[:, None]).to(dtype)
+    u = torch.rand(5, generator=g)
+    for kw in (dict(), dict(p=0.5), dict(p=0.9, T=2.0), dict(p=0.9, k=vocab // 2), dict(m=0.7, T=0.5)):
+        check(x, u, where=kw, **kw)
