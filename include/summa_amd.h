@@ -691,10 +691,12 @@ int sm_sample_ex(const float* logits, int64_t rows, int64_t ld, int64_t vocab,
  * tokens [rows]; logprobs (nullable) [rows] f32: log_softmax(logits)[token] of the raw logits.
  * Weights and their sums are held in 64 bits, sums in a fixed order: a weight is within 2^-44 of
  * itself down to 2^-80 of the row's largest and within 2^-42 below, and those under 2^-900 of the largest
- * may count as none; a row's token does not depend on the others. Rows with
- * more equal logits at the border of a filter than a list of 1024 holds (512 up to 16384 logits), with
- * top_k above half of that, with +inf, or with a temperature outside 1e-30 .. 1e30, take several
- * passes over the row, 3 to 10 times as long.
+ * may count as none; a row's token does not depend on the others. Rows take
+ * several passes over memory, 8 to 20 times as long (256 rows of 65536: 0.4-0.8 ms, not 0.05), with
+ * more logits than a list of 1024 holds (512 up to 16384 logits) equal at the border of top_k or close to that
+ * of top_p (within some 0.02 temperature of it, 0.08 up to 16384 logits: a row whose logits spread over less than
+ * 0.2 temperature has them), with top_k above half of that, with +inf, with a temperature outside 1e-30 ..
+ * 1e30, or with more than 262144 logits.
  * workspace: sm_sample_rows_workspace_bytes(...) bytes (0 but for a few rows of a large vocabulary, which
  * are shared out over the chip; -1 for a bad shape), 16-byte aligned; calls that share one must
  * not overlap. rows below 2^22, vocab below 2^30. */

@@ -44,6 +44,10 @@ struct Cut {  // keys above T are kept, and those at T up to index `last`
   }
 };
 
+// What is called for every step, and what takes the rows' state by reference, is not left to the
+// compiler's measure of size: a call puts that in scratch (256 rows of 65536 with top-p 52 -> 72 us).
+#define SM_INLINE __attribute__((always_inline)) inline
+
 // Sums of weights by atomics, in any order: whole numbers of 128 bits, in units of 2^-96 of the
 // largest weight, so that the sums of 2^30 logits hold and are off by less than 2^-66 of it.
 struct Wide {
@@ -258,7 +262,7 @@ __device__ Cut select(const Row<T>& row, const Cut& outer, Wide target, Shared<T
 // One row by passes over memory: takes every row, and is what rows that the kernel below does not
 // hold in its lists come to. Bound by its passes, each with an exponential in f64 for every logit.
 template <int THREADS, typename T>
-__device__ void by_passes(const RowsArgs& a, int r, const Row<T>& row, int top_k, float top_p,
+__device__ SM_INLINE void by_passes(const RowsArgs& a, int r, const Row<T>& row, int top_k, float top_p,
                           float min_p, Shared<THREADS>& sh) {
   const int tid = threadIdx.x;
   int first = 0x7fffffff;
@@ -351,9 +355,6 @@ __device__ void by_passes(const RowsArgs& a, int r, const Row<T>& row, int top_k
       a.logprobs[r] = (row.m == INFINITY ? 0.f : row.at(token) - row.m) - __logf(exps);
   }
 }
-
-// (what is called for every step is not left to the compiler's measure of size)
-#define SM_INLINE __attribute__((always_inline)) inline
 
 // Four at a time, step by step: left to itself the compiler makes one after the other, and each
 // operation waits for the one before it.
@@ -637,8 +638,10 @@ struct RowShare {
 //   and of those above the list, and the exact border is found in the list;
 // - the draw: sums of 512 consecutive logits are kept by the 64-bit pass; those that u falls in are
 //   read again. One wave does it.
-// Rows that the list does not hold (hundreds of equal logits at a border, a larger top-k), and those
-// with +inf, go by passes.
+// Rows that the list does not hold (more logits at a border than it has room for, a larger top-k), and those
+// with +inf, go by passes: 256 rows of 65536 f32 640 us with top-p where all logits are nearly equal, 420 with
+// top-k 3000. Entries that a wave's part of the list has no room for go to the others' through one LDS counter:
+// rows in falling order with top-p 90 us (493 by passes), flat ones (spread 0.1) with top-p 0.9 109 (643).
 //
 // Bound by instructions, not by memory. 256 rows of 65536 f32 with top-p 54 us (1.24 TB/s; the logits are 14
 // us of HBM): 13 us until the row is there, 8 for the bins, 22 for the 64-bit pass (an f64
@@ -819,7 +822,8 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
   float list_lo = m, list_hi = m;  // the list: logits from list_lo to list_hi
   int n = 0;
   // Adds what piece j of a step has of it, in no order: with top-k, where few pieces have any, to the
-  // list; else to the wave's part of it, which needs no answer from LDS.
+  // list; else to the wave's part of it, which needs no answer from LDS, until that is full (a border
+  // that lies in one stretch of the vocabulary).
   int mine = 0;
   auto to_list = [&](int i, int j, const float* x) __attribute__((always_inline)) {
     bool hit[H::G];
@@ -847,12 +851,28 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
     }
     int skip;
     const int place = held.place(i, j, skip);
+    int before = 0;  // of this lane's hits
 #pragma unroll
     for (int e = 0; e < H::G; ++e)
       if (hit[e]) {
         if (put < end) to[put] = (unsigned long long)key_of(x[e]) << 32 | (uint32_t)~(place + e);
         ++put;
+        ++before;
       }
+    if (!PARTS && !by_k && mine > end) {  // (uniform; seldom)
+      const int from = max(mine - hits, end);  // the first that the part does not hold
+      int base = 0;
+      if (lane == 0) base = atomicAdd(&sh.listed, mine - from);
+      base = __builtin_amdgcn_readfirstlane(base) - from;
+      put -= before;
+#pragma unroll
+      for (int e = 0; e < H::G; ++e)
+        if (hit[e]) {
+          if (put >= end && base + put < L::CAP)
+            sh.c.key[base + put] = (unsigned long long)key_of(x[e]) << 32 | (uint32_t)~(place + e);
+          ++put;
+        }
+    }
   };
   if constexpr (PHASE == 4) {
     list_lo = lane_f32(rs->list_lo, 0);
@@ -1014,7 +1034,7 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
       if (lane == 0) {
         (PARTS ? rs->all : sh.all)[nth * NW + wave] = all;
         (PARTS ? rs->above : sh.above)[nth * NW + wave] = above;
-        sh.n[wave] = mine;
+        sh.n[wave] = min(mine, L::CAP / NW);
       }
     } else {
       for (int i = lane; i < a.steps; i += kWave)
@@ -1064,17 +1084,17 @@ __global__ __launch_bounds__(THREADS, sizeof(T) * STEPS <= 32 ? 4 : 2) void samp
   } else if (fits && by_k) {
     n = sh.listed;
     fits = n <= L::CAP;
-  } else if (fits && by_p) {  // the waves' parts, one behind the other
-    int most = 0, at = 0;
+  } else if (fits && by_p) {  // the waves' parts, behind what they did not hold
+    n = sh.listed;
+    int at = n;
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
       if (i < wave) at += sh.n[i];
       n += sh.n[i];
-      most = max(most, sh.n[i]);
     }
-    fits = most <= L::CAP / NW;
+    fits = n <= L::CAP;
     if (fits)
-      for (int i = lane; i < mine; i += kWave) sh.c.key[at + i] = sh.own[wave][i];
+      for (int i = lane; i < sh.n[wave]; i += kWave) sh.c.key[at + i] = sh.own[wave][i];
     __syncthreads();
   }
   if (!fits) {

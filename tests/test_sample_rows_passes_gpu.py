@@ -87,3 +87,26 @@ def test_flat_rows(dev, vocab, dtype):
     u = torch.rand(5, generator=g)
     for kw in (dict(), dict(p=0.5), dict(p=0.9, T=2.0), dict(p=0.9, k=vocab // 2), dict(m=0.7, T=0.5)):
         check(x, u, where=kw, **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,vocab", [(5, 9000), (5, 16384), (5, 32768), (70, 65536), (70, 131072), (2, 131072)])
+@pytest.mark.parametrize("order", ["falling", "rising", "together"])
+def test_borders_in_one_stretch_of_the_vocabulary(dev, rows, vocab, dtype, order):
+    """A vocabulary in the order of its frequencies, and one whose border's logits lie side by side: more of
+    them in one wave's range than its part of the list holds, up to the list's 512 or 1024 and past it."""
+    print(f"case stretch {rows} {vocab} {dtype} {order}", flush=True)
+    g = torch.Generator().manual_seed(vocab)
+    if order == "together":
+        x = torch.randn(rows, vocab, generator=g) * 2 - 12
+        near = [40, 60, 130, 500, 900, 1500, 0][: rows]
+        for r in range(rows):
+            at = vocab // 3 + 17 * r
+            x[r, at:at + near[r % len(near)]] = 2e-4 * torch.rand(near[r % len(near)], generator=g)
+            x[r, 11] = 3.0
+    else:
+        x = torch.sort(torch.randn(rows, vocab, generator=g) * 2, 1, descending=order == "falling")[0]
+    x = x.to(dtype)
+    u = torch.rand(rows, generator=g)
+    for kw in (dict(p=0.97), dict(p=0.6, T=1.3), dict(p=0.9, m=1e-3)):
+        check(x, u, where=(order, kw), **kw)
