@@ -640,7 +640,7 @@ struct RowShare {
 //   read again. One wave does it.
 // Rows that the list does not hold (more logits at a border than it has room for, a larger top-k), and those
 // with +inf, go by passes: 256 rows of 65536 f32 640 us with top-p where all logits are nearly equal, 420 with
-// top-k 3000. Entries that a wave's part of the list has no room for go to the others' through one LDS counter:
+// top-k 3000. What a wave's part of the list has no room for takes places of the others' through one LDS counter:
 // rows in falling order with top-p 90 us (493 by passes), flat ones (spread 0.1) with top-p 0.9 109 (643).
 //
 // Bound by instructions, not by memory. 256 rows of 65536 f32 with top-p 54 us (1.24 TB/s; the logits are 14

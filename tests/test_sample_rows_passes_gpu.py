@@ -110,3 +110,25 @@ def test_borders_in_one_stretch_of_the_vocabulary(dev, rows, vocab, dtype, order
     u = torch.rand(rows, generator=g)
     for kw in (dict(p=0.97), dict(p=0.6, T=1.3), dict(p=0.9, m=1e-3)):
         check(x, u, where=(order, kw), **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [49153, 65536, 131072])
+def test_a_row_is_the_same_in_every_batch(dev, vocab, dtype):
+    """Shared out over the chip in small batches, in one workgroup in large ones: the rows' tokens are the
+    definition's and each other's, log-probs the same within their f32 sums."""
+    from summa_amd import sampling
+    print(f"case batches {vocab} {dtype}", flush=True)
+    x = (torch.randn(300, vocab) * 2).to(dtype)
+    u = torch.rand(300)
+    xd, ud = x.to(dev), u.to(dev)
+    for kw in (dict(), dict(top_k=300), dict(top_p=0.9), dict(top_k=400, top_p=0.8, min_p=1e-3),
+               dict(temperature=0.0), dict(min_p=0.05, temperature=1.4)):
+        tok, lp = sampling.sample_rows(xd, ud, **kw)
+        for rows in (1, 3, 8, 31, 32, 33, 63, 64, 65, 128):
+            t, l = sampling.sample_rows(xd[:rows], ud[:rows], **kw)
+            assert torch.equal(t, tok[:rows]), (kw, rows)
+            assert float((l - lp[:rows]).abs().max()) <= 2.0 ** -15, (kw, rows)
+        names = dict(top_k="k", top_p="p", min_p="m", temperature="T")
+        got = check(x[:4], u[:4], **{names[k]: v for k, v in kw.items()})
+        assert got == tok[:4].tolist()
