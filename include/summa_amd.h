@@ -694,9 +694,9 @@ int sm_sample_ex(const float* logits, int64_t rows, int64_t ld, int64_t vocab,
  * may count as none; a row's token does not depend on the others. Rows take
  * several passes over memory, 8 to 20 times as long (256 rows of 65536: 0.4-0.8 ms, not 0.05), with
  * more logits than a list of 1024 holds (512 up to 16384 logits) equal at the border of top_k or close to that
- * of top_p (within some 0.02 temperature of it, 0.08 up to 16384 logits: a row whose logits spread over less than
- * 0.2 temperature has them), with top_k above half of that, with +inf, with a temperature outside 1e-30 ..
- * 1e30, or with more than 262144 logits.
+ * of top_p (within some 0.02 temperature of it, 0.08 up to 16384 logits: 65536 logits of a standard deviation
+ * of 0.3 temperature may have them), with top_k above half of that, with +inf, with a temperature outside
+ * 1e-30 .. 1e30, or with more than 262144 logits.
  * workspace: sm_sample_rows_workspace_bytes(...) bytes (0 but for a few rows of a large vocabulary, which
  * are shared out over the chip; -1 for a bad shape), 16-byte aligned; calls that share one must
  * not overlap. rows below 2^22, vocab below 2^30. */

@@ -643,13 +643,13 @@ struct RowShare {
 // top-k 3000. What a wave's part of the list has no room for takes places of the others' through one LDS counter:
 // rows in falling order with top-p 90 us (493 by passes), flat ones (spread 0.1) with top-p 0.9 109 (643).
 //
-// Bound by instructions, not by memory. 256 rows of 65536 f32 with top-p 54 us (1.24 TB/s; the logits are 14
-// us of HBM): 13 us until the row is there, 8 for the bins, 22 for the 64-bit pass (an f64
+// Bound by instructions, not by memory. 256 rows of 65536 f32 with top-p 49 us (1.36 TB/s; the logits are 14
+// us of HBM): 20 us until the row is there and in bins, 2 for the border's, 19 for the 64-bit pass (an f64
 // operation takes 4.9 clocks of a SIMD with four waves, of which a weight needs 16 and its sums 3
-// and a logit's share of the rest 14 of 3.3), 8 for list and draw. Without a filter 25 us for 128 rows, with top-k 22.
+// and a logit's share of the rest 14 of 3.3), 7 for list and draw. Without a filter 25 us for 128 rows, with top-k 22.
 // 768 rows of 50001 bf16 with options of all kinds 98 us: 17 us a row with top-k, most of it eight
-// barriers' waits with one workgroup a unit, 36 with top-p.
-// Tried: 512 threads with twice the registers (54 us -> 66: two waves a SIMD issue 5.7 clocks apart), two
+// barriers' waits with one workgroup a unit, 38 with top-p.
+// Tried, where 256 rows took 54 us: 512 threads with twice the registers (66: two waves a SIMD issue 5.7 clocks apart), two
 // workgroups of 64 registers a thread a unit (16 bits: spills, 98 -> 466) or of 512 threads (117: a row
 // takes twice as long), the rows in the order of their length (94, for a scan before the first load), loops unrolled over the
 // row's registers (code of 120 KB, fetched anew by every phase: 87), 64-bit bins (8 -> 12).
