@@ -132,3 +132,21 @@ def test_a_row_is_the_same_in_every_batch(dev, vocab, dtype):
         names = dict(top_k="k", top_p="p", min_p="m", temperature="T")
         got = check(x[:4], u[:4], **{names[k]: v for k, v in kw.items()})
         assert got == tok[:4].tolist()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_equal_logits_of_a_very_large_vocabulary(dev, dtype):
+    """Counts past 2^24: every token, border and draw follows from the number of logits."""
+    from summa_amd import sampling
+    n = 2 ** 25 + 3
+    print(f"case equal {n} {dtype}", flush=True)
+    x = torch.full((1, n), -3.0, dtype=dtype, device=dev)
+    for u in (0.0, 2.0 ** -26, 0.7, 1 - 2.0 ** -24):
+        for kw, kept in ((dict(), n), (dict(top_k=2 ** 24 + 5), 2 ** 24 + 5), (dict(top_p=0.75), math.ceil(0.75 * n)),
+                         (dict(top_k=2 ** 24 + 5, top_p=0.5), math.ceil((2 ** 24 + 5) * 0.5)),
+                         (dict(min_p=1.0, temperature=0.3), n)):
+            ud = torch.tensor([u], device=dev)
+            tok, lp = sampling.sample_rows(x, ud, **kw)
+            # the first at which i + 1 > u kept, in 64 bits exact up to one rounding (2^-27 of a token)
+            assert int(tok) == int(Fraction(float(ud)) * kept), (u, kw)
+            assert abs(float(lp) + math.log(n)) <= 2.0 ** -20 * math.log(n)
